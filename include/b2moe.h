@@ -58,7 +58,15 @@ enum b2moe_type {
      * stores every weight as a 4-bit code (grid lookup and sign applied once, at load time): 134 bytes per 256 weights
      * in HBM instead of 110, the same fp32 values bit for bit, and decode kernels that need no codebook lookup. The
      * layout to choose when HBM capacity allows (21.8 % more bytes per expert); B2MOE_IQ3_S keeps the GGUF size. */
-    B2MOE_IQ3_S_X4 = 0x1015
+    B2MOE_IQ3_S_X4 = 0x1015,
+    /* Not a GGUF type: plain rows of 8-bit integers, one fp32 scale a row (an 8-bit checkpoint with scales per output
+     * channel). data is int8 [experts][rows][cols], aux fp32 [experts][rows], the weight is their product; cols is a multiple of
+     * 16 and below 2^17. There is nothing to repack (b2moe_bank_load does not know the type): a bank is the caller's
+     * arrays, or what b2moe_quantize_rows makes of floating-point rows. The expert products and the layer calls take such banks, a
+     * layer may mix them with others; activation rows are quantised to 8 bits each (b2moe_quantize_rows has the rule) and the
+     * sums of products are exact. Scratch: b2moe_expert_workspace_bytes; with b2moe_expert_slot_workspace_bytes gate/up calls of
+     * many tokens per expert run on the grouped tensor-core form, with the same bits. */
+    B2MOE_I8 = 0x1008
 };
 enum b2moe_dtype { B2MOE_F32 = 0, B2MOE_F16 = 1, B2MOE_BF16 = 2 };
 /* MoeGating values, src/experts/moe.hpp:20-26 (the two the device path implements) */
@@ -258,6 +266,47 @@ B2MOE_API int32_t b2moe_combine(const float * y, const int32_t * ids, const floa
 B2MOE_API int32_t b2moe_combine_residual(const float * y, const int32_t * ids, const float * weights, const float * shared_weights,
                                const void * residual, int32_t n, int32_t topk, int32_t hidden, int32_t shared_tokens, void * out,
                                int32_t out_dtype, b2moe_stream stream);
+
+/* ---- 8-bit integers with a scale for each row and each channel ------------------------------------------------------
+ * They have no counterpart in the reference.
+ * b2moe_quantize_rows: x [n][k] of x_dtype, rows ldx elements apart -> q int8, rows ldq bytes apart, and scale [n]:
+ *   scale = max|x| / 127 (fp32), q = the integer nearest to 127 x / max|x|, halves to even, exactly. A row of zeros has
+ *   scale 0; a row that holds an infinity or a NaN has a NaN as its scale (and with it in everything that is made of it). k and
+ *   ldq are multiples of 16, k below 2^17, ldx a multiple of 16 bytes; x and q 16-byte aligned. Bytes between k and ldq are
+ *   left as they are.
+ * b2moe_linear_i8: y[t][r] = (sum_j q[t][j] w[r][j]) * (scale[t] * aux[r]) rounded once to y_dtype, rows of y ldy elements
+ *   apart; the sum is exact. w is a bank of type B2MOE_I8 with one expert; q as b2moe_quantize_rows leaves it (any values of int8).
+ *   status (device int32, may be null): set to a nonzero value where a kernel gave up a bounded wait (the output is then
+ *   invalid), otherwise left as it is. */
+B2MOE_API int32_t b2moe_quantize_rows(const void * x, int32_t x_dtype, int64_t ldx, int32_t n, int32_t k, int8_t * q, int64_t ldq, float * scale,
+                            b2moe_stream stream);
+B2MOE_API int32_t b2moe_linear_i8(const int8_t * q, int64_t ldq, const float * scale, const b2moe_bank * w, int32_t n, void * y, int32_t y_dtype,
+                        int64_t ldy, int32_t * status, b2moe_stream stream);
+
+/* ---- balance loss ------------------------------------------------------------------------------------------------
+ * The auxiliary loss that keeps a router's load even, with the counts per expert and sequence, and its gradient on the
+ * logits. It has no counterpart in the reference (which serves).
+ *   p[t] = softmax of logits[t][0..experts) (B2MOE_SOFTMAX), or their sigmoids divided by their sum (B2MOE_SIGMOID; no bias);
+ *   a row whose logits are all -inf has p = 0; any NaN makes its row, its sequence's means and the loss NaN
+ *   tokens[s] = tokens of sequence s that the mask keeps; counts[s][e] = their assignments to e; prob[s][e] = their mean p[t][e]
+ *   loss = coef / S * sum over the S sequences with tokens of experts / (topk tokens[s]) * sum_e counts[s][e] prob[s][e]
+ * logits fp32, rows ld apart (further columns, as a shared expert's, are not read); ids [n][topk], ids outside [0, experts) are
+ * not counted; mask [n] bytes, 0 = the token does not take part (null: all do; its logits and ids are not looked at);
+ * offsets: int32 [sequences + 1] (device), sequence s = the tokens offsets[s] .. offsets[s + 1) (null: one sequence of all n;
+ * an empty sequence counts nothing). Written: loss [1], counts [sequences][experts], prob [sequences][experts], tokens
+ * [sequences + 1] (the last one: S). experts <= 4096, sequences <= 65535. The sums run in a fixed order.
+ * backward: grad_logits[t][e] = (accumulate: +) grad_loss[0] (null: 1) * dloss / dlogits, with the counts held fixed, from the counts and
+ *   tokens that the loss wrote; rows ldg apart. Rows that the mask leaves out, and rows of no sequence, get 0 (accumulate: stay); columns
+ *   from `experts` on are left as they are. grad_logits may not overlap logits.
+ * workspace: b2moe_balance_workspace_bytes(experts, n, sequences) bytes, 16-byte aligned, used by one call at a time. */
+B2MOE_API size_t b2moe_balance_workspace_bytes(int32_t experts, int32_t n, int32_t sequences);
+B2MOE_API int32_t b2moe_balance_loss(int32_t gating, const float * logits, int32_t ld, const int32_t * ids, int32_t topk, const uint8_t * mask,
+                           const int32_t * offsets, int32_t sequences, int32_t experts, int32_t n, float coef, float * loss, int32_t * counts,
+                           float * prob, int32_t * tokens, void * workspace, size_t workspace_bytes, b2moe_stream stream);
+B2MOE_API int32_t b2moe_balance_loss_backward(int32_t gating, const float * logits, int32_t ld, int32_t topk, const uint8_t * mask,
+                                    const int32_t * offsets, int32_t sequences, int32_t experts, int32_t n, float coef, const int32_t * counts,
+                                    const int32_t * tokens, const float * grad_loss, float * grad_logits, int32_t ldg, int32_t accumulate,
+                                    b2moe_stream stream);
 
 /* ---- expert parallelism --------------------------------------------------------------------------------------
  * Rank r of G owns the contiguous experts [first_expert, first_expert + local_experts); tokens are data-parallel and

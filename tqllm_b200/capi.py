@@ -16,6 +16,7 @@ OK, ERR_SHAPE, ERR_ALIGN, ERR_FORMAT, ERR_NULL, ERR_WORKSPACE, ERR_CUDA, ERR_CAP
 F32, F16, BF16 = 0, 1, 2
 Q4_K, IQ4_NL, IQ3_S, IQ4_XS, NVFP4G = 12, 20, 21, 23, 323
 IQ3_S_X4 = 0x1015        # bank layout of IQ3_S blocks as 4-bit codes (b2moe_type)
+I8 = 0x1008              # plain 8-bit rows with a scale each (b2moe_type)
 FAMILY = {"auto": 0, "generic": 1, "decode": 2, "gemm": 3, "decode_kernels": 4}
 SOFTMAX, SIGMOID = 1, 2
 
@@ -100,6 +101,11 @@ SIGNATURES = {
     "b2moe_expert_down_static": (_i32, [C.POINTER(Bank)] * 2 + [_vp, _vp, _i32, _i32, _i32, _vp, _vp]),
     "b2moe_combine": (_i32, [_vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _vp, _i32, _vp]),
     "b2moe_combine_residual": (_i32, [_vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _vp, _i32, _vp]),
+    "b2moe_quantize_rows": (_i32, [_vp, _i32, _i64, _i32, _i32, _vp, _i64, _vp, _vp]),
+    "b2moe_linear_i8": (_i32, [_vp, _i64, _vp, C.POINTER(Bank), _i32, _vp, _i32, _i64, _vp, _vp]),
+    "b2moe_balance_workspace_bytes": (_sz, [_i32, _i32, _i32]),
+    "b2moe_balance_loss": (_i32, [_i32, _vp, _i32, _vp, _i32, _vp, _vp, _i32, _i32, _i32, _f32, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "b2moe_balance_loss_backward": (_i32, [_i32, _vp, _i32, _i32, _vp, _vp, _i32, _i32, _i32, _f32, _vp, _vp, _vp, _vp, _i32, _i32, _vp]),
     "b2moe_gguf_open": (_i32, [C.c_char_p, C.POINTER(C.c_void_p)]),
     "b2moe_gguf_close": (None, [_vp]),
     "b2moe_gguf_tensor_count": (_i32, [_vp]),

@@ -3,8 +3,10 @@
 // formats.cuh against dequantize_host (src/formats/weight/dequant.cpp:393-606).
 #include "common.cuh"
 #include "formats.cuh"
+#include "int8.cuh"
 
 namespace b2 {
+int32_t i8_dump(const b2moe_bank & b, float * out, cudaStream_t s);
 namespace {
 
 template <uint32_t T>
@@ -67,6 +69,11 @@ int32_t dump_t(const b2moe_bank & b, float * out, cudaStream_t s) {
 int32_t check_bank(const b2moe_bank * b) {
     FmtInfo f;
     if (!b) return B2MOE_ERR_NULL;
+    if (b->type == B2MOE_I8) {                                         // plain rows and a scale each: nothing of the block formats applies
+        if (b->experts <= 0 || b->rows <= 0 || !i8_cols(b->cols)) return B2MOE_ERR_SHAPE;
+        if (!b->data || !b->aux) return B2MOE_ERR_NULL;
+        return aligned16(b->data) ? B2MOE_OK : B2MOE_ERR_ALIGN;
+    }
     if (!fmt_info(b->type, f)) return B2MOE_ERR_FORMAT;
     if (b->experts <= 0 || b->rows <= 0 || b->cols <= 0 || b->cols % f.kt) return B2MOE_ERR_SHAPE;
     if (!b->data || (f.aux && !b->aux)) return B2MOE_ERR_NULL;
@@ -85,11 +92,13 @@ extern "C" B2MOE_API size_t b2moe_raw_bytes(uint32_t type, int32_t rows, int32_t
 }
 extern "C" B2MOE_API size_t b2moe_bank_bytes(uint32_t type, int32_t rows, int32_t cols) {
     FmtInfo f;
+    if (type == B2MOE_I8) return rows > 0 && i8_cols(cols) ? size_t(rows) * cols : 0;
     if (!fmt_info(type, f) || rows <= 0 || cols <= 0 || cols % f.kt) return 0;
     return size_t(ceil_div(rows, 16)) * (cols / f.kt) * f.tile;
 }
 extern "C" B2MOE_API size_t b2moe_bank_aux_bytes(uint32_t type, int32_t rows, int32_t cols) {
     FmtInfo f;
+    if (type == B2MOE_I8) return rows > 0 && i8_cols(cols) ? size_t(rows) * sizeof(float) : 0;
     if (!fmt_info(type, f) || rows <= 0 || cols <= 0 || cols % f.kt || !f.aux) return 0;
     return size_t(ceil_div(rows, 16)) * 16 * sizeof(float);
 }
@@ -173,6 +182,7 @@ extern "C" B2MOE_API int32_t b2moe_dequant_dump(const b2moe_bank * bank, float *
     if (!out) return B2MOE_ERR_NULL;
     cudaStream_t s = as_stream(stream);
     switch (bank->type) {
+        case B2MOE_I8: return i8_dump(*bank, out, s);
         case T_Q4_K: return dump_t<T_Q4_K>(*bank, out, s);
         case T_IQ3_S: return dump_t<T_IQ3_S>(*bank, out, s);
         case T_IQ3S4: return dump_t<T_IQ3S4>(*bank, out, s);

@@ -1,0 +1,223 @@
+// Products of 8-bit integers with a scale for each activation row and each weight row: dense (b2moe_linear_i8) and grouped by expert, the expert
+// products over a plan on banks of type B2MOE_I8.
+//
+//   sum_tr = sum_j q_tj w_rj   exactly, in 32-bit integers (so K may be split in any way and the order does not show in the result)
+//   y_tr = sum_tr * (s_t v_r);   gate/up: act_tr = silu(g_tr) u_tr
+//
+// The sum is exact, y has three roundings (the sum to fp32, the product of the scales, their product) and the one to its own type.
+#include <type_traits>
+
+#include "int8.cuh"
+
+namespace b2 {
+int32_t check_bank(const b2moe_bank * b);
+namespace {
+
+struct I8Args {
+    const int8_t * w[2], * shared_w[2];          // gate and up, or one matrix: [experts][rows][cols]
+    const float * v[2], * shared_v[2];           // their scales, [experts][rows]
+    int experts, rows, cols;
+    const int8_t * q;                            // rows in operand form
+    long long ldq;
+    const float * s;
+    const int * plan;                            // null: one matrix, rows 0..n of q
+    int n, assignments, topk, per_token, slots;  // slots: row i of q belongs to slot i of the plan; else to its token (per_token) or assignment
+    void * y;
+    int y_dtype;
+    long long ldy;
+};
+
+__device__ __forceinline__ void mma_i8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// weights are read once: past the L1
+__device__ __forceinline__ uint4 load_stream(const int8_t * p) {
+    uint4 r;
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(__cvta_generic_to_global(p)));
+    return r;
+}
+__device__ __forceinline__ int source_row(const I8Args & p, int slot, int a) {
+    return p.slots ? slot : !p.per_token ? a : a < p.assignments ? a / p.topk : a - p.assignments;
+}
+
+// A few tokens per expert: bound by streaming the weights. A block takes 16 weight rows of one expert (of both matrices with MATS = 2) and all the
+// expert's tokens, 8 NT at a time; its warps share the columns in pieces of 64, 16 bytes a lane and row, straight from memory into the fragments of the tensor
+// core: lane (g, t) holds bytes 16 t.. of rows g and g + 8, so word i of both operands stands for the same four columns, which is all that a sum over columns needs.
+template <int MATS, int NT>
+__global__ void __launch_bounds__(256) i8_stream_k(const I8Args p) {
+    extern __shared__ int red[];                                       // [warps][MATS][NT][16 rows][8 tokens]
+    constexpr int UNROLL = NT > 2 ? 2 : 4;
+    grid_wait();
+    grid_release();                                                    // after the wait: a down product behind this launch may read the plan above its own
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, g = lane >> 2, t = lane & 3;
+    int e = 0, count = p.n, first = 0;
+    const int * perm = nullptr;
+    if (p.plan) {
+        const int e1 = p.experts + 1;
+        if (int(blockIdx.y) >= p.plan[PLAN_NACTIVE]) return;
+        e = p.plan[PLAN_HDR + 2 * e1 + 1 + blockIdx.y];
+        count = p.plan[PLAN_HDR + e];
+        first = p.plan[PLAN_HDR + e1 + e];
+        perm = p.plan + PLAN_HDR + 3 * e1 + 1 + first;
+    }
+    const bool shared = p.plan && e == p.experts;
+    const int r0 = blockIdx.x * 16, rg = min(r0 + g, p.rows - 1), rh = min(r0 + g + 8, p.rows - 1);
+    const int8_t * wg[MATS], * wh[MATS];
+    const float * v[MATS];
+#pragma unroll
+    for (int m = 0; m < MATS; ++m) {
+        const int8_t * w = shared ? p.shared_w[m] : p.w[m] + size_t(e) * p.rows * p.cols;
+        wg[m] = w + size_t(rg) * p.cols + 16 * t;
+        wh[m] = w + size_t(rh) * p.cols + 16 * t;
+        v[m] = shared ? p.shared_v[m] : p.v[m] + size_t(e) * p.rows;
+    }
+    const int steps = (p.cols + 63) / 64;
+#pragma unroll 1
+    for (int j0 = 0; j0 < count; j0 += 8 * NT) {
+        const int8_t * b[NT];
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+            const int j = min(j0 + 8 * i + g, count - 1);
+            b[i] = p.q + size_t(p.plan ? source_row(p, first + j, perm[j]) : j) * p.ldq + 16 * t;
+        }
+        int acc[MATS][NT][4] = {};
+#pragma unroll 1
+        for (int s0 = warp; s0 < steps; s0 += UNROLL * warps) {
+            uint4 x[UNROLL][NT], ag[UNROLL][MATS], ah[UNROLL][MATS];
+#pragma unroll
+            for (int u = 0; u < UNROLL; ++u) {
+                const int k = 64 * (s0 + u * warps);
+                const bool in = k + 16 * t < p.cols;
+#pragma unroll
+                for (int m = 0; m < MATS; ++m) {
+                    ag[u][m] = in ? load_stream(wg[m] + k) : make_uint4(0, 0, 0, 0);
+                    ah[u][m] = in ? load_stream(wh[m] + k) : make_uint4(0, 0, 0, 0);
+                }
+#pragma unroll
+                for (int i = 0; i < NT; ++i) x[u][i] = in ? *reinterpret_cast<const uint4 *>(b[i] + k) : make_uint4(0, 0, 0, 0);
+            }
+#pragma unroll
+            for (int u = 0; u < UNROLL; ++u)
+#pragma unroll
+                for (int m = 0; m < MATS; ++m)
+#pragma unroll
+                    for (int i = 0; i < NT; ++i) {
+                        mma_i8(acc[m][i], ag[u][m].x, ah[u][m].x, ag[u][m].y, ah[u][m].y, x[u][i].x, x[u][i].y);
+                        mma_i8(acc[m][i], ag[u][m].z, ah[u][m].z, ag[u][m].w, ah[u][m].w, x[u][i].z, x[u][i].w);
+                    }
+        }
+        if (j0) __syncthreads();                                       // the sums of the tokens before have been read
+#pragma unroll
+        for (int m = 0; m < MATS; ++m)
+#pragma unroll
+            for (int i = 0; i < NT; ++i) {
+                int2 * d = reinterpret_cast<int2 *>(red + ((warp * MATS + m) * NT + i) * 128);
+                d[g * 4 + t] = make_int2(acc[m][i][0], acc[m][i][1]);
+                d[(g + 8) * 4 + t] = make_int2(acc[m][i][2], acc[m][i][3]);
+            }
+        __syncthreads();
+        for (int x = threadIdx.x; x < 128 * NT; x += blockDim.x) {
+            const int r = x & 15, jj = x >> 4, j = j0 + jj, row = r0 + r;
+            if (row >= p.rows || j >= count) continue;
+            int sum[MATS];
+#pragma unroll
+            for (int m = 0; m < MATS; ++m) {
+                sum[m] = 0;
+                for (int w = 0; w < warps; ++w) sum[m] += red[((w * MATS + m) * NT + (jj >> 3)) * 128 + r * 8 + (jj & 7)];
+            }
+            const int a = p.plan ? perm[j] : j;
+            const float s = p.s[p.plan ? source_row(p, first + j, a) : j];
+            float out = float(sum[0]) * (s * v[0][row]);
+            if (MATS == 2) {
+                const float u = float(sum[MATS - 1]) * (s * v[MATS - 1][row]);
+                out = out / (1.f + expf(-out)) * u;
+            }
+            store_act(p.y, p.y_dtype, size_t(a) * p.ldy + row, out);
+        }
+    }
+}
+
+template <int MATS, int NT>
+int32_t launch_stream(const I8Args & a, int groups, cudaStream_t s) {
+    // Warps that share a block's columns: eight where a launch has few blocks, else four
+    const int blocks = ceil_div(a.rows, 16), warps = (long long)blocks * groups < 148 * 4 ? 8 : 4;
+    launch_overlapped(i8_stream_k<MATS, NT>, dim3(blocks, groups), dim3(32 * warps), size_t(warps) * MATS * NT * 128 * sizeof(int), s, a);
+    return launch_status();
+}
+template <int MATS>
+int32_t i8_stream(const I8Args & a, int groups, long long tokens, cudaStream_t s) {
+    if (tokens <= 8LL * groups) return launch_stream<MATS, 1>(a, groups, s);
+    if (tokens <= 16LL * groups) return launch_stream<MATS, 2>(a, groups, s);
+    return launch_stream<MATS, 4>(a, groups, s);
+}
+int groups_of(int experts, int n, int topk, int shared_tokens) { return int(std::min((long long)n * topk, (long long)experts)) + (shared_tokens ? 1 : 0); }
+
+I8Args grouped(const b2moe_bank * a, const b2moe_bank * b, const b2moe_bank * sa, const b2moe_bank * sb, const int * plan, int n, int topk, int shared_tokens, void * y, int y_dtype) {
+    I8Args p{};
+    const b2moe_bank * m[2] = {a, b}, * sm[2] = {sa, sb};
+    for (int i = 0; i < 2; ++i) {
+        if (m[i]) { p.w[i] = static_cast<const int8_t *>(m[i]->data); p.v[i] = static_cast<const float *>(m[i]->aux); }
+        if (shared_tokens && sm[i]) { p.shared_w[i] = static_cast<const int8_t *>(sm[i]->data); p.shared_v[i] = static_cast<const float *>(sm[i]->aux); }
+    }
+    p.experts = a->experts; p.rows = a->rows; p.cols = a->cols;
+    p.plan = plan; p.n = n; p.assignments = n * topk; p.topk = topk;
+    p.y = y; p.y_dtype = y_dtype; p.ldy = a->rows;
+    return p;
+}
+
+}  // namespace
+
+size_t i8_workspace_bytes(int rows_x, int k) { return i8_rows_bytes(rows_x, k); }
+
+// x [n][cols]; the workspace holds the rows of the n tokens
+int32_t i8_gateup(const b2moe_bank * gate, const b2moe_bank * up, const b2moe_bank * shared_gate, const b2moe_bank * shared_up, const void * x, int x_dtype, const int * plan, int n,
+                  int topk, int shared_tokens, long long live, void * act, int act_dtype, void * ws, void * rows_buf, size_t rows_buf_bytes, cudaStream_t s) {
+    I8Args p = grouped(gate, up, shared_gate, shared_up, plan, n, topk, shared_tokens, act, act_dtype);
+    const I8Rows rows = i8_rows(ws, n);
+    if (int32_t rc = i8_quantize(x, x_dtype, gate->cols, n, gate->cols, rows.q, gate->cols, rows.scale, nullptr, 0, 0, 1, false, s)) return rc;
+    p.q = rows.q; p.ldq = gate->cols; p.s = rows.scale; p.per_token = 1;
+    return i8_stream<2>(p, groups_of(gate->experts, n, topk, shared_tokens), live + shared_tokens, s);
+}
+// x [assignments][cols] (per_token: [n][cols]); the workspace holds a row per assignment, in slot order
+int32_t i8_down(const b2moe_bank * down, const b2moe_bank * shared_down, const void * x, int x_dtype, bool per_token, const int * plan, int n, int topk, int shared_tokens, long long live,
+                void * y, int y_dtype, void * ws, cudaStream_t s) {
+    I8Args p = grouped(down, nullptr, shared_down, nullptr, plan, n, topk, shared_tokens, y, y_dtype);
+    const int total = n * topk + shared_tokens;
+    const I8Rows rows = i8_rows(ws, total);
+    if (int32_t rc = i8_quantize(x, x_dtype, down->cols, total, down->cols, rows.q, down->cols, rows.scale, plan, down->experts, n * topk, topk, per_token, s)) return rc;
+    p.q = rows.q; p.ldq = down->cols; p.s = rows.scale; p.slots = 1;
+    return i8_stream<1>(p, groups_of(down->experts, n, topk, shared_tokens), live + shared_tokens, s);
+}
+
+namespace {
+__global__ void i8_dump_k(const int8_t * w, const float * v, int rows, int cols, float * out) {
+    const size_t row = blockIdx.x;
+    for (int j = threadIdx.x; j < cols; j += blockDim.x) out[row * cols + j] = float(w[row * cols + j]) * v[row];
+}
+}  // namespace
+int32_t i8_dump(const b2moe_bank & b, float * out, cudaStream_t s) {
+    const long long rows = (long long)b.experts * b.rows;
+    if (rows > 0x7fffffffLL) return B2MOE_ERR_SHAPE;
+    i8_dump_k<<<unsigned(rows), 128, 0, s>>>(static_cast<const int8_t *>(b.data), static_cast<const float *>(b.aux), b.rows, b.cols, out);
+    return launch_status();
+}
+
+}  // namespace b2
+
+using namespace b2;
+
+extern "C" B2MOE_API int32_t b2moe_linear_i8(const int8_t * q, int64_t ldq, const float * scale, const b2moe_bank * w, int32_t n, void * y, int32_t y_dtype, int64_t ldy, int32_t * status,
+                                             b2moe_stream stream) {
+    if (int32_t rc = check_bank(w)) return rc;
+    if (w->type != B2MOE_I8) return B2MOE_ERR_FORMAT;
+    if (n <= 0 || w->experts != 1 || !valid_dtype(y_dtype) || ldq < w->cols || ldq % 16 || ldy < w->rows) return B2MOE_ERR_SHAPE;
+    if (!q || !scale || !y) return B2MOE_ERR_NULL;
+    if (!aligned16(q)) return B2MOE_ERR_ALIGN;
+    I8Args p{};
+    p.w[0] = static_cast<const int8_t *>(w->data); p.v[0] = static_cast<const float *>(w->aux);
+    p.experts = 1; p.rows = w->rows; p.cols = w->cols;
+    p.q = q; p.ldq = ldq; p.s = scale; p.n = n;
+    p.y = y; p.y_dtype = y_dtype; p.ldy = ldy;
+    return i8_stream<1>(p, 1, n, as_stream(stream));
+}

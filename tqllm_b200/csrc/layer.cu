@@ -5,6 +5,7 @@
 
 #include "common.cuh"
 #include "formats.cuh"
+#include "int8.cuh"
 
 namespace b2 {
 int32_t check_bank(const b2moe_bank * b);
@@ -51,6 +52,10 @@ size_t gemm_exact_bytes(int slot_rows, int k, int dtype);
 int32_t gemm_exact_gateup(const b2moe_bank *, const b2moe_bank *, const b2moe_bank *, const b2moe_bank *, const void *, int, const int *, int, int, int, void *, int act_dtype,
                           void * rows, bool slots, cudaStream_t);
 int32_t gemm_exact_down(const b2moe_bank *, const b2moe_bank *, const void *, int, bool per_token, const int *, int, int, int, void *, int y_dtype, void * rows, bool plan_ready, cudaStream_t);
+size_t i8_workspace_bytes(int rows_x, int k);
+int32_t i8_gateup(const b2moe_bank *, const b2moe_bank *, const b2moe_bank *, const b2moe_bank *, const void *, int, const int *, int, int, int, long long live, void *, int act_dtype,
+                  void * ws, void * rows_buf, size_t rows_buf_bytes, cudaStream_t);
+int32_t i8_down(const b2moe_bank *, const b2moe_bank *, const void *, int, bool per_token, const int *, int, int, int, long long live, void *, int y_dtype, void * ws, cudaStream_t);
 
 namespace {
 int32_t same_shape(const b2moe_bank * a, const b2moe_bank * b, bool same_experts) {
@@ -118,6 +123,7 @@ int32_t product_typed(const b2moe_bank * m, const void * x, int x_dtype, bool pe
                       void * ws, void * rows_buf, size_t rows_buf_bytes, cudaStream_t s, bool * took) {
     const int path = expert_path(m->type, m->cols, B2MOE_F32, m->experts, (long long)n * topk);
     *took = true;
+    if (m->type == B2MOE_I8) return i8_down(m, nullptr, x, x_dtype, per_token, plan, n, topk, 0, (long long)n * topk, y, y_dtype, ws, s);
     if (exact_path(m->type, m->cols, x_dtype, m->experts, (long long)n * topk) && rows_buf_bytes >= gemm_exact_bytes(n * topk, m->cols, x_dtype))
         return gemm_exact_down(m, nullptr, x, x_dtype, per_token, plan, n, topk, 0, y, y_dtype, rows_buf, false, s);
     if (path == B2MOE_FAMILY_GEMM) return gemm_tc_down(m, nullptr, x, x_dtype, per_token, plan, n, topk, 0, (long long)n * topk, y, y_dtype, ws, false, s);
@@ -131,6 +137,8 @@ int32_t gateup_typed(const b2moe_bank * gate, const b2moe_bank * up, const void 
                      void * ws, void * rows_buf, size_t rows_buf_bytes, cudaStream_t s, bool * took) {
     const int path = expert_path(gate->type, gate->cols, x_dtype, gate->experts, (long long)n * topk);
     *took = true;
+    if (gate->type == B2MOE_I8)
+        return i8_gateup(gate, up, nullptr, nullptr, x, x_dtype, plan, n, topk, 0, (long long)n * topk, act, act_dtype, ws, rows_buf, rows_buf_bytes, s);
     if (exact_path(gate->type, gate->cols, x_dtype, gate->experts, (long long)n * topk)) {
         if (rows_buf_bytes >= gemm_exact_bytes(n * topk, gate->cols, x_dtype))
             return gemm_exact_gateup(gate, up, nullptr, nullptr, x, x_dtype, plan, n, topk, 0, act, act_dtype, rows_buf, true, s);
@@ -146,7 +154,7 @@ int32_t gateup_typed(const b2moe_bank * gate, const b2moe_bank * up, const void 
 }
 // true when b2moe_expert_down would take the format-generic kernels (which use no scratch) for this call
 bool expert_down_is_generic(const b2moe_bank * down, int n, int topk) {
-    return expert_path(down->type, down->cols, B2MOE_F32, down->experts, (long long)n * topk) == B2MOE_FAMILY_GENERIC;
+    return down->type != B2MOE_I8 && expert_path(down->type, down->cols, B2MOE_F32, down->experts, (long long)n * topk) == B2MOE_FAMILY_GENERIC;
 }
 }  // namespace b2
 
@@ -185,6 +193,7 @@ extern "C" B2MOE_API uint64_t b2moe_harness_launches(void) { return g_launch_cou
 
 extern "C" B2MOE_API size_t b2moe_expert_workspace_bytes(uint32_t type, int32_t rows_x, int32_t k, int32_t x_dtype) {
     if (rows_x <= 0 || k <= 0 || !valid_dtype(x_dtype)) return 0;
+    if (type == B2MOE_I8) return i8_cols(k) ? i8_workspace_bytes(rows_x, k) : 0;
     FmtInfo f;
     if (!fmt_info(type, f)) return 0;
     // the largest of what the families that can serve this type would take (the family is chosen per call)
@@ -195,7 +204,7 @@ extern "C" B2MOE_API size_t b2moe_expert_workspace_bytes(uint32_t type, int32_t 
 }
 extern "C" B2MOE_API size_t b2moe_expert_slot_workspace_bytes(const b2moe_bank * bank, int32_t slot_rows, int32_t x_dtype) {
     const size_t base = bank ? b2moe_expert_workspace_bytes(bank->type, slot_rows, bank->cols, x_dtype) : 0;
-    if (!base) return 0;
+    if (!base || bank->type == B2MOE_I8) return base;
     const bool exact = dec4_supported(bank->type, bank->cols) && gemm_exact_supported(bank->type, bank->cols, bank->experts);
     return std::max({base, gemm_tc_slot_bytes(slot_rows, bank->cols), exact ? gemm_exact_bytes(slot_rows, bank->cols, x_dtype) : size_t(0)});
 }
@@ -225,13 +234,15 @@ static int32_t expert_gateup(const b2moe_bank * gate, const b2moe_bank * up, con
     if (int32_t rc = check_gateup(gate, up, shared_gate, shared_up, x, x_dtype, plan, n, topk, shared_tokens, act)) return rc;
     if (live < 0) live = (long long)n * topk;
     const int path = expert_path(gate->type, gate->cols, x_dtype, gate->experts, live);
-    if (path != B2MOE_FAMILY_GENERIC) {
+    const bool i8 = gate->type == B2MOE_I8;
+    if (path != B2MOE_FAMILY_GENERIC || i8) {
         const size_t need = b2moe_expert_workspace_bytes(gate->type, n, gate->cols, x_dtype);
         if (need && !workspace) return B2MOE_ERR_NULL;
         if (need && !aligned16(workspace)) return B2MOE_ERR_ALIGN;
         if (workspace_bytes < need) return B2MOE_ERR_WORKSPACE;
         void * const spare = rows_buf ? rows_buf : workspace;
         const size_t spare_bytes = rows_buf ? rows_buf_bytes : workspace_bytes;
+        if (i8) return i8_gateup(gate, up, shared_gate, shared_up, x, x_dtype, plan, n, topk, shared_tokens, live, act, B2MOE_F32, workspace, spare, spare_bytes, as_stream(stream));
         bool slots;
         if (exact_gateup(gate, x_dtype, live, n * topk + shared_tokens, spare_bytes, &slots))
             return gemm_exact_gateup(gate, up, shared_gate, shared_up, x, x_dtype, plan, n, topk, shared_tokens, act, B2MOE_F32, slots ? spare : workspace, slots, as_stream(stream));
@@ -269,11 +280,13 @@ static int32_t expert_down(const b2moe_bank * down, const b2moe_bank * shared_do
     if (!aligned16(act) || !aligned16(y)) return B2MOE_ERR_ALIGN;
     if (live < 0) live = (long long)n * topk;
     const int path = expert_path(down->type, down->cols, B2MOE_F32, down->experts, live);
-    if (path != B2MOE_FAMILY_GENERIC) {
+    const bool i8 = down->type == B2MOE_I8;
+    if (path != B2MOE_FAMILY_GENERIC || i8) {
         const int rows_x = n * topk + shared_tokens;
         if (!workspace) return B2MOE_ERR_NULL;
         if (!aligned16(workspace)) return B2MOE_ERR_ALIGN;
         if (workspace_bytes < b2moe_expert_workspace_bytes(down->type, rows_x, down->cols, B2MOE_F32)) return B2MOE_ERR_WORKSPACE;
+        if (i8) return i8_down(down, shared_down, act, B2MOE_F32, false, plan, n, topk, shared_tokens, live, y, B2MOE_F32, workspace, as_stream(stream));
         if (exact_path(down->type, down->cols, B2MOE_F32, down->experts, live) && workspace_bytes >= gemm_exact_bytes(rows_x, down->cols, B2MOE_F32))
             return gemm_exact_down(down, shared_down, act, B2MOE_F32, false, plan, n, topk, shared_tokens, y, B2MOE_F32, workspace, plan_ready, as_stream(stream));
         if (path == B2MOE_FAMILY_GEMM)

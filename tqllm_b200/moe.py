@@ -7,6 +7,7 @@ dispatch plan (counts, offsets, permutation), the layer forward.
 from __future__ import annotations
 
 import ctypes as C
+from typing import NamedTuple
 
 import torch
 
@@ -50,6 +51,28 @@ class DeviceBank:
         self.aux = None if aux is None else torch.as_tensor(aux).to(device)
         self.c = capi.Bank(self.data.data_ptr(), _ptr(self.aux), type_id, experts, rows, cols)
         return self
+
+    @classmethod
+    def from_int8(cls, data: torch.Tensor, scale: torch.Tensor, experts: int = 1):
+        """A bank of 8-bit rows over the caller's arrays, which it keeps and does not copy: data int8 [experts * rows, cols] (or
+        [experts, rows, cols]), scale float32 with one value a row."""
+        rows, cols = data.shape[-2] if data.dim() == 3 else data.shape[0] // experts, data.shape[-1]
+        experts = data.shape[0] if data.dim() == 3 else experts
+        if data.dtype != torch.int8 or scale.dtype != torch.float32 or not data.is_contiguous() or not scale.is_contiguous():
+            raise capi.B2moeError(capi.ERR_FORMAT, "DeviceBank.from_int8: contiguous int8 rows and float32 scales are wanted")
+        if data.numel() != experts * rows * cols or scale.numel() != experts * rows or data.device != scale.device:
+            raise capi.B2moeError(capi.ERR_SHAPE, "DeviceBank.from_int8: a scale for each row is wanted, on the same device")
+        self = cls.__new__(cls)
+        self.type, self.experts, self.rows, self.cols = capi.I8, experts, rows, cols
+        self.data, self.aux = data, scale
+        self.c = capi.Bank(data.data_ptr(), scale.data_ptr(), capi.I8, experts, rows, cols)
+        return self
+
+    @classmethod
+    def from_float(cls, w: torch.Tensor):
+        """floating-point weights [experts, rows, cols] (or [rows, cols]) quantised to a bank of 8-bit rows (b2moe_quantize_rows)"""
+        q, scale = quantize_rows(w.reshape(-1, w.shape[-1]))
+        return cls.from_int8(q.view(w.shape), scale.view(w.shape[:-1]), 1)
 
     def dequant(self) -> torch.Tensor:
         out = torch.empty(self.experts * self.rows, self.cols, dtype=torch.float32, device=self.data.device)
@@ -98,6 +121,81 @@ def route_sigmoid(logits, experts, k, bias=None, norm=True, scale=0.0):
     check(lib.b2moe_route_sigmoid(logits.data_ptr(), ld, _ptr(bias), ids.data_ptr(), w.data_ptr(), experts, k, int(norm), scale, n,
                                   _stream()), "b2moe_route_sigmoid")
     return ids, w
+
+
+def quantize_rows(x: torch.Tensor):
+    """(q int8 [n, k], scale float32 [n]) of the rows of x (b2moe_quantize_rows); x may be rows of a wider matrix"""
+    n, k = x.shape
+    if x.stride(1) != 1 and k > 1:
+        raise capi.B2moeError(capi.ERR_SHAPE, "quantize_rows: the values of a row have to be neighbours")
+    q = torch.empty(n, k, dtype=torch.int8, device=x.device)
+    scale = torch.empty(n, dtype=torch.float32, device=x.device)
+    check(lib.b2moe_quantize_rows(x.data_ptr(), _DT[x.dtype], x.stride(0) if n > 1 else k, n, k, q.data_ptr(), k, scale.data_ptr(), _stream()), "b2moe_quantize_rows")
+    return q, scale
+
+
+def linear_i8(q: torch.Tensor, scale: torch.Tensor, bank: DeviceBank, out_dtype=torch.bfloat16, out: torch.Tensor | None = None, status: torch.Tensor | None = None):
+    """y [n, rows] = (q . w) * scale[t] * bank scale[r] of 8-bit rows (b2moe_linear_i8); q and out may be rows of wider matrices"""
+    n, k = q.shape
+    if out is None:
+        out = torch.empty(n, bank.rows, dtype=out_dtype, device=q.device)
+    if q.dtype != torch.int8 or k != bank.cols or scale.dtype != torch.float32 or scale.numel() != n or not scale.is_contiguous() or out.shape != (n, bank.rows):
+        raise capi.B2moeError(capi.ERR_SHAPE, "linear_i8: int8 rows of the bank's columns, a float32 scale for each, and an output [n, rows] are wanted")
+    if (q.stride(1) != 1 and k > 1) or (out.stride(1) != 1 and bank.rows > 1):
+        raise capi.B2moeError(capi.ERR_SHAPE, "linear_i8: the values of a row have to be neighbours")
+    check(lib.b2moe_linear_i8(q.data_ptr(), q.stride(0) if n > 1 else k, scale.data_ptr(), C.byref(bank.c), n, out.data_ptr(), _DT[out.dtype],
+                              out.stride(0) if n > 1 else bank.rows, _ptr(status), _stream()), "b2moe_linear_i8")
+    return out
+
+
+class Balance(NamedTuple):
+    """what b2moe_balance_loss writes: loss (a scalar), counts and prob [sequences, experts], tokens [sequences + 1]"""
+    loss: torch.Tensor
+    counts: torch.Tensor
+    prob: torch.Tensor
+    tokens: torch.Tensor
+
+
+def _balance_args(logits, mask, offsets):
+    n = logits.shape[0]
+    if logits.dtype != torch.float32 or logits.stride(1) != 1:
+        raise capi.B2moeError(capi.ERR_SHAPE, "balance loss: float32 logits whose rows are contiguous are wanted")
+    if mask is not None and (mask.numel() != n or mask.dtype not in (torch.bool, torch.uint8) or not mask.is_contiguous()):
+        raise capi.B2moeError(capi.ERR_SHAPE, "balance loss: the mask has a byte for each token")
+    if offsets is not None and (offsets.dtype != torch.int32 or offsets.numel() < 2 or not offsets.is_contiguous()):
+        raise capi.B2moeError(capi.ERR_SHAPE, "balance loss: the offsets are int32, one more than sequences")
+    return n, logits.stride(0) if n > 1 else logits.shape[1], 1 if offsets is None else offsets.numel() - 1
+
+
+def balance_loss(logits, ids, experts, coef, gating=capi.SOFTMAX, mask=None, offsets=None) -> Balance:
+    """The router's balance loss over logits [n, >= experts] and the ids [n, topk] that were routed (b2moe_balance_loss)."""
+    n, ld, seqs = _balance_args(logits, mask, offsets)
+    if ids.shape[0] != n or ids.dtype != torch.int32 or not ids.is_contiguous():
+        raise capi.B2moeError(capi.ERR_SHAPE, "balance loss: contiguous int32 ids [n, topk] are wanted")
+    dev = logits.device
+    out = Balance(torch.empty((), dtype=torch.float32, device=dev), torch.empty(seqs, experts, dtype=torch.int32, device=dev),
+                  torch.empty(seqs, experts, dtype=torch.float32, device=dev), torch.empty(seqs + 1, dtype=torch.int32, device=dev))
+    ws = torch.empty(max(16, lib.b2moe_balance_workspace_bytes(experts, n, seqs)), dtype=torch.uint8, device=dev)
+    check(lib.b2moe_balance_loss(gating, logits.data_ptr(), ld, ids.data_ptr(), ids.shape[1], _ptr(mask), _ptr(offsets), seqs, experts, n, coef, out.loss.data_ptr(),
+                                 out.counts.data_ptr(), out.prob.data_ptr(), out.tokens.data_ptr(), ws.data_ptr(), ws.numel(), _stream()), "b2moe_balance_loss")
+    return out
+
+
+def balance_loss_backward(logits, saved: Balance, topk, coef, gating=capi.SOFTMAX, mask=None, offsets=None, grad_loss=None, out=None):
+    """The gradient of the balance loss on the logits, [n, experts]; into `out` (rows of at least `experts` columns) it is added."""
+    n, ld, seqs = _balance_args(logits, mask, offsets)
+    experts = saved.counts.shape[1]
+    if saved.counts.shape[0] != seqs or (grad_loss is not None and grad_loss.dtype != torch.float32):
+        raise capi.B2moeError(capi.ERR_SHAPE, "balance loss: the counts of the same sequences and a float32 gradient are wanted")
+    grad = out
+    if grad is None:
+        grad = torch.empty(n, experts, dtype=torch.float32, device=logits.device)
+    if grad.dtype != torch.float32 or grad.shape[0] != n or grad.shape[1] < experts or grad.stride(1) != 1:
+        raise capi.B2moeError(capi.ERR_SHAPE, "balance loss: the gradient has float32 rows like the logits")
+    check(lib.b2moe_balance_loss_backward(gating, logits.data_ptr(), ld, topk, _ptr(mask), _ptr(offsets), seqs, experts, n, coef, saved.counts.data_ptr(),
+                                          saved.tokens.data_ptr(), _ptr(grad_loss), grad.data_ptr(), grad.stride(0) if n > 1 else grad.shape[1], int(out is not None),
+                                          _stream()), "b2moe_balance_loss_backward")
+    return grad
 
 
 def count_ids(ids: torch.Tensor, counts: torch.Tensor) -> torch.Tensor:
@@ -168,9 +266,11 @@ def _bref(b: DeviceBank | None):
     return C.byref(b.c) if b is not None else None
 
 
-def expert_gateup_swiglu(gate, up, x, plan: Plan, sh_gate=None, sh_up=None):
+def expert_gateup_swiglu(gate, up, x, plan: Plan, sh_gate=None, sh_up=None, act: torch.Tensor | None = None):
+    """act [assignments, ff]; a buffer that is given keeps the rows of skipped assignments, without one they are zeros"""
     total = plan.n * plan.topk + plan.shared_tokens
-    act = torch.zeros(total, gate.rows, dtype=torch.float32, device=x.device)
+    act = torch.zeros(total, gate.rows, dtype=torch.float32, device=x.device) if act is None else act
+    assert act.dtype == torch.float32 and act.shape == (total, gate.rows) and act.is_contiguous()
     # room for a row per assignment: the grouped GEMM reads the rows of an expert as boxes then and does not gather them
     ws = _scratch(lib.b2moe_expert_slot_workspace_bytes(_bref(gate), total, _DT[x.dtype]), x.device)
     check(lib.b2moe_expert_gateup_swiglu(_bref(gate), _bref(up), _bref(sh_gate), _bref(sh_up), x.data_ptr(), _DT[x.dtype],
@@ -179,8 +279,10 @@ def expert_gateup_swiglu(gate, up, x, plan: Plan, sh_gate=None, sh_up=None):
     return act
 
 
-def expert_down(down, act, plan: Plan, sh_down=None):
-    y = torch.zeros(act.shape[0], down.rows, dtype=torch.float32, device=act.device)
+def expert_down(down, act, plan: Plan, sh_down=None, y: torch.Tensor | None = None):
+    """y [assignments, hidden]; a buffer that is given keeps the rows of skipped assignments, without one they are zeros"""
+    y = torch.zeros(act.shape[0], down.rows, dtype=torch.float32, device=act.device) if y is None else y
+    assert y.dtype == torch.float32 and y.shape == (act.shape[0], down.rows) and y.is_contiguous()
     ws = _scratch(lib.b2moe_expert_slot_workspace_bytes(_bref(down), act.shape[0], capi.F32), act.device)
     check(lib.b2moe_expert_down(_bref(down), _bref(sh_down), act.data_ptr(), plan.buf.data_ptr(), plan.n, plan.topk,
                                 plan.shared_tokens, y.data_ptr(), _ptr(ws), 0 if ws is None else ws.numel(), _stream()),
@@ -255,6 +357,17 @@ class MoeLayer:
         mk = lambda b, n: DeviceBank.from_packed(b[0], b[3], b[4], n, b[1], b[2], device)
         self.gate, self.up, self.down = (mk(b, E) for b in banks)
         self.sh = tuple(mk(b, 1) for b in shared) if shared else None
+        self._finish()
+        return self
+
+    @classmethod
+    def from_banks(cls, shape, router_w, banks, shared_banks=None, sel_bias=None, shared_gate_vec=None):
+        """A layer over finished banks (DeviceBank: gate, up, down, of any types, 8-bit ones among them) that it keeps; shape.types is not looked at"""
+        self = cls.__new__(cls)
+        self.shape, self.experts, self.device = shape, banks[0].experts, router_w.device
+        self.router_w, self.sel_bias, self.shared_gate_vec = router_w, sel_bias, shared_gate_vec
+        self.gate, self.up, self.down = banks
+        self.sh = tuple(shared_banks) if shared_banks is not None else None
         self._finish()
         return self
 
