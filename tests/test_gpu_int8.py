@@ -98,7 +98,14 @@ def linear_case(n, m, k, seed):
 
 @pytest.mark.parametrize("n", (1, 2, 8, 9, 17, 33, 64, 100, 129, 300, 515))
 @pytest.mark.parametrize("m,k", ((1, 16), (15, 48), (16, 64), (17, 80), (100, 1024), (257, 1040), (1411, 2560)))
-def test_linear(n, m, k):
+@pytest.mark.parametrize("family", ("auto", "gemm", "decode"))
+def test_linear(n, m, k, family):
+    from tqllm_b200 import capi
+    with capi.family(family):
+        linear(n, m, k)
+
+
+def linear(n, m, k):
     from tqllm_b200 import moe
     q, s, w, v = linear_case(n, m, k, n * 7 + m)
     bank = moe.DeviceBank.from_int8(w.cuda(), v.cuda())
@@ -207,7 +214,14 @@ SHAPES = [  # n, e, k, h, f, shared, route
 @pytest.mark.parametrize("n,e,k,h,f,shared,route", SHAPES)
 @pytest.mark.parametrize("dtype", (torch.bfloat16, torch.float16, torch.float32))
 @pytest.mark.parametrize("room", ("rows", "slots"))
-def test_expert_products(n, e, k, h, f, shared, route, dtype, room):
+@pytest.mark.parametrize("family", ("auto", "gemm", "decode"))
+def test_expert_products(n, e, k, h, f, shared, route, dtype, room, family):
+    from tqllm_b200 import capi
+    with capi.family(family):
+        expert_products(n, e, k, h, f, shared, route, dtype, room)
+
+
+def expert_products(n, e, k, h, f, shared, route, dtype, room):
     import ctypes as C
 
     from tqllm_b200 import capi, moe

@@ -17,9 +17,33 @@ inline I8Rows i8_rows(void * ws, int rows) {
     return {reinterpret_cast<int8_t *>(ws) + align_up(size_t(rows) * sizeof(float), 256), static_cast<float *>(ws)};
 }
 
+// One product, or gate and up together
+struct I8Args {
+    const int8_t * w[2], * shared_w[2];          // gate and up, or one matrix: [experts][rows][cols]
+    const float * v[2], * shared_v[2];           // their scales, [experts][rows]
+    int experts, rows, cols;
+    const int8_t * q;                            // rows in operand form
+    long long ldq;
+    const float * s;
+    const int * plan;                            // null: one matrix, rows 0..n of q
+    int n, assignments, topk, per_token, slots;  // slots: row i of q belongs to slot i of the plan; else to its token (per_token) or assignment
+    void * y;
+    int y_dtype;
+    long long ldy;
+};
+
+__device__ __forceinline__ int source_row(const I8Args & p, int slot, int a) {
+    return p.slots ? slot : !p.per_token ? a : a < p.assignments ? a / p.topk : a - p.assignments;
+}
+
 // rows x[0..n) of ldx elements -> q (stride ldq), scale. plan: the rows of the grouped assignments in slot order instead (slot i holds assignment
 // perm[i], whose row is its token's with per_token and its own otherwise), at most n of them
 int32_t i8_quantize(const void * x, int x_dtype, long long ldx, int n, int k, int8_t * q, long long ldq, float * scale, const int * plan, int experts,
                     int assignments, int topk, bool per_token, cudaStream_t s);
+
+// the tensor-core form for many rows (int8_gemm.cu): true when it takes banks of this many experts; status: where a wait that runs out is noted (may be null);
+// per_group: expected rows per expert. Rows of grouped calls lie in slot order
+bool i8_gemm_supported(int experts);
+template <int MATS> int32_t i8_gemm(const I8Args & a, long long q_rows, int per_group, int * status, cudaStream_t s);
 
 }  // namespace b2

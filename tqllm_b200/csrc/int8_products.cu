@@ -11,21 +11,8 @@
 
 namespace b2 {
 int32_t check_bank(const b2moe_bank * b);
+int harness_family();
 namespace {
-
-struct I8Args {
-    const int8_t * w[2], * shared_w[2];          // gate and up, or one matrix: [experts][rows][cols]
-    const float * v[2], * shared_v[2];           // their scales, [experts][rows]
-    int experts, rows, cols;
-    const int8_t * q;                            // rows in operand form
-    long long ldq;
-    const float * s;
-    const int * plan;                            // null: one matrix, rows 0..n of q
-    int n, assignments, topk, per_token, slots;  // slots: row i of q belongs to slot i of the plan; else to its token (per_token) or assignment
-    void * y;
-    int y_dtype;
-    long long ldy;
-};
 
 __device__ __forceinline__ void mma_i8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -37,10 +24,6 @@ __device__ __forceinline__ uint4 load_stream(const int8_t * p) {
     asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(__cvta_generic_to_global(p)));
     return r;
 }
-__device__ __forceinline__ int source_row(const I8Args & p, int slot, int a) {
-    return p.slots ? slot : !p.per_token ? a : a < p.assignments ? a / p.topk : a - p.assignments;
-}
-
 // A few tokens per expert: bound by streaming the weights. A block takes 16 weight rows of one expert (of both matrices with MATS = 2) and all the
 // expert's tokens, 8 NT at a time; its warps share the columns in pieces of 64, 16 bytes a lane and row, straight from memory into the fragments of the tensor
 // core: lane (g, t) holds bytes 16 t.. of rows g and g + 8, so word i of both operands stands for the same four columns, which is all that a sum over columns needs.
@@ -170,10 +153,26 @@ I8Args grouped(const b2moe_bank * a, const b2moe_bank * b, const b2moe_bank * sa
 
 size_t i8_workspace_bytes(int rows_x, int k) { return i8_rows_bytes(rows_x, k); }
 
+// The form of a product: the tensor-core GEMM from I8_GEMM_MIN_PER rows per expert on, else the streaming kernel
+constexpr int I8_GEMM_MIN_PER = 9;
+bool i8_takes_gemm(int experts, long long rows) {
+    const int family = harness_family();
+    if (!i8_gemm_supported(experts) || family == B2MOE_FAMILY_GENERIC || family == B2MOE_FAMILY_DECODE || family == B2MOE_FAMILY_DECODE_KERNELS) return false;
+    return family == B2MOE_FAMILY_GEMM || rows >= (long long)I8_GEMM_MIN_PER * experts;
+}
+int per_group(int experts, long long rows) { return int(std::min<long long>(1 << 20, (rows + experts - 1) / experts)); }
+
 // x [n][cols]; the workspace holds the rows of the n tokens
 int32_t i8_gateup(const b2moe_bank * gate, const b2moe_bank * up, const b2moe_bank * shared_gate, const b2moe_bank * shared_up, const void * x, int x_dtype, const int * plan, int n,
                   int topk, int shared_tokens, long long live, void * act, int act_dtype, void * ws, void * rows_buf, size_t rows_buf_bytes, cudaStream_t s) {
     I8Args p = grouped(gate, up, shared_gate, shared_up, plan, n, topk, shared_tokens, act, act_dtype);
+    const int total = n * topk + shared_tokens;
+    if (i8_takes_gemm(gate->experts, live) && rows_buf_bytes >= i8_rows_bytes(total, gate->cols)) {
+        const I8Rows rows = i8_rows(rows_buf, total);
+        if (int32_t rc = i8_quantize(x, x_dtype, gate->cols, total, gate->cols, rows.q, gate->cols, rows.scale, plan, gate->experts, n * topk, topk, true, s)) return rc;
+        p.q = rows.q; p.ldq = gate->cols; p.s = rows.scale; p.slots = 1;
+        return i8_gemm<2>(p, total, per_group(gate->experts, live), const_cast<int *>(plan) + PLAN_STATUS, s);
+    }
     const I8Rows rows = i8_rows(ws, n);
     if (int32_t rc = i8_quantize(x, x_dtype, gate->cols, n, gate->cols, rows.q, gate->cols, rows.scale, nullptr, 0, 0, 1, false, s)) return rc;
     p.q = rows.q; p.ldq = gate->cols; p.s = rows.scale; p.per_token = 1;
@@ -187,6 +186,7 @@ int32_t i8_down(const b2moe_bank * down, const b2moe_bank * shared_down, const v
     const I8Rows rows = i8_rows(ws, total);
     if (int32_t rc = i8_quantize(x, x_dtype, down->cols, total, down->cols, rows.q, down->cols, rows.scale, plan, down->experts, n * topk, topk, per_token, s)) return rc;
     p.q = rows.q; p.ldq = down->cols; p.s = rows.scale; p.slots = 1;
+    if (i8_takes_gemm(down->experts, live)) return i8_gemm<1>(p, total, per_group(down->experts, live), const_cast<int *>(plan) + PLAN_STATUS, s);
     return i8_stream<1>(p, groups_of(down->experts, n, topk, shared_tokens), live + shared_tokens, s);
 }
 
@@ -219,5 +219,6 @@ extern "C" B2MOE_API int32_t b2moe_linear_i8(const int8_t * q, int64_t ldq, cons
     p.experts = 1; p.rows = w->rows; p.cols = w->cols;
     p.q = q; p.ldq = ldq; p.s = scale; p.n = n;
     p.y = y; p.y_dtype = y_dtype; p.ldy = ldy;
+    if (i8_takes_gemm(1, n)) return i8_gemm<1>(p, n, n, status, as_stream(stream));
     return i8_stream<1>(p, 1, n, as_stream(stream));
 }

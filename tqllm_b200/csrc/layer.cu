@@ -152,6 +152,7 @@ int32_t gateup_typed(const b2moe_bank * gate, const b2moe_bank * up, const void 
     *took = false;
     return B2MOE_OK;
 }
+int harness_family() { return g_family; }
 // true when b2moe_expert_down would take the format-generic kernels (which use no scratch) for this call
 bool expert_down_is_generic(const b2moe_bank * down, int n, int topk) {
     return down->type != B2MOE_I8 && expert_path(down->type, down->cols, B2MOE_F32, down->experts, (long long)n * topk) == B2MOE_FAMILY_GENERIC;
