@@ -98,3 +98,27 @@ def test_chunk_numbers_of_sequences_never_meet(n):
         off = [0, *cuts, n]
         taken = [off[s] // chunk + s + j for s in range(seqs) for j in range(-(-(off[s + 1] - off[s]) // chunk))]
         assert len(set(taken)) == len(taken) and max(taken) < n // chunk + seqs
+
+
+@pytest.mark.parametrize("bits", (8, 11))
+def test_roundings_of_16_bit_rows(bits):
+    """every pair of mantissas of bf16 (8 bits) and fp16 (11): the nearest integer to x * inv, inv = 127 / top rounded up, is the nearest to the quotient
+    with halves to the even side, except where 127 divides the mantissa of top and inv is rounded"""
+    import numpy as np
+    lo, hi = 1 << (bits - 1), 1 << bits
+    left = 0
+    for top in range(lo, hi):
+        inv = np.float32(127.0 / top)
+        if float(inv) * top < 127.0:                                   # whole numbers of 35 bits: exact
+            inv = np.nextafter(inv, np.float32(np.inf))
+        if top % 127 == 0 and float(inv) * top != 127.0:
+            left += 1
+            continue
+        for e in range(0, -11, -1):
+            x = np.arange(lo, hi) * 2.0 ** e
+            x = x[x <= top]
+            m = np.floor(127.0 * x / top)
+            a, h = 127.0 * x, (m + 0.5) * top
+            want = np.where(a > h, m + 1, np.where(a < h, m, m + m % 2))
+            assert np.array_equal(np.rint(x * float(inv)), want), (top, e)
+    assert left == (0 if bits == 8 else 7)

@@ -36,10 +36,12 @@ __device__ __forceinline__ int source_row(const I8Args & p, int slot, int a) {
     return p.slots ? slot : !p.per_token ? a : a < p.assignments ? a / p.topk : a - p.assignments;
 }
 
-// rows x[0..n) of ldx elements -> q (stride ldq), scale. plan: the rows of the grouped assignments in slot order instead (slot i holds assignment
-// perm[i], whose row is its token's with per_token and its own otherwise), at most n of them
-int32_t i8_quantize(const void * x, int x_dtype, long long ldx, int n, int k, int8_t * q, long long ldq, float * scale, const int * plan, int experts,
-                    int assignments, int topk, bool per_token, cudaStream_t s);
+// rows x[0..n) of ldx elements -> q (stride ldq), scale
+int32_t i8_quantize(const void * x, int x_dtype, long long ldx, int n, int k, int8_t * q, long long ldq, float * scale, cudaStream_t s);
+// the rows of the grouped assignments in slot order: slot i holds assignment perm[i], whose row is its token's (per_token) or its own
+int32_t i8_quantize_slots(const void * x, int x_dtype, bool per_token, int n, int k, const I8Rows & rows, const int * plan, int experts, int topk, int shared_tokens, cudaStream_t s);
+// the same for rows of tokens, each quantised once and written to all its slots; inverse: scratch, a word per assignment
+int32_t i8_quantize_scatter(const void * x, int x_dtype, int n, int k, const I8Rows & rows, int * inverse, const int * plan, int experts, int topk, int shared_tokens, cudaStream_t s);
 
 // the tensor-core form for many rows (int8_gemm.cu): true when it takes banks of this many experts; status: where a wait that runs out is noted (may be null);
 // per_group: expected rows per expert. Rows of grouped calls lie in slot order

@@ -24,7 +24,7 @@ constexpr int TC_A_BYTES = 128 * 128, TC_SMEM = 227 * 1024;
 
 struct TcMaps { CUtensorMap a[2], shared[2], b; };
 struct TcArgs {
-    int nt, stages, row_blocks, tiles;          // activation rows of an item; ring; blocks of weight rows; items of a dense call in the row direction
+    int nt, box, stages, row_blocks, tiles;     // activation rows of an item, of a copy; ring; blocks of weight rows; items of a dense call in the row direction
     uint32_t tmem_cols;
     int * status;
 };
@@ -39,16 +39,17 @@ __device__ __forceinline__ void epi_sync() { asm volatile("bar.sync 1, %0;" ::"n
 
 struct TcItem { int e, first, count, rb; };      // expert, first row (slot), rows, block of weight rows
 
-// the item's outputs from tensor memory; t: (output row, scale) of its activation rows
+// this lane's weight row of an item
+template <int MATS>
+__device__ __forceinline__ int weight_row(const TcItem & im, int quarter, int lane) {
+    return MATS == 2 ? im.rb * 64 + 16 * quarter + (lane & 15) : im.rb * 128 + 32 * quarter + lane;
+}
+// the item's outputs from tensor memory; t: (output row, scale) of its activation rows, v: the scales of the lane's weight row
 template <int MATS, class T>
-__device__ __forceinline__ void store_item(const I8Args & p, const TcItem & im, uint32_t taddr, const int2 * t, int quarter, int half, int lane) {
-    constexpr int ROWS = MATS == 2 ? 64 : 128;
+__device__ __forceinline__ void store_item(const I8Args & p, const TcItem & im, uint32_t taddr, const int2 * t, const float (&v)[MATS], int quarter, int half, int lane) {
     const bool upper = MATS == 2 && lane >= 16;
-    const int row = im.rb * ROWS + (MATS == 2 ? 16 * quarter + (lane & 15) : 32 * quarter + lane);
-    const bool in = row < p.rows, shared = p.plan && im.e == p.experts;
-    float v[MATS];
-#pragma unroll
-    for (int m = 0; m < MATS; ++m) v[m] = in ? (shared ? p.shared_v[m] : p.v[m] + size_t(im.e) * p.rows)[row] : 0.f;
+    const int row = weight_row<MATS>(im, quarter, lane);
+    const bool in = row < p.rows;
     T * const y = static_cast<T *>(p.y) + row;
     auto put = [&](int at, float f) {
         T * d = y + size_t(uint32_t(at)) * p.ldy;
@@ -90,7 +91,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) i8_gemm_k(const I8Args p, const
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const uint32_t stage_bytes = TC_A_BYTES + c.nt * 128;
     uint8_t * const ring = tc_mem + (1024u - (saddr(tc_mem) & 1023u)) % 1024u;
-    int * const ends = reinterpret_cast<int *>(ring + size_t(c.stages) * stage_bytes);      // tiles up to and with expert e
+    const int e1 = p.experts + 1;
+    int * const ends = reinterpret_cast<int *>(ring + size_t(c.stages) * stage_bytes), * const offs = ends + e1;      // tiles up to and with expert e, its first slot
     const uint32_t full = saddr(bars), empty = full + 8 * TC_MAX_STAGES, acc_full = empty + 8 * TC_MAX_STAGES, acc_empty = acc_full + 16, drain = acc_empty + 16;
     if (threadIdx.x == 0) {
         for (int i = 0; i < c.stages; ++i) { bar_init(full + 8 * i, 1); bar_init(empty + 8 * i, 1); }
@@ -108,7 +110,6 @@ __global__ void __launch_bounds__(TC_THREADS, 1) i8_gemm_k(const I8Args p, const
     const uint32_t tmem = tmem_slot;
     grid_wait();
     grid_release();                                                    // after the wait: a down product behind this launch may read the plan above its own
-    const int e1 = p.experts + 1;
     const int * counts = p.plan + PLAN_HDR, * offsets = counts + e1, * perm = offsets + e1 + 1 + e1;
     int tiles = c.tiles;
     if (p.plan) {
@@ -129,7 +130,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1) i8_gemm_k(const I8Args p, const
         for (int e = lo; e < hi; ++e) {
             run += (counts[e] + c.nt - 1) / c.nt;
             ends[e] = run;
+            offs[e] = offsets[e];
         }
+        if (threadIdx.x == 0) offs[e1] = offsets[e1];
         __syncthreads();
         tiles = ends[e1 - 1];
     }
@@ -151,8 +154,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) i8_gemm_k(const I8Args p, const
             }
             im.e = lo;
             t = tile - (lo ? ends[lo - 1] : 0);
-            im.first = offsets[lo];
-            im.count = counts[lo];
+            im.first = offs[lo];
+            im.count = offs[lo + 1] - offs[lo];
         }
         im.first += t * c.nt;
         im.count = min(c.nt, im.count - t * c.nt);
@@ -173,13 +176,13 @@ __global__ void __launch_bounds__(TC_THREADS, 1) i8_gemm_k(const I8Args p, const
             const TcItem im = locate(it);
             const bool shared = p.plan && im.e == p.experts;
             const CUtensorMap * a = shared ? maps.shared : maps.a;
-            const int e = shared ? 0 : im.e;
+            const int e = shared ? 0 : im.e, boxes = (im.count + c.box - 1) / c.box;
 #pragma unroll 1
             for (int k = 0; k < steps; ++k) {
                 if (issued >= uint32_t(c.stages) && !warp_wait(empty + 8 * slot, phase)) { ok = false; break; }
                 if (lead) {
                     const uint32_t bar = full + 8 * slot, dst = saddr(ring) + slot * stage_bytes;
-                    bar_expect_tx(bar, stage_bytes);
+                    bar_expect_tx(bar, TC_A_BYTES + uint32_t(boxes * c.box) * 128);
                     if (MATS == 2) {
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
@@ -189,7 +192,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) i8_gemm_k(const I8Args p, const
                     } else {
                         tma_load_3d(dst, a, 128 * k, 128 * im.rb, e, bar);
                     }
-                    tma_load_2d(dst + TC_A_BYTES, &maps.b, 128 * k, im.first, bar);
+                    for (int i = 0; i < boxes; ++i) tma_load_2d(dst + TC_A_BYTES + i * c.box * 128, &maps.b, 128 * k, im.first + i * c.box, bar);
                 }
                 __syncwarp();
                 ++issued;
@@ -203,12 +206,12 @@ __global__ void __launch_bounds__(TC_THREADS, 1) i8_gemm_k(const I8Args p, const
     } else if (warp == 1) {
         // ---- products: the whole warp walks the loop, one lane issues ----
         const bool lead = elect_one();
-        const uint32_t id = idesc_i8(128, c.nt), a0 = sw128_desc_lo(saddr(ring)), step = stage_bytes >> 4;
+        const uint32_t a0 = sw128_desc_lo(saddr(ring)), step = stage_bytes >> 4;
         uint32_t slot = 0, phase = 0, done = 0;
         bool ok = true;
 #pragma unroll 1
         for (int it = blockIdx.x; it < items && ok && !abort_flag; it += gridDim.x, ++done) {
-            const uint32_t h = done & 1u, d = tmem + h * c.nt;
+            const uint32_t h = done & 1u, d = tmem + h * c.nt, id = idesc_i8(128, uint32_t(__shfl_sync(0xffffffffu, locate(it).count, 0) + 15) & ~15u);
             if (done >= 2 && !warp_wait(acc_empty + 8 * h, ((done >> 1) - 1) & 1u)) { ok = false; break; }
             fence_after();
 #pragma unroll 1
@@ -230,24 +233,42 @@ __global__ void __launch_bounds__(TC_THREADS, 1) i8_gemm_k(const I8Args p, const
     } else if (warp >= TC_EPI_WARP0) {
         // ---- results: warp q of either half reads the lanes 32 (q mod 4) of tensor memory, the halves take 16 columns in turn ----
         const int tid = threadIdx.x - 32 * TC_EPI_WARP0, quarter = warp & 3, half = (warp - TC_EPI_WARP0) >> 2;
+        // what the stores of an item need to know (its rows' places and scales, the weight row's scales) is asked for an item ahead
+        int2 mine = make_int2(0, 0);
+        float v[MATS];
+        auto fetch = [&](const TcItem & im) {
+            if (tid < im.count) mine = make_int2(p.plan ? perm[im.first + tid] : im.first + tid, __float_as_int(p.s[im.first + tid]));
+            const int row = weight_row<MATS>(im, quarter, lane);
+#pragma unroll
+            for (int m = 0; m < MATS; ++m) v[m] = row < p.rows ? (p.plan && im.e == p.experts ? p.shared_v[m] : p.v[m] + size_t(im.e) * p.rows)[row] : 0.f;
+        };
         uint32_t done = 0;
         bool ok = true;
+        TcItem im{}, next{};
+        if (int(blockIdx.x) < items) {
+            next = locate(blockIdx.x);
+            fetch(next);
+        }
 #pragma unroll 1
         for (int it = blockIdx.x; it < items; it += gridDim.x, ++done) {
-            const TcItem im = locate(it);
             const uint32_t h = done & 1u;
-            if (tid < im.count) {
-                const int at = p.plan ? perm[im.first + tid] : im.first + tid;
-                table[h][tid] = make_int2(at, __float_as_int(p.s[im.first + tid]));
-            }
+            im = next;
+            if (tid < im.count) table[h][tid] = mine;
+            float scale[MATS];
+#pragma unroll
+            for (int m = 0; m < MATS; ++m) scale[m] = v[m];
             epi_sync();                                                // the table is there; the other one's item has been read by every warp
+            if (it + int(gridDim.x) < items) {
+                next = locate(it + gridDim.x);
+                fetch(next);
+            }
             ok = ok && !abort_flag && warp_wait(acc_full + 8 * h, (done >> 1) & 1u);
             fence_after();
             if (ok) {
                 const uint32_t taddr = tmem + h * c.nt + (uint32_t(32 * quarter) << 16);
-                if (p.y_dtype == B2MOE_F32) store_item<MATS, float>(p, im, taddr, table[h], quarter, half, lane);
-                else if (p.y_dtype == B2MOE_F16) store_item<MATS, __half>(p, im, taddr, table[h], quarter, half, lane);
-                else store_item<MATS, __nv_bfloat16>(p, im, taddr, table[h], quarter, half, lane);
+                if (p.y_dtype == B2MOE_F32) store_item<MATS, float>(p, im, taddr, table[h], scale, quarter, half, lane);
+                else if (p.y_dtype == B2MOE_F16) store_item<MATS, __half>(p, im, taddr, table[h], scale, quarter, half, lane);
+                else store_item<MATS, __nv_bfloat16>(p, im, taddr, table[h], scale, quarter, half, lane);
             } else if (lane == 0) {
                 give_up();
             }
@@ -263,9 +284,11 @@ __global__ void __launch_bounds__(TC_THREADS, 1) i8_gemm_k(const I8Args p, const
 }
 
 int sm_count() {
-    int dev = 0, n = 148;
-    if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
-    return n;
+    static const int count = [] {                                      // the library runs on one kind of GPU
+        int dev = 0, n = 0;
+        return cudaGetDevice(&dev) == cudaSuccess && cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess && n > 0 ? n : 148;
+    }();
+    return count;
 }
 bool map_rows(CUtensorMap & m, const int8_t * base, int cols, long long rows, long long stride, int experts, int box) {
     if (experts) {
@@ -285,18 +308,21 @@ bool i8_gemm_supported(int experts) { return experts <= TC_MAX_EXPERTS; }
 template <int MATS>
 int32_t i8_gemm(const I8Args & p, long long q_rows, int per_group, int * status, cudaStream_t s) {
     TcArgs c{};
-    c.nt = 16;
-    while (c.nt < 256 && c.nt < per_group) c.nt *= 2;
     c.row_blocks = ceil_div(p.rows, MATS == 2 ? 64 : 128);
+    // Items of 256 rows halve what the weights cost in copies and products (8192 x 4096 x 4096: 96 us, with 128 rows 153), items of 128 leave room for six ring
+    // stages instead of four and waste less where an expert has fewer (512 experts at 80 each, gate/up 211 against 225 us; 128 experts at 16 each 242 and 263, at 128 each with a
+    // skewed load 385 and 333); below that nothing is gained (64 rows, 16 each: 248). A dense call takes the large ones where they fill the SMs
+    c.nt = per_group > 96 && (p.plan || (long long)ceil_div(p.n, 256) * c.row_blocks >= sm_count()) ? 256 : 128;
+    c.box = 64;                                                        // rows of a copy: an item takes as many copies as it has rows for
     c.tiles = p.plan ? 0 : ceil_div(p.n, c.nt);
     c.tmem_cols = std::max(32, 2 * c.nt);
     c.status = status;
-    const size_t table = p.plan ? size_t(p.experts + 1) * sizeof(int) : 0, fixed = 8 * 1024;      // static arrays and the alignment of the ring
+    const size_t table = p.plan ? size_t(2 * (p.experts + 1) + 1) * sizeof(int) : 0, fixed = 8 * 1024;      // static arrays and the alignment of the ring
     c.stages = int(std::min<size_t>(TC_MAX_STAGES, (TC_SMEM - fixed - table) / (TC_A_BYTES + size_t(c.nt) * 128)));
     TcMaps maps;
     std::memset(&maps, 0, sizeof(maps));
     const int box = MATS == 2 ? 16 : 128;
-    bool ok = map_rows(maps.b, p.q, p.cols, q_rows, p.ldq, 0, c.nt);
+    bool ok = map_rows(maps.b, p.q, p.cols, q_rows, p.ldq, 0, c.box);
     for (int m = 0; m < MATS; ++m) {
         ok = ok && map_rows(maps.a[m], p.w[m], p.cols, p.rows, p.cols, p.experts, box);
         if (p.shared_w[m]) ok = ok && map_rows(maps.shared[m], p.shared_w[m], p.cols, p.rows, p.cols, 1, box);

@@ -152,6 +152,8 @@ I8Args grouped(const b2moe_bank * a, const b2moe_bank * b, const b2moe_bank * sa
 }  // namespace
 
 size_t i8_workspace_bytes(int rows_x, int k) { return i8_rows_bytes(rows_x, k); }
+// rows in slot order, and the slot of every assignment
+size_t i8_slot_bytes(int slot_rows, int k) { return i8_rows_bytes(slot_rows, k) + align_up(size_t(slot_rows) * sizeof(int), 256); }
 
 // The form of a product: the tensor-core GEMM from I8_GEMM_MIN_PER rows per expert on, else the streaming kernel
 constexpr int I8_GEMM_MIN_PER = 9;
@@ -167,14 +169,15 @@ int32_t i8_gateup(const b2moe_bank * gate, const b2moe_bank * up, const b2moe_ba
                   int topk, int shared_tokens, long long live, void * act, int act_dtype, void * ws, void * rows_buf, size_t rows_buf_bytes, cudaStream_t s) {
     I8Args p = grouped(gate, up, shared_gate, shared_up, plan, n, topk, shared_tokens, act, act_dtype);
     const int total = n * topk + shared_tokens;
-    if (i8_takes_gemm(gate->experts, live) && rows_buf_bytes >= i8_rows_bytes(total, gate->cols)) {
+    if (i8_takes_gemm(gate->experts, live) && rows_buf_bytes >= i8_slot_bytes(total, gate->cols)) {
         const I8Rows rows = i8_rows(rows_buf, total);
-        if (int32_t rc = i8_quantize(x, x_dtype, gate->cols, total, gate->cols, rows.q, gate->cols, rows.scale, plan, gate->experts, n * topk, topk, true, s)) return rc;
+        int * inverse = reinterpret_cast<int *>(static_cast<char *>(rows_buf) + i8_rows_bytes(total, gate->cols));
+        if (int32_t rc = i8_quantize_scatter(x, x_dtype, n, gate->cols, rows, inverse, plan, gate->experts, topk, shared_tokens, s)) return rc;
         p.q = rows.q; p.ldq = gate->cols; p.s = rows.scale; p.slots = 1;
         return i8_gemm<2>(p, total, per_group(gate->experts, live), const_cast<int *>(plan) + PLAN_STATUS, s);
     }
     const I8Rows rows = i8_rows(ws, n);
-    if (int32_t rc = i8_quantize(x, x_dtype, gate->cols, n, gate->cols, rows.q, gate->cols, rows.scale, nullptr, 0, 0, 1, false, s)) return rc;
+    if (int32_t rc = i8_quantize(x, x_dtype, gate->cols, n, gate->cols, rows.q, gate->cols, rows.scale, s)) return rc;
     p.q = rows.q; p.ldq = gate->cols; p.s = rows.scale; p.per_token = 1;
     return i8_stream<2>(p, groups_of(gate->experts, n, topk, shared_tokens), live + shared_tokens, s);
 }
@@ -184,7 +187,7 @@ int32_t i8_down(const b2moe_bank * down, const b2moe_bank * shared_down, const v
     I8Args p = grouped(down, nullptr, shared_down, nullptr, plan, n, topk, shared_tokens, y, y_dtype);
     const int total = n * topk + shared_tokens;
     const I8Rows rows = i8_rows(ws, total);
-    if (int32_t rc = i8_quantize(x, x_dtype, down->cols, total, down->cols, rows.q, down->cols, rows.scale, plan, down->experts, n * topk, topk, per_token, s)) return rc;
+    if (int32_t rc = i8_quantize_slots(x, x_dtype, per_token, n, down->cols, rows, plan, down->experts, topk, shared_tokens, s)) return rc;
     p.q = rows.q; p.ldq = down->cols; p.s = rows.scale; p.slots = 1;
     if (i8_takes_gemm(down->experts, live)) return i8_gemm<1>(p, total, per_group(down->experts, live), const_cast<int *>(plan) + PLAN_STATUS, s);
     return i8_stream<1>(p, groups_of(down->experts, n, topk, shared_tokens), live + shared_tokens, s);

@@ -53,6 +53,7 @@ int32_t gemm_exact_gateup(const b2moe_bank *, const b2moe_bank *, const b2moe_ba
                           void * rows, bool slots, cudaStream_t);
 int32_t gemm_exact_down(const b2moe_bank *, const b2moe_bank *, const void *, int, bool per_token, const int *, int, int, int, void *, int y_dtype, void * rows, bool plan_ready, cudaStream_t);
 size_t i8_workspace_bytes(int rows_x, int k);
+size_t i8_slot_bytes(int slot_rows, int k);
 int32_t i8_gateup(const b2moe_bank *, const b2moe_bank *, const b2moe_bank *, const b2moe_bank *, const void *, int, const int *, int, int, int, long long live, void *, int act_dtype,
                   void * ws, void * rows_buf, size_t rows_buf_bytes, cudaStream_t);
 int32_t i8_down(const b2moe_bank *, const b2moe_bank *, const void *, int, bool per_token, const int *, int, int, int, long long live, void *, int y_dtype, void * ws, cudaStream_t);
@@ -205,7 +206,8 @@ extern "C" B2MOE_API size_t b2moe_expert_workspace_bytes(uint32_t type, int32_t 
 }
 extern "C" B2MOE_API size_t b2moe_expert_slot_workspace_bytes(const b2moe_bank * bank, int32_t slot_rows, int32_t x_dtype) {
     const size_t base = bank ? b2moe_expert_workspace_bytes(bank->type, slot_rows, bank->cols, x_dtype) : 0;
-    if (!base || bank->type == B2MOE_I8) return base;
+    if (base && bank->type == B2MOE_I8) return i8_slot_bytes(slot_rows, bank->cols);
+    if (!base) return 0;
     const bool exact = dec4_supported(bank->type, bank->cols) && gemm_exact_supported(bank->type, bank->cols, bank->experts);
     return std::max({base, gemm_tc_slot_bytes(slot_rows, bank->cols), exact ? gemm_exact_bytes(slot_rows, bank->cols, x_dtype) : size_t(0)});
 }

@@ -18,7 +18,8 @@ _DT = {torch.float32: capi.F32, torch.float16: capi.F16, torch.bfloat16: capi.BF
 
 
 def _stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    """handle of the current device's current stream (torch.cuda.current_stream().cuda_stream makes a Stream object for it: 3.3 us a call)"""
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 def _ptr(t: torch.Tensor | None) -> int | None:
