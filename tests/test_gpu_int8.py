@@ -117,8 +117,15 @@ def linear(n, m, k):
     assert int(status) == 0
 
 
-@pytest.mark.parametrize("n,m,k", ((1, 4096, 4096), (64, 4096, 4096), (1000, 520, 4096), (2100, 1408, 1408)))
-def test_linear_of_real_sizes(n, m, k):
+@pytest.mark.parametrize("n,m,k", ((1, 4096, 4096), (64, 4096, 4096), (200, 4096, 4096), (256, 130, 8192), (17, 70, 16400), (1000, 520, 4096), (2100, 1408, 1408)))
+@pytest.mark.parametrize("family", ("auto", "gemm"))
+def test_linear_of_real_sizes(n, m, k, family):
+    from tqllm_b200 import capi
+    with capi.family(family):
+        linear_of_real_sizes(n, m, k)
+
+
+def linear_of_real_sizes(n, m, k):
     from tqllm_b200 import moe
     q, s, w, v = linear_case(n, m, k, 3)
     y = moe.linear_i8(q.cuda(), s.cuda(), moe.DeviceBank.from_int8(w.cuda(), v.cuda()), out_dtype=torch.float32)

@@ -7,8 +7,10 @@
 //
 // One block per SM walks the items (tile of activation rows, block of weight rows): one thread issues the copies into a ring, one the products, eight warps
 // empty one accumulator while the next one fills.
+#include <cooperative_groups.h>
 #include <cuda.h>
 
+#include <array>
 #include <cstring>
 
 #include "int8.cuh"
@@ -20,7 +22,7 @@ namespace {
 using namespace tc;
 
 constexpr int TC_THREADS = 384, TC_EPI_WARP0 = 4, TC_EPI_WARPS = 8, TC_EPI_THREADS = 32 * TC_EPI_WARPS, TC_MAX_STAGES = 12, TC_MAX_EXPERTS = 4096;
-constexpr int TC_A_BYTES = 128 * 128, TC_SMEM = 227 * 1024;
+constexpr int TC_A_BYTES = 128 * 128, TC_SMEM = 227 * 1024, TC_MAX_SPLIT = 8;
 
 struct TcMaps { CUtensorMap a[2], shared[2], b; };
 struct TcArgs {
@@ -80,7 +82,9 @@ __device__ __forceinline__ void store_item(const I8Args & p, const TcItem & im, 
     }
 }
 
-template <int MATS>
+// SPLIT (dense calls with few items): the blocks of a cluster take parts of an item's columns each, and then a share of its activation rows each, whose parts they
+// read from one another's shared memory: whole numbers, so the sum is the same
+template <int MATS, bool SPLIT>
 __global__ void __launch_bounds__(TC_THREADS, 1) i8_gemm_k(const I8Args p, const TcArgs c, const __grid_constant__ TcMaps maps) {
     extern __shared__ __align__(1024) uint8_t tc_mem[];
     __shared__ __align__(16) int2 table[2][256];
@@ -136,7 +140,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) i8_gemm_k(const I8Args p, const
         __syncthreads();
         tiles = ends[e1 - 1];
     }
-    const int items = tiles * c.row_blocks, steps = (p.cols + 127) / 128;
+    const int items = tiles * c.row_blocks, all_steps = (p.cols + 127) / 128;
+    const int k0 = SPLIT ? all_steps * int(blockIdx.z) / int(gridDim.z) : 0, k1 = SPLIT ? all_steps * (int(blockIdx.z) + 1) / int(gridDim.z) : all_steps;
     auto locate = [&](int it) {
         TcItem im;
         const int tile = it / c.row_blocks;
@@ -178,7 +183,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) i8_gemm_k(const I8Args p, const
             const CUtensorMap * a = shared ? maps.shared : maps.a;
             const int e = shared ? 0 : im.e, boxes = (im.count + c.box - 1) / c.box;
 #pragma unroll 1
-            for (int k = 0; k < steps; ++k) {
+            for (int k = k0; k < k1; ++k) {
                 if (issued >= uint32_t(c.stages) && !warp_wait(empty + 8 * slot, phase)) { ok = false; break; }
                 if (lead) {
                     const uint32_t bar = full + 8 * slot, dst = saddr(ring) + slot * stage_bytes;
@@ -215,12 +220,12 @@ __global__ void __launch_bounds__(TC_THREADS, 1) i8_gemm_k(const I8Args p, const
             if (done >= 2 && !warp_wait(acc_empty + 8 * h, ((done >> 1) - 1) & 1u)) { ok = false; break; }
             fence_after();
 #pragma unroll 1
-            for (int k = 0; k < steps; ++k) {
+            for (int k = k0; k < k1; ++k) {
                 if (!warp_wait(full + 8 * slot, phase)) { ok = false; break; }
                 fence_after();
                 const uint32_t a = a0 + slot * step, b = a + (TC_A_BYTES >> 4);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) mma_i8(lead, d, a + 2 * i, b + 2 * i, id, k > 0 || i > 0);
+                for (int i = 0; i < 4; ++i) mma_i8(lead, d, a + 2 * i, b + 2 * i, id, k > k0 || i > 0);
                 mma_commit(lead, empty + 8 * slot);
                 if (++slot == uint32_t(c.stages)) { slot = 0; phase ^= 1u; }
             }
@@ -230,7 +235,24 @@ __global__ void __launch_bounds__(TC_THREADS, 1) i8_gemm_k(const I8Args p, const
         // nothing may be in flight when the tensor memory is freed
         mma_commit(lead, drain);
         warp_wait(drain, 0);
-    } else if (warp >= TC_EPI_WARP0) {
+    } else if (SPLIT && warp >= TC_EPI_WARP0) {
+        // ---- this block's part: from tensor memory to the ring, which nothing uses any more, 128 weight rows for each activation row ----
+        const int quarter = warp & 3, half = (warp - TC_EPI_WARP0) >> 2;
+        const TcItem im = locate(blockIdx.x);
+        if (warp_wait(acc_full, 0)) {
+            fence_after();
+#pragma unroll 1
+            for (int col = 16 * half; col < im.count; col += 32) {
+                uint32_t d[16];
+                tmem_ld16(tmem + (uint32_t(32 * quarter) << 16) + col, d);
+                tmem_ld_wait();
+#pragma unroll
+                for (int j = 0; j < 16; ++j) reinterpret_cast<uint32_t *>(ring)[(col + j) * 128 + 32 * quarter + lane] = d[j];
+            }
+        } else if (lane == 0) {
+            give_up();
+        }
+    } else if (!SPLIT && warp >= TC_EPI_WARP0) {
         // ---- results: warp q of either half reads the lanes 32 (q mod 4) of tensor memory, the halves take 16 columns in turn ----
         const int tid = threadIdx.x - 32 * TC_EPI_WARP0, quarter = warp & 3, half = (warp - TC_EPI_WARP0) >> 2;
         // what the stores of an item need to know (its rows' places and scales, the weight row's scales) is asked for an item ahead
@@ -281,6 +303,41 @@ __global__ void __launch_bounds__(TC_THREADS, 1) i8_gemm_k(const I8Args p, const
     __syncthreads();
     fence_after();
     if (warp == 1) tmem_free(tmem, c.tmem_cols);
+    if constexpr (SPLIT) {
+        namespace cg = cooperative_groups;
+        cg::cluster_group cluster = cg::this_cluster();
+        const TcItem im = locate(blockIdx.x);
+        const int parts = gridDim.z, lo = im.count * int(blockIdx.z) / parts, hi = im.count * (int(blockIdx.z) + 1) / parts, r = threadIdx.x & 127, row = 128 * im.rb + r;
+        const bool in = row < p.rows;
+        const float v = in ? p.v[0][row] : 0.f;
+        uint32_t place[TC_MAX_SPLIT];
+#pragma unroll
+        for (int z = 0; z < TC_MAX_SPLIT; ++z) asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(place[z]) : "r"(saddr(ring) + 4 * r), "r"(z < parts ? z : 0));
+        cluster.sync();
+        // four activation rows of a thread at a time: a read of another block's memory takes several hundred cycles
+        constexpr int STEP = TC_THREADS / 128;
+        for (int col = lo + (threadIdx.x >> 7); col < hi && in; col += 4 * STEP) {
+            int part[4][TC_MAX_SPLIT];
+            float s[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int at = min(col + i * STEP, hi - 1);
+                s[i] = p.s[im.first + at];
+#pragma unroll
+                for (int z = 0; z < TC_MAX_SPLIT; ++z)
+                    if (z < parts) asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(part[i][z]) : "r"(place[z] + uint32_t(at) * 512u) : "memory");
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                int sum = 0;
+#pragma unroll
+                for (int z = 0; z < TC_MAX_SPLIT; ++z)
+                    if (z < parts) sum += part[i][z];
+                if (col + i * STEP < hi) store_act(p.y, p.y_dtype, size_t(im.first + col + i * STEP) * p.ldy + row, float(sum) * (s[i] * v));
+            }
+        }
+        cluster.sync();                                                // the parts stay until every block has read them
+    }
 }
 
 int sm_count() {
@@ -301,6 +358,36 @@ bool map_rows(CUtensorMap & m, const int8_t * base, int cols, long long rows, lo
     return encode_map(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, base, dims, strides, b, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
+// the most clusters of this many blocks that run at once (a cluster stays inside a GPC: 148 SMs hold fewer than 148 / 8 of eight)
+int clusters_at_once(int size) {
+    static const std::array<int, TC_MAX_SPLIT + 1> most = [] {
+        std::array<int, TC_MAX_SPLIT + 1> m{};
+        constexpr int smem = TC_SMEM - 8 * 1024;
+        if (cudaFuncSetAttribute(i8_gemm_k<1, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return m;
+        for (int size = 2; size <= TC_MAX_SPLIT; ++size) {
+            cudaLaunchConfig_t cfg{};
+            cfg.gridDim = dim3(1, 1, size); cfg.blockDim = dim3(TC_THREADS); cfg.dynamicSmemBytes = smem;
+            cudaLaunchAttribute at[1];
+            at[0].id = cudaLaunchAttributeClusterDimension;
+            at[0].val.clusterDim.x = 1; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = size;
+            cfg.attrs = at; cfg.numAttrs = 1;
+            if (cudaOccupancyMaxActiveClusters(&m[size], i8_gemm_k<1, true>, &cfg) != cudaSuccess) m[size] = 0;
+        }
+        cudaGetLastError();
+        return m;
+    }();
+    return most[size];
+}
+// Blocks that share an item's columns: as many as one round of clusters has room for, with four steps of 128 columns each at least, and none where an item has fewer
+// than 16: a step takes such a block 0.3 us, the meeting at the end 1.5 to 2 us and more with many rows. us, one block / this: 16 rows 4096 x 4096 11.2 / 7.9, 1411 x 2560 7.6 / 5.7, 2048 x 8192
+// 19.3 / 8.3, 8192 x 1024 4.9 / 6.4 with two; 128 rows 13.8 / 10.0, 10.1 / 7.5, 22.6 / 10.3, 7.1 / 9.9
+int split_of(long long items, int steps) {
+    int split = 1;
+    for (int s = 2; s <= TC_MAX_SPLIT; ++s)
+        if (steps >= 16 && s * 4 <= steps && items <= clusters_at_once(s)) split = s;
+    return split;
+}
+
 }  // namespace
 
 bool i8_gemm_supported(int experts) { return experts <= TC_MAX_EXPERTS; }
@@ -311,10 +398,13 @@ int32_t i8_gemm(const I8Args & p, long long q_rows, int per_group, int * status,
     c.row_blocks = ceil_div(p.rows, MATS == 2 ? 64 : 128);
     // Items of 256 rows halve what the weights cost in copies and products (8192 x 4096 x 4096: 96 us, with 128 rows 153), items of 128 leave room for six ring
     // stages instead of four and waste less where an expert has fewer (512 experts at 80 each, gate/up 211 against 225 us; 128 experts at 16 each 242 and 263, at 128 each with a
-    // skewed load 385 and 333); below that nothing is gained (64 rows, 16 each: 248). A dense call takes the large ones where they fill the SMs
-    c.nt = per_group > 96 && (p.plan || (long long)ceil_div(p.n, 256) * c.row_blocks >= sm_count()) ? 256 : 128;
+    // skewed load 385 and 333); below that nothing is gained (64 rows, 16 each: 248). A dense call takes the large ones where they fill the SMs (256 rows of 4096 x 4096: 17.5 us in items of 256, 14.0 of 128)
+    const int sms = sm_count();
+    c.nt = p.plan ? (per_group > 96 ? 256 : 128) : (long long)ceil_div(p.n, 256) * c.row_blocks >= sms ? 256 : 128;
     c.box = 64;                                                        // rows of a copy: an item takes as many copies as it has rows for
     c.tiles = p.plan ? 0 : ceil_div(p.n, c.nt);
+    // A dense call with few items: as many blocks an item as run at once
+    const int split = MATS == 1 && !p.plan ? split_of((long long)c.tiles * c.row_blocks, ceil_div(p.cols, 128)) : 1;
     c.tmem_cols = std::max(32, 2 * c.nt);
     c.status = status;
     const size_t table = p.plan ? size_t(2 * (p.experts + 1) + 1) * sizeof(int) : 0, fixed = 8 * 1024;      // static arrays and the alignment of the ring
@@ -330,9 +420,23 @@ int32_t i8_gemm(const I8Args & p, long long q_rows, int per_group, int * status,
     }
     if (!ok) return B2MOE_ERR_CUDA;
     const size_t smem = 1024 + size_t(c.stages) * (TC_A_BYTES + size_t(c.nt) * 128) + table;
-    if (cudaFuncSetAttribute(i8_gemm_k<MATS>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)) != cudaSuccess) return B2MOE_ERR_CUDA;
-    const long long most = p.plan ? (long long)sm_count() : (long long)c.tiles * c.row_blocks;
-    launch_overlapped(i8_gemm_k<MATS>, dim3(unsigned(std::min<long long>(sm_count(), most))), dim3(TC_THREADS), smem, s, p, c, maps);
+    const long long items = (long long)c.tiles * c.row_blocks;
+    if constexpr (MATS == 1)
+        if (split > 1) {
+            if (cudaFuncSetAttribute(i8_gemm_k<1, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)) != cudaSuccess) return B2MOE_ERR_CUDA;
+            cudaLaunchConfig_t cfg{};
+            cfg.gridDim = dim3(unsigned(items), 1, split); cfg.blockDim = dim3(TC_THREADS); cfg.dynamicSmemBytes = smem; cfg.stream = s;
+            cudaLaunchAttribute at[2];
+            at[0].id = cudaLaunchAttributeClusterDimension;
+            at[0].val.clusterDim.x = 1; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = split;
+            at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+            at[1].val.programmaticStreamSerializationAllowed = 1;
+            cfg.attrs = at; cfg.numAttrs = g_overlap ? 2 : 1;
+            if (cudaLaunchKernelEx(&cfg, i8_gemm_k<1, true>, p, c, maps) != cudaSuccess) return B2MOE_ERR_CUDA;
+            return launch_status();
+        }
+    if (cudaFuncSetAttribute(i8_gemm_k<MATS, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)) != cudaSuccess) return B2MOE_ERR_CUDA;
+    launch_overlapped(i8_gemm_k<MATS, false>, dim3(unsigned(p.plan ? sms : std::min<long long>(sms, items))), dim3(TC_THREADS), smem, s, p, c, maps);
     return launch_status();
 }
 template int32_t i8_gemm<1>(const I8Args &, long long, int, int *, cudaStream_t);

@@ -31,9 +31,12 @@ template <int MATS, int NT>
 __global__ void __launch_bounds__(256) i8_stream_k(const I8Args p) {
     extern __shared__ int red[];                                       // [warps][MATS][NT][16 rows][8 tokens]
     constexpr int UNROLL = NT > 2 ? 2 : 4;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, g = lane >> 2, t = lane & 3, r0 = blockIdx.x * 16;
+    // a dense call's weights are asked into the L2 while the launch in front of this one runs (they are not read before it is through): 4096 x 4096, one row 5.0 -> 4.6 us
+    if (!p.plan && threadIdx.x < 16 && r0 + int(threadIdx.x) < p.rows)
+        asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(__cvta_generic_to_global(p.w[0] + size_t(r0 + threadIdx.x) * p.cols)), "r"(uint32_t(p.cols)) : "memory");
     grid_wait();
     grid_release();                                                    // after the wait: a down product behind this launch may read the plan above its own
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, g = lane >> 2, t = lane & 3;
     int e = 0, count = p.n, first = 0;
     const int * perm = nullptr;
     if (p.plan) {
@@ -45,7 +48,7 @@ __global__ void __launch_bounds__(256) i8_stream_k(const I8Args p) {
         perm = p.plan + PLAN_HDR + 3 * e1 + 1 + first;
     }
     const bool shared = p.plan && e == p.experts;
-    const int r0 = blockIdx.x * 16, rg = min(r0 + g, p.rows - 1), rh = min(r0 + g + 8, p.rows - 1);
+    const int rg = min(r0 + g, p.rows - 1), rh = min(r0 + g + 8, p.rows - 1);
     const int8_t * wg[MATS], * wh[MATS];
     const float * v[MATS];
 #pragma unroll
@@ -130,6 +133,7 @@ int32_t launch_stream(const I8Args & a, int groups, cudaStream_t s) {
 }
 template <int MATS>
 int32_t i8_stream(const I8Args & a, int groups, long long tokens, cudaStream_t s) {
+    // rows that a pass over the weights serves: a second pass of some experts (from the L2) costs less than the registers of 16 rows (512 experts at five each: 184 and 222 us)
     if (tokens <= 8LL * groups) return launch_stream<MATS, 1>(a, groups, s);
     if (tokens <= 16LL * groups) return launch_stream<MATS, 2>(a, groups, s);
     return launch_stream<MATS, 4>(a, groups, s);
@@ -155,13 +159,18 @@ size_t i8_workspace_bytes(int rows_x, int k) { return i8_rows_bytes(rows_x, k); 
 // rows in slot order, and the slot of every assignment
 size_t i8_slot_bytes(int slot_rows, int k) { return i8_rows_bytes(slot_rows, k) + align_up(size_t(slot_rows) * sizeof(int), 256); }
 
-// The form of a product: the tensor-core GEMM from I8_GEMM_MIN_PER rows per expert on, else the streaming kernel
-constexpr int I8_GEMM_MIN_PER = 9;
-bool i8_takes_gemm(int experts, long long rows) {
+// The form of a product: the streaming kernel for a few rows, the tensor-core GEMM (int8_gemm.cu) for more. us, streamed / GEMM:
+//   dense, from 17 rows on: 4096 x 4096 16 rows 7.7 / 7.9, 24 10.3 / 8.0; 1411 x 2560 16 4.4 / 5.7, 32 6.7 / 5.9; 8192 x 1024 16 4.4 / 4.9, 32 5.7 / 5.1
+//   gate/up, from seven rows per expert on: 128 experts of 1408 x 4096 at 4 each 221 / 233, at 8 307 / 245; 512 of 512 x 2048 at 2.5 155 / 168, at 5 184 / 187; 32 of 512 x 1024 at 4 8.9 / 14.2, at 16
+//   17.1 / 15.3 (the GEMM's times have a launch more in them, since its rows lie in slot order)
+//   down, where they are in slot order anyway, also where the SMs get eight items each: 128 of 4096 x 1408 at 0.5 59 / 56, at 1 95 / 79, at 4 136 / 119; 512 of 2048 x 512 at 0.2 25 / 24, at 1.2 111 / 82
+constexpr int I8_DENSE_ROWS = 16, I8_GEMM_MIN_PER = 7, I8_MANY_ITEMS = 148 * 8;
+bool i8_takes_gemm(int experts, bool worth) {
     const int family = harness_family();
     if (!i8_gemm_supported(experts) || family == B2MOE_FAMILY_GENERIC || family == B2MOE_FAMILY_DECODE || family == B2MOE_FAMILY_DECODE_KERNELS) return false;
-    return family == B2MOE_FAMILY_GEMM || rows >= (long long)I8_GEMM_MIN_PER * experts;
+    return family == B2MOE_FAMILY_GEMM || worth;
 }
+bool dense_enough(int experts, long long rows) { return rows >= (long long)I8_GEMM_MIN_PER * experts; }
 int per_group(int experts, long long rows) { return int(std::min<long long>(1 << 20, (rows + experts - 1) / experts)); }
 
 // x [n][cols]; the workspace holds the rows of the n tokens
@@ -169,7 +178,7 @@ int32_t i8_gateup(const b2moe_bank * gate, const b2moe_bank * up, const b2moe_ba
                   int topk, int shared_tokens, long long live, void * act, int act_dtype, void * ws, void * rows_buf, size_t rows_buf_bytes, cudaStream_t s) {
     I8Args p = grouped(gate, up, shared_gate, shared_up, plan, n, topk, shared_tokens, act, act_dtype);
     const int total = n * topk + shared_tokens;
-    if (i8_takes_gemm(gate->experts, live) && rows_buf_bytes >= i8_slot_bytes(total, gate->cols)) {
+    if (i8_takes_gemm(gate->experts, dense_enough(gate->experts, live)) && rows_buf_bytes >= i8_slot_bytes(total, gate->cols)) {
         const I8Rows rows = i8_rows(rows_buf, total);
         int * inverse = reinterpret_cast<int *>(static_cast<char *>(rows_buf) + i8_rows_bytes(total, gate->cols));
         if (int32_t rc = i8_quantize_scatter(x, x_dtype, n, gate->cols, rows, inverse, plan, gate->experts, topk, shared_tokens, s)) return rc;
@@ -189,7 +198,8 @@ int32_t i8_down(const b2moe_bank * down, const b2moe_bank * shared_down, const v
     const I8Rows rows = i8_rows(ws, total);
     if (int32_t rc = i8_quantize_slots(x, x_dtype, per_token, n, down->cols, rows, plan, down->experts, topk, shared_tokens, s)) return rc;
     p.q = rows.q; p.ldq = down->cols; p.s = rows.scale; p.slots = 1;
-    if (i8_takes_gemm(down->experts, live)) return i8_gemm<1>(p, total, per_group(down->experts, live), const_cast<int *>(plan) + PLAN_STATUS, s);
+    const bool many = (long long)groups_of(down->experts, n, topk, shared_tokens) * ceil_div(down->rows, 128) >= I8_MANY_ITEMS;
+    if (i8_takes_gemm(down->experts, dense_enough(down->experts, live) || (many && live == (long long)n * topk))) return i8_gemm<1>(p, total, per_group(down->experts, live), const_cast<int *>(plan) + PLAN_STATUS, s);
     return i8_stream<1>(p, groups_of(down->experts, n, topk, shared_tokens), live + shared_tokens, s);
 }
 
@@ -222,6 +232,6 @@ extern "C" B2MOE_API int32_t b2moe_linear_i8(const int8_t * q, int64_t ldq, cons
     p.experts = 1; p.rows = w->rows; p.cols = w->cols;
     p.q = q; p.ldq = ldq; p.s = scale; p.n = n;
     p.y = y; p.y_dtype = y_dtype; p.ldy = ldy;
-    if (i8_takes_gemm(1, n)) return i8_gemm<1>(p, n, n, status, as_stream(stream));
+    if (i8_takes_gemm(1, n > I8_DENSE_ROWS)) return i8_gemm<1>(p, n, n, status, as_stream(stream));
     return i8_stream<1>(p, 1, n, as_stream(stream));
 }
