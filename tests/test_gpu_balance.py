@@ -118,6 +118,19 @@ def test_sequences_and_masks(gating, e):
     assert bool(torch.isfinite(g).all())
 
 
+@pytest.mark.parametrize("n", (1, 33, 64, 65))
+@pytest.mark.parametrize("e", (40, 600, 2048, 2049))
+@pytest.mark.parametrize("span", ((0, None), (1, None), (5, 30), (64, 64), (0, 0)))
+def test_one_sequence_of_a_few_tokens(n, e, span):
+    """with rows in front and behind, a mask, nothing at all"""
+    logits, ids, gen = make(n, e, 3, n + e)
+    a, z = min(span[0], n), n if span[1] is None else min(span[1], n)
+    offsets = torch.tensor([a, max(a, z)], dtype=torch.int32)
+    for mask in (None, torch.rand(n, generator=gen) < 0.6):
+        b, g = run(logits, ids, e, 0.1, 1, mask, offsets)
+        check(logits, ids, e, 0.1, 1, mask, offsets, b=b, grad=g)
+
+
 @pytest.mark.parametrize("e", (40, 600))
 def test_nothing_left(e):
     from tqllm_b200 import moe

@@ -173,12 +173,11 @@ def balance_loss(logits, ids, experts, coef, gating=capi.SOFTMAX, mask=None, off
     n, ld, seqs = _balance_args(logits, mask, offsets)
     if ids.shape[0] != n or ids.dtype != torch.int32 or not ids.is_contiguous():
         raise capi.B2moeError(capi.ERR_SHAPE, "balance loss: contiguous int32 ids [n, topk] are wanted")
-    dev = logits.device
-    out = Balance(torch.empty((), dtype=torch.float32, device=dev), torch.empty(seqs, experts, dtype=torch.int32, device=dev),
-                  torch.empty(seqs, experts, dtype=torch.float32, device=dev), torch.empty(seqs + 1, dtype=torch.int32, device=dev))
-    ws = torch.empty(max(16, lib.b2moe_balance_workspace_bytes(experts, n, seqs)), dtype=torch.uint8, device=dev)
+    new, ints = logits.new_empty, ids.new_empty
+    out = Balance(new(()), ints((seqs, experts)), new((seqs, experts)), ints(seqs + 1))
+    ws = new(max(4, lib.b2moe_balance_workspace_bytes(experts, n, seqs) // 4))
     check(lib.b2moe_balance_loss(gating, logits.data_ptr(), ld, ids.data_ptr(), ids.shape[1], _ptr(mask), _ptr(offsets), seqs, experts, n, coef, out.loss.data_ptr(),
-                                 out.counts.data_ptr(), out.prob.data_ptr(), out.tokens.data_ptr(), ws.data_ptr(), ws.numel(), _stream()), "b2moe_balance_loss")
+                                 out.counts.data_ptr(), out.prob.data_ptr(), out.tokens.data_ptr(), ws.data_ptr(), 4 * ws.numel(), _stream()), "b2moe_balance_loss")
     return out
 
 
@@ -190,7 +189,7 @@ def balance_loss_backward(logits, saved: Balance, topk, coef, gating=capi.SOFTMA
         raise capi.B2moeError(capi.ERR_SHAPE, "balance loss: the counts of the same sequences and a float32 gradient are wanted")
     grad = out
     if grad is None:
-        grad = torch.empty(n, experts, dtype=torch.float32, device=logits.device)
+        grad = logits.new_empty((n, experts))
     if grad.dtype != torch.float32 or grad.shape[0] != n or grad.shape[1] < experts or grad.stride(1) != 1:
         raise capi.B2moeError(capi.ERR_SHAPE, "balance loss: the gradient has float32 rows like the logits")
     check(lib.b2moe_balance_loss_backward(gating, logits.data_ptr(), ld, topk, _ptr(mask), _ptr(offsets), seqs, experts, n, coef, saved.counts.data_ptr(),
