@@ -117,7 +117,7 @@ def linear(n, m, k):
     assert int(status) == 0
 
 
-@pytest.mark.parametrize("n,m,k", ((1, 4096, 4096), (64, 4096, 4096), (200, 4096, 4096), (256, 130, 8192), (17, 70, 16400), (1000, 520, 4096), (2100, 1408, 1408)))
+@pytest.mark.parametrize("n,m,k", ((1, 4096, 4096), (64, 4096, 4096), (200, 4096, 4096), (256, 130, 8192), (17, 70, 16400), (1000, 520, 4096), (2100, 1408, 1408), (700, 6500, 2688), (3000, 1700, 4096)))
 @pytest.mark.parametrize("family", ("auto", "gemm"))
 def test_linear_of_real_sizes(n, m, k, family):
     from tqllm_b200 import capi
@@ -215,6 +215,7 @@ SHAPES = [  # n, e, k, h, f, shared, route
     (1, 8, 2, 64, 16, False, "even"), (3, 5, 5, 80, 48, True, "even"), (7, 16, 4, 256, 144, False, "skip"), (9, 4, 2, 48, 80, True, "skip"),
     (40, 3, 1, 128, 64, False, "one"), (17, 40, 6, 1040, 272, False, "even"), (130, 4, 2, 192, 208, True, "even"), (300, 6, 3, 144, 128, False, "skip"),
     (260, 2, 1, 128, 336, False, "one"), (5, 8, 2, 64, 32, False, "none"), (700, 8, 4, 512, 256, True, "even"), (1, 2, 1, 16, 16, False, "even"),
+    (60, 6, 2, 2576, 80, True, "even"), (600, 3, 2, 2688, 208, False, "skip"),
 ]
 
 
@@ -360,3 +361,42 @@ def test_streams_and_graphs():
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(out, moe.linear_i8(*moe.quantize_rows(x), bank))
+
+
+@pytest.mark.parametrize("n,m,k", ((40, 300, 2560), (300, 300, 256), (1100, 4096, 2688)))
+def test_a_wait_that_runs_out_is_reported(n, m, k):
+    """one step's copies are left out (harness hook): the launch ends, sets the status word, and the next one is clean; the launches share columns in a cluster, walk
+    alone and in pairs"""
+    from tqllm_b200 import capi, moe
+    q, s, w, v = linear_case(n, m, k, 6)
+    bank, status = moe.DeviceBank.from_int8(w.cuda(), v.cuda()), torch.zeros(1, dtype=torch.int32, device="cuda")
+    q, s = q.cuda(), s.cuda()
+    clean = moe.linear_i8(q, s, bank, status=status)
+    assert int(status) == 0
+    capi.lib.b2moe_harness_wait_probe(1, 0)
+    try:
+        moe.linear_i8(q, s, bank, status=status)
+        torch.cuda.synchronize()
+    finally:
+        capi.lib.b2moe_harness_wait_probe(-1, 0)
+    assert int(status) != 0
+    status.zero_()
+    assert torch.equal(moe.linear_i8(q, s, bank, status=status), clean) and int(status) == 0
+
+
+def test_a_wait_of_grouped_products_that_runs_out():
+    from tqllm_b200 import capi, moe
+    x, ids, banks, _ = experts_case(200, 4, 2, 256, 272, 3)
+    dev = [moe.DeviceBank.from_int8(w.cuda(), v.cuda()) for w, v in banks]
+    plan = moe.dispatch(ids.cuda(), 4)
+    xd = x.cuda()
+    clean = moe.expert_gateup_swiglu(dev[0], dev[1], xd, plan)
+    capi.lib.b2moe_harness_wait_probe(1, 0)
+    try:
+        moe.expert_gateup_swiglu(dev[0], dev[1], xd, plan)
+        torch.cuda.synchronize()
+    finally:
+        capi.lib.b2moe_harness_wait_probe(-1, 0)
+    assert int(plan.buf[3]) != 0
+    plan = moe.dispatch(ids.cuda(), 4)
+    assert torch.equal(moe.expert_gateup_swiglu(dev[0], dev[1], xd, plan), clean) and int(plan.buf[3]) == 0

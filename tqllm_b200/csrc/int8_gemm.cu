@@ -6,7 +6,8 @@
 // l + 16 of the epilogue hold both sums of an output.
 //
 // One block per SM walks the items (tile of activation rows, block of weight rows): one thread issues the copies into a ring, one the products, eight warps
-// empty one accumulator while the next one fills.
+// empty one accumulator while the next one fills. 8192 rows of 4096 x 4096: 85.7 us, 3.2e15 operations a second (1.93 of the measured bf16 rate; 96 without pairs, 150 with items of
+// 128 rows). The grouped products are bound by reading the weights: gate/up of 128 experts of 1408 x 4096 at 16 rows each 241 us, 6.1 TB/s (0.94 of measured).
 #include <cooperative_groups.h>
 #include <cuda.h>
 
@@ -29,7 +30,9 @@ struct TcArgs {
     int nt, box, stages, row_blocks, tiles;     // activation rows of an item, of a copy; ring; blocks of weight rows; items of a dense call in the row direction
     uint32_t tmem_cols;
     int * status;
+    int drop;                                   // test hook: the copies of this step of every block are left out (-1: none)
 };
+int g_drop_step = -1;
 
 // kind::i8: A and B signed 8-bit, D signed 32-bit, both K-major
 __device__ __forceinline__ uint32_t idesc_i8(uint32_t m, uint32_t n) { return (2u << 4) | (1u << 7) | (1u << 10) | ((n >> 3) << 17) | ((m >> 4) << 24); }
@@ -37,6 +40,38 @@ __device__ __forceinline__ void mma_i8(bool lead, uint32_t d, uint32_t a_lo, uin
     asm volatile("{\n .reg .pred p, q;\n .reg .b64 da, db;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %6, 0;\n mov.b64 da, {%1, %5};\n mov.b64 db, {%2, %5};\n"
                  " @q tcgen05.mma.cta_group::1.kind::i8 [%0], da, db, %3, p;\n}" ::"r"(d), "r"(a_lo), "r"(b_lo), "r"(id), "r"(acc), "r"(SW128_DESC_HI), "r"(uint32_t(lead)) : "memory");
 }
+// The same across a pair of blocks (the even one of a cluster issues): 256 rows of D, 128 in either block's tensor memory; A and B lie half in either block's shared memory
+__device__ __forceinline__ void mma_i8_pair(bool lead, uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t id, uint32_t acc) {
+    asm volatile("{\n .reg .pred p, q;\n .reg .b64 da, db;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %6, 0;\n mov.b64 da, {%1, %5};\n mov.b64 db, {%2, %5};\n"
+                 " @q tcgen05.mma.cta_group::2.kind::i8 [%0], da, db, %3, p;\n}" ::"r"(d), "r"(a_lo), "r"(b_lo), "r"(id), "r"(acc), "r"(SW128_DESC_HI), "r"(uint32_t(lead)) : "memory");
+}
+// one arrival at the barrier of this place in both blocks
+__device__ __forceinline__ void mma_commit_pair(bool lead, uint32_t bar) {
+    asm volatile("{\n .reg .pred q;\n .reg .b16 m;\n setp.ne.b32 q, %1, 0;\n mov.b16 m, 3;\n"
+                 " @q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], m;\n}" ::"r"(bar), "r"(uint32_t(lead)) : "memory");
+}
+__device__ __forceinline__ void tmem_alloc_pair(uint32_t slot_saddr, uint32_t cols) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot_saddr), "r"(cols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_free_pair(uint32_t base, uint32_t cols) {
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(cols) : "memory");
+}
+// copies into this block's shared memory whose completion goes to a barrier of either block of the pair
+__device__ __forceinline__ void pair_load_3d(uint32_t dst, const void * map, int x, int y, int z, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3, %4}], [%5];"
+                 ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void pair_load_2d(uint32_t dst, const void * map, int x, int y, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3}], [%4];"
+                 ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
+}
+__device__ __forceinline__ uint32_t at_rank(uint32_t addr, int rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ void bar_arrive_cluster(uint32_t bar) { asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
 __device__ __forceinline__ void epi_sync() { asm volatile("bar.sync 1, %0;" ::"n"(TC_EPI_THREADS) : "memory"); }
 
 struct TcItem { int e, first, count, rb; };      // expert, first row (slot), rows, block of weight rows
@@ -84,7 +119,10 @@ __device__ __forceinline__ void store_item(const I8Args & p, const TcItem & im, 
 
 // SPLIT (dense calls with few items): the blocks of a cluster take parts of an item's columns each, and then a share of its activation rows each, whose parts they
 // read from one another's shared memory: whole numbers, so the sum is the same
-template <int MATS, bool SPLIT>
+// PAIR (long rows): two blocks take neighbouring blocks of weight rows of the same activation rows, of which each brings a half: the copies from the L2, which set the pace of
+// large calls, are a third fewer. The even block issues the products of both and has the barriers of the operands and of the sums that have been read.
+enum { TC_SPLIT = 1, TC_PAIR = 2 };
+template <int MATS, int MODE>
 __global__ void __launch_bounds__(TC_THREADS, 1) i8_gemm_k(const I8Args p, const TcArgs c, const __grid_constant__ TcMaps maps) {
     extern __shared__ __align__(1024) uint8_t tc_mem[];
     __shared__ __align__(16) int2 table[2][256];
@@ -92,24 +130,30 @@ __global__ void __launch_bounds__(TC_THREADS, 1) i8_gemm_k(const I8Args p, const
     __shared__ int scan[TC_THREADS / 32];
     __shared__ uint32_t tmem_slot;
     __shared__ volatile int abort_flag;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const uint32_t stage_bytes = TC_A_BYTES + c.nt * 128;
+    constexpr bool SPLIT = MODE == TC_SPLIT, PAIR = MODE == TC_PAIR;
+    namespace cg = cooperative_groups;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rank = PAIR ? blockIdx.x & 1 : 0;
+    const uint32_t stage_bytes = TC_A_BYTES + c.nt * (PAIR ? 64 : 128);
     uint8_t * const ring = tc_mem + (1024u - (saddr(tc_mem) & 1023u)) % 1024u;
     const int e1 = p.experts + 1;
     int * const ends = reinterpret_cast<int *>(ring + size_t(c.stages) * stage_bytes), * const offs = ends + e1;      // tiles up to and with expert e, its first slot
     const uint32_t full = saddr(bars), empty = full + 8 * TC_MAX_STAGES, acc_full = empty + 8 * TC_MAX_STAGES, acc_empty = acc_full + 16, drain = acc_empty + 16;
     if (threadIdx.x == 0) {
         for (int i = 0; i < c.stages; ++i) { bar_init(full + 8 * i, 1); bar_init(empty + 8 * i, 1); }
-        for (int i = 0; i < 2; ++i) { bar_init(acc_full + 8 * i, 1); bar_init(acc_empty + 8 * i, TC_EPI_WARPS); }
+        for (int i = 0; i < 2; ++i) { bar_init(acc_full + 8 * i, 1); bar_init(acc_empty + 8 * i, (PAIR ? 2 : 1) * TC_EPI_WARPS); }
         bar_init(drain, 1);
         bar_init_fence();
         abort_flag = 0;
         for (int m = 0; m < MATS; ++m) { prefetch_map(maps.a + m); if (p.plan) prefetch_map(maps.shared + m); }
         prefetch_map(&maps.b);
     }
-    if (warp == 1) tmem_alloc(saddr(&tmem_slot), c.tmem_cols);
+    if (warp == 1) {
+        if (PAIR) tmem_alloc_pair(saddr(&tmem_slot), c.tmem_cols);
+        else tmem_alloc(saddr(&tmem_slot), c.tmem_cols);
+    }
     fence_before();
-    __syncthreads();
+    if (PAIR) cg::this_cluster().sync();                               // the other block's barriers are there
+    else __syncthreads();
     fence_after();
     const uint32_t tmem = tmem_slot;
     grid_wait();
@@ -140,12 +184,14 @@ __global__ void __launch_bounds__(TC_THREADS, 1) i8_gemm_k(const I8Args p, const
         __syncthreads();
         tiles = ends[e1 - 1];
     }
-    const int items = tiles * c.row_blocks, all_steps = (p.cols + 127) / 128;
+    // an item: a tile of activation rows and a block (PAIR: two) of weight rows; the blocks of a pair walk the same items
+    const int item_blocks = PAIR ? (c.row_blocks + 1) / 2 : c.row_blocks, it0 = PAIR ? blockIdx.x >> 1 : blockIdx.x, it_step = PAIR ? gridDim.x >> 1 : gridDim.x;
+    const int items = tiles * item_blocks, all_steps = (p.cols + 127) / 128;
     const int k0 = SPLIT ? all_steps * int(blockIdx.z) / int(gridDim.z) : 0, k1 = SPLIT ? all_steps * (int(blockIdx.z) + 1) / int(gridDim.z) : all_steps;
     auto locate = [&](int it) {
         TcItem im;
-        const int tile = it / c.row_blocks;
-        im.rb = it - tile * c.row_blocks;
+        const int tile = it / item_blocks;
+        im.rb = PAIR ? 2 * (it - tile * item_blocks) + rank : it - tile * item_blocks;
         im.e = 0;
         int t = tile;
         im.first = 0;
@@ -176,19 +222,32 @@ __global__ void __launch_bounds__(TC_THREADS, 1) i8_gemm_k(const I8Args p, const
         uint32_t issued = 0, slot = 0, phase = 1;                      // phase: of the empty barrier's wait (none in the first round)
         bool ok = true;
         const bool lead = elect_one();
+        const uint32_t full0 = PAIR ? at_rank(full, 0) : full;
 #pragma unroll 1
-        for (int it = blockIdx.x; it < items && ok && !abort_flag; it += gridDim.x) {
+        for (int it = it0; it < items && ok && !abort_flag; it += it_step) {
             const TcItem im = locate(it);
             const bool shared = p.plan && im.e == p.experts;
             const CUtensorMap * a = shared ? maps.shared : maps.a;
-            const int e = shared ? 0 : im.e, boxes = (im.count + c.box - 1) / c.box;
+            const int e = shared ? 0 : im.e, boxes = PAIR ? (im.count + 2 * c.box - 1) / (2 * c.box) : (im.count + c.box - 1) / c.box;      // PAIR: of this block's half
+            const int first = im.first + (PAIR ? rank * boxes * c.box : 0);
 #pragma unroll 1
             for (int k = k0; k < k1; ++k) {
                 if (issued >= uint32_t(c.stages) && !warp_wait(empty + 8 * slot, phase)) { ok = false; break; }
-                if (lead) {
-                    const uint32_t bar = full + 8 * slot, dst = saddr(ring) + slot * stage_bytes;
-                    bar_expect_tx(bar, TC_A_BYTES + uint32_t(boxes * c.box) * 128);
-                    if (MATS == 2) {
+                if (lead && int(issued) != c.drop) {
+                    const uint32_t bar = PAIR ? full0 + 8 * slot : full + 8 * slot, dst = saddr(ring) + slot * stage_bytes;
+                    if (!PAIR || rank == 0) bar_expect_tx(full + 8 * slot, (PAIR ? 2 : 1) * (TC_A_BYTES + uint32_t(boxes * c.box) * 128));
+                    if (PAIR) {
+                        if (MATS == 2) {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                pair_load_3d(dst + 4096 * i, a, 128 * k, 64 * im.rb + 16 * i, e, bar);
+                                pair_load_3d(dst + 4096 * i + 2048, a + 1, 128 * k, 64 * im.rb + 16 * i, e, bar);
+                            }
+                        } else {
+                            pair_load_3d(dst, a, 128 * k, 128 * im.rb, e, bar);
+                        }
+                        for (int i = 0; i < boxes; ++i) pair_load_2d(dst + TC_A_BYTES + i * c.box * 128, &maps.b, 128 * k, first + i * c.box, bar);
+                    } else if (MATS == 2) {
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             tma_load_3d(dst + 4096 * i, a, 128 * k, 64 * im.rb + 16 * i, e, bar);
@@ -197,7 +256,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) i8_gemm_k(const I8Args p, const
                     } else {
                         tma_load_3d(dst, a, 128 * k, 128 * im.rb, e, bar);
                     }
-                    for (int i = 0; i < boxes; ++i) tma_load_2d(dst + TC_A_BYTES + i * c.box * 128, &maps.b, 128 * k, im.first + i * c.box, bar);
+                    if (!PAIR) for (int i = 0; i < boxes; ++i) tma_load_2d(dst + TC_A_BYTES + i * c.box * 128, &maps.b, 128 * k, first + i * c.box, bar);
                 }
                 __syncwarp();
                 ++issued;
@@ -205,18 +264,25 @@ __global__ void __launch_bounds__(TC_THREADS, 1) i8_gemm_k(const I8Args p, const
             }
         }
         if (!ok && lane == 0) give_up();
-        // before leaving, every copy must have landed (after a clean run these waits return at once)
+        // before leaving, every copy must have landed (after a clean run these waits return at once). The odd block of a pair has no barrier for its own: the even one waits for them, and the
+        // blocks meet at the end; after a wait that ran out it leaves them two milliseconds
+        if (PAIR && rank == 1) {
+            if (!ok || abort_flag)
+                for (int i = 0; i < 2000; ++i) __nanosleep(1000);
+        } else
 #pragma unroll 1
-        for (uint32_t i = issued > uint32_t(c.stages) ? issued - c.stages : 0; i < issued; ++i) bar_wait(full + 8 * (i % c.stages), (i / c.stages) & 1u);
-    } else if (warp == 1) {
+        for (uint32_t i = issued > uint32_t(c.stages) ? issued - c.stages : 0; i < issued; ++i)
+            if (int(i) != c.drop) bar_wait(full + 8 * (i % c.stages), (i / c.stages) & 1u);
+    } else if (warp == 1 && rank == 0) {
         // ---- products: the whole warp walks the loop, one lane issues ----
         const bool lead = elect_one();
         const uint32_t a0 = sw128_desc_lo(saddr(ring)), step = stage_bytes >> 4;
         uint32_t slot = 0, phase = 0, done = 0;
         bool ok = true;
 #pragma unroll 1
-        for (int it = blockIdx.x; it < items && ok && !abort_flag; it += gridDim.x, ++done) {
-            const uint32_t h = done & 1u, d = tmem + h * c.nt, id = idesc_i8(128, uint32_t(__shfl_sync(0xffffffffu, locate(it).count, 0) + 15) & ~15u);
+        for (int it = it0; it < items && ok && !abort_flag; it += it_step, ++done) {
+            const uint32_t h = done & 1u, d = tmem + h * c.nt, count = __shfl_sync(0xffffffffu, locate(it).count, 0);
+            const uint32_t id = PAIR ? idesc_i8(256, (count + 2 * c.box - 1) / (2 * c.box) * (2 * c.box)) : idesc_i8(128, (count + 15) & ~15u);
             if (done >= 2 && !warp_wait(acc_empty + 8 * h, ((done >> 1) - 1) & 1u)) { ok = false; break; }
             fence_after();
 #pragma unroll 1
@@ -225,15 +291,23 @@ __global__ void __launch_bounds__(TC_THREADS, 1) i8_gemm_k(const I8Args p, const
                 fence_after();
                 const uint32_t a = a0 + slot * step, b = a + (TC_A_BYTES >> 4);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) mma_i8(lead, d, a + 2 * i, b + 2 * i, id, k > k0 || i > 0);
-                mma_commit(lead, empty + 8 * slot);
+                for (int i = 0; i < 4; ++i) {
+                    if (PAIR) mma_i8_pair(lead, d, a + 2 * i, b + 2 * i, id, k > k0 || i > 0);
+                    else mma_i8(lead, d, a + 2 * i, b + 2 * i, id, k > k0 || i > 0);
+                }
+                if (PAIR) mma_commit_pair(lead, empty + 8 * slot);
+                else mma_commit(lead, empty + 8 * slot);
                 if (++slot == uint32_t(c.stages)) { slot = 0; phase ^= 1u; }
             }
-            if (ok) mma_commit(lead, acc_full + 8 * h);
+            if (ok) {
+                if (PAIR) mma_commit_pair(lead, acc_full + 8 * h);
+                else mma_commit(lead, acc_full + 8 * h);
+            }
         }
         if (!ok && lane == 0) give_up();
         // nothing may be in flight when the tensor memory is freed
-        mma_commit(lead, drain);
+        if (PAIR) mma_commit_pair(lead, drain);
+        else mma_commit(lead, drain);
         warp_wait(drain, 0);
     } else if (SPLIT && warp >= TC_EPI_WARP0) {
         // ---- this block's part: from tensor memory to the ring, which nothing uses any more, 128 weight rows for each activation row ----
@@ -264,15 +338,16 @@ __global__ void __launch_bounds__(TC_THREADS, 1) i8_gemm_k(const I8Args p, const
 #pragma unroll
             for (int m = 0; m < MATS; ++m) v[m] = row < p.rows ? (p.plan && im.e == p.experts ? p.shared_v[m] : p.v[m] + size_t(im.e) * p.rows)[row] : 0.f;
         };
+        const uint32_t acc_empty0 = PAIR ? at_rank(acc_empty, 0) : acc_empty;
         uint32_t done = 0;
         bool ok = true;
         TcItem im{}, next{};
-        if (int(blockIdx.x) < items) {
-            next = locate(blockIdx.x);
+        if (it0 < items) {
+            next = locate(it0);
             fetch(next);
         }
 #pragma unroll 1
-        for (int it = blockIdx.x; it < items; it += gridDim.x, ++done) {
+        for (int it = it0; it < items; it += it_step, ++done) {
             const uint32_t h = done & 1u;
             im = next;
             if (tid < im.count) table[h][tid] = mine;
@@ -280,8 +355,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) i8_gemm_k(const I8Args p, const
 #pragma unroll
             for (int m = 0; m < MATS; ++m) scale[m] = v[m];
             epi_sync();                                                // the table is there; the other one's item has been read by every warp
-            if (it + int(gridDim.x) < items) {
-                next = locate(it + gridDim.x);
+            if (it + it_step < items) {
+                next = locate(it + it_step);
                 fetch(next);
             }
             ok = ok && !abort_flag && warp_wait(acc_full + 8 * h, (done >> 1) & 1u);
@@ -296,15 +371,21 @@ __global__ void __launch_bounds__(TC_THREADS, 1) i8_gemm_k(const I8Args p, const
             }
             fence_before();
             __syncwarp();
-            if (lane == 0) bar_arrive(acc_empty + 8 * h);
+            if (lane == 0) {
+                if (PAIR) bar_arrive_cluster(acc_empty0 + 8 * h);
+                else bar_arrive(acc_empty + 8 * h);
+            }
         }
     }
     fence_before();
-    __syncthreads();
+    if (PAIR) cg::this_cluster().sync();                               // nothing of either block arrives at the other one any more
+    else __syncthreads();
     fence_after();
-    if (warp == 1) tmem_free(tmem, c.tmem_cols);
+    if (warp == 1) {
+        if (PAIR) tmem_free_pair(tmem, c.tmem_cols);
+        else tmem_free(tmem, c.tmem_cols);
+    }
     if constexpr (SPLIT) {
-        namespace cg = cooperative_groups;
         cg::cluster_group cluster = cg::this_cluster();
         const TcItem im = locate(blockIdx.x);
         const int parts = gridDim.z, lo = im.count * int(blockIdx.z) / parts, hi = im.count * (int(blockIdx.z) + 1) / parts, r = threadIdx.x & 127, row = 128 * im.rb + r;
@@ -347,6 +428,19 @@ int sm_count() {
     }();
     return count;
 }
+template <class K>
+int32_t launch_cluster(K kernel, dim3 grid, dim3 cluster, size_t smem, cudaStream_t s, const I8Args & p, const TcArgs & c, const TcMaps & maps) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid; cfg.blockDim = dim3(TC_THREADS); cfg.dynamicSmemBytes = smem; cfg.stream = s;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = cluster.x; at[0].val.clusterDim.y = cluster.y; at[0].val.clusterDim.z = cluster.z;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at; cfg.numAttrs = g_overlap ? 2 : 1;
+    if (cudaLaunchKernelEx(&cfg, kernel, p, c, maps) != cudaSuccess) return B2MOE_ERR_CUDA;
+    return launch_status();
+}
 bool map_rows(CUtensorMap & m, const int8_t * base, int cols, long long rows, long long stride, int experts, int box) {
     if (experts) {
         const cuuint64_t dims[3] = {cuuint64_t(cols), cuuint64_t(rows), cuuint64_t(experts)}, strides[2] = {cuuint64_t(stride), cuuint64_t(stride) * rows};
@@ -363,7 +457,7 @@ int clusters_at_once(int size) {
     static const std::array<int, TC_MAX_SPLIT + 1> most = [] {
         std::array<int, TC_MAX_SPLIT + 1> m{};
         constexpr int smem = TC_SMEM - 8 * 1024;
-        if (cudaFuncSetAttribute(i8_gemm_k<1, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return m;
+        if (cudaFuncSetAttribute(i8_gemm_k<1, TC_SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return m;
         for (int size = 2; size <= TC_MAX_SPLIT; ++size) {
             cudaLaunchConfig_t cfg{};
             cfg.gridDim = dim3(1, 1, size); cfg.blockDim = dim3(TC_THREADS); cfg.dynamicSmemBytes = smem;
@@ -371,7 +465,7 @@ int clusters_at_once(int size) {
             at[0].id = cudaLaunchAttributeClusterDimension;
             at[0].val.clusterDim.x = 1; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = size;
             cfg.attrs = at; cfg.numAttrs = 1;
-            if (cudaOccupancyMaxActiveClusters(&m[size], i8_gemm_k<1, true>, &cfg) != cudaSuccess) m[size] = 0;
+            if (cudaOccupancyMaxActiveClusters(&m[size], i8_gemm_k<1, TC_SPLIT>, &cfg) != cudaSuccess) m[size] = 0;
         }
         cudaGetLastError();
         return m;
@@ -390,25 +484,32 @@ int split_of(long long items, int steps) {
 
 }  // namespace
 
+void i8_drop_step(int step) { g_drop_step = step; }
 bool i8_gemm_supported(int experts) { return experts <= TC_MAX_EXPERTS; }
 
 template <int MATS>
 int32_t i8_gemm(const I8Args & p, long long q_rows, int per_group, int * status, cudaStream_t s) {
     TcArgs c{};
     c.row_blocks = ceil_div(p.rows, MATS == 2 ? 64 : 128);
-    // Items of 256 rows halve what the weights cost in copies and products (8192 x 4096 x 4096: 96 us, with 128 rows 153), items of 128 leave room for six ring
-    // stages instead of four and waste less where an expert has fewer (512 experts at 80 each, gate/up 211 against 225 us; 128 experts at 16 each 242 and 263, at 128 each with a
-    // skewed load 385 and 333); below that nothing is gained (64 rows, 16 each: 248). A dense call takes the large ones where they fill the SMs (256 rows of 4096 x 4096: 17.5 us in items of 256, 14.0 of 128)
+    // Items of 256 rows halve what the weights cost in copies and products (8192 x 4096 x 4096: 96 us, with 128 rows 150), items of 128 leave room for six ring
+    // stages instead of four and waste less where an expert has fewer (512 experts at 80 each, gate/up 211 against 225 us; 128 experts at 128 each with a
+    // skewed load 385 and 333); below that nothing is gained (64 rows, 16 each: 248 and 242). A dense call takes the large ones where they fill the SMs (256 rows of 4096 x 4096: 17.5 us in items of 256,
+    // 14.0 of 128). Pairs pay from long rows on, where the products of an item outlast what its blocks tell each other: us, single / pair: 8192 x 4096 rows of 4096 columns 96.5 / 87.1, of 2048 59.6 / 60.3,
+    // of 1024 49.1 / 53.6; 8192 x 8192 of 8192 378.6 / 353.0; gate/up, 128 experts of 4096 columns at 16 each 248.5 (items of 128) / 246.2, at 160 344.9 / 326.2, at 320 613 / 584; 512 of 2048 at 160 304 / 318;
+    // down, 512 of 512 columns at 80 193 / 242
     const int sms = sm_count();
-    c.nt = p.plan ? (per_group > 96 ? 256 : 128) : (long long)ceil_div(p.n, 256) * c.row_blocks >= sms ? 256 : 128;
-    c.box = 64;                                                        // rows of a copy: an item takes as many copies as it has rows for
+    const bool longer = p.cols > 2560;
+    c.nt = p.plan ? (per_group > 96 || longer ? 256 : 128) : (long long)ceil_div(p.n, 256) * c.row_blocks >= sms ? 256 : 128;
     c.tiles = p.plan ? 0 : ceil_div(p.n, c.nt);
     // A dense call with few items: as many blocks an item as run at once
     const int split = MATS == 1 && !p.plan ? split_of((long long)c.tiles * c.row_blocks, ceil_div(p.cols, 128)) : 1;
+    const bool pair = split == 1 && longer && c.nt == 256;
+    c.box = pair ? 32 : 64;                                            // rows of a copy: an item takes as many copies as it has rows for
     c.tmem_cols = std::max(32, 2 * c.nt);
     c.status = status;
+    c.drop = g_drop_step;
     const size_t table = p.plan ? size_t(2 * (p.experts + 1) + 1) * sizeof(int) : 0, fixed = 8 * 1024;      // static arrays and the alignment of the ring
-    c.stages = int(std::min<size_t>(TC_MAX_STAGES, (TC_SMEM - fixed - table) / (TC_A_BYTES + size_t(c.nt) * 128)));
+    c.stages = int(std::min<size_t>(TC_MAX_STAGES, (TC_SMEM - fixed - table) / (TC_A_BYTES + size_t(c.nt) * (pair ? 64 : 128))));
     TcMaps maps;
     std::memset(&maps, 0, sizeof(maps));
     const int box = MATS == 2 ? 16 : 128;
@@ -419,24 +520,20 @@ int32_t i8_gemm(const I8Args & p, long long q_rows, int per_group, int * status,
         else maps.shared[m] = maps.a[m];
     }
     if (!ok) return B2MOE_ERR_CUDA;
-    const size_t smem = 1024 + size_t(c.stages) * (TC_A_BYTES + size_t(c.nt) * 128) + table;
+    const size_t smem = 1024 + size_t(c.stages) * (TC_A_BYTES + size_t(c.nt) * (pair ? 64 : 128)) + table;
     const long long items = (long long)c.tiles * c.row_blocks;
     if constexpr (MATS == 1)
         if (split > 1) {
-            if (cudaFuncSetAttribute(i8_gemm_k<1, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)) != cudaSuccess) return B2MOE_ERR_CUDA;
-            cudaLaunchConfig_t cfg{};
-            cfg.gridDim = dim3(unsigned(items), 1, split); cfg.blockDim = dim3(TC_THREADS); cfg.dynamicSmemBytes = smem; cfg.stream = s;
-            cudaLaunchAttribute at[2];
-            at[0].id = cudaLaunchAttributeClusterDimension;
-            at[0].val.clusterDim.x = 1; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = split;
-            at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-            at[1].val.programmaticStreamSerializationAllowed = 1;
-            cfg.attrs = at; cfg.numAttrs = g_overlap ? 2 : 1;
-            if (cudaLaunchKernelEx(&cfg, i8_gemm_k<1, true>, p, c, maps) != cudaSuccess) return B2MOE_ERR_CUDA;
-            return launch_status();
+            if (cudaFuncSetAttribute(i8_gemm_k<1, TC_SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)) != cudaSuccess) return B2MOE_ERR_CUDA;
+            return launch_cluster(i8_gemm_k<1, TC_SPLIT>, dim3(unsigned(items), 1, split), dim3(1, 1, split), smem, s, p, c, maps);
         }
-    if (cudaFuncSetAttribute(i8_gemm_k<MATS, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)) != cudaSuccess) return B2MOE_ERR_CUDA;
-    launch_overlapped(i8_gemm_k<MATS, false>, dim3(unsigned(p.plan ? sms : std::min<long long>(sms, items))), dim3(TC_THREADS), smem, s, p, c, maps);
+    if (pair) {
+        if (cudaFuncSetAttribute(i8_gemm_k<MATS, TC_PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)) != cudaSuccess) return B2MOE_ERR_CUDA;
+        const long long pairs = (long long)c.tiles * ceil_div(c.row_blocks, 2);
+        return launch_cluster(i8_gemm_k<MATS, TC_PAIR>, dim3(unsigned(2 * (p.plan ? sms / 2 : std::min<long long>(sms / 2, pairs)))), dim3(2), smem, s, p, c, maps);
+    }
+    if (cudaFuncSetAttribute(i8_gemm_k<MATS, 0>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)) != cudaSuccess) return B2MOE_ERR_CUDA;
+    launch_overlapped(i8_gemm_k<MATS, 0>, dim3(unsigned(p.plan ? sms : std::min<long long>(sms, items))), dim3(TC_THREADS), smem, s, p, c, maps);
     return launch_status();
 }
 template int32_t i8_gemm<1>(const I8Args &, long long, int, int *, cudaStream_t);
