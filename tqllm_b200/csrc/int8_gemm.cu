@@ -5,9 +5,9 @@
 // expert has few, and a warp of the epilogue stores neighbouring outputs of one activation row. Gate and up share a tile, 16 rows of each in turn, so that lanes l and
 // l + 16 of the epilogue hold both sums of an output.
 //
-// One block per SM walks the items (tile of activation rows, block of weight rows): one thread issues the copies into a ring, one the products, eight warps
+// One block per SM (two for short rows) walks the items (tile of activation rows, block of weight rows): one thread issues the copies into a ring, one the products, eight warps
 // empty one accumulator while the next one fills. 8192 rows of 4096 x 4096: 85.7 us, 3.2e15 operations a second (1.93 of the measured bf16 rate; 96 without pairs, 150 with items of
-// 128 rows). The grouped products are bound by reading the weights: gate/up of 128 experts of 1408 x 4096 at 16 rows each 241 us, 6.1 TB/s (0.94 of measured).
+// 128 rows). The grouped products are bound by reading the weights: gate/up of 128 experts of 1408 x 4096 at 16 rows each 241 us, 6.1 TB/s (0.94 of measured), down of 512 of 2048 x 512 at 1.2 rows each 62 us, 5.9 TB/s.
 #include <cooperative_groups.h>
 #include <cuda.h>
 
@@ -123,7 +123,7 @@ __device__ __forceinline__ void store_item(const I8Args & p, const TcItem & im, 
 // large calls, are a third fewer. The even block issues the products of both and has the barriers of the operands and of the sums that have been read.
 enum { TC_SPLIT = 1, TC_PAIR = 2 };
 template <int MATS, int MODE>
-__global__ void __launch_bounds__(TC_THREADS, 1) i8_gemm_k(const I8Args p, const TcArgs c, const __grid_constant__ TcMaps maps) {
+__global__ void __launch_bounds__(TC_THREADS, MODE ? 1 : 2) i8_gemm_k(const I8Args p, const TcArgs c, const __grid_constant__ TcMaps maps) {
     extern __shared__ __align__(1024) uint8_t tc_mem[];
     __shared__ __align__(16) int2 table[2][256];
     __shared__ __align__(8) uint64_t bars[2 * TC_MAX_STAGES + 5];
@@ -497,19 +497,27 @@ int32_t i8_gemm(const I8Args & p, long long q_rows, int per_group, int * status,
     // 14.0 of 128). Pairs pay from long rows on, where the products of an item outlast what its blocks tell each other: us, single / pair: 8192 x 4096 rows of 4096 columns 96.5 / 87.1, of 2048 59.6 / 60.3,
     // of 1024 49.1 / 53.6; 8192 x 8192 of 8192 378.6 / 353.0; gate/up, 128 experts of 4096 columns at 16 each 248.5 (items of 128) / 246.2, at 160 344.9 / 326.2, at 320 613 / 584; 512 of 2048 at 160 304 / 318;
     // down, 512 of 512 columns at 80 193 / 242
+    // Short rows: two blocks an SM with half the ring each, since an item of a few steps takes longer from its first copy to its last store than its copies alone, and one block's items hide
+    // behind the other's. us, one / two: down, 512 experts of 512 columns at one row each 76 / 60, at 80 192 / 178, at 320 650 / 498, of 768 columns at 40 64 / 67; gate/up of 512 columns at 8 107 / 78;
+    // dense 8192 rows, 4096 x 512 44 / 36, 4096 x 1024 49 / 42; gate/up of 2048 columns at 80 242 / 258. A dense call takes smaller items then where those fill more of the SMs (256 rows 6.2 / 5.0)
     const int sms = sm_count();
-    const bool longer = p.cols > 2560;
-    c.nt = p.plan ? (per_group > 96 || longer ? 256 : 128) : (long long)ceil_div(p.n, 256) * c.row_blocks >= sms ? 256 : 128;
+    const bool longer = p.cols > 2560, two = p.cols <= I8_SHORT_COLS;
+    if (two) {
+        c.nt = 128;
+        while (!p.plan && c.nt > 32 && (long long)ceil_div(p.n, c.nt) * c.row_blocks < sms) c.nt /= 2;
+    } else {
+        c.nt = p.plan ? (per_group > 96 || longer ? 256 : 128) : (long long)ceil_div(p.n, 256) * c.row_blocks >= sms ? 256 : 128;
+    }
     c.tiles = p.plan ? 0 : ceil_div(p.n, c.nt);
     // A dense call with few items: as many blocks an item as run at once
     const int split = MATS == 1 && !p.plan ? split_of((long long)c.tiles * c.row_blocks, ceil_div(p.cols, 128)) : 1;
     const bool pair = split == 1 && longer && c.nt == 256;
-    c.box = pair ? 32 : 64;                                            // rows of a copy: an item takes as many copies as it has rows for
+    c.box = pair || two ? 32 : 64;                                     // rows of a copy: an item takes as many copies as it has rows for
     c.tmem_cols = std::max(32, 2 * c.nt);
     c.status = status;
     c.drop = g_drop_step;
     const size_t table = p.plan ? size_t(2 * (p.experts + 1) + 1) * sizeof(int) : 0, fixed = 8 * 1024;      // static arrays and the alignment of the ring
-    c.stages = int(std::min<size_t>(TC_MAX_STAGES, (TC_SMEM - fixed - table) / (TC_A_BYTES + size_t(c.nt) * (pair ? 64 : 128))));
+    c.stages = int(std::min<size_t>(TC_MAX_STAGES, ((two ? TC_SMEM / 2 : TC_SMEM) - fixed - table) / (TC_A_BYTES + size_t(c.nt) * (pair ? 64 : 128))));
     TcMaps maps;
     std::memset(&maps, 0, sizeof(maps));
     const int box = MATS == 2 ? 16 : 128;
@@ -533,7 +541,8 @@ int32_t i8_gemm(const I8Args & p, long long q_rows, int per_group, int * status,
         return launch_cluster(i8_gemm_k<MATS, TC_PAIR>, dim3(unsigned(2 * (p.plan ? sms / 2 : std::min<long long>(sms / 2, pairs)))), dim3(2), smem, s, p, c, maps);
     }
     if (cudaFuncSetAttribute(i8_gemm_k<MATS, 0>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)) != cudaSuccess) return B2MOE_ERR_CUDA;
-    launch_overlapped(i8_gemm_k<MATS, 0>, dim3(unsigned(p.plan ? sms : std::min<long long>(sms, items))), dim3(TC_THREADS), smem, s, p, c, maps);
+    const int blocks = two ? 2 * sms : sms;
+    launch_overlapped(i8_gemm_k<MATS, 0>, dim3(unsigned(p.plan ? blocks : std::min<long long>(blocks, items))), dim3(TC_THREADS), smem, s, p, c, maps);
     return launch_status();
 }
 template int32_t i8_gemm<1>(const I8Args &, long long, int, int *, cudaStream_t);

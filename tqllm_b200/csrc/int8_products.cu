@@ -163,14 +163,14 @@ size_t i8_slot_bytes(int slot_rows, int k) { return i8_rows_bytes(slot_rows, k) 
 //   dense, from 17 rows on: 4096 x 4096 16 rows 7.7 / 7.9, 24 10.3 / 8.0; 1411 x 2560 16 4.4 / 5.7, 32 6.7 / 5.9; 8192 x 1024 16 4.4 / 4.9, 32 5.7 / 5.1
 //   gate/up, from seven rows per expert on: 128 experts of 1408 x 4096 at 4 each 221 / 233, at 8 307 / 245; 512 of 512 x 2048 at 2.5 155 / 168, at 5 184 / 187; 32 of 512 x 1024 at 4 8.9 / 14.2, at 16
 //   17.1 / 15.3 (the GEMM's times have a launch more in them, since its rows lie in slot order)
-//   down, where they are in slot order anyway, also where the SMs get eight items each: 128 of 4096 x 1408 at 0.5 59 / 56, at 1 95 / 79, at 4 136 / 119; 512 of 2048 x 512 at 0.2 25 / 24, at 1.2 111 / 82
-constexpr int I8_DENSE_ROWS = 16, I8_GEMM_MIN_PER = 7, I8_MANY_ITEMS = 148 * 8;
+//   down, where they are in slot order anyway, also where the SMs get eight items each, and for short rows from three per expert or four items an SM on: 128 of 4096 x 1408 at 0.5 63 / 60, at 1
+//   95 / 80, at 4 138 / 120; 512 of 2048 x 512 two tokens of ten 9.5 / 9.7, four 14.8 / 11.9, 64 110 / 67; 32 of 1024 x 512 at 2 7.8 / 7.7, at 4 9.6 / 7.6
+constexpr int I8_DENSE_ROWS = 16, I8_GEMM_MIN_PER = 7, I8_SHORT_MIN_PER = 3, I8_MANY_ITEMS = 148 * 8, I8_SHORT_ITEMS = 148 * 4;
 bool i8_takes_gemm(int experts, bool worth) {
     const int family = harness_family();
     if (!i8_gemm_supported(experts) || family == B2MOE_FAMILY_GENERIC || family == B2MOE_FAMILY_DECODE || family == B2MOE_FAMILY_DECODE_KERNELS) return false;
     return family == B2MOE_FAMILY_GEMM || worth;
 }
-bool dense_enough(int experts, long long rows) { return rows >= (long long)I8_GEMM_MIN_PER * experts; }
 int per_group(int experts, long long rows) { return int(std::min<long long>(1 << 20, (rows + experts - 1) / experts)); }
 
 // x [n][cols]; the workspace holds the rows of the n tokens
@@ -178,7 +178,7 @@ int32_t i8_gateup(const b2moe_bank * gate, const b2moe_bank * up, const b2moe_ba
                   int topk, int shared_tokens, long long live, void * act, int act_dtype, void * ws, void * rows_buf, size_t rows_buf_bytes, cudaStream_t s) {
     I8Args p = grouped(gate, up, shared_gate, shared_up, plan, n, topk, shared_tokens, act, act_dtype);
     const int total = n * topk + shared_tokens;
-    if (i8_takes_gemm(gate->experts, dense_enough(gate->experts, live)) && rows_buf_bytes >= i8_slot_bytes(total, gate->cols)) {
+    if (i8_takes_gemm(gate->experts, live >= (long long)I8_GEMM_MIN_PER * gate->experts) && rows_buf_bytes >= i8_slot_bytes(total, gate->cols)) {
         const I8Rows rows = i8_rows(rows_buf, total);
         int * inverse = reinterpret_cast<int *>(static_cast<char *>(rows_buf) + i8_rows_bytes(total, gate->cols));
         if (int32_t rc = i8_quantize_scatter(x, x_dtype, n, gate->cols, rows, inverse, plan, gate->experts, topk, shared_tokens, s)) return rc;
@@ -198,8 +198,10 @@ int32_t i8_down(const b2moe_bank * down, const b2moe_bank * shared_down, const v
     const I8Rows rows = i8_rows(ws, total);
     if (int32_t rc = i8_quantize_slots(x, x_dtype, per_token, n, down->cols, rows, plan, down->experts, topk, shared_tokens, s)) return rc;
     p.q = rows.q; p.ldq = down->cols; p.s = rows.scale; p.slots = 1;
-    const bool many = (long long)groups_of(down->experts, n, topk, shared_tokens) * ceil_div(down->rows, 128) >= I8_MANY_ITEMS;
-    if (i8_takes_gemm(down->experts, dense_enough(down->experts, live) || (many && live == (long long)n * topk))) return i8_gemm<1>(p, total, per_group(down->experts, live), const_cast<int *>(plan) + PLAN_STATUS, s);
+    const bool short_rows = down->cols <= I8_SHORT_COLS, all = live == (long long)n * topk;
+    const long long items = (long long)groups_of(down->experts, n, topk, shared_tokens) * ceil_div(down->rows, 128);
+    if (i8_takes_gemm(down->experts, live >= (long long)(short_rows ? I8_SHORT_MIN_PER : I8_GEMM_MIN_PER) * down->experts || (all && items >= (short_rows ? I8_SHORT_ITEMS : I8_MANY_ITEMS))))
+        return i8_gemm<1>(p, total, per_group(down->experts, live), const_cast<int *>(plan) + PLAN_STATUS, s);
     return i8_stream<1>(p, groups_of(down->experts, n, topk, shared_tokens), live + shared_tokens, s);
 }
 
