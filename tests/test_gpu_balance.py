@@ -63,7 +63,7 @@ def check(logits, ids, e, coef, gating, mask=None, offsets=None, grad_scale=1.0,
     loss, counts, means, tokens, _ = plain(x, ids, e, coef, gating, mask, offsets)
     assert torch.equal(b.counts.cpu().double(), counts) and b.tokens.tolist() == tokens
     assert bool(((b.prob.cpu().double() - means).abs() <= C * means + 1e-36).all())
-    assert abs(float(b.loss) - float(loss)) <= C * abs(float(loss)) + 1e-36
+    assert abs(float(b.loss) - float(loss.detach())) <= C * abs(float(loss.detach())) + 1e-36
     want, = torch.autograd.grad(loss * grad_scale, x) if loss.requires_grad else (torch.zeros_like(x),)
     want = torch.nan_to_num(want[:, :e].detach(), nan=0.0)
     # the size of what is subtracted: p (c + dot) factor, from the gradient of the definition with its parts

@@ -340,27 +340,106 @@ def test_per_matrix_calls():
         assert torch.equal(out, moe.expert_down(down, act.float(), plan).half())
 
 
-def test_streams_and_graphs():
-    """a call on another stream, and a captured decode step replayed with new tokens in the same buffers"""
+@pytest.mark.parametrize("n,m,k", ((2, 130, 256), (200, 130, 256), (40, 300, 2560), (1100, 4096, 2688)))
+def test_streams_and_graphs(n, m, k):
+    """a call on another stream, and a captured decode step replayed with new tokens in the same buffers: every form of the product"""
     from tqllm_b200 import moe
-    for n in (2, 200):
-        q, s, w, v = linear_case(n, 130, 256, 8)
+    q, s, w, v = linear_case(n, m, k, 8)
+    bank = moe.DeviceBank.from_int8(w.cuda(), v.cuda())
+    x = torch.randn(n, k, generator=gen(1)).cuda()
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        side = moe.linear_i8(*moe.quantize_rows(x), bank)
+    stream.synchronize()
+    assert torch.equal(side, moe.linear_i8(*moe.quantize_rows(x), bank))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        out = moe.linear_i8(*moe.quantize_rows(x), bank)
+    for seed in (2, 3):
+        x.copy_(torch.randn(n, k, generator=gen(seed)))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, moe.linear_i8(*moe.quantize_rows(x), bank))
+
+
+def test_two_calls_at_once():
+    """products on two streams whose blocks share the SMs and their tensor memory"""
+    from tqllm_b200 import moe
+    jobs = []
+    for n, m, k in ((1000, 2000, 512), (1100, 4096, 2688), (40, 300, 2560), (3, 4096, 1024)):
+        q, s, w, v = linear_case(n, m, k, n)
         bank = moe.DeviceBank.from_int8(w.cuda(), v.cuda())
-        x = torch.randn(n, 256, generator=gen(1)).cuda()
-        stream = torch.cuda.Stream()
-        stream.wait_stream(torch.cuda.current_stream())
-        with torch.cuda.stream(stream):
-            side = moe.linear_i8(*moe.quantize_rows(x), bank)
-        stream.synchronize()
-        assert torch.equal(side, moe.linear_i8(*moe.quantize_rows(x), bank))
-        graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(graph, stream=stream):
-            out = moe.linear_i8(*moe.quantize_rows(x), bank)
-        for seed in (2, 3):
-            x.copy_(torch.randn(n, 256, generator=gen(seed)))
-            graph.replay()
-            torch.cuda.synchronize()
-            assert torch.equal(out, moe.linear_i8(*moe.quantize_rows(x), bank))
+        jobs.append((q.cuda(), s.cuda(), bank, moe.linear_i8(q.cuda(), s.cuda(), bank)))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in jobs]
+    outs = [[] for _ in jobs]
+    for _ in range(20):
+        for (q, s, bank, _), stream, out in zip(jobs, streams, outs):
+            with torch.cuda.stream(stream):
+                out.append(moe.linear_i8(q, s, bank))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, job[3]) for job, out in zip(jobs, outs) for o in out)
+
+
+@pytest.mark.parametrize("n", (2, 90))
+def test_a_captured_expert_block(n):
+    """dispatch, gate/up, down and the weighted sum in one graph, replayed with other tokens and other ids"""
+    from tqllm_b200 import moe
+    e, k, h, f = 6, 3, 2688, 272
+    _, _, banks, _ = experts_case(n, e, k, h, f, 5)
+    dev = [moe.DeviceBank.from_int8(w.cuda(), v.cuda()) for w, v in banks]
+    x, ids, w = torch.zeros(n, h, device="cuda"), torch.zeros(n, k, dtype=torch.int32, device="cuda"), torch.rand(n, k, generator=gen(1)).cuda()
+
+    def block():
+        plan = moe.dispatch(ids, e)
+        y = moe.expert_down(dev[2], moe.expert_gateup_swiglu(dev[0], dev[1], x, plan), plan)
+        return moe.combine(y, w, n, k, h, ids=ids, out_dtype=torch.bfloat16)
+
+    def fill(seed):
+        a, b, _, _ = experts_case(n, e, k, h, f, seed, route="skip" if seed % 2 else "even")
+        x.copy_(a)
+        ids.copy_(b)
+
+    fill(1)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        block()
+    stream.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        out = block()
+    for seed in (2, 3, 4):
+        fill(seed)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, block())
+
+
+@pytest.mark.parametrize("n", (3, 120))
+@pytest.mark.parametrize("which", ("gate", "down"))
+def test_a_layer_of_two_kinds_of_banks(n, which):
+    """Q4_K experts on one side and 8-bit ones on the other: the layer call gives the bits of its parts"""
+    from tqllm_b200 import moe, synth
+    e, k, h, f = 16, 3, 256, 512
+    shape = synth.LayerShape("mixed", h, e, k, f)
+    raw = synth.make_layer(shape, 3, "cpu", experts=e)
+    q4 = [moe.DeviceBank(synth.Q4_K, r.cuda(), e, *d) for r, d in zip(raw.raw, ((f, h), (f, h), (h, f)))]
+    i8 = [moe.DeviceBank.from_float((torch.randn(e, *d, generator=gen(i)) * 0.02).cuda()) for i, d in enumerate(((f, h), (f, h), (h, f)))]
+    banks = i8[:2] + q4[2:] if which == "gate" else q4[:2] + i8[2:]
+    layer = moe.MoeLayer.from_banks(shape, raw.router_w.cuda(), banks)
+    x = torch.randn(n, h, generator=gen(9)).bfloat16().cuda()
+    out = layer.forward(x)
+    art = layer.artefacts()
+    assert art["status"] == 0 and torch.equal(out, layer.forward(x))
+    # the parts: each side's product has the bits of a call of its own on what the layer handed it
+    plan = moe.dispatch(art["ids"].clone(), e)
+    if which == "gate":
+        assert torch.equal(moe.expert_gateup_swiglu(*banks[:2], x, plan), art["act"])
+    else:
+        assert torch.equal(moe.expert_down(banks[2], art["act"].clone(), plan), art["y"])
+    assert torch.equal(moe.combine(art["y"].clone(), art["weights"], n, k, h), out)
 
 
 @pytest.mark.parametrize("n,m,k", ((40, 300, 2560), (300, 300, 256), (1100, 4096, 2688)))

@@ -176,6 +176,7 @@ int per_group(int experts, long long rows) { return int(std::min<long long>(1 <<
 // x [n][cols]; the workspace holds the rows of the n tokens
 int32_t i8_gateup(const b2moe_bank * gate, const b2moe_bank * up, const b2moe_bank * shared_gate, const b2moe_bank * shared_up, const void * x, int x_dtype, const int * plan, int n,
                   int topk, int shared_tokens, long long live, void * act, int act_dtype, void * ws, void * rows_buf, size_t rows_buf_bytes, cudaStream_t s) {
+    if ((long long)n * topk > 0x3fffffffLL) return B2MOE_ERR_SHAPE;
     I8Args p = grouped(gate, up, shared_gate, shared_up, plan, n, topk, shared_tokens, act, act_dtype);
     const int total = n * topk + shared_tokens;
     if (i8_takes_gemm(gate->experts, live >= (long long)I8_GEMM_MIN_PER * gate->experts) && rows_buf_bytes >= i8_slot_bytes(total, gate->cols)) {
@@ -193,6 +194,7 @@ int32_t i8_gateup(const b2moe_bank * gate, const b2moe_bank * up, const b2moe_ba
 // x [assignments][cols] (per_token: [n][cols]); the workspace holds a row per assignment, in slot order
 int32_t i8_down(const b2moe_bank * down, const b2moe_bank * shared_down, const void * x, int x_dtype, bool per_token, const int * plan, int n, int topk, int shared_tokens, long long live,
                 void * y, int y_dtype, void * ws, cudaStream_t s) {
+    if ((long long)n * topk > 0x3fffffffLL) return B2MOE_ERR_SHAPE;
     I8Args p = grouped(down, nullptr, shared_down, nullptr, plan, n, topk, shared_tokens, y, y_dtype);
     const int total = n * topk + shared_tokens;
     const I8Rows rows = i8_rows(ws, total);

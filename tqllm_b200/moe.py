@@ -157,10 +157,10 @@ class Balance(NamedTuple):
     tokens: torch.Tensor
 
 
-def _balance_args(logits, mask, offsets):
+def _balance_args(logits, experts, mask, offsets):
     n = logits.shape[0]
-    if logits.dtype != torch.float32 or logits.stride(1) != 1:
-        raise capi.B2moeError(capi.ERR_SHAPE, "balance loss: float32 logits whose rows are contiguous are wanted")
+    if logits.dtype != torch.float32 or logits.shape[1] < experts or (logits.stride(1) != 1 and experts > 1):
+        raise capi.B2moeError(capi.ERR_SHAPE, "balance loss: float32 logits with contiguous rows of at least as many columns as experts are wanted")
     if mask is not None and (mask.numel() != n or mask.dtype not in (torch.bool, torch.uint8) or not mask.is_contiguous()):
         raise capi.B2moeError(capi.ERR_SHAPE, "balance loss: the mask has a byte for each token")
     if offsets is not None and (offsets.dtype != torch.int32 or offsets.numel() < 2 or not offsets.is_contiguous()):
@@ -170,7 +170,7 @@ def _balance_args(logits, mask, offsets):
 
 def balance_loss(logits, ids, experts, coef, gating=capi.SOFTMAX, mask=None, offsets=None) -> Balance:
     """The router's balance loss over logits [n, >= experts] and the ids [n, topk] that were routed (b2moe_balance_loss)."""
-    n, ld, seqs = _balance_args(logits, mask, offsets)
+    n, ld, seqs = _balance_args(logits, experts, mask, offsets)
     if ids.shape[0] != n or ids.dtype != torch.int32 or not ids.is_contiguous():
         raise capi.B2moeError(capi.ERR_SHAPE, "balance loss: contiguous int32 ids [n, topk] are wanted")
     new, ints = logits.new_empty, ids.new_empty
@@ -183,14 +183,14 @@ def balance_loss(logits, ids, experts, coef, gating=capi.SOFTMAX, mask=None, off
 
 def balance_loss_backward(logits, saved: Balance, topk, coef, gating=capi.SOFTMAX, mask=None, offsets=None, grad_loss=None, out=None):
     """The gradient of the balance loss on the logits, [n, experts]; into `out` (rows of at least `experts` columns) it is added."""
-    n, ld, seqs = _balance_args(logits, mask, offsets)
     experts = saved.counts.shape[1]
+    n, ld, seqs = _balance_args(logits, experts, mask, offsets)
     if saved.counts.shape[0] != seqs or (grad_loss is not None and grad_loss.dtype != torch.float32):
         raise capi.B2moeError(capi.ERR_SHAPE, "balance loss: the counts of the same sequences and a float32 gradient are wanted")
     grad = out
     if grad is None:
         grad = logits.new_empty((n, experts))
-    if grad.dtype != torch.float32 or grad.shape[0] != n or grad.shape[1] < experts or grad.stride(1) != 1:
+    if grad.dtype != torch.float32 or grad.shape[0] != n or grad.shape[1] < experts or (grad.stride(1) != 1 and experts > 1):
         raise capi.B2moeError(capi.ERR_SHAPE, "balance loss: the gradient has float32 rows like the logits")
     check(lib.b2moe_balance_loss_backward(gating, logits.data_ptr(), ld, topk, _ptr(mask), _ptr(offsets), seqs, experts, n, coef, saved.counts.data_ptr(),
                                           saved.tokens.data_ptr(), _ptr(grad_loss), grad.data_ptr(), grad.stride(0) if n > 1 else grad.shape[1], int(out is not None),
