@@ -268,7 +268,8 @@ B2MOE_API int32_t b2moe_combine_residual(const float * y, const int32_t * ids, c
                                int32_t out_dtype, b2moe_stream stream);
 
 /* ---- 8-bit integers with a scale for each row and each channel ------------------------------------------------------
- * They have no counterpart in the reference.
+ * The scale of a row is that of the reference's activation quantiser (quant_act_rows_k, src/formats/weight/quant_u4h.inc:790-821: the largest
+ * magnitude / 127); weights of 8 bits with a scale a channel are not among its GGUF types.
  * b2moe_quantize_rows: x [n][k] of x_dtype, rows ldx elements apart -> q int8, rows ldq bytes apart, and scale [n]:
  *   scale = max|x| / 127 (fp32), q = the integer nearest to 127 x / max|x|, halves to even, exactly. A row of zeros has
  *   scale 0; a row that holds an infinity or a NaN has a NaN as its scale (and with it in everything that is made of it). k and

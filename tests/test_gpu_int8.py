@@ -195,6 +195,8 @@ def experts_case(n, e, k, h, f, seed, shared=False, route="even"):
         ids[:, 0] = e - 1
     elif route == "none":
         ids[:] = -1
+    elif route == "twice":                                             # the same expert in several slots of a token
+        ids[:, 1:] = ids[:, :1]
     return torch.randn(n, h, generator=g), ids, banks, sh
 
 
@@ -215,7 +217,7 @@ SHAPES = [  # n, e, k, h, f, shared, route
     (1, 8, 2, 64, 16, False, "even"), (3, 5, 5, 80, 48, True, "even"), (7, 16, 4, 256, 144, False, "skip"), (9, 4, 2, 48, 80, True, "skip"),
     (40, 3, 1, 128, 64, False, "one"), (17, 40, 6, 1040, 272, False, "even"), (130, 4, 2, 192, 208, True, "even"), (300, 6, 3, 144, 128, False, "skip"),
     (260, 2, 1, 128, 336, False, "one"), (5, 8, 2, 64, 32, False, "none"), (700, 8, 4, 512, 256, True, "even"), (1, 2, 1, 16, 16, False, "even"),
-    (60, 6, 2, 2576, 80, True, "even"), (600, 3, 2, 2688, 208, False, "skip"),
+    (5, 4, 4, 64, 48, True, "twice"), (70, 3, 3, 128, 144, False, "twice"), (60, 6, 2, 2576, 80, True, "even"), (600, 3, 2, 2688, 208, False, "skip"),
 ]
 
 
@@ -301,6 +303,23 @@ def test_layer_on_8_bit_banks(n, gating, shared):
     want = moe.combine(y, art["weights"], n, k, h, st, art["shared_weights"] if shared else None)
     assert torch.equal(out, want) and torch.equal(out, again) and art["status"] == 0
     assert bool(torch.isfinite(out).all()) and bool(((with_res - out - res).abs() <= 2.0 ** -22 * (out.abs() + res.abs()) + 1e-30).all())
+
+
+@pytest.mark.parametrize("n", (3, 200))
+def test_a_plan_with_a_shared_expert_and_a_call_without(n):
+    """the shared expert's assignments are left alone"""
+    from tqllm_b200 import capi, moe
+    e, k, h, f = 4, 2, 128, 144
+    x, ids, banks, _ = experts_case(n, e, k, h, f, 2, route="skip")
+    dev = [moe.DeviceBank.from_int8(w.cuda(), v.cuda()) for w, v in banks]
+    shared, plain = moe.dispatch(ids.cuda(), e, n), moe.dispatch(ids.cuda(), e)
+    for family in ("decode", "gemm"):
+        with capi.family(family):
+            want = moe.expert_gateup_swiglu(dev[0], dev[1], x.cuda(), plain)
+            shared.shared_tokens = 0
+            got = moe.expert_gateup_swiglu(dev[0], dev[1], x.cuda(), shared)
+            assert torch.equal(got, want)
+            assert torch.equal(moe.expert_down(dev[2], want, shared), moe.expert_down(dev[2], want, plain))
 
 
 def test_per_matrix_calls():

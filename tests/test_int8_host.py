@@ -45,7 +45,7 @@ def test_quantize_refusals():
     assert [f(n=0), f(k=0), f(k=24), f(k=1 << 17, ldx=1 << 17, ldq=1 << 17), f(dt=3), f(ldx=56), f(ldx=68), f(ldq=48), f(ldq=72)] == [capi.ERR_SHAPE] * 9
     assert f(ldx=66, dt=capi.F32) == capi.ERR_SHAPE
     assert [f(x=None), f(q=None), f(s=None)] == [capi.ERR_NULL] * 3
-    assert [f(x=24), f(q=8)] == [capi.ERR_ALIGN] * 2
+    assert [f(x=24), f(q=8), f(s=18)] == [capi.ERR_ALIGN] * 3
 
 
 def test_linear_refusals():
@@ -53,7 +53,7 @@ def test_linear_refusals():
     one = bank(1)
     assert [f(bank(2)), f(one, n=0), f(one, dt=5), f(one, ldq=240), f(one, ldq=264), f(one, ldy=31), f(bank(1, cols=250)), f(bank(1, rows=0))] == [capi.ERR_SHAPE] * 8
     assert [f(one, q=None), f(one, s=None), f(one, y=None), f(bank(1, data=None)), f(bank(1, aux=None))] == [capi.ERR_NULL] * 5
-    assert [f(one, q=8), f(bank(1, data=24))] == [capi.ERR_ALIGN] * 2
+    assert [f(one, q=8), f(bank(1, data=24)), f(one, y=17), f(one, y=18, dt=capi.F32), f(one, s=18), f(bank(1, aux=18))] == [capi.ERR_ALIGN] * 6
     assert f(capi.Bank(16, None, 12, 1, 32, 256)) == capi.ERR_FORMAT
     assert lib.b2moe_linear_i8(16, 256, 16, None, 2, 16, 0, 32, None, None) == capi.ERR_NULL
 
@@ -77,12 +77,14 @@ def test_balance_refusals():
     assert bad == [capi.ERR_SHAPE] * len(bad)
     null = [loss(**{k: None}) for k in ("logits", "ids", "out", "counts", "prob", "tokens", "ws")]
     assert null == [capi.ERR_NULL] * len(null)
-    assert loss(ws=24) == capi.ERR_ALIGN and loss(size=lib.b2moe_balance_workspace_bytes(8, 4, 2) - 1) == capi.ERR_WORKSPACE
+    assert [loss(ws=24), loss(logits=18), loss(ids=18), loss(offsets=18), loss(counts=17), loss(prob=18), loss(tokens=18), loss(out=18)] == [capi.ERR_ALIGN] * 8
+    assert loss(size=lib.b2moe_balance_workspace_bytes(8, 4, 2) - 1) == capi.ERR_WORKSPACE
 
     def back(gating=1, logits=16, ld=8, topk=2, offsets=16, seqs=2, experts=8, n=4, counts=16, tokens=16, grad=16, ldg=8):
         return lib.b2moe_balance_loss_backward(gating, logits, ld, topk, None, offsets, seqs, experts, n, 0.1, counts, tokens, None, grad, ldg, 0, None)
     bad = [back(gating=5), back(ld=7), back(ldg=7), back(topk=9), back(offsets=None), back(seqs=0), back(experts=4097, ld=5000, ldg=5000), back(n=-1)]
     assert bad == [capi.ERR_SHAPE] * len(bad)
+    assert [back(**{k: 18}) for k in ("logits", "offsets", "counts", "tokens", "grad")] == [capi.ERR_ALIGN] * 5
     null = [back(**{k: None}) for k in ("logits", "counts", "tokens", "grad")]
     assert null == [capi.ERR_NULL] * len(null)
 

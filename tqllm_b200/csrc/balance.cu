@@ -417,7 +417,8 @@ extern "C" B2MOE_API int32_t b2moe_balance_loss(int32_t gating, const float * lo
                                                 b2moe_stream stream) {
     if (int32_t rc = bal_check(gating, ld, topk, offsets, sequences, experts, n)) return rc;
     if (!logits || !ids || !loss || !counts || !prob || !tokens || !workspace) return B2MOE_ERR_NULL;
-    if (!aligned16(workspace)) return B2MOE_ERR_ALIGN;
+    if (!aligned16(workspace) || !aligned_to(logits, 4) || !aligned_to(ids, 4) || !aligned_to(offsets, 4) || !aligned_to(loss, 4) || !aligned_to(counts, 4) || !aligned_to(prob, 4) ||
+        !aligned_to(tokens, 4)) return B2MOE_ERR_ALIGN;
     const BalSpace w = bal_space(experts, n, sequences);
     if (workspace_bytes < w.total) return B2MOE_ERR_WORKSPACE;
     char * base = static_cast<char *>(workspace);
@@ -441,6 +442,7 @@ extern "C" B2MOE_API int32_t b2moe_balance_loss_backward(int32_t gating, const f
     if (int32_t rc = bal_check(gating, ld, topk, offsets, sequences, experts, n)) return rc;
     if (ldg < experts) return B2MOE_ERR_SHAPE;
     if (!logits || !counts || !tokens || !grad_logits) return B2MOE_ERR_NULL;
+    if (!aligned_to(logits, 4) || !aligned_to(offsets, 4) || !aligned_to(counts, 4) || !aligned_to(tokens, 4) || !aligned_to(grad_loss, 4) || !aligned_to(grad_logits, 4)) return B2MOE_ERR_ALIGN;
     const BalBackArgs a{logits, ld, topk, mask, offsets, sequences, experts, n, bal_chunk(n), coef, counts, tokens, grad_loss, grad_logits, ldg, accumulate};
     return launch_rows<BackKernel>(a, gating, bal_chunks(n, sequences), [](int, int) { return size_t(0); }, as_stream(stream));
 }

@@ -72,7 +72,7 @@ int32_t check_bank(const b2moe_bank * b) {
     if (b->type == B2MOE_I8) {                                         // plain rows and a scale each: nothing of the block formats applies
         if (b->experts <= 0 || b->rows <= 0 || !i8_cols(b->cols)) return B2MOE_ERR_SHAPE;
         if (!b->data || !b->aux) return B2MOE_ERR_NULL;
-        return aligned16(b->data) ? B2MOE_OK : B2MOE_ERR_ALIGN;
+        return aligned16(b->data) && aligned_to(b->aux, 4) ? B2MOE_OK : B2MOE_ERR_ALIGN;
     }
     if (!fmt_info(b->type, f)) return B2MOE_ERR_FORMAT;
     if (b->experts <= 0 || b->rows <= 0 || b->cols <= 0 || b->cols % f.kt) return B2MOE_ERR_SHAPE;

@@ -57,6 +57,7 @@ __device__ __forceinline__ void bulk_g2s_first_out(uint32_t dst, const void * sr
                  ::"r"(dst), "l"(__cvta_generic_to_global(src)), "r"(bytes), "r"(bar), "l"(policy) : "memory");
 }
 inline bool aligned16(const void * p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+inline bool aligned_to(const void * p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 inline cudaStream_t as_stream(b2moe_stream s) { return static_cast<cudaStream_t>(s); }
 inline int ceil_div(int a, int b) { return (a + b - 1) / b; }
 inline size_t align_up(size_t v, size_t a) { return (v + a - 1) / a * a; }

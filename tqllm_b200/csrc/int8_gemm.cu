@@ -159,10 +159,11 @@ __global__ void __launch_bounds__(TC_THREADS, MODE ? 1 : 2) i8_gemm_k(const I8Ar
     grid_wait();
     grid_release();                                                    // after the wait: a down product behind this launch may read the plan above its own
     const int * counts = p.plan + PLAN_HDR, * offsets = counts + e1, * perm = offsets + e1 + 1 + e1;
+    const int ne = p.shared_w[0] ? e1 : p.experts;
     int tiles = c.tiles;
     if (p.plan) {
-        // inclusive prefix sums of the experts' tiles: a span of experts a thread
-        const int span = (e1 + TC_THREADS - 1) / TC_THREADS, lo = min(e1, int(threadIdx.x) * span), hi = min(e1, lo + span);
+        // inclusive prefix sums of the experts' tiles: a span of experts a thread (a call without a shared expert leaves that of the plan out)
+        const int span = (ne + TC_THREADS - 1) / TC_THREADS, lo = min(ne, int(threadIdx.x) * span), hi = min(ne, lo + span);
         int mine = 0;
         for (int e = lo; e < hi; ++e) mine += (counts[e] + c.nt - 1) / c.nt;
         int run = mine;
@@ -180,9 +181,9 @@ __global__ void __launch_bounds__(TC_THREADS, MODE ? 1 : 2) i8_gemm_k(const I8Ar
             ends[e] = run;
             offs[e] = offsets[e];
         }
-        if (threadIdx.x == 0) offs[e1] = offsets[e1];
+        if (threadIdx.x == 0) offs[ne] = offsets[ne];
         __syncthreads();
-        tiles = ends[e1 - 1];
+        tiles = ends[ne - 1];
     }
     // an item: a tile of activation rows and a block (PAIR: two) of weight rows; the blocks of a pair walk the same items
     const int item_blocks = PAIR ? (c.row_blocks + 1) / 2 : c.row_blocks, it0 = PAIR ? blockIdx.x >> 1 : blockIdx.x, it_step = PAIR ? gridDim.x >> 1 : gridDim.x;
@@ -197,7 +198,7 @@ __global__ void __launch_bounds__(TC_THREADS, MODE ? 1 : 2) i8_gemm_k(const I8Ar
         im.first = 0;
         im.count = p.n;
         if (p.plan) {
-            int lo = 0, hi = e1 - 1;                                   // the first expert whose tiles end behind this one
+            int lo = 0, hi = ne - 1;                                   // the first expert whose tiles end behind this one
             while (lo < hi) {
                 const int mid = (lo + hi) >> 1;
                 if (ends[mid] > tile) hi = mid;

@@ -24,6 +24,7 @@ __device__ __forceinline__ uint4 load_stream(const int8_t * p) {
     asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(__cvta_generic_to_global(p)));
     return r;
 }
+
 // A few tokens per expert: bound by streaming the weights. A block takes 16 weight rows of one expert (of both matrices with MATS = 2) and all the
 // expert's tokens, 8 NT at a time; its warps share the columns in pieces of 64, 16 bytes a lane and row, straight from memory into the fragments of the tensor
 // core: lane (g, t) holds bytes 16 t.. of rows g and g + 8, so word i of both operands stands for the same four columns, which is all that a sum over columns needs.
@@ -48,6 +49,7 @@ __global__ void __launch_bounds__(256) i8_stream_k(const I8Args p) {
         perm = p.plan + PLAN_HDR + 3 * e1 + 1 + first;
     }
     const bool shared = p.plan && e == p.experts;
+    if (shared && !p.shared_w[0]) return;                              // a plan with a shared expert, a call without one
     const int rg = min(r0 + g, p.rows - 1), rh = min(r0 + g + 8, p.rows - 1);
     const int8_t * wg[MATS], * wh[MATS];
     const float * v[MATS];
@@ -230,7 +232,7 @@ extern "C" B2MOE_API int32_t b2moe_linear_i8(const int8_t * q, int64_t ldq, cons
     if (w->type != B2MOE_I8) return B2MOE_ERR_FORMAT;
     if (n <= 0 || w->experts != 1 || !valid_dtype(y_dtype) || ldq < w->cols || ldq % 16 || ldy < w->rows) return B2MOE_ERR_SHAPE;
     if (!q || !scale || !y) return B2MOE_ERR_NULL;
-    if (!aligned16(q)) return B2MOE_ERR_ALIGN;
+    if (!aligned16(q) || !aligned_to(y, dtype_bytes(y_dtype)) || !aligned_to(scale, 4) || !aligned_to(status, 4)) return B2MOE_ERR_ALIGN;
     I8Args p{};
     p.w[0] = static_cast<const int8_t *>(w->data); p.v[0] = static_cast<const float *>(w->aux);
     p.experts = 1; p.rows = w->rows; p.cols = w->cols;

@@ -156,6 +156,7 @@ __global__ void __launch_bounds__(256) quant_rows_k(const QuantArgs p) {
     if (!SCATTER && p.plan) {
         if (i >= p.plan[PLAN_NGROUPED]) return;
         const int a = perm[i];
+        if (a >= p.assignments && !p.shared) return;                   // a plan with a shared expert, a call without one
         src = !p.per_token ? a : a < p.assignments ? a / p.topk : a - p.assignments;
     } else if (i >= p.n) {
         return;
@@ -268,7 +269,7 @@ int32_t i8_quantize(const void * x, int x_dtype, long long ldx, int n, int k, in
 }
 int32_t i8_quantize_slots(const void * x, int x_dtype, bool per_token, int n, int k, const I8Rows & rows, const int * plan, int experts, int topk, int shared_tokens, cudaStream_t s) {
     const int A = n * topk;
-    return quantize<false>(QuantArgs{x, k, k, A + shared_tokens, k, rows.q, rows.scale, plan, experts, A, topk, per_token}, x_dtype, s);
+    return quantize<false>(QuantArgs{x, k, k, A + shared_tokens, k, rows.q, rows.scale, plan, experts, A, topk, per_token, shared_tokens ? 1 : 0}, x_dtype, s);
 }
 int32_t i8_quantize_scatter(const void * x, int x_dtype, int n, int k, const I8Rows & rows, int * inverse, const int * plan, int experts, int topk, int shared_tokens, cudaStream_t s) {
     launch_overlapped(inverse_k, dim3(ceil_div(n * topk + shared_tokens, 256)), dim3(256), 0, s, plan, experts, inverse);
@@ -284,6 +285,6 @@ extern "C" B2MOE_API int32_t b2moe_quantize_rows(const void * x, int32_t x_dtype
                                                  b2moe_stream stream) {
     if (n <= 0 || !i8_cols(k) || !valid_dtype(x_dtype) || ldx < k || ldx % (x_dtype == B2MOE_F32 ? 4 : 8) || ldq < k || ldq % 16) return B2MOE_ERR_SHAPE;
     if (!x || !q || !scale) return B2MOE_ERR_NULL;
-    if (!aligned16(x) || !aligned16(q)) return B2MOE_ERR_ALIGN;
+    if (!aligned16(x) || !aligned16(q) || !aligned_to(scale, 4)) return B2MOE_ERR_ALIGN;
     return i8_quantize(x, x_dtype, ldx, n, k, q, ldq, scale, as_stream(stream));
 }
