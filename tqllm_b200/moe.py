@@ -127,25 +127,32 @@ def route_sigmoid(logits, experts, k, bias=None, norm=True, scale=0.0):
 def quantize_rows(x: torch.Tensor):
     """(q int8 [n, k], scale float32 [n]) of the rows of x (b2moe_quantize_rows); x may be rows of a wider matrix"""
     n, k = x.shape
-    if x.stride(1) != 1 and k > 1:
+    ldx, one = x.stride()
+    if one != 1 and k > 1:
         raise capi.B2moeError(capi.ERR_SHAPE, "quantize_rows: the values of a row have to be neighbours")
     q = torch.empty(n, k, dtype=torch.int8, device=x.device)
     scale = torch.empty(n, dtype=torch.float32, device=x.device)
-    check(lib.b2moe_quantize_rows(x.data_ptr(), _DT[x.dtype], x.stride(0) if n > 1 else k, n, k, q.data_ptr(), k, scale.data_ptr(), _stream()), "b2moe_quantize_rows")
+    check(lib.b2moe_quantize_rows(x.data_ptr(), _DT[x.dtype], ldx if n > 1 else k, n, k, q.data_ptr(), k, scale.data_ptr(), _stream()), "b2moe_quantize_rows")
     return q, scale
 
 
 def linear_i8(q: torch.Tensor, scale: torch.Tensor, bank: DeviceBank, out_dtype=torch.bfloat16, out: torch.Tensor | None = None, status: torch.Tensor | None = None):
     """y [n, rows] = (q . w) * scale[t] * bank scale[r] of 8-bit rows (b2moe_linear_i8); q and out may be rows of wider matrices"""
     n, k = q.shape
-    if out is None:
-        out = torch.empty(n, bank.rows, dtype=out_dtype, device=q.device)
-    if q.dtype != torch.int8 or k != bank.cols or scale.dtype != torch.float32 or scale.numel() != n or not scale.is_contiguous() or out.shape != (n, bank.rows):
-        raise capi.B2moeError(capi.ERR_SHAPE, "linear_i8: int8 rows of the bank's columns, a float32 scale for each, and an output [n, rows] are wanted")
-    if (q.stride(1) != 1 and k > 1) or (out.stride(1) != 1 and bank.rows > 1):
+    ldq, one = q.stride()
+    ldy = rows = bank.rows
+    if q.dtype is not torch.int8 or k != bank.cols or scale.dtype is not torch.float32 or scale.numel() != n or not scale.is_contiguous():
+        raise capi.B2moeError(capi.ERR_SHAPE, "linear_i8: int8 rows of the bank's columns and a float32 scale for each are wanted")
+    if one != 1 and k > 1:
         raise capi.B2moeError(capi.ERR_SHAPE, "linear_i8: the values of a row have to be neighbours")
-    check(lib.b2moe_linear_i8(q.data_ptr(), q.stride(0) if n > 1 else k, scale.data_ptr(), C.byref(bank.c), n, out.data_ptr(), _DT[out.dtype],
-                              out.stride(0) if n > 1 else bank.rows, _ptr(status), _stream()), "b2moe_linear_i8")
+    if out is None:
+        out = torch.empty(n, rows, dtype=out_dtype, device=q.device)
+    elif out.shape != (n, rows) or (out.stride(1) != 1 and rows > 1):
+        raise capi.B2moeError(capi.ERR_SHAPE, "linear_i8: an output [n, rows] with contiguous rows is wanted")
+    else:
+        out_dtype = out.dtype
+        ldy = out.stride(0) if n > 1 else rows
+    check(lib.b2moe_linear_i8(q.data_ptr(), ldq if n > 1 else k, scale.data_ptr(), C.byref(bank.c), n, out.data_ptr(), _DT[out_dtype], ldy, _ptr(status), _stream()), "b2moe_linear_i8")
     return out
 
 
@@ -158,43 +165,50 @@ class Balance(NamedTuple):
 
 
 def _balance_args(logits, experts, mask, offsets):
-    n = logits.shape[0]
-    if logits.dtype != torch.float32 or logits.shape[1] < experts or (logits.stride(1) != 1 and experts > 1):
+    n, cols = logits.shape
+    ld, one = logits.stride()
+    if logits.dtype is not torch.float32 or cols < experts or (one != 1 and experts > 1):
         raise capi.B2moeError(capi.ERR_SHAPE, "balance loss: float32 logits with contiguous rows of at least as many columns as experts are wanted")
     if mask is not None and (mask.numel() != n or mask.dtype not in (torch.bool, torch.uint8) or not mask.is_contiguous()):
         raise capi.B2moeError(capi.ERR_SHAPE, "balance loss: the mask has a byte for each token")
-    if offsets is not None and (offsets.dtype != torch.int32 or offsets.numel() < 2 or not offsets.is_contiguous()):
+    if offsets is None:
+        return n, ld if n > 1 else cols, 1
+    sequences = offsets.numel() - 1
+    if offsets.dtype is not torch.int32 or sequences < 1 or not offsets.is_contiguous():
         raise capi.B2moeError(capi.ERR_SHAPE, "balance loss: the offsets are int32, one more than sequences")
-    return n, logits.stride(0) if n > 1 else logits.shape[1], 1 if offsets is None else offsets.numel() - 1
+    return n, ld if n > 1 else cols, sequences
 
 
 def balance_loss(logits, ids, experts, coef, gating=capi.SOFTMAX, mask=None, offsets=None) -> Balance:
     """The router's balance loss over logits [n, >= experts] and the ids [n, topk] that were routed (b2moe_balance_loss)."""
     n, ld, seqs = _balance_args(logits, experts, mask, offsets)
-    if ids.shape[0] != n or ids.dtype != torch.int32 or not ids.is_contiguous():
+    tokens, topk = ids.shape
+    if tokens != n or ids.dtype is not torch.int32 or not ids.is_contiguous():
         raise capi.B2moeError(capi.ERR_SHAPE, "balance loss: contiguous int32 ids [n, topk] are wanted")
     new, ints = logits.new_empty, ids.new_empty
     out = Balance(new(()), ints((seqs, experts)), new((seqs, experts)), ints(seqs + 1))
-    ws = new(max(4, lib.b2moe_balance_workspace_bytes(experts, n, seqs) // 4))
-    check(lib.b2moe_balance_loss(gating, logits.data_ptr(), ld, ids.data_ptr(), ids.shape[1], _ptr(mask), _ptr(offsets), seqs, experts, n, coef, out.loss.data_ptr(),
-                                 out.counts.data_ptr(), out.prob.data_ptr(), out.tokens.data_ptr(), ws.data_ptr(), 4 * ws.numel(), _stream()), "b2moe_balance_loss")
+    size = lib.b2moe_balance_workspace_bytes(experts, n, seqs)
+    ws = new(max(4, size // 4))
+    check(lib.b2moe_balance_loss(gating, logits.data_ptr(), ld, ids.data_ptr(), topk, _ptr(mask), _ptr(offsets), seqs, experts, n, coef, out.loss.data_ptr(),
+                                 out.counts.data_ptr(), out.prob.data_ptr(), out.tokens.data_ptr(), ws.data_ptr(), size, _stream()), "b2moe_balance_loss")
     return out
 
 
 def balance_loss_backward(logits, saved: Balance, topk, coef, gating=capi.SOFTMAX, mask=None, offsets=None, grad_loss=None, out=None):
     """The gradient of the balance loss on the logits, [n, experts]; into `out` (rows of at least `experts` columns) it is added."""
-    experts = saved.counts.shape[1]
+    counted, experts = saved.counts.shape
     n, ld, seqs = _balance_args(logits, experts, mask, offsets)
-    if saved.counts.shape[0] != seqs or (grad_loss is not None and grad_loss.dtype != torch.float32):
+    if counted != seqs or (grad_loss is not None and grad_loss.dtype is not torch.float32):
         raise capi.B2moeError(capi.ERR_SHAPE, "balance loss: the counts of the same sequences and a float32 gradient are wanted")
-    grad = out
+    grad, ldg = out, experts
     if grad is None:
         grad = logits.new_empty((n, experts))
-    if grad.dtype != torch.float32 or grad.shape[0] != n or grad.shape[1] < experts or (grad.stride(1) != 1 and experts > 1):
+    elif grad.dtype is not torch.float32 or grad.shape[0] != n or grad.shape[1] < experts or (grad.stride(1) != 1 and experts > 1):
         raise capi.B2moeError(capi.ERR_SHAPE, "balance loss: the gradient has float32 rows like the logits")
+    else:
+        ldg = grad.stride(0) if n > 1 else grad.shape[1]
     check(lib.b2moe_balance_loss_backward(gating, logits.data_ptr(), ld, topk, _ptr(mask), _ptr(offsets), seqs, experts, n, coef, saved.counts.data_ptr(),
-                                          saved.tokens.data_ptr(), _ptr(grad_loss), grad.data_ptr(), grad.stride(0) if n > 1 else grad.shape[1], int(out is not None),
-                                          _stream()), "b2moe_balance_loss_backward")
+                                          saved.tokens.data_ptr(), _ptr(grad_loss), grad.data_ptr(), ldg, int(out is not None), _stream()), "b2moe_balance_loss_backward")
     return grad
 
 
