@@ -236,8 +236,9 @@ void launch_quant(const QuantArgs & a, cudaStream_t s) {
     auto go = [&](auto kernel, int blocks, int threads) { launch_overlapped(kernel, dim3(blocks), dim3(threads), 0, s, a); };
     const int pieces = a.k / 16, by_warp = ceil_div(pieces, 32);
     // Many rows (they fill the SMs with 16 warps each): four pieces a thread, a warp a row where that does. 8192 x 4096 bf16 with 256 / 128 / 64 threads a row 28.6 / 22.2 / 18.5 us,
-    // 40960 x 512 fp32 with a warp a block / eight warps of a row each 43.4 / 19.2
-    if (a.n >= 148 * 16) {
+    // 40960 x 512 fp32 with a warp a block / eight warps of a row each 43.4 / 19.2. Rows that are written to several slots have more stores than loads and take the other shape (4096 x 2048 to ten slots
+    // each 26 / 18)
+    if (!SCATTER && a.n >= 148 * 16) {
         const int blocks = ceil_div(a.n, 8);
         if (by_warp == 1) return go(quant_rows_k<DT, 1, true, SCATTER>, blocks, 256);
         if (by_warp == 2) return go(quant_rows_k<DT, 2, true, SCATTER>, blocks, 256);
