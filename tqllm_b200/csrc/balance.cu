@@ -17,7 +17,7 @@
 namespace b2 {
 namespace {
 
-constexpr int BAL_THREADS = 256, BAL_WARPS = BAL_THREADS / 32, BAL_MAX_EXPERTS = 4096, SUM_COLS = 32, SUM_ROWS = 16, SUM_ASK = 8;
+constexpr int ALONE_THREADS = 512, BAL_THREADS = 256, BAL_WARPS = BAL_THREADS / 32, BAL_MAX_EXPERTS = 4096, SUM_COLS = 32, SUM_ROWS = 16, SUM_ASK = 8;
 
 struct BalArgs {
     const float * logits;
@@ -119,9 +119,10 @@ struct Row {
 // column sums of a warp's rows stay in registers until the chunk is through.
 // ALONE: a batch of one sequence and a few tokens is one block's, which writes the results itself.
 template <int V, int G, bool SIGMOID, bool ALONE>
-__global__ void __launch_bounds__(BAL_THREADS) balance_rows_k(const BalArgs p) {
-    extern __shared__ float cols[];                                    // [BAL_WARPS / G][experts], then the counters; ALONE: the counters behind them
-    __shared__ float red[BAL_WARPS];
+__global__ void __launch_bounds__(ALONE ? ALONE_THREADS : BAL_THREADS) balance_rows_k(const BalArgs p) {
+    extern __shared__ float cols[];                                    // [WARPS / G][experts], then the counters; ALONE: the counters behind them
+    constexpr int THREADS = ALONE ? ALONE_THREADS : BAL_THREADS, WARPS = THREADS / 32;
+    __shared__ float red[WARPS];
     grid_release();
     grid_wait();
     int3 c;
@@ -134,7 +135,7 @@ __global__ void __launch_bounds__(BAL_THREADS) balance_rows_k(const BalArgs p) {
         if (c.x < 0) return;
     }
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, group = warp / G;
-    constexpr int ROWS = BAL_WARPS / G;
+    constexpr int ROWS = WARPS / G;
     Row<V, G> row;
     row.red = red;
     row.first = (warp % G) * 32 + lane;
@@ -158,7 +159,7 @@ __global__ void __launch_bounds__(BAL_THREADS) balance_rows_k(const BalArgs p) {
         if (row.first + 32 * G * i < p.experts) cols[size_t(group) * p.experts + row.first + 32 * G * i] = acc[i];
     __syncthreads();
     if (!ALONE) {
-        for (int e = threadIdx.x; e < p.experts; e += BAL_THREADS) {
+        for (int e = threadIdx.x; e < p.experts; e += THREADS) {
             float sum = cols[e];
 #pragma unroll
             for (int i = 1; i < ROWS; ++i) sum += cols[size_t(i) * p.experts + e];
@@ -167,9 +168,9 @@ __global__ void __launch_bounds__(BAL_THREADS) balance_rows_k(const BalArgs p) {
         __syncthreads();
     }
     int * hist = reinterpret_cast<int *>(cols) + (ALONE ? ROWS * p.experts : 0);
-    for (int e = threadIdx.x; e < p.experts; e += BAL_THREADS) hist[e] = 0;
+    for (int e = threadIdx.x; e < p.experts; e += THREADS) hist[e] = 0;
     __syncthreads();
-    for (long long i = (long long)c.y * p.topk + threadIdx.x; i < (long long)c.z * p.topk; i += BAL_THREADS) {
+    for (long long i = (long long)c.y * p.topk + threadIdx.x; i < (long long)c.z * p.topk; i += THREADS) {
         const int id = p.ids[i];
         if (id >= 0 && id < p.experts && !(p.mask && !p.mask[i / p.topk])) atomicAdd(&hist[id], 1);      // whole numbers: any order gives the same
     }
@@ -177,7 +178,7 @@ __global__ void __launch_bounds__(BAL_THREADS) balance_rows_k(const BalArgs p) {
     const int tokens = __syncthreads_count(mine < c.z && !(p.mask && !p.mask[mine]));
     if (ALONE) {
         float dot = 0.f;
-        for (int e = threadIdx.x; e < p.experts; e += BAL_THREADS) {
+        for (int e = threadIdx.x; e < p.experts; e += THREADS) {
             float sum = cols[e];
 #pragma unroll
             for (int i = 1; i < ROWS; ++i) sum += cols[size_t(i) * p.experts + e];
@@ -192,7 +193,7 @@ __global__ void __launch_bounds__(BAL_THREADS) balance_rows_k(const BalArgs p) {
         __syncthreads();
         if (threadIdx.x == 0) {
             dot = 0.f;
-            for (int w = 0; w < BAL_WARPS; ++w) dot += red[w];
+            for (int w = 0; w < WARPS; ++w) dot += red[w];
             p.tokens[0] = tokens;
             p.tokens[1] = tokens > 0;
             *p.loss = tokens ? float(double(p.coef) * p.experts / p.topk * (double(dot) / double(tokens))) : 0.f;
@@ -200,7 +201,7 @@ __global__ void __launch_bounds__(BAL_THREADS) balance_rows_k(const BalArgs p) {
         return;
     }
     if (threadIdx.x == 0) p.part_tokens[blockIdx.x] = tokens;
-    for (int e = threadIdx.x; e < p.experts; e += BAL_THREADS) p.part_count[size_t(blockIdx.x) * p.experts + e] = hist[e];
+    for (int e = threadIdx.x; e < p.experts; e += THREADS) p.part_count[size_t(blockIdx.x) * p.experts + e] = hist[e];
 }
 
 // One block per sequence and SUM_COLS experts adds the chunks up; the last block of all adds the sequences.
@@ -356,12 +357,12 @@ inline int bal_chunk(int n) { return 8 * std::min(16, std::max(1, ceil_div(n, 14
 inline long long bal_chunks(int n, int sequences) { return n / bal_chunk(n) + (long long)sequences; }
 
 template <template <int, int, bool> class K, class Args>
-int32_t launch_rows(const Args & a, int gating, long long chunks, size_t (*smem)(int, int), cudaStream_t s) {
+int32_t launch_rows(const Args & a, int gating, long long chunks, int threads, size_t (*smem)(int, int), cudaStream_t s) {
     auto go = [&](auto v, auto g) {
         constexpr int V = decltype(v)::value, G = decltype(g)::value;
         const size_t bytes = smem(a.experts, G);
-        if (gating == B2MOE_SIGMOID) launch_overlapped(K<V, G, true>::fn(), dim3(unsigned(chunks)), dim3(BAL_THREADS), bytes, s, a);
-        else launch_overlapped(K<V, G, false>::fn(), dim3(unsigned(chunks)), dim3(BAL_THREADS), bytes, s, a);
+        if (gating == B2MOE_SIGMOID) launch_overlapped(K<V, G, true>::fn(), dim3(unsigned(chunks)), dim3(threads), bytes, s, a);
+        else launch_overlapped(K<V, G, false>::fn(), dim3(unsigned(chunks)), dim3(threads), bytes, s, a);
         return launch_status();
     };
     using std::integral_constant;
@@ -427,10 +428,10 @@ extern "C" B2MOE_API int32_t b2moe_balance_loss(int32_t gating, const float * lo
                     reinterpret_cast<float *>(base + w.prob), reinterpret_cast<int *>(base + w.count), reinterpret_cast<int *>(base + w.tokens),
                     reinterpret_cast<float *>(base + w.dots), reinterpret_cast<int *>(base + w.ticket), loss, prob, counts, tokens};
     cudaStream_t s = as_stream(stream);
-    // one launch in place of two: 48 tokens of 32 experts, loss and gradient 12.4 -> 8.3 us. Eight rows a warp at most; the counters fit behind the sums up to 2048 experts
-    if (sequences == 1 && n <= 8 * BAL_WARPS && experts <= 2048)
-        return launch_rows<AloneKernel>(a, gating, 1, [](int e, int g) { return size_t(BAL_WARPS / g + 1) * e * sizeof(float); }, s);
-    if (int32_t rc = launch_rows<RowsKernel>(a, gating, chunks, [](int e, int g) { return size_t(BAL_WARPS / g) * e * sizeof(float); }, s)) return rc;
+    // one launch in place of two: 48 tokens of 32 experts, loss and gradient 12.4 -> 8.3 us (the launch alone 4.6 us with eight warps, 3.6 with sixteen). Four rows a warp at most; the counters fit behind the sums up to 2048 experts
+    if (sequences == 1 && n <= 64 && experts <= 2048)
+        return launch_rows<AloneKernel>(a, gating, 1, ALONE_THREADS, [](int e, int g) { return size_t(ALONE_THREADS / 32 / g + 1) * e * sizeof(float); }, s);
+    if (int32_t rc = launch_rows<RowsKernel>(a, gating, chunks, BAL_THREADS, [](int e, int g) { return size_t(BAL_WARPS / g) * e * sizeof(float); }, s)) return rc;
     launch_overlapped(balance_sum_k, dim3(ceil_div(experts, SUM_COLS), sequences), dim3(SUM_COLS * SUM_ROWS), 0, s, a);
     return launch_status();
 }
@@ -444,5 +445,5 @@ extern "C" B2MOE_API int32_t b2moe_balance_loss_backward(int32_t gating, const f
     if (!logits || !counts || !tokens || !grad_logits) return B2MOE_ERR_NULL;
     if (!aligned_to(logits, 4) || !aligned_to(offsets, 4) || !aligned_to(counts, 4) || !aligned_to(tokens, 4) || !aligned_to(grad_loss, 4) || !aligned_to(grad_logits, 4)) return B2MOE_ERR_ALIGN;
     const BalBackArgs a{logits, ld, topk, mask, offsets, sequences, experts, n, bal_chunk(n), coef, counts, tokens, grad_loss, grad_logits, ldg, accumulate};
-    return launch_rows<BackKernel>(a, gating, bal_chunks(n, sequences), [](int, int) { return size_t(0); }, as_stream(stream));
+    return launch_rows<BackKernel>(a, gating, bal_chunks(n, sequences), BAL_THREADS, [](int, int) { return size_t(0); }, as_stream(stream));
 }
