@@ -28,6 +28,8 @@ constexpr int TC_A_BYTES = 128 * 128, TC_SMEM = 227 * 1024, TC_MAX_SPLIT = 8;
 struct TcMaps { CUtensorMap a[2], shared[2], b; };
 struct TcArgs {
     int nt, box, stages, row_blocks, tiles;     // activation rows of an item, of a copy; ring; blocks of weight rows; items of a dense call in the row direction
+    int half;                                   // columns of an accumulator
+    int b_rows;                                 // a block's copies of an item's rows
     uint32_t tmem_cols;
     int * status;
     int drop;                                   // test hook: the copies of this step of every block are left out (-1: none)
@@ -133,7 +135,7 @@ __global__ void __launch_bounds__(TC_THREADS, MODE ? 1 : 2) i8_gemm_k(const I8Ar
     constexpr bool SPLIT = MODE == TC_SPLIT, PAIR = MODE == TC_PAIR;
     namespace cg = cooperative_groups;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rank = PAIR ? blockIdx.x & 1 : 0;
-    const uint32_t stage_bytes = TC_A_BYTES + c.nt * (PAIR ? 64 : 128);
+    const uint32_t stage_bytes = TC_A_BYTES + c.b_rows * 128;
     uint8_t * const ring = tc_mem + (1024u - (saddr(tc_mem) & 1023u)) % 1024u;
     const int e1 = p.experts + 1;
     int * const ends = reinterpret_cast<int *>(ring + size_t(c.stages) * stage_bytes), * const offs = ends + e1;      // tiles up to and with expert e, its first slot
@@ -282,7 +284,7 @@ __global__ void __launch_bounds__(TC_THREADS, MODE ? 1 : 2) i8_gemm_k(const I8Ar
         bool ok = true;
 #pragma unroll 1
         for (int it = it0; it < items && ok && !abort_flag; it += it_step, ++done) {
-            const uint32_t h = done & 1u, d = tmem + h * c.nt, count = __shfl_sync(0xffffffffu, locate(it).count, 0);
+            const uint32_t h = done & 1u, d = tmem + h * c.half, count = __shfl_sync(0xffffffffu, locate(it).count, 0);
             const uint32_t id = PAIR ? idesc_i8(256, (count + 2 * c.box - 1) / (2 * c.box) * (2 * c.box)) : idesc_i8(128, (count + 15) & ~15u);
             if (done >= 2 && !warp_wait(acc_empty + 8 * h, ((done >> 1) - 1) & 1u)) { ok = false; break; }
             fence_after();
@@ -363,7 +365,7 @@ __global__ void __launch_bounds__(TC_THREADS, MODE ? 1 : 2) i8_gemm_k(const I8Ar
             ok = ok && !abort_flag && warp_wait(acc_full + 8 * h, (done >> 1) & 1u);
             fence_after();
             if (ok) {
-                const uint32_t taddr = tmem + h * c.nt + (uint32_t(32 * quarter) << 16);
+                const uint32_t taddr = tmem + h * c.half + (uint32_t(32 * quarter) << 16);
                 if (p.y_dtype == B2MOE_F32) store_item<MATS, float>(p, im, taddr, table[h], scale, quarter, half, lane);
                 else if (p.y_dtype == B2MOE_F16) store_item<MATS, __half>(p, im, taddr, table[h], scale, quarter, half, lane);
                 else store_item<MATS, __nv_bfloat16>(p, im, taddr, table[h], scale, quarter, half, lane);
@@ -483,6 +485,26 @@ int split_of(long long items, int steps) {
     return split;
 }
 
+// Activation rows of an item of a dense call: the rows are cut alike into the number of tiles that is expected to cost least. In steps of an item of 256 rows: a round of items takes its steps
+// in proportion to 128 + rows (its weights, its rows), those that share columns meet for six of 128 rows. us, with items of 128 or 256 rows / cut alike: 515 rows of 4096 x 4096 21.9 / 15.4, 1000
+// 24.7 / 18.3, 1500 27.3 / 25.7; 2100 of 1411 x 2560 17.6 / 13.0; 1500 of 4096 x 1408 17.6 / 15.0; 515 of 4096 x 512 6.4 / 5.6
+int dense_rows(int n, int row_blocks, int steps, bool longer, bool two, int sms) {
+    const int most = two ? 128 : 256, least = two ? 32 : 96, first = ceil_div(n, most);
+    int best = most;
+    float cost = 1e30f;
+    for (int tiles = first; tiles <= std::max(first + 8, ceil_div(n, least)); ++tiles) {
+        const int rows = (ceil_div(n, tiles) + 15) / 16 * 16;
+        if (rows < least && tiles > first) break;
+        const bool pair = longer && rows > 128;
+        const long long items = (long long)ceil_div(n, rows) * (pair ? ceil_div(row_blocks, 2) : row_blocks), at_once = pair ? sms / 2 : two ? 2 * sms : sms;
+        const int split = split_of((long long)ceil_div(n, rows) * row_blocks, steps);
+        const float each = float(128 + (pair ? (rows + 63) / 64 * 64 : rows)) / 384.f;
+        const float c = split > 1 ? float(steps) / split * each + 6.f * rows / 128.f : float((items + at_once - 1) / at_once) * steps * each;
+        if (c < cost) { cost = c; best = rows; }
+    }
+    return best;
+}
+
 }  // namespace
 
 void i8_drop_step(int step) { g_drop_step = step; }
@@ -494,31 +516,30 @@ int32_t i8_gemm(const I8Args & p, long long q_rows, int per_group, int * status,
     c.row_blocks = ceil_div(p.rows, MATS == 2 ? 64 : 128);
     // Items of 256 rows halve what the weights cost in copies and products (8192 x 4096 x 4096: 96 us, with 128 rows 150), items of 128 leave room for six ring
     // stages instead of four and waste less where an expert has fewer (512 experts at 80 each, gate/up 211 against 225 us; 128 experts at 128 each with a
-    // skewed load 385 and 333); below that nothing is gained (64 rows, 16 each: 248 and 242). A dense call takes the large ones where they fill the SMs (256 rows of 4096 x 4096: 17.5 us in items of 256,
-    // 14.0 of 128). Pairs pay from long rows on, where the products of an item outlast what its blocks tell each other: us, single / pair: 8192 x 4096 rows of 4096 columns 96.5 / 87.1, of 2048 59.6 / 60.3,
+    // skewed load 385 and 333); below that nothing is gained (64 rows, 16 each: 248 and 242). Pairs pay from long rows on, where the products of an item outlast what its blocks tell each other: us, single / pair: 8192 x 4096 rows of 4096 columns 96.5 / 87.1, of 2048 59.6 / 60.3,
     // of 1024 49.1 / 53.6; 8192 x 8192 of 8192 378.6 / 353.0; gate/up, 128 experts of 4096 columns at 16 each 248.5 (items of 128) / 246.2, at 160 344.9 / 326.2, at 320 613 / 584; 512 of 2048 at 160 304 / 318;
     // down, 512 of 512 columns at 80 193 / 242
     // Short rows: two blocks an SM with half the ring each, since an item of a few steps takes longer from its first copy to its last store than its copies alone, and one block's items hide
     // behind the other's. us, one / two: down, 512 experts of 512 columns at one row each 76 / 60, at 80 192 / 178, at 320 650 / 498, of 768 columns at 40 64 / 67; gate/up of 512 columns at 8 107 / 78;
-    // dense 8192 rows, 4096 x 512 44 / 36, 4096 x 1024 49 / 42; gate/up of 2048 columns at 80 242 / 258. A dense call takes smaller items then where those fill more of the SMs (256 rows 6.2 / 5.0)
+    // dense 8192 rows, 4096 x 512 44 / 36, 4096 x 1024 49 / 42; gate/up of 2048 columns at 80 242 / 258.
     const int sms = sm_count();
     const bool longer = p.cols > 2560, two = p.cols <= I8_SHORT_COLS;
-    if (two) {
-        c.nt = 128;
-        while (!p.plan && c.nt > 32 && (long long)ceil_div(p.n, c.nt) * c.row_blocks < sms) c.nt /= 2;
-    } else {
-        c.nt = p.plan ? (per_group > 96 || longer ? 256 : 128) : (long long)ceil_div(p.n, 256) * c.row_blocks >= sms ? 256 : 128;
-    }
+    if (p.plan) c.nt = two ? 128 : per_group > 96 || longer ? 256 : 128;
+    else c.nt = dense_rows(p.n, c.row_blocks, ceil_div(p.cols, 128), longer, two, sms);
     c.tiles = p.plan ? 0 : ceil_div(p.n, c.nt);
     // A dense call with few items: as many blocks an item as run at once
     const int split = MATS == 1 && !p.plan ? split_of((long long)c.tiles * c.row_blocks, ceil_div(p.cols, 128)) : 1;
-    const bool pair = split == 1 && longer && c.nt == 256;
+    const bool pair = split == 1 && longer && c.nt > 128;
     c.box = pair || two ? 32 : 64;                                     // rows of a copy: an item takes as many copies as it has rows for
-    c.tmem_cols = std::max(32, 2 * c.nt);
+    c.tmem_cols = 32;
+    while (c.tmem_cols < 2 * uint32_t(c.nt)) c.tmem_cols *= 2;
+    c.b_rows = (pair ? ceil_div(c.nt, 2 * c.box) : ceil_div(c.nt, c.box)) * c.box;
+    const size_t stage_bytes = TC_A_BYTES + size_t(c.b_rows) * 128;
+    c.half = c.tmem_cols / 2;
     c.status = status;
     c.drop = g_drop_step;
     const size_t table = p.plan ? size_t(2 * (p.experts + 1) + 1) * sizeof(int) : 0, fixed = 8 * 1024;      // static arrays and the alignment of the ring
-    c.stages = int(std::min<size_t>(TC_MAX_STAGES, ((two ? TC_SMEM / 2 : TC_SMEM) - fixed - table) / (TC_A_BYTES + size_t(c.nt) * (pair ? 64 : 128))));
+    c.stages = int(std::min<size_t>(TC_MAX_STAGES, ((two ? TC_SMEM / 2 : TC_SMEM) - fixed - table) / stage_bytes));
     TcMaps maps;
     std::memset(&maps, 0, sizeof(maps));
     const int box = MATS == 2 ? 16 : 128;
@@ -529,7 +550,7 @@ int32_t i8_gemm(const I8Args & p, long long q_rows, int per_group, int * status,
         else maps.shared[m] = maps.a[m];
     }
     if (!ok) return B2MOE_ERR_CUDA;
-    const size_t smem = 1024 + size_t(c.stages) * (TC_A_BYTES + size_t(c.nt) * (pair ? 64 : 128)) + table;
+    const size_t smem = 1024 + size_t(c.stages) * stage_bytes + table;
     const long long items = (long long)c.tiles * c.row_blocks;
     if constexpr (MATS == 1)
         if (split > 1) {
