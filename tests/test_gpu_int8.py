@@ -217,7 +217,7 @@ SHAPES = [  # n, e, k, h, f, shared, route
     (1, 8, 2, 64, 16, False, "even"), (3, 5, 5, 80, 48, True, "even"), (7, 16, 4, 256, 144, False, "skip"), (9, 4, 2, 48, 80, True, "skip"),
     (40, 3, 1, 128, 64, False, "one"), (17, 40, 6, 1040, 272, False, "even"), (130, 4, 2, 192, 208, True, "even"), (300, 6, 3, 144, 128, False, "skip"),
     (260, 2, 1, 128, 336, False, "one"), (5, 8, 2, 64, 32, False, "none"), (700, 8, 4, 512, 256, True, "even"), (1, 2, 1, 16, 16, False, "even"),
-    (5, 4, 4, 64, 48, True, "twice"), (70, 3, 3, 128, 144, False, "twice"), (60, 6, 2, 2576, 80, True, "even"), (600, 3, 2, 2688, 208, False, "skip"),
+    (150, 4096, 2, 64, 32, False, "even"), (100, 4097, 2, 64, 32, True, "skip"), (5, 4, 4, 64, 48, True, "twice"), (70, 3, 3, 128, 144, False, "twice"), (60, 6, 2, 2576, 80, True, "even"), (600, 3, 2, 2688, 208, False, "skip"),
 ]
 
 
@@ -498,3 +498,19 @@ def test_a_wait_of_grouped_products_that_runs_out():
     assert int(plan.buf[3]) != 0
     plan = moe.dispatch(ids.cuda(), 4)
     assert torch.equal(moe.expert_gateup_swiglu(dev[0], dev[1], xd, plan), clean) and int(plan.buf[3]) == 0
+
+
+def test_tensors_on_the_host_beside_those_on_the_device():
+    from tqllm_b200 import capi, moe
+    q, s, w, v = linear_case(4, 6, 32, 1)
+    bank = moe.DeviceBank.from_int8(w.cuda(), v.cuda())
+    l, ids = torch.zeros(5, 8).cuda(), torch.zeros(5, 2, dtype=torch.int32).cuda()
+    b = moe.balance_loss(l, ids, 8, 0.1)
+    calls = [lambda: moe.linear_i8(q.cuda(), s, bank), lambda: moe.linear_i8(q.cuda(), s.cuda(), moe.DeviceBank.from_int8(w, v)), lambda: moe.linear_i8(q.cuda(), s.cuda(), bank, out=torch.zeros(4, 6)),
+             lambda: moe.balance_loss(l, ids.cpu(), 8, 0.1), lambda: moe.balance_loss(l, ids, 8, 0.1, mask=torch.ones(5, dtype=torch.bool)),
+             lambda: moe.balance_loss(l, ids, 8, 0.1, offsets=torch.tensor([0, 5], dtype=torch.int32)), lambda: moe.balance_loss_backward(l, b, 2, 0.1, grad_loss=torch.tensor(1.0)),
+             lambda: moe.balance_loss_backward(l, b, 2, 0.1, out=torch.zeros(5, 8))]
+    for call in calls:
+        with pytest.raises(capi.B2moeError) as e:
+            call()
+        assert e.value.status == capi.ERR_CUDA

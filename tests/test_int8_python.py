@@ -38,3 +38,14 @@ def test_balance():
     for bad in (dict(offsets=torch.tensor([0, 2, 5], dtype=torch.int32)), dict(grad_loss=torch.zeros((), dtype=torch.float64)), dict(out=torch.zeros(5, 7)), dict(out=torch.zeros(4, 8)),
                 dict(out=torch.zeros(5, 8, dtype=torch.float64)), dict(out=torch.zeros(8, 5).t()), dict(logits=l[:, :7])):
         refused(capi.ERR_SHAPE, moe.balance_loss_backward, **{**dict(logits=l, saved=saved, topk=2, coef=0.1), **bad})
+
+
+def test_tensors_that_are_not_on_the_current_device():
+    x, q, s = torch.zeros(4, 32), torch.zeros(4, 32, dtype=torch.int8), torch.zeros(4)
+    bank = moe.DeviceBank.from_int8(torch.zeros(6, 32, dtype=torch.int8), torch.zeros(6))
+    l, ids = torch.zeros(5, 8), torch.zeros(5, 2, dtype=torch.int32)
+    saved = moe.Balance(torch.zeros(()), torch.zeros(1, 8, dtype=torch.int32), torch.zeros(1, 8), torch.zeros(2, dtype=torch.int32))
+    refused(capi.ERR_CUDA, moe.quantize_rows, x)
+    refused(capi.ERR_CUDA, moe.linear_i8, q, s, bank)
+    refused(capi.ERR_CUDA, moe.balance_loss, l, ids, 8, 0.1)
+    refused(capi.ERR_CUDA, moe.balance_loss_backward, l, saved, 2, 0.1)

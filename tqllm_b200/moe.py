@@ -26,6 +26,18 @@ def _ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
 
+def _stream_of(t: torch.Tensor, *others: torch.Tensor | None) -> int:
+    """the current stream, for tensors that are all on the current device (a launch there on another one's memory would fault)"""
+    dev = t.get_device()
+    if dev >= 0 and dev == torch._C._cuda_getDevice():
+        for o in others:
+            if o is not None and o.get_device() != dev:
+                break
+        else:
+            return torch._C._cuda_getCurrentRawStream(dev)
+    raise capi.B2moeError(capi.ERR_CUDA, "tensors on the current CUDA device are wanted")
+
+
 class DeviceBank:
     """One stacked expert matrix [experts * rows][cols] in bank layout on the device."""
 
@@ -130,9 +142,10 @@ def quantize_rows(x: torch.Tensor):
     ldx, one = x.stride()
     if one != 1 and k > 1:
         raise capi.B2moeError(capi.ERR_SHAPE, "quantize_rows: the values of a row have to be neighbours")
+    stream = _stream_of(x)
     q = torch.empty(n, k, dtype=torch.int8, device=x.device)
     scale = torch.empty(n, dtype=torch.float32, device=x.device)
-    check(lib.b2moe_quantize_rows(x.data_ptr(), _DT[x.dtype], ldx if n > 1 else k, n, k, q.data_ptr(), k, scale.data_ptr(), _stream()), "b2moe_quantize_rows")
+    check(lib.b2moe_quantize_rows(x.data_ptr(), _DT[x.dtype], ldx if n > 1 else k, n, k, q.data_ptr(), k, scale.data_ptr(), stream), "b2moe_quantize_rows")
     return q, scale
 
 
@@ -145,14 +158,15 @@ def linear_i8(q: torch.Tensor, scale: torch.Tensor, bank: DeviceBank, out_dtype=
         raise capi.B2moeError(capi.ERR_SHAPE, "linear_i8: int8 rows of the bank's columns and a float32 scale for each are wanted")
     if one != 1 and k > 1:
         raise capi.B2moeError(capi.ERR_SHAPE, "linear_i8: the values of a row have to be neighbours")
-    if out is None:
-        out = torch.empty(n, rows, dtype=out_dtype, device=q.device)
-    elif out.shape != (n, rows) or (out.stride(1) != 1 and rows > 1):
-        raise capi.B2moeError(capi.ERR_SHAPE, "linear_i8: an output [n, rows] with contiguous rows is wanted")
-    else:
+    if out is not None:
+        if out.shape != (n, rows) or (out.stride(1) != 1 and rows > 1):
+            raise capi.B2moeError(capi.ERR_SHAPE, "linear_i8: an output [n, rows] with contiguous rows is wanted")
         out_dtype = out.dtype
         ldy = out.stride(0) if n > 1 else rows
-    check(lib.b2moe_linear_i8(q.data_ptr(), ldq if n > 1 else k, scale.data_ptr(), C.byref(bank.c), n, out.data_ptr(), _DT[out_dtype], ldy, _ptr(status), _stream()), "b2moe_linear_i8")
+    stream = _stream_of(q, scale, bank.data, bank.aux, out, status)
+    if out is None:
+        out = torch.empty(n, rows, dtype=out_dtype, device=q.device)
+    check(lib.b2moe_linear_i8(q.data_ptr(), ldq if n > 1 else k, scale.data_ptr(), C.byref(bank.c), n, out.data_ptr(), _DT[out_dtype], ldy, _ptr(status), stream), "b2moe_linear_i8")
     return out
 
 
@@ -185,12 +199,13 @@ def balance_loss(logits, ids, experts, coef, gating=capi.SOFTMAX, mask=None, off
     tokens, topk = ids.shape
     if tokens != n or ids.dtype is not torch.int32 or not ids.is_contiguous():
         raise capi.B2moeError(capi.ERR_SHAPE, "balance loss: contiguous int32 ids [n, topk] are wanted")
+    stream = _stream_of(logits, ids, mask, offsets)
     new, ints = logits.new_empty, ids.new_empty
     out = Balance(new(()), ints((seqs, experts)), new((seqs, experts)), ints(seqs + 1))
     size = lib.b2moe_balance_workspace_bytes(experts, n, seqs)
     ws = new(max(4, size // 4))
     check(lib.b2moe_balance_loss(gating, logits.data_ptr(), ld, ids.data_ptr(), topk, _ptr(mask), _ptr(offsets), seqs, experts, n, coef, out.loss.data_ptr(),
-                                 out.counts.data_ptr(), out.prob.data_ptr(), out.tokens.data_ptr(), ws.data_ptr(), size, _stream()), "b2moe_balance_loss")
+                                 out.counts.data_ptr(), out.prob.data_ptr(), out.tokens.data_ptr(), ws.data_ptr(), size, stream), "b2moe_balance_loss")
     return out
 
 
@@ -201,14 +216,15 @@ def balance_loss_backward(logits, saved: Balance, topk, coef, gating=capi.SOFTMA
     if counted != seqs or (grad_loss is not None and grad_loss.dtype is not torch.float32):
         raise capi.B2moeError(capi.ERR_SHAPE, "balance loss: the counts of the same sequences and a float32 gradient are wanted")
     grad, ldg = out, experts
+    if grad is not None:
+        if grad.dtype is not torch.float32 or grad.shape[0] != n or grad.shape[1] < experts or (grad.stride(1) != 1 and experts > 1):
+            raise capi.B2moeError(capi.ERR_SHAPE, "balance loss: the gradient has float32 rows like the logits")
+        ldg = grad.stride(0) if n > 1 else grad.shape[1]
+    stream = _stream_of(logits, saved.counts, saved.tokens, mask, offsets, grad_loss, out)
     if grad is None:
         grad = logits.new_empty((n, experts))
-    elif grad.dtype is not torch.float32 or grad.shape[0] != n or grad.shape[1] < experts or (grad.stride(1) != 1 and experts > 1):
-        raise capi.B2moeError(capi.ERR_SHAPE, "balance loss: the gradient has float32 rows like the logits")
-    else:
-        ldg = grad.stride(0) if n > 1 else grad.shape[1]
     check(lib.b2moe_balance_loss_backward(gating, logits.data_ptr(), ld, topk, _ptr(mask), _ptr(offsets), seqs, experts, n, coef, saved.counts.data_ptr(),
-                                          saved.tokens.data_ptr(), _ptr(grad_loss), grad.data_ptr(), ldg, int(out is not None), _stream()), "b2moe_balance_loss_backward")
+                                          saved.tokens.data_ptr(), _ptr(grad_loss), grad.data_ptr(), ldg, int(out is not None), stream), "b2moe_balance_loss_backward")
     return grad
 
 
