@@ -514,3 +514,18 @@ def test_tensors_on_the_host_beside_those_on_the_device():
         with pytest.raises(capi.B2moeError) as e:
             call()
         assert e.value.status == capi.ERR_CUDA
+
+
+@pytest.mark.parametrize("n,e,k,h,f,shared,route", [s for s in SHAPES if s[1] < 100])
+def test_the_forms_give_the_same_bits(n, e, k, h, f, shared, route):
+    from tqllm_b200 import capi, moe
+    x, ids, banks, sh = experts_case(n, e, k, h, f, n * e, shared, route)
+    dev = [moe.DeviceBank.from_int8(w.cuda(), v.cuda()) for w, v in banks]
+    dsh = [moe.DeviceBank.from_int8(w.cuda(), v.cuda()) for w, v in sh] if shared else [None] * 3
+    plan = moe.dispatch(ids.cuda(), e, n if shared else 0)
+    got = []
+    for family in ("decode", "gemm"):
+        with capi.family(family):
+            act = moe.expert_gateup_swiglu(dev[0], dev[1], x.cuda(), plan, dsh[0], dsh[1])
+            got.append((act, moe.expert_down(dev[2], act, plan, dsh[2]), moe.linear_i8(*moe.quantize_rows(x.cuda()), moe.DeviceBank.from_int8(dev[0].data[0], dev[0].aux[0]), out_dtype=torch.float32)))
+    assert all(torch.equal(a, b) for a, b in zip(*got))
