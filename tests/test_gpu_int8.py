@@ -529,3 +529,12 @@ def test_the_forms_give_the_same_bits(n, e, k, h, f, shared, route):
             act = moe.expert_gateup_swiglu(dev[0], dev[1], x.cuda(), plan, dsh[0], dsh[1])
             got.append((act, moe.expert_down(dev[2], act, plan, dsh[2]), moe.linear_i8(*moe.quantize_rows(x.cuda()), moe.DeviceBank.from_int8(dev[0].data[0], dev[0].aux[0]), out_dtype=torch.float32)))
     assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+# 16 warps (at most 296 blocks of 16 rows, 32 steps of 64 columns or more) and 8, with eight steps at once and the remainder behind them
+@pytest.mark.parametrize("m,k", ((4736, 2048), (4737, 2048), (40, 2032), (40, 8192), (33, 9104), (4750, 4112), (9500, 2064), (7, 16400)))
+@pytest.mark.parametrize("n", (1, 8, 9, 33))
+def test_linear_streamed_by_few_and_many_warps(n, m, k):
+    from tqllm_b200 import capi
+    with capi.family("decode"):
+        linear_of_real_sizes(n, m, k)

@@ -28,12 +28,12 @@ __device__ __forceinline__ uint4 load_stream(const int8_t * p) {
 // A few tokens per expert: bound by streaming the weights. A block takes 16 weight rows of one expert (of both matrices with MATS = 2) and all the
 // expert's tokens, 8 NT at a time; its warps share the columns in pieces of 64, 16 bytes a lane and row, straight from memory into the fragments of the tensor
 // core: lane (g, t) holds bytes 16 t.. of rows g and g + 8, so word i of both operands stands for the same four columns, which is all that a sum over columns needs.
-template <int MATS, int NT>
-__global__ void __launch_bounds__(256) i8_stream_k(const I8Args p) {
+// UNROLL: steps that a warp asks for at once.
+template <int MATS, int NT, int UNROLL>
+__global__ void __launch_bounds__(512) i8_stream_k(const I8Args p) {
     extern __shared__ int red[];                                       // [warps][MATS][NT][16 rows][8 tokens]
-    constexpr int UNROLL = NT > 2 ? 2 : 4;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, g = lane >> 2, t = lane & 3, r0 = blockIdx.x * 16;
-    // a dense call's weights are asked into the L2 while the launch in front of this one runs (they are not read before it is through): 4096 x 4096, one row 5.0 -> 4.6 us
+    // a dense call's weights are asked into the L2 while the launch in front of this one runs (they are not read before it is through): 4096 x 4096, one row, 5.0 -> 4.6 us
     if (!p.plan && threadIdx.x < 16 && r0 + int(threadIdx.x) < p.rows)
         asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(__cvta_generic_to_global(p.w[0] + size_t(r0 + threadIdx.x) * p.cols)), "r"(uint32_t(p.cols)) : "memory");
     grid_wait();
@@ -126,11 +126,17 @@ __global__ void __launch_bounds__(256) i8_stream_k(const I8Args p) {
     }
 }
 
+// Warps that share a block's columns: eight where a launch has few blocks, else four; sixteen for long rows of a dense call whose blocks are all on the SMs at once. us with 4 / 8 / 16, one row:
+// 4096 x 4096 10.0 / 6.5 / 4.6, 2048 x 8192 15.7 / 9.3 / 6.2, 1411 x 2560 5.1 / 3.6 / 2.9, 1024 x 2048 4.2 / 3.0 / 2.7, 512 x 1024 2.4 / 2.2 / 2.4, 8192 x 1024 3.7 / 3.4 / 5.5; gate/up of one token of
+// ten experts 11.3 / 9.0 / 12.1. Eight steps at once where a warp has as many (8192 x 8192 16.1 -> 15.3, 2048 x 8192 6.1 -> 5.7; where it has fewer it loses: 4096 x 4096 4.5 -> 4.8)
 template <int MATS, int NT>
 int32_t launch_stream(const I8Args & a, int groups, cudaStream_t s) {
-    // Warps that share a block's columns: eight where a launch has few blocks, else four
-    const int blocks = ceil_div(a.rows, 16), warps = (long long)blocks * groups < 148 * 4 ? 8 : 4;
-    launch_overlapped(i8_stream_k<MATS, NT>, dim3(blocks, groups), dim3(32 * warps), size_t(warps) * MATS * NT * 128 * sizeof(int), s, a);
+    const int blocks = ceil_div(a.rows, 16), steps = ceil_div(a.cols, 64);
+    const int warps = !a.plan && blocks <= 148 * 2 && steps >= 32 ? 16 : (long long)blocks * groups < 148 * 4 ? 8 : 4;
+    auto kernel = i8_stream_k<MATS, NT, (NT > 2 ? 2 : 4)>;
+    if constexpr (MATS == 1 && NT == 1)
+        if (steps >= 8 * warps) kernel = i8_stream_k<1, 1, 8>;
+    launch_overlapped(kernel, dim3(blocks, groups), dim3(32 * warps), size_t(warps) * MATS * NT * 128 * sizeof(int), s, a);
     return launch_status();
 }
 template <int MATS>
@@ -162,7 +168,7 @@ size_t i8_workspace_bytes(int rows_x, int k) { return i8_rows_bytes(rows_x, k); 
 size_t i8_slot_bytes(int slot_rows, int k) { return i8_rows_bytes(slot_rows, k) + align_up(size_t(slot_rows) * sizeof(int), 256); }
 
 // The form of a product: the streaming kernel for a few rows, the tensor-core GEMM (int8_gemm.cu) for more. us, streamed / GEMM:
-//   dense, from 17 rows on: 4096 x 4096 16 rows 7.7 / 7.9, 24 10.3 / 8.0; 1411 x 2560 16 4.4 / 5.7, 32 6.7 / 5.9; 8192 x 1024 16 4.4 / 4.9, 32 5.7 / 5.1
+//   dense, from 17 rows on: 4096 x 4096 16 rows 5.5 / 8.0, 24 7.9 / 8.0, 48 13.1 / 8.2; 2048 x 8192 16 6.9 / 8.8, 17 10.4 / 8.9; 1411 x 2560 16 3.6 / 5.9, 32 5.7 / 6.0; 8192 x 8192 16 17.3 / 15.5, 17 22.4 / 15.3
 //   gate/up, from seven rows per expert on: 128 experts of 1408 x 4096 at 4 each 221 / 233, at 8 307 / 245; 512 of 512 x 2048 at 2.5 155 / 168, at 5 184 / 187; 32 of 512 x 1024 at 4 8.9 / 14.2, at 16
 //   17.1 / 15.3 (the GEMM's times have a launch more in them, since its rows lie in slot order)
 //   down, where they are in slot order anyway, also where the SMs get eight items each, and for short rows from three per expert or four items an SM on: 128 of 4096 x 1408 at 0.5 63 / 60, at 1
