@@ -492,8 +492,8 @@ int dense_rows(int n, int row_blocks, int steps, bool longer, bool two, int sms)
     const int most = two ? 128 : 256, least = two ? 32 : 96, first = ceil_div(n, most);
     int best = most;
     float cost = 1e30f;
-    for (int tiles = first; tiles <= std::max(first + 8, ceil_div(n, least)); ++tiles) {
-        const int rows = (ceil_div(n, tiles) + 15) / 16 * 16;
+    for (int r = most; r >= least; r -= 16) {                          // multiples of 16, made as small as their number of tiles allows
+        const int tiles = ceil_div(n, r), rows = (ceil_div(n, tiles) + 15) / 16 * 16;
         if (rows < least && tiles > first) break;
         const bool pair = longer && rows > 128;
         const long long items = (long long)ceil_div(n, rows) * (pair ? ceil_div(row_blocks, 2) : row_blocks), at_once = pair ? sms / 2 : two ? 2 * sms : sms;
