@@ -61,7 +61,7 @@ enum b2moe_type {
     B2MOE_IQ3_S_X4 = 0x1015,
     /* Not a GGUF type: plain rows of 8-bit integers, one fp32 scale a row (an 8-bit checkpoint with scales per output
      * channel). data is int8 [experts][rows][cols], aux fp32 [experts][rows], the weight is their product; cols is a multiple of
-     * 16 and below 2^17. There is nothing to repack (b2moe_bank_load does not know the type): a bank is the caller's
+     * 16 and below 2^17, rows below 2^30. There is nothing to repack (b2moe_bank_load does not know the type): a bank is the caller's
      * arrays, or what b2moe_quantize_rows makes of floating-point rows. The expert products and the layer calls take such banks, a
      * layer may mix them with others; activation rows are quantised to 8 bits each (b2moe_quantize_rows has the rule) and the
      * sums of products are exact. Scratch: b2moe_expert_workspace_bytes; with b2moe_expert_slot_workspace_bytes gate/up calls of
@@ -273,7 +273,7 @@ B2MOE_API int32_t b2moe_combine_residual(const float * y, const int32_t * ids, c
  * b2moe_quantize_rows: x [n][k] of x_dtype, rows ldx elements apart -> q int8, rows ldq bytes apart, and scale [n]:
  *   scale = max|x| / 127 (fp32), q = the integer nearest to 127 x / max|x|, halves to even, exactly. A row of zeros has
  *   scale 0; a row that holds an infinity or a NaN has a NaN as its scale (and with it in everything that is made of it). k and
- *   ldq are multiples of 16, k below 2^17, ldx a multiple of 16 bytes; x and q 16-byte aligned. Bytes between k and ldq are
+ *   ldq are multiples of 16, k below 2^17, n below 2^30 (in b2moe_linear_i8 too), ldx a multiple of 16 bytes; x and q 16-byte aligned. Bytes between k and ldq are
  *   left as they are.
  * b2moe_linear_i8: y[t][r] = (sum_j q[t][j] w[r][j]) * (scale[t] * aux[r]) rounded once to y_dtype, rows of y ldy elements
  *   apart; the sum is exact. w is a bank of type B2MOE_I8 with one expert; q as b2moe_quantize_rows leaves it (any values of int8).

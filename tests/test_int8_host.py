@@ -124,3 +124,16 @@ def test_roundings_of_16_bit_rows(bits):
             want = np.where(a > h, m + 1, np.where(a < h, m, m + m % 2))
             assert np.array_equal(np.rint(x * float(inv)), want), (top, e)
     assert left == (0 if bits == 8 else 7)
+
+
+def test_row_counts_whose_tiles_pass_32_bits():
+    most = (1 << 30) - 1
+    for n in (most + 1, (1 << 31) - 1):
+        assert lib.b2moe_quantize_rows(16, capi.BF16, 16, n, 16, 16, 16, 16, None) == capi.ERR_SHAPE
+        assert lib.b2moe_linear_i8(16, 16, 16, C.byref(bank(1, 1, 16)), n, 16, capi.BF16, 1, None, None) == capi.ERR_SHAPE
+        assert lib.b2moe_linear_i8(16, 16, 16, C.byref(bank(1, n, 16)), 1, 16, capi.BF16, n, None, None) == capi.ERR_SHAPE
+        assert lib.b2moe_dequant_dump(C.byref(bank(1, n, 16)), 16, None) == capi.ERR_SHAPE
+    down = bank(4, 16, 16)
+    n = 1 << 29                                                        # two assignments a token and a shared row: 3 * 2^29
+    size = lib.b2moe_expert_workspace_bytes(I8, most, 16, capi.F32) * 2
+    assert lib.b2moe_expert_down(C.byref(down), C.byref(bank(1, 16, 16)), 16, 16, n, 1, n, 16, 16, size, None) == capi.ERR_SHAPE

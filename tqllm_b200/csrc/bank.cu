@@ -70,7 +70,7 @@ int32_t check_bank(const b2moe_bank * b) {
     FmtInfo f;
     if (!b) return B2MOE_ERR_NULL;
     if (b->type == B2MOE_I8) {                                         // plain rows and a scale each: nothing of the block formats applies
-        if (b->experts <= 0 || b->rows <= 0 || !i8_cols(b->cols)) return B2MOE_ERR_SHAPE;
+        if (b->experts <= 0 || b->rows <= 0 || b->rows > I8_MAX_ROWS || !i8_cols(b->cols)) return B2MOE_ERR_SHAPE;
         if (!b->data || !b->aux) return B2MOE_ERR_NULL;
         return aligned16(b->data) && aligned_to(b->aux, 4) ? B2MOE_OK : B2MOE_ERR_ALIGN;
     }

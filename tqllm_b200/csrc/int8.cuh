@@ -10,6 +10,8 @@ namespace b2 {
 constexpr int I8_MAX_COLS = (1 << 17) - 16;
 // rows up to here are short: the tensor-core form runs two blocks an SM
 constexpr int I8_SHORT_COLS = 1024;
+// rows of a call or of an expert, assignments: tile arithmetic stays inside 32 bits
+constexpr int I8_MAX_ROWS = (1 << 30) - 1;
 inline bool i8_cols(int cols) { return cols > 0 && cols % 16 == 0 && cols <= I8_MAX_COLS; }
 
 // Operand form of activation rows inside a workspace: `rows` 8-bit rows of k values, a scale each

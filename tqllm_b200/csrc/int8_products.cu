@@ -141,6 +141,7 @@ int32_t launch_stream(const I8Args & a, int groups, cudaStream_t s) {
 }
 template <int MATS>
 int32_t i8_stream(const I8Args & a, int groups, long long tokens, cudaStream_t s) {
+    if (groups > 65535) return B2MOE_ERR_SHAPE;                        // the grid's second extent
     // rows that a pass over the weights serves: a second pass of some experts (from the L2) costs less than the registers of 16 rows (512 experts at five each: 184 and 222 us)
     if (tokens <= 8LL * groups) return launch_stream<MATS, 1>(a, groups, s);
     if (tokens <= 16LL * groups) return launch_stream<MATS, 2>(a, groups, s);
@@ -184,7 +185,7 @@ int per_group(int experts, long long rows) { return int(std::min<long long>(1 <<
 // x [n][cols]; the workspace holds the rows of the n tokens
 int32_t i8_gateup(const b2moe_bank * gate, const b2moe_bank * up, const b2moe_bank * shared_gate, const b2moe_bank * shared_up, const void * x, int x_dtype, const int * plan, int n,
                   int topk, int shared_tokens, long long live, void * act, int act_dtype, void * ws, void * rows_buf, size_t rows_buf_bytes, cudaStream_t s) {
-    if ((long long)n * topk > 0x3fffffffLL) return B2MOE_ERR_SHAPE;
+    if ((long long)n * topk + shared_tokens > I8_MAX_ROWS) return B2MOE_ERR_SHAPE;
     I8Args p = grouped(gate, up, shared_gate, shared_up, plan, n, topk, shared_tokens, act, act_dtype);
     const int total = n * topk + shared_tokens;
     if (i8_takes_gemm(gate->experts, live >= (long long)I8_GEMM_MIN_PER * gate->experts) && rows_buf_bytes >= i8_slot_bytes(total, gate->cols)) {
@@ -202,7 +203,7 @@ int32_t i8_gateup(const b2moe_bank * gate, const b2moe_bank * up, const b2moe_ba
 // x [assignments][cols] (per_token: [n][cols]); the workspace holds a row per assignment, in slot order
 int32_t i8_down(const b2moe_bank * down, const b2moe_bank * shared_down, const void * x, int x_dtype, bool per_token, const int * plan, int n, int topk, int shared_tokens, long long live,
                 void * y, int y_dtype, void * ws, cudaStream_t s) {
-    if ((long long)n * topk > 0x3fffffffLL) return B2MOE_ERR_SHAPE;
+    if ((long long)n * topk + shared_tokens > I8_MAX_ROWS) return B2MOE_ERR_SHAPE;
     I8Args p = grouped(down, nullptr, shared_down, nullptr, plan, n, topk, shared_tokens, y, y_dtype);
     const int total = n * topk + shared_tokens;
     const I8Rows rows = i8_rows(ws, total);
@@ -236,7 +237,7 @@ extern "C" B2MOE_API int32_t b2moe_linear_i8(const int8_t * q, int64_t ldq, cons
                                              b2moe_stream stream) {
     if (int32_t rc = check_bank(w)) return rc;
     if (w->type != B2MOE_I8) return B2MOE_ERR_FORMAT;
-    if (n <= 0 || w->experts != 1 || !valid_dtype(y_dtype) || ldq < w->cols || ldq % 16 || ldy < w->rows) return B2MOE_ERR_SHAPE;
+    if (n <= 0 || n > I8_MAX_ROWS || w->experts != 1 || !valid_dtype(y_dtype) || ldq < w->cols || ldq % 16 || ldy < w->rows) return B2MOE_ERR_SHAPE;
     if (!q || !scale || !y) return B2MOE_ERR_NULL;
     if (!aligned16(q) || !aligned_to(y, dtype_bytes(y_dtype)) || !aligned_to(scale, 4) || !aligned_to(status, 4)) return B2MOE_ERR_ALIGN;
     I8Args p{};

@@ -284,7 +284,7 @@ using namespace b2;
 
 extern "C" B2MOE_API int32_t b2moe_quantize_rows(const void * x, int32_t x_dtype, int64_t ldx, int32_t n, int32_t k, int8_t * q, int64_t ldq, float * scale,
                                                  b2moe_stream stream) {
-    if (n <= 0 || !i8_cols(k) || !valid_dtype(x_dtype) || ldx < k || ldx % (x_dtype == B2MOE_F32 ? 4 : 8) || ldq < k || ldq % 16) return B2MOE_ERR_SHAPE;
+    if (n <= 0 || n > I8_MAX_ROWS || !i8_cols(k) || !valid_dtype(x_dtype) || ldx < k || ldx % (x_dtype == B2MOE_F32 ? 4 : 8) || ldq < k || ldq % 16) return B2MOE_ERR_SHAPE;
     if (!x || !q || !scale) return B2MOE_ERR_NULL;
     if (!aligned16(x) || !aligned16(q) || !aligned_to(scale, 4)) return B2MOE_ERR_ALIGN;
     return i8_quantize(x, x_dtype, ldx, n, k, q, ldq, scale, as_stream(stream));
