@@ -27,6 +27,8 @@ def test_rows_and_products():
         refused(capi.ERR_SHAPE, moe.linear_i8, *bad, bank)
     for out in (torch.zeros(4, 5), torch.zeros(3, 6), torch.zeros(6, 4).t()):
         refused(capi.ERR_SHAPE, moe.linear_i8, q, s, bank, out=out)
+    for status in (torch.zeros(1), torch.zeros(4, dtype=torch.uint8), torch.zeros(0, dtype=torch.int32)):
+        refused(capi.ERR_SHAPE, lambda: moe.linear_i8(q, s, bank, status=status))
 
 
 def test_balance():
@@ -38,6 +40,15 @@ def test_balance():
     for bad in (dict(offsets=torch.tensor([0, 2, 5], dtype=torch.int32)), dict(grad_loss=torch.zeros((), dtype=torch.float64)), dict(out=torch.zeros(5, 7)), dict(out=torch.zeros(4, 8)),
                 dict(out=torch.zeros(5, 8, dtype=torch.float64)), dict(out=torch.zeros(8, 5).t()), dict(logits=l[:, :7])):
         refused(capi.ERR_SHAPE, moe.balance_loss_backward, **{**dict(logits=l, saved=saved, topk=2, coef=0.1), **bad})
+
+
+def test_what_the_balance_gradient_is_given():
+    """counts as they come back from a reduction over ranks, say"""
+    l, f = torch.zeros(5, 8), torch.zeros(())
+    counts, tokens = torch.zeros(1, 8, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+    for c, t, g in ((counts.long(), tokens, None), (counts.float(), tokens, None), (torch.zeros(1, 16, dtype=torch.int32)[:, ::2], tokens, None),
+                    (counts, tokens.long(), None), (counts, tokens[:1], None), (counts, torch.zeros(4, dtype=torch.int32)[::2], None), (counts, tokens, torch.zeros(0)), (counts, tokens, torch.zeros(2))):
+        refused(capi.ERR_SHAPE, moe.balance_loss_backward, l, moe.Balance(f, c, f, t), 2, 0.1, grad_loss=g)
 
 
 def test_tensors_that_are_not_on_the_current_device():

@@ -158,6 +158,8 @@ def linear_i8(q: torch.Tensor, scale: torch.Tensor, bank: DeviceBank, out_dtype=
         raise capi.B2moeError(capi.ERR_SHAPE, "linear_i8: int8 rows of the bank's columns and a float32 scale for each are wanted")
     if one != 1 and k > 1:
         raise capi.B2moeError(capi.ERR_SHAPE, "linear_i8: the values of a row have to be neighbours")
+    if status is not None and (status.dtype is not torch.int32 or status.numel() < 1):
+        raise capi.B2moeError(capi.ERR_SHAPE, "linear_i8: the status is an int32 word")
     if out is not None:
         if out.shape != (n, rows) or (out.stride(1) != 1 and rows > 1):
             raise capi.B2moeError(capi.ERR_SHAPE, "linear_i8: an output [n, rows] with contiguous rows is wanted")
@@ -213,8 +215,11 @@ def balance_loss_backward(logits, saved: Balance, topk, coef, gating=capi.SOFTMA
     """The gradient of the balance loss on the logits, [n, experts]; into `out` (rows of at least `experts` columns) it is added."""
     counted, experts = saved.counts.shape
     n, ld, seqs = _balance_args(logits, experts, mask, offsets)
-    if counted != seqs or (grad_loss is not None and grad_loss.dtype is not torch.float32):
-        raise capi.B2moeError(capi.ERR_SHAPE, "balance loss: the counts of the same sequences and a float32 gradient are wanted")
+    if counted != seqs or saved.tokens.shape != (seqs + 1,) or saved.counts.dtype is not torch.int32 or saved.tokens.dtype is not torch.int32 or not (
+            saved.counts.is_contiguous() and saved.tokens.is_contiguous()):
+        raise capi.B2moeError(capi.ERR_SHAPE, "balance loss: int32 counts and tokens of the same sequences are wanted, as the loss leaves them")
+    if grad_loss is not None and (grad_loss.dtype is not torch.float32 or grad_loss.numel() != 1):
+        raise capi.B2moeError(capi.ERR_SHAPE, "balance loss: the loss's gradient is one float32")
     grad, ldg = out, experts
     if grad is not None:
         if grad.dtype is not torch.float32 or grad.shape[0] != n or grad.shape[1] < experts or (grad.stride(1) != 1 and experts > 1):
