@@ -128,7 +128,8 @@ __global__ void __launch_bounds__(512) i8_stream_k(const I8Args p) {
 
 // Warps that share a block's columns: eight where a launch has few blocks, else four; sixteen for long rows of a dense call whose blocks are all on the SMs at once. us with 4 / 8 / 16, one row:
 // 4096 x 4096 10.0 / 6.5 / 4.6, 2048 x 8192 15.7 / 9.3 / 6.2, 1411 x 2560 5.1 / 3.6 / 2.9, 1024 x 2048 4.2 / 3.0 / 2.7, 512 x 1024 2.4 / 2.2 / 2.4, 8192 x 1024 3.7 / 3.4 / 5.5; gate/up of one token of
-// ten experts 11.3 / 9.0 / 12.1. Eight steps at once where a warp has as many (8192 x 8192 16.1 -> 15.3, 2048 x 8192 6.1 -> 5.7; where it has fewer it loses: 4096 x 4096 4.5 -> 4.8)
+// ten experts 11.3 / 9.0 / 12.1. Eight steps at once where a warp has as many (8192 x 8192 16.1 -> 15.3, 2048 x 8192 6.1 -> 5.7; down of 64 experts of 4096 x 4096 at
+// three each 181.6 -> 171.8, of eight of 2048 x 4096 17.9 -> 17.0; where it has fewer it loses: 4096 x 4096 4.5 -> 4.8)
 template <int MATS, int NT>
 int32_t launch_stream(const I8Args & a, int groups, cudaStream_t s) {
     const int blocks = ceil_div(a.rows, 16), steps = ceil_div(a.cols, 64);
