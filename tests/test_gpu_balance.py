@@ -228,3 +228,37 @@ def test_counts_place_experts():
     hist = moe.count_ids(ids, torch.zeros(32, dtype=torch.int64, device="cuda"))
     assert torch.equal(b.counts[0].long(), hist)
     assert torch.equal(torch.from_numpy(moe.place_experts(b.counts[0], 4)[0]), torch.from_numpy(moe.place_experts(hist, 4)[0]))
+
+
+@pytest.mark.parametrize("e,k,n", ((1, 1, 5), (6, 6, 70), (40, 40, 9), (700, 7, 100), (64, 8, 4000), (2100, 3, 700)))
+@pytest.mark.parametrize("gating", (1, 2))
+def test_an_even_load_has_no_gradient(e, k, n, gating):
+    """equal counts: c - sum p c is zero whatever p is, and no rounding of the sum is left in its place"""
+    logits, _, _ = make(n, e, k, e)
+    ids = (torch.arange(n * k) % e).view(n, k).int()
+    assert n * k % e == 0
+    b, g = run(logits, ids, e, 3.0, gating)
+    assert torch.equal(b.counts.cpu(), torch.full((1, e), n * k // e, dtype=torch.int32))
+    assert not bool(g.any())
+
+
+@pytest.mark.parametrize("e", (60, 700))
+@pytest.mark.parametrize("gating", (1, 2))
+def test_a_nearly_even_load(e, gating):
+    """Counts of 1,000 (or 200) and a few: the error is relative to what they have more than the least, which is little of them. Scores are sums of positive numbers: the bound of the definition, C as above."""
+    k, coef = 5, 1.0
+    n = (1000 if e == 60 else 200) * e // k
+    logits, _, gen = make(300, e, k, e)
+    logits = logits.repeat(-(-n // 300), 1)[:n]
+    ids = (torch.arange(n * k) % e).view(n, k).int()
+    ids[:40, 0] = torch.randint(0, e // 2, (40,), generator=gen).int()
+    b, g = run(logits, ids, e, coef, gating)
+    c = torch.bincount(ids.flatten().long(), minlength=e).double()
+    assert torch.equal(b.counts[0].cpu().double(), c)
+    x = c - c.min()
+    u = logits.double()
+    p = torch.softmax(torch.nn.functional.logsigmoid(u) if gating == 2 else u, -1)
+    f = coef * e / (k * float(n) ** 2) * (torch.sigmoid(-u) if gating == 2 else 1.0)
+    want, size = p * (x - p @ x[:, None]) * f, p * (x + p @ x[:, None]) * f
+    C = (100 + float(2 * logits.abs().max())) * 2.0 ** -24
+    assert bool(((g.cpu().double() - want).abs() <= C * size + 1e-36).all())

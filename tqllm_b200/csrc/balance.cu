@@ -4,6 +4,8 @@
 //   c_se = assignments of sequence s to expert e,  T_s = its unmasked tokens,  P_se = sum_t p_te / T_s
 //   L = coef / S+ * sum_s E / (k T_s) * sum_e c_se P_se                       (S+: sequences with T_s > 0)
 //   dL/dl_tj = g coef / S+ * E / (k T_s^2) * p_tj (c_sj - sum_e p_te c_se) * (1 | 1 - sigmoid(l_tj))
+// The p_te of a token add up to one, so any number may be taken off the c_se. The gradient takes off their least: what is left stays positive and no larger than it was, an even load
+// has a gradient of zero instead of the rounding of the sum, and a nearly even one, which the loss makes for, loses fewer bits to the difference.
 //
 // The batch is cut into chunks of tokens that lie in one sequence each. Chunk j of sequence s has the number offsets[s] / chunk + s + j: the
 // numbers of two sequences never meet (a sequence of len tokens has at most ceil(len / chunk) <= floor((offsets[s] + len) / chunk) - floor(offsets[s] / chunk) + 1
@@ -315,12 +317,16 @@ __global__ void __launch_bounds__(BAL_THREADS) balance_backward_k(const BalBackA
     row.first = (warp % G) * 32 + lane;
     const float tokens = float(p.tokens[c.x]);
     const float factor = (p.grad_loss ? *p.grad_loss : 1.f) * p.coef / float(max(p.tokens[p.sequences], 1)) * float(p.experts) / (float(p.topk) * tokens * tokens);
-    float weight[V];
+    float weight[V], least = INFINITY;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
         const int e = row.first + 32 * G * i;
-        weight[i] = e < p.experts ? float(p.counts[size_t(c.x) * p.experts + e]) : 0.f;
+        weight[i] = e < p.experts ? float(p.counts[size_t(c.x) * p.experts + e]) : INFINITY;
+        least = fminf(least, weight[i]);
     }
+    least = -row.all(-least, true);
+#pragma unroll
+    for (int i = 0; i < V; ++i) weight[i] = row.first + 32 * G * i < p.experts ? weight[i] - least : 0.f;
 #pragma unroll 1
     for (int t0 = c.y; t0 < c.z; t0 += ROWS) {
         const int t = t0 + group;
