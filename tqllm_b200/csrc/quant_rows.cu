@@ -223,12 +223,15 @@ __global__ void __launch_bounds__(256) quant_rows_k(const QuantArgs p) {
     }
 }
 
-// slot of every grouped assignment
-__global__ void __launch_bounds__(256) inverse_k(const int * plan, int experts, int * inverse) {
+// Slot of every grouped assignment below `words`, what the array has room for: a plan with a shared expert holds assignments behind the routed ones, which a call without one
+// has no words for
+__global__ void __launch_bounds__(256) inverse_k(const int * plan, int experts, int words, int * inverse) {
     grid_release();
     grid_wait();
     const int i = blockIdx.x * 256 + threadIdx.x;
-    if (i < plan[PLAN_NGROUPED]) inverse[plan[PLAN_HDR + 3 * (experts + 1) + 1 + i]] = i;
+    if (i >= plan[PLAN_NGROUPED]) return;
+    const int a = plan[PLAN_HDR + 3 * (experts + 1) + 1 + i];
+    if (a < words) inverse[a] = i;
 }
 
 template <int DT, bool SCATTER>
@@ -273,7 +276,8 @@ int32_t i8_quantize_slots(const void * x, int x_dtype, bool per_token, int n, in
     return quantize<false>(QuantArgs{x, k, k, A + shared_tokens, k, rows.q, rows.scale, plan, experts, A, topk, per_token, shared_tokens ? 1 : 0}, x_dtype, s);
 }
 int32_t i8_quantize_scatter(const void * x, int x_dtype, int n, int k, const I8Rows & rows, int * inverse, const int * plan, int experts, int topk, int shared_tokens, cudaStream_t s) {
-    launch_overlapped(inverse_k, dim3(ceil_div(n * topk + shared_tokens, 256)), dim3(256), 0, s, plan, experts, inverse);
+    const int words = n * topk + shared_tokens;
+    launch_overlapped(inverse_k, dim3(ceil_div(words, 256)), dim3(256), 0, s, plan, experts, words, inverse);
     if (int32_t rc = launch_status()) return rc;
     return quantize<true>(QuantArgs{x, k, k, n, k, rows.q, rows.scale, plan, experts, n * topk, topk, 1, shared_tokens ? 1 : 0, inverse}, x_dtype, s);
 }
