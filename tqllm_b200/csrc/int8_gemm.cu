@@ -267,11 +267,16 @@ __global__ void __launch_bounds__(TC_THREADS, MODE ? 1 : 2) i8_gemm_k(const I8Ar
             }
         }
         if (!ok && lane == 0) give_up();
-        // before leaving, every copy must have landed (after a clean run these waits return at once). The odd block of a pair has no barrier for its own: the even one waits for them, and the
-        // blocks meet at the end; after a wait that ran out it leaves them two milliseconds
+        // Before leaving, every copy must have landed (after a clean run these waits return at once). The barriers of a pair's copies are the even block's, which waits for those that it has
+        // announced. The odd block knows that its copies have landed, and that the arrivals which the products send to its own barriers are here, when the last product of every stage has reported to
+        // it; where that does not come, it leaves its copies a tenth of a second (by the SM's clock, 2 GHz at most), a thousand times what one takes.
         if (PAIR && rank == 1) {
-            if (!ok || abort_flag)
-                for (int i = 0; i < 2000; ++i) __nanosleep(1000);
+#pragma unroll 1
+            for (uint32_t i = issued > uint32_t(c.stages) ? issued - c.stages : 0; ok && i < issued; ++i) ok = warp_wait(empty + 8 * (i % c.stages), (i / c.stages) & 1u);
+            if (!ok) {
+                const long long begin = clock64();
+                while (clock64() - begin < 200000000LL) __nanosleep(1000);
+            }
         } else
 #pragma unroll 1
         for (uint32_t i = issued > uint32_t(c.stages) ? issued - c.stages : 0; i < issued; ++i)
@@ -312,6 +317,8 @@ __global__ void __launch_bounds__(TC_THREADS, MODE ? 1 : 2) i8_gemm_k(const I8Ar
         if (PAIR) mma_commit_pair(lead, drain);
         else mma_commit(lead, drain);
         warp_wait(drain, 0);
+    } else if (PAIR && warp == 1) {
+        warp_wait(drain, 0);                                           // the even block's last word to this one: it arrives whether or not a wait of its own ran out
     } else if (SPLIT && warp >= TC_EPI_WARP0) {
         // ---- this block's part: from tensor memory to the ring, which nothing uses any more, 128 weight rows for each activation row ----
         const int quarter = warp & 3, half = (warp - TC_EPI_WARP0) >> 2;
@@ -381,7 +388,7 @@ __global__ void __launch_bounds__(TC_THREADS, MODE ? 1 : 2) i8_gemm_k(const I8Ar
         }
     }
     fence_before();
-    if (PAIR) cg::this_cluster().sync();                               // nothing of either block arrives at the other one any more
+    if (PAIR) cg::this_cluster().sync();                               // what either block sends to the other has arrived: each waited for what it was sent (above), arrivals of threads come before this
     else __syncthreads();
     fence_after();
     if (warp == 1) {
