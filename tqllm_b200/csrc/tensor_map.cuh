@@ -18,8 +18,16 @@ inline bool encode_map(CUtensorMap & m, CUtensorMapDataType type, int rank, cons
                        const cuuint32_t * box, CUtensorMapSwizzle swizzle) {
     const cuuint32_t steps[4] = {1, 1, 1, 1};
     const auto encode = map_encoder();
-    return encode && encode(&m, type, rank, const_cast<void *>(base), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
-                            CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    if (!encode) return false;
+    auto made = [&] {
+        return encode(&m, type, rank, const_cast<void *>(base), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    };
+    const CUresult rc = made();
+    if (rc != CUDA_ERROR_INVALID_CONTEXT) return rc == CUDA_SUCCESS;
+    // a host thread that has made no call of the runtime yet, which binds the device's context at its first one (the driver's functions do not): allowed while a stream is captured
+    int dev = 0;
+    return cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess && made() == CUDA_SUCCESS;
 }
 
 }  // namespace b2
