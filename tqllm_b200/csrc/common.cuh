@@ -56,6 +56,9 @@ __device__ __forceinline__ void bulk_g2s_first_out(uint32_t dst, const void * sr
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1], %2, [%3], %4;"
                  ::"r"(dst), "l"(__cvta_generic_to_global(src)), "r"(bytes), "r"(bar), "l"(policy) : "memory");
 }
+// Lets a kernel take `most` bytes of dynamic shared memory: the same number at every call, whatever the launch behind it takes, since the limit is the kernel's and host threads call at once. A limit set
+// to each launch's own size refused another thread's larger launch
+template <typename K> inline bool allow_smem(K kernel, size_t most) { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(most)) == cudaSuccess; }
 inline bool aligned16(const void * p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 inline bool aligned_to(const void * p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 inline cudaStream_t as_stream(b2moe_stream s) { return static_cast<cudaStream_t>(s); }

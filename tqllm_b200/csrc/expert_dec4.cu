@@ -784,7 +784,7 @@ int32_t launch_dec4(Dec4Args a, cudaStream_t s, typename std::conditional<ROUTED
         if (smem + sizeof(Routed) > SMEM_LIMIT + 1024) return B2MOE_OK;
         *took = true;
     }
-    if (cudaFuncSetAttribute(dec4_k<T, MODE, FEW, ROUTED>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)) != cudaSuccess) return B2MOE_ERR_CUDA;
+    if (!allow_smem(dec4_k<T, MODE, FEW, ROUTED>, ROUTED ? SMEM_LIMIT + 1024 - align_up(sizeof(Routed), 128) : SMEM_LIMIT)) return B2MOE_ERR_CUDA;
     a.wait_limit = g_wait_limit;
     a.drop_tile = g_drop_tile;
     launch_overlapped(dec4_k<T, MODE, FEW, ROUTED>, dim3(sms), dim3(threads_of<FEW && MODE == 1>()), smem, s, a, route);       // a block's share of the (pass, row tile) jobs: an equal one, or (FEW) whole passes

@@ -1062,7 +1062,7 @@ int32_t gemm_launch_t(GemmArgs a, long long live, const b2moe_bank * const * m, 
             if (a.out_dtype != B2MOE_F32) return B2MOE_ERR_SHAPE;      // calls with 16-bit results bring scratch for the rows in slot order
             kernel = gemm_tc_k<T, MODE, true, true>;
         }
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)) != cudaSuccess) return B2MOE_ERR_CUDA;
+    if (!allow_smem(kernel, GEMM_SMEM_LIMIT)) return B2MOE_ERR_CUDA;
     launch_overlapped(kernel, dim3(sms), dim3(g_threads(!slots)), smem, s, a, maps);
     return launch_status();
 }
@@ -1109,7 +1109,7 @@ int32_t exact_launch_t(GemmArgs a, const b2moe_bank * const * m, const void * x,
             return B2MOE_ERR_SHAPE;
         }
     }
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)) != cudaSuccess) return B2MOE_ERR_CUDA;
+    if (!allow_smem(kernel, GEMM_SMEM_LIMIT)) return B2MOE_ERR_CUDA;
     launch_overlapped(kernel, dim3(sms), dim3(g_threads(!slots)), smem, s, a, maps);
     return launch_status();
 }

@@ -346,8 +346,7 @@ int32_t launch_grouped(Iq3sArgs a, long long max_items, cudaStream_t s) {
     a.nbuf = fixed + xs_bytes(k, NTERM, 2) <= SMEM_LIMIT ? 2 : 1;
     const size_t smem = fixed + xs_bytes(k, NTERM, a.nbuf);
     if (smem > SMEM_LIMIT) return B2MOE_ERR_SHAPE;
-    if (cudaFuncSetAttribute(iq3s_grouped_k<MODE, NTERM, OP>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)) != cudaSuccess)
-        return B2MOE_ERR_CUDA;
+    if (!allow_smem(iq3s_grouped_k<MODE, NTERM, OP>, SMEM_LIMIT)) return B2MOE_ERR_CUDA;
     const int blocks = int(std::min<long long>(sms, std::max<long long>(1, max_items)));
     iq3s_grouped_k<MODE, NTERM, OP><<<blocks, CTA_WARPS * 32, smem, s>>>(a);
     return launch_status();

@@ -24,8 +24,7 @@ using namespace tc;
 
 constexpr int TC_THREADS = 384, TC_EPI_WARP0 = 4, TC_EPI_WARPS = 8, TC_EPI_THREADS = 32 * TC_EPI_WARPS, TC_MAX_STAGES = 12, TC_MAX_EXPERTS = 4096;
 constexpr int TC_A_BYTES = 128 * 128, TC_SMEM = 227 * 1024, TC_MAX_SPLIT = 8;
-// Static arrays and the alignment of the ring; what a launch asks for at most. Every call allows the kernel that much, whatever its own launch takes: a limit of its own would be the limit of another
-// host thread's launch, too
+// static arrays and the alignment of the ring; what a launch asks for at most
 constexpr int TC_FIXED = 8 * 1024, TC_ALIGN = 1024, TC_SMEM_MOST = TC_SMEM - TC_FIXED + TC_ALIGN;
 
 struct TcMaps { CUtensorMap a[2], shared[2], b; };
@@ -442,8 +441,6 @@ int sm_count() {
     return count;
 }
 template <class K>
-bool allow_smem(K kernel) { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, TC_SMEM_MOST) == cudaSuccess; }
-template <class K>
 int32_t launch_cluster(K kernel, dim3 grid, dim3 cluster, size_t smem, cudaStream_t s, const I8Args & p, const TcArgs & c, const TcMaps & maps) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = grid; cfg.blockDim = dim3(TC_THREADS); cfg.dynamicSmemBytes = smem; cfg.stream = s;
@@ -471,7 +468,7 @@ bool map_rows(CUtensorMap & m, const int8_t * base, int cols, long long rows, lo
 int clusters_at_once(int size) {
     static const std::array<int, TC_MAX_SPLIT + 1> most = [] {
         std::array<int, TC_MAX_SPLIT + 1> m{};
-        if (!allow_smem(i8_gemm_k<1, TC_SPLIT>)) return m;
+        if (!allow_smem(i8_gemm_k<1, TC_SPLIT>, TC_SMEM_MOST)) return m;
         for (int size = 2; size <= TC_MAX_SPLIT; ++size) {
             cudaLaunchConfig_t cfg{};
             cfg.gridDim = dim3(1, 1, size); cfg.blockDim = dim3(TC_THREADS); cfg.dynamicSmemBytes = TC_SMEM_MOST;
@@ -565,15 +562,15 @@ int32_t i8_gemm(const I8Args & p, long long q_rows, int per_group, int * status,
     const long long items = (long long)c.tiles * c.row_blocks;
     if constexpr (MATS == 1)
         if (split > 1) {
-            if (!allow_smem(i8_gemm_k<1, TC_SPLIT>)) return B2MOE_ERR_CUDA;
+            if (!allow_smem(i8_gemm_k<1, TC_SPLIT>, TC_SMEM_MOST)) return B2MOE_ERR_CUDA;
             return launch_cluster(i8_gemm_k<1, TC_SPLIT>, dim3(unsigned(items), 1, split), dim3(1, 1, split), smem, s, p, c, maps);
         }
     if (pair) {
-        if (!allow_smem(i8_gemm_k<MATS, TC_PAIR>)) return B2MOE_ERR_CUDA;
+        if (!allow_smem(i8_gemm_k<MATS, TC_PAIR>, TC_SMEM_MOST)) return B2MOE_ERR_CUDA;
         const long long pairs = (long long)c.tiles * ceil_div(c.row_blocks, 2);
         return launch_cluster(i8_gemm_k<MATS, TC_PAIR>, dim3(unsigned(2 * (p.plan ? sms / 2 : std::min<long long>(sms / 2, pairs)))), dim3(2), smem, s, p, c, maps);
     }
-    if (!allow_smem(i8_gemm_k<MATS, 0>)) return B2MOE_ERR_CUDA;
+    if (!allow_smem(i8_gemm_k<MATS, 0>, TC_SMEM_MOST)) return B2MOE_ERR_CUDA;
     const int blocks = two ? 2 * sms : sms;
     launch_overlapped(i8_gemm_k<MATS, 0>, dim3(unsigned(p.plan ? blocks : std::min<long long>(blocks, items))), dim3(TC_THREADS), smem, s, p, c, maps);
     return launch_status();

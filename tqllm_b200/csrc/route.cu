@@ -240,6 +240,11 @@ constexpr int RT_ROWS = 64, RT_TOK = 128, RT_K = 32, RT_THREADS = 256, RT_LD = R
 constexpr int RT_SPLIT_BELOW = 100, RT_MAX_PARTS = 64, RT_COLS = 256, RT_PLD = RT_ROWS + 4, RT_PART = RT_TOK * RT_PLD * 4;           // columns of a partial sum; a tile of them in shared memory, [token][row]
 constexpr int RT_W_STAGE = 3 * RT_ROWS * RT_LD * 2, RT_X_TERM = RT_TOK * RT_LD * 2;
 template <int DT> constexpr int rt_stages_bytes() { return 2 * (RT_W_STAGE + x_terms<DT>() * RT_X_TERM); }
+// what a split launch takes at most: a block's partial sums behind the stages, as many as fit beside 256 bytes of static arrays (eight blocks share RT_MAX_PARTS at most, the last sum takes the stages' place)
+template <int DT> constexpr int rt_split_most() {
+    const int fits = (227 * 1024 - 256 - rt_stages_bytes<DT>()) / RT_PART, most = RT_MAX_PARTS / 8 - 1;
+    return rt_stages_bytes<DT>() + (fits < most ? fits : most) * RT_PART;
+}
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
 }
@@ -539,7 +544,7 @@ __global__ void route2_k(const RouteSet a, const RouteSet b, int ld, const float
 // Top-k routing and dispatch in one launch for decode-sized batches: the block's 16 warps route the tokens (round
 // robin), then the same block builds the plan from the ids it just wrote. Saves a launch and a device-wide drain.
 // 512 threads: the register-resident top-k keeps 32 values per lane, which a 1024-thread block's 64 registers would spill.
-constexpr int RD_THREADS = 512;
+constexpr int RD_THREADS = 512, RD_SMEM = 160 * 1024;
 template <int GATING>
 __global__ void __launch_bounds__(RD_THREADS) route_dispatch_k(const float * logits, int ld, const float * __restrict__ bias,
                                                          int * __restrict__ ids, float * __restrict__ weights,
@@ -605,7 +610,7 @@ int32_t route_launch(const float * logits, int ld, const float * bias, int * ids
 // true when the one-cluster routing launch takes this shape: a warp per token, the plan built by one block
 bool route_cluster_fits(int experts, int topk, int n) {
     return n >= 1 && n <= RC_BLOCKS * (RD_THREADS / 32) && dispatch_small_path(experts, n * topk) &&
-           size_t(RD_THREADS / 32) * 2 * experts * sizeof(float) <= 160 * 1024;
+           size_t(RD_THREADS / 32) * 2 * experts * sizeof(float) <= RD_SMEM;
 }
 // Top-k + dispatch (+ staging of the n activation rows x[n][k] for the 4-bit decode kernels when x is given) as one cluster
 // launch. *took = false and B2MOE_OK when the shape does not fit: the caller takes the separate launches.
@@ -629,11 +634,11 @@ int32_t route_plan_stage(int gating, const float * logits, int ld, const float *
     cfg.attrs = attr;
     cfg.numAttrs = g_overlap ? 2 : 1;
     if (gating == B2MOE_SOFTMAX) {
-        if (cudaFuncSetAttribute(route_cluster_k<B2MOE_SOFTMAX>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)) != cudaSuccess) return B2MOE_ERR_CUDA;
+        if (!allow_smem(route_cluster_k<B2MOE_SOFTMAX>, RD_SMEM)) return B2MOE_ERR_CUDA;
         cudaLaunchKernelEx(&cfg, route_cluster_k<B2MOE_SOFTMAX>, logits, ld, (const float *)nullptr, ids, weights, shared_weights, experts, topk, 1, scale, n,
                            shared_first, shared_count, plan, st);
     } else {
-        if (cudaFuncSetAttribute(route_cluster_k<B2MOE_SIGMOID>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)) != cudaSuccess) return B2MOE_ERR_CUDA;
+        if (!allow_smem(route_cluster_k<B2MOE_SIGMOID>, RD_SMEM)) return B2MOE_ERR_CUDA;
         cudaLaunchKernelEx(&cfg, route_cluster_k<B2MOE_SIGMOID>, logits, ld, bias, ids, weights, (float *)nullptr, experts, topk, norm, scale, n,
                            shared_first, shared_count, plan, st);
     }
@@ -717,7 +722,7 @@ int32_t router_launch(const float * w, const float * shared, const void * xv, fl
         const bool split = n_part > 1 && tiles.x * tiles.y < RT_SPLIT_BELOW && n_part <= RT_MAX_PARTS && smem <= 227 * 1024;
         const auto kernel = split ? router_tile_k<DT, true> : router_tile_k<DT, false>;
         const size_t bytes = split ? smem : size_t(rt_stages_bytes<DT>());
-        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes)) != cudaSuccess) return B2MOE_ERR_CUDA;
+        if (!allow_smem(kernel, split ? rt_split_most<DT>() : bytes)) return B2MOE_ERR_CUDA;
         return launch_cluster_z(kernel, dim3(tiles.x, tiles.y, split ? ks : 1), RT_THREADS, bytes, s, w, shared, x, logits, ld, h, e, rows, n);
     }
     if (h % 16 == 0 && ceil_div(n, 64) <= GRID_Y) {
@@ -799,14 +804,14 @@ extern "C" B2MOE_API int32_t b2moe_route_dispatch(int32_t gating, const float * 
     // one launch only while every token has a warp of its own: the single block routes its tokens RD_THREADS / 32 at a time,
     // and a token's selection rounds are a dependent chain (measured: 64 tokens, 512 experts: 53 us fused against 12 + 10 us as
     // two launches)
-    if (n <= RD_THREADS / 32 && dispatch_small_path(experts, n * topk) && smem <= 160 * 1024) {
+    if (n <= RD_THREADS / 32 && dispatch_small_path(experts, n * topk) && smem <= RD_SMEM) {
         cudaStream_t s = as_stream(stream);
         if (gating == B2MOE_SOFTMAX) {
-            if (cudaFuncSetAttribute(route_dispatch_k<B2MOE_SOFTMAX>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)) != cudaSuccess) return B2MOE_ERR_CUDA;
+            if (!allow_smem(route_dispatch_k<B2MOE_SOFTMAX>, RD_SMEM)) return B2MOE_ERR_CUDA;
             launch_overlapped(route_dispatch_k<B2MOE_SOFTMAX>, dim3(1), dim3(RD_THREADS), smem, s, logits, ld, nullptr, ids, weights, shared_weights, experts,
                               topk, 1, scale, n, shared_first, shared_count, plan);
         } else {
-            if (cudaFuncSetAttribute(route_dispatch_k<B2MOE_SIGMOID>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)) != cudaSuccess) return B2MOE_ERR_CUDA;
+            if (!allow_smem(route_dispatch_k<B2MOE_SIGMOID>, RD_SMEM)) return B2MOE_ERR_CUDA;
             launch_overlapped(route_dispatch_k<B2MOE_SIGMOID>, dim3(1), dim3(RD_THREADS), smem, s, logits, ld, bias, ids, weights, nullptr, experts, topk,
                               norm, scale, n, shared_first, shared_count, plan);
         }
