@@ -88,9 +88,15 @@ class DeviceBank:
         return cls.from_int8(q.view(w.shape), scale.view(w.shape[:-1]), 1)
 
     def dequant(self) -> torch.Tensor:
+        stream = _stream_of(*_tensors(self))
         out = torch.empty(self.experts * self.rows, self.cols, dtype=torch.float32, device=self.data.device)
-        check(lib.b2moe_dequant_dump(C.byref(self.c), out.data_ptr(), _stream()), "b2moe_dequant_dump")
+        check(lib.b2moe_dequant_dump(C.byref(self.c), out.data_ptr(), stream), "b2moe_dequant_dump")
         return out
+
+
+def _tensors(*banks: DeviceBank | None) -> list:
+    """the arrays of banks, which may be the caller's own (DeviceBank.from_int8) and lie anywhere"""
+    return [t for b in banks if b is not None for t in (b.data, b.aux)]
 
 
 def router(router_w, x, shared_gate=None, ld=None):
@@ -304,23 +310,25 @@ def _bref(b: DeviceBank | None):
 def expert_gateup_swiglu(gate, up, x, plan: Plan, sh_gate=None, sh_up=None, act: torch.Tensor | None = None):
     """act [assignments, ff]; a buffer that is given keeps the rows of skipped assignments, without one they are zeros"""
     total = plan.n * plan.topk + plan.shared_tokens
+    stream = _stream_of(x, plan.buf, act, *_tensors(gate, up, sh_gate, sh_up))
     act = torch.zeros(total, gate.rows, dtype=torch.float32, device=x.device) if act is None else act
     assert act.dtype == torch.float32 and act.shape == (total, gate.rows) and act.is_contiguous()
     # room for a row per assignment: the grouped GEMM reads the rows of an expert as boxes then and does not gather them
     ws = _scratch(lib.b2moe_expert_slot_workspace_bytes(_bref(gate), total, _DT[x.dtype]), x.device)
     check(lib.b2moe_expert_gateup_swiglu(_bref(gate), _bref(up), _bref(sh_gate), _bref(sh_up), x.data_ptr(), _DT[x.dtype],
                                          plan.buf.data_ptr(), plan.n, plan.topk, plan.shared_tokens, act.data_ptr(),
-                                         _ptr(ws), 0 if ws is None else ws.numel(), _stream()), "b2moe_expert_gateup_swiglu")
+                                         _ptr(ws), 0 if ws is None else ws.numel(), stream), "b2moe_expert_gateup_swiglu")
     return act
 
 
 def expert_down(down, act, plan: Plan, sh_down=None, y: torch.Tensor | None = None):
     """y [assignments, hidden]; a buffer that is given keeps the rows of skipped assignments, without one they are zeros"""
+    stream = _stream_of(act, plan.buf, y, *_tensors(down, sh_down))
     y = torch.zeros(act.shape[0], down.rows, dtype=torch.float32, device=act.device) if y is None else y
     assert y.dtype == torch.float32 and y.shape == (act.shape[0], down.rows) and y.is_contiguous()
     ws = _scratch(lib.b2moe_expert_slot_workspace_bytes(_bref(down), act.shape[0], capi.F32), act.device)
     check(lib.b2moe_expert_down(_bref(down), _bref(sh_down), act.data_ptr(), plan.buf.data_ptr(), plan.n, plan.topk,
-                                plan.shared_tokens, y.data_ptr(), _ptr(ws), 0 if ws is None else ws.numel(), _stream()),
+                                plan.shared_tokens, y.data_ptr(), _ptr(ws), 0 if ws is None else ws.numel(), stream),
           "b2moe_expert_down")
     return y
 
@@ -398,6 +406,7 @@ class MoeLayer:
     @classmethod
     def from_banks(cls, shape, router_w, banks, shared_banks=None, sel_bias=None, shared_gate_vec=None):
         """A layer over finished banks (DeviceBank: gate, up, down, of any types, 8-bit ones among them) that it keeps; shape.types is not looked at"""
+        _stream_of(router_w, sel_bias, shared_gate_vec, *_tensors(*banks, *(shared_banks or ())))
         self = cls.__new__(cls)
         self.shape, self.experts, self.device = shape, banks[0].experts, router_w.device
         self.router_w, self.sel_bias, self.shared_gate_vec = router_w, sel_bias, shared_gate_vec
@@ -422,16 +431,17 @@ class MoeLayer:
     def forward(self, x: torch.Tensor, out: torch.Tensor | None = None, out_dtype=torch.float32, residual: torch.Tensor | None = None) -> torch.Tensor:
         """out = layer(x), or residual + layer(x) when a residual [n][hidden] of the output's dtype is given (it may be `out`)"""
         n = x.shape[0]
+        stream = _stream_of(self.router_w, x, out, residual)
         self.reserve(n)
         if out is None:
             out = torch.empty(n, self.shape.hidden, dtype=out_dtype if residual is None else residual.dtype, device=self.device)
         if residual is None:
             check(lib.b2moe_layer_forward(C.byref(self.c), x.data_ptr(), _DT[x.dtype], n, out.data_ptr(), _DT[out.dtype],
-                                          self.ws.data_ptr(), self.ws.numel(), _stream()), "b2moe_layer_forward")
+                                          self.ws.data_ptr(), self.ws.numel(), stream), "b2moe_layer_forward")
         else:
             assert residual.dtype == out.dtype and residual.shape == out.shape
             check(lib.b2moe_layer_forward_residual(C.byref(self.c), x.data_ptr(), _DT[x.dtype], n, residual.data_ptr(), out.data_ptr(),
-                                                   _DT[out.dtype], self.ws.data_ptr(), self.ws.numel(), _stream()), "b2moe_layer_forward_residual")
+                                                   _DT[out.dtype], self.ws.data_ptr(), self.ws.numel(), stream), "b2moe_layer_forward_residual")
         return out
 
     def artefacts(self) -> dict:
