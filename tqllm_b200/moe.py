@@ -405,7 +405,11 @@ class MoeLayer:
 
     @classmethod
     def from_banks(cls, shape, router_w, banks, shared_banks=None, sel_bias=None, shared_gate_vec=None):
-        """A layer over finished banks (DeviceBank: gate, up, down, of any types, 8-bit ones among them) that it keeps; shape.types is not looked at"""
+        """A layer over finished banks (DeviceBank: gate, up, down, of any types, 8-bit ones among them) that it keeps, with router_w [experts, hidden],
+        sel_bias [experts] and shared_gate_vec [hidden] in contiguous float32; shape.types is not looked at"""
+        for t, dims in ((router_w, (banks[0].experts, shape.hidden)), (sel_bias, (banks[0].experts,)), (shared_gate_vec, (shape.hidden,))):
+            if t is not None and (t.dtype is not torch.float32 or tuple(t.shape) != dims or not t.is_contiguous()):
+                raise capi.B2moeError(capi.ERR_SHAPE, "MoeLayer.from_banks: contiguous float32 router weights, selection bias and shared gate of the layer's sizes are wanted")
         _stream_of(router_w, sel_bias, shared_gate_vec, *_tensors(*banks, *(shared_banks or ())))
         self = cls.__new__(cls)
         self.shape, self.experts, self.device = shape, banks[0].experts, router_w.device
