@@ -15,6 +15,7 @@ from . import capi
 from .capi import check, lib
 
 _DT = {torch.float32: capi.F32, torch.float16: capi.F16, torch.bfloat16: capi.BF16}
+_INT = (1 << 31) - 1                       # the C ABI's int32: ctypes would take a larger number's low bits
 
 
 def _stream() -> int:
@@ -75,6 +76,8 @@ class DeviceBank:
             raise capi.B2moeError(capi.ERR_FORMAT, "DeviceBank.from_int8: contiguous int8 rows and float32 scales are wanted")
         if data.numel() != experts * rows * cols or scale.numel() != experts * rows or data.device != scale.device:
             raise capi.B2moeError(capi.ERR_SHAPE, "DeviceBank.from_int8: a scale for each row is wanted, on the same device")
+        if max(experts, rows, cols) > _INT:
+            raise capi.B2moeError(capi.ERR_SHAPE, "DeviceBank.from_int8: experts, rows and columns are 32-bit numbers")
         self = cls.__new__(cls)
         self.type, self.experts, self.rows, self.cols = capi.I8, experts, rows, cols
         self.data, self.aux = data, scale
@@ -148,6 +151,8 @@ def quantize_rows(x: torch.Tensor):
     ldx, one = x.stride()
     if one != 1 and k > 1:
         raise capi.B2moeError(capi.ERR_SHAPE, "quantize_rows: the values of a row have to be neighbours")
+    if max(n, k) > _INT:
+        raise capi.B2moeError(capi.ERR_SHAPE, "quantize_rows: rows and columns are 32-bit numbers")
     stream = _stream_of(x)
     q = torch.empty(n, k, dtype=torch.int8, device=x.device)
     scale = torch.empty(n, dtype=torch.float32, device=x.device)
@@ -164,6 +169,8 @@ def linear_i8(q: torch.Tensor, scale: torch.Tensor, bank: DeviceBank, out_dtype=
         raise capi.B2moeError(capi.ERR_SHAPE, "linear_i8: int8 rows of the bank's columns and a float32 scale for each are wanted")
     if one != 1 and k > 1:
         raise capi.B2moeError(capi.ERR_SHAPE, "linear_i8: the values of a row have to be neighbours")
+    if n > _INT:
+        raise capi.B2moeError(capi.ERR_SHAPE, "linear_i8: the number of rows is a 32-bit number")
     if status is not None and (status.dtype is not torch.int32 or status.numel() < 1):
         raise capi.B2moeError(capi.ERR_SHAPE, "linear_i8: the status is an int32 word")
     if out is not None:
@@ -191,12 +198,14 @@ def _balance_args(logits, experts, mask, offsets):
     ld, one = logits.stride()
     if logits.dtype is not torch.float32 or cols < experts or (one != 1 and experts > 1):
         raise capi.B2moeError(capi.ERR_SHAPE, "balance loss: float32 logits with contiguous rows of at least as many columns as experts are wanted")
+    if max(n, ld if n > 1 else cols) > _INT:                           # (experts are no more than the columns)
+        raise capi.B2moeError(capi.ERR_SHAPE, "balance loss: tokens, columns and the row stride of the logits are 32-bit numbers")
     if mask is not None and (mask.numel() != n or mask.dtype not in (torch.bool, torch.uint8) or not mask.is_contiguous()):
         raise capi.B2moeError(capi.ERR_SHAPE, "balance loss: the mask has a byte for each token")
     if offsets is None:
         return n, ld if n > 1 else cols, 1
     sequences = offsets.numel() - 1
-    if offsets.dtype is not torch.int32 or sequences < 1 or not offsets.is_contiguous():
+    if offsets.dtype is not torch.int32 or sequences < 1 or sequences > _INT or not offsets.is_contiguous():
         raise capi.B2moeError(capi.ERR_SHAPE, "balance loss: the offsets are int32, one more than sequences")
     return n, ld if n > 1 else cols, sequences
 
@@ -231,6 +240,8 @@ def balance_loss_backward(logits, saved: Balance, topk, coef, gating=capi.SOFTMA
         if grad.dtype is not torch.float32 or grad.shape[0] != n or grad.shape[1] < experts or (grad.stride(1) != 1 and experts > 1):
             raise capi.B2moeError(capi.ERR_SHAPE, "balance loss: the gradient has float32 rows like the logits")
         ldg = grad.stride(0) if n > 1 else grad.shape[1]
+        if ldg > _INT:
+            raise capi.B2moeError(capi.ERR_SHAPE, "balance loss: the row stride of the gradient is a 32-bit number")
     stream = _stream_of(logits, saved.counts, saved.tokens, mask, offsets, grad_loss, out)
     if grad is None:
         grad = logits.new_empty((n, experts))
