@@ -12,6 +12,7 @@
 // chunks), so a block finds its chunk from the offsets alone, without a scan and without the host knowing them. Each chunk leaves the sums of its
 // rows of probabilities and its counts in the workspace; a second launch adds them up in a fixed order, so that a batch gives the same bits every time.
 #include <algorithm>
+#include <climits>
 #include <type_traits>
 
 #include "common.cuh"
@@ -80,6 +81,21 @@ struct Row {
             x = red[w / G * G];
 #pragma unroll
             for (int i = 1; i < G; ++i) x = largest ? fmaxf(x, red[w / G * G + i]) : x + red[w / G * G + i];
+        }
+        return x;
+    }
+    // the least of whole numbers, as all()
+    __device__ __forceinline__ int least(int x) {
+        x = __reduce_min_sync(0xffffffffu, x);
+        if (G > 1) {
+            const int w = threadIdx.x >> 5;
+            int * words = reinterpret_cast<int *>(red);
+            __syncthreads();
+            if ((threadIdx.x & 31) == 0) words[w] = x;
+            __syncthreads();
+            x = words[w / G * G];
+#pragma unroll
+            for (int i = 1; i < G; ++i) x = min(x, words[w / G * G + i]);
         }
         return x;
     }
@@ -317,16 +333,18 @@ __global__ void __launch_bounds__(BAL_THREADS) balance_backward_k(const BalBackA
     row.first = (warp % G) * 32 + lane;
     const float tokens = float(p.tokens[c.x]);
     const float factor = (p.grad_loss ? *p.grad_loss : 1.f) * p.coef / float(max(p.tokens[p.sequences], 1)) * float(p.experts) / (float(p.topk) * tokens * tokens);
-    float weight[V], least = INFINITY;
+    // what the counts have more than the least, from whole numbers: 32-bit floats do not hold counts from 2^24 on
+    int count[V], least = INT_MAX;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
         const int e = row.first + 32 * G * i;
-        weight[i] = e < p.experts ? float(p.counts[size_t(c.x) * p.experts + e]) : INFINITY;
-        least = fminf(least, weight[i]);
+        count[i] = e < p.experts ? p.counts[size_t(c.x) * p.experts + e] : INT_MAX;
+        least = min(least, count[i]);
     }
-    least = -row.all(-least, true);
+    least = row.least(least);
+    float weight[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) weight[i] = row.first + 32 * G * i < p.experts ? weight[i] - least : 0.f;
+    for (int i = 0; i < V; ++i) weight[i] = row.first + 32 * G * i < p.experts ? float(count[i] - least) : 0.f;
 #pragma unroll 1
     for (int t0 = c.y; t0 < c.z; t0 += ROWS) {
         const int t = t0 + group;
