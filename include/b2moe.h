@@ -277,8 +277,8 @@ B2MOE_API int32_t b2moe_combine_residual(const float * y, const int32_t * ids, c
  *   left as they are.
  * b2moe_linear_i8: y[t][r] = (sum_j q[t][j] w[r][j]) * (scale[t] * aux[r]) rounded once to y_dtype, rows of y ldy elements
  *   apart; the sum is exact. w is a bank of type B2MOE_I8 with one expert; q as b2moe_quantize_rows leaves it (any values of int8).
- *   status (device int32, may be null): set to a nonzero value where a kernel gave up a bounded wait (the output is then
- *   invalid), otherwise left as it is. */
+ *   status (device int32, may be null): set to a nonzero value where a kernel gave up a bounded wait, otherwise left as it is.
+ *   Outputs that such a launch did not finish are NaN, with or without the word (those of the expert products on such banks, too). */
 B2MOE_API int32_t b2moe_quantize_rows(const void * x, int32_t x_dtype, int64_t ldx, int32_t n, int32_t k, int8_t * q, int64_t ldq, float * scale,
                             b2moe_stream stream);
 B2MOE_API int32_t b2moe_linear_i8(const int8_t * q, int64_t ldq, const float * scale, const b2moe_bank * w, int32_t n, void * y, int32_t y_dtype,

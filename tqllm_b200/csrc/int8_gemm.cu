@@ -121,6 +121,13 @@ __device__ __forceinline__ void store_item(const I8Args & p, const TcItem & im, 
     }
 }
 
+// The outputs of an item that was left unfinished by a wait that ran out: NaN, since the call may have no status word to tell. One weight row; of the item's activation rows this half's 16 of every 32.
+// Not inlined, so that it takes no registers from what happens
+__device__ __noinline__ void spoil_rows(void * y, int dtype, long long ldy, int row, const int2 * t, int count, int half) {
+    for (int c = 16 * half; c < count; c += 32)
+        for (int j = c; j < min(c + 16, count); ++j) store_act(y, dtype, size_t(uint32_t(t[j].x)) * ldy + row, __int_as_float(0x7fc00000));
+}
+
 // SPLIT (dense calls with few items): the blocks of a cluster take parts of an item's columns each, and then a share of its activation rows each, whose parts they
 // read from one another's shared memory: whole numbers, so the sum is the same
 // PAIR (long rows): two blocks take neighbouring blocks of weight rows of the same activation rows, of which each brings a half: the copies from the L2, which set the pace of
@@ -378,8 +385,10 @@ __global__ void __launch_bounds__(TC_THREADS, MODE ? 1 : 2) i8_gemm_k(const I8Ar
                 if (p.y_dtype == B2MOE_F32) store_item<MATS, float>(p, im, taddr, table[h], scale, quarter, half, lane);
                 else if (p.y_dtype == B2MOE_F16) store_item<MATS, __half>(p, im, taddr, table[h], scale, quarter, half, lane);
                 else store_item<MATS, __nv_bfloat16>(p, im, taddr, table[h], scale, quarter, half, lane);
-            } else if (lane == 0) {
-                give_up();
+            } else {
+                if (lane == 0) give_up();
+                const int row = weight_row<MATS>(im, quarter, lane);
+                if (row < p.rows) spoil_rows(p.y, p.y_dtype, p.ldy, row, table[h], im.count, half);
             }
             fence_before();
             __syncwarp();
@@ -430,6 +439,8 @@ __global__ void __launch_bounds__(TC_THREADS, MODE ? 1 : 2) i8_gemm_k(const I8Ar
             }
         }
         cluster.sync();                                                // the parts stay until every block has read them
+        if (abort_flag && in)                                          // and where this block has no part, what the cluster stored of the item is none
+            for (int col = threadIdx.x >> 7; col < im.count; col += STEP) store_act(p.y, p.y_dtype, size_t(im.first + col) * p.ldy + row, __int_as_float(0x7fc00000));
     }
 }
 

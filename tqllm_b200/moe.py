@@ -161,7 +161,8 @@ def quantize_rows(x: torch.Tensor):
 
 
 def linear_i8(q: torch.Tensor, scale: torch.Tensor, bank: DeviceBank, out_dtype=torch.bfloat16, out: torch.Tensor | None = None, status: torch.Tensor | None = None):
-    """y [n, rows] = (q . w) * scale[t] * bank scale[r] of 8-bit rows (b2moe_linear_i8); q and out may be rows of wider matrices"""
+    """y [n, rows] = (q . w) * scale[t] * bank scale[r] of 8-bit rows (b2moe_linear_i8); q and out may be rows of wider matrices. A launch that gives up a bounded
+    wait leaves NaN in what it did not finish, and a nonzero value in `status` where that is given"""
     n, k = q.shape
     ldq, one = q.stride()
     ldy = rows = bank.rows
