@@ -241,13 +241,14 @@ void launch_quant(const QuantArgs & a, cudaStream_t s) {
     // Many rows (they fill the SMs with 16 warps each): four pieces a thread, a warp a row where that does. 8192 x 4096 bf16 with 256 / 128 / 64 threads a row 28.6 / 22.2 / 18.5 us,
     // 40960 x 512 fp32 with a warp a block / eight warps of a row each 43.4 / 19.2. Rows that are written to several slots have more stores than loads and take the other shape (4096 x 2048 to ten slots
     // each 26 / 18)
-    if (!SCATTER && a.n >= 148 * 16) {
-        const int blocks = ceil_div(a.n, 8);
-        if (by_warp == 1) return go(quant_rows_k<DT, 1, true, SCATTER>, blocks, 256);
-        if (by_warp == 2) return go(quant_rows_k<DT, 2, true, SCATTER>, blocks, 256);
-        if (by_warp <= 4) return go(quant_rows_k<DT, 4, true, SCATTER>, blocks, 256);
-        if (by_warp <= 32) return go(quant_rows_k<DT, 4, false, SCATTER>, a.n, ceil_div(by_warp, 4) * 32);
-    }
+    if constexpr (!SCATTER)
+        if (a.n >= 148 * 16) {
+            const int blocks = ceil_div(a.n, 8);
+            if (by_warp == 1) return go(quant_rows_k<DT, 1, true, false>, blocks, 256);
+            if (by_warp == 2) return go(quant_rows_k<DT, 2, true, false>, blocks, 256);
+            if (by_warp <= 4) return go(quant_rows_k<DT, 4, true, false>, blocks, 256);
+            if (by_warp <= 32) return go(quant_rows_k<DT, 4, false, false>, a.n, ceil_div(by_warp, 4) * 32);
+        }
     // a few: as many threads as the row has pieces, up to 256
     const int threads = std::min(256, by_warp * 32), per = ceil_div(pieces, threads);
     if (per == 1) go(quant_rows_k<DT, 1, false, SCATTER>, a.n, threads);
