@@ -6,8 +6,9 @@
 // l + 16 of the epilogue hold both sums of an output.
 //
 // One block per SM (two for short rows) walks the items (tile of activation rows, block of weight rows): one thread issues the copies into a ring, one the products, eight warps
-// empty one accumulator while the next one fills. 8192 rows of 4096 x 4096: 85.7 us, 3.2e15 operations a second (1.93 of the measured bf16 rate; 96 without pairs, 150 with items of
-// 128 rows). The grouped products are bound by reading the weights: gate/up of 128 experts of 1408 x 4096 at 16 rows each 241 us, 6.1 TB/s (0.94 of measured), down of 512 of 2048 x 512 at 1.2 rows each 62 us, 5.9 TB/s.
+// empty one accumulator while the next one fills.
+//   8192 rows of 4096 x 4096: 86 to 90 us by card, 3.2e15 operations a second (1.93 of the measured bf16 rate); 96 without pairs, 150 with items of 128 rows. Bound by the tensor pipe.
+//   gate/up of 128 experts of 1408 x 4096 at 16 rows each: 241 us, 6.1 TB/s (0.94 of measured); down of 512 of 2048 x 512 at 1.2 rows each: 62 us, 5.9 TB/s. Bound by reading the weights.
 #include <cooperative_groups.h>
 #include <cuda.h>
 
@@ -494,9 +495,11 @@ int clusters_at_once(int size) {
     }();
     return most[size];
 }
-// Blocks that share an item's columns: as many as one round of clusters has room for, with four steps of 128 columns each at least, and none where an item has fewer
-// than 16: a step takes such a block 0.3 us, the meeting at the end 1.5 to 2 us and more with many rows. us, one block / this: 16 rows 4096 x 4096 11.2 / 7.9, 1411 x 2560 7.6 / 5.7, 2048 x 8192
-// 19.3 / 8.3, 8192 x 1024 4.9 / 6.4 with two; 128 rows 13.8 / 10.0, 10.1 / 7.5, 22.6 / 10.3, 7.1 / 9.9
+// Blocks that share an item's columns: as many as one round of clusters has room for, with four steps of 128 columns each at least, and none where an item has fewer than 16: a step takes such a
+// block 0.3 us, the meeting at the end 1.5 to 2 us and more with many rows. us, one block / this:
+//              4096 x 4096    1411 x 2560    2048 x 8192    8192 x 1024 (with two)
+//    16 rows   11.2 / 7.9      7.6 / 5.7     19.3 / 8.3      4.9 / 6.4
+//   128 rows   13.8 / 10.0    10.1 / 7.5     22.6 / 10.3     7.1 / 9.9
 int split_of(long long items, int steps) {
     int split = 1;
     for (int s = 2; s <= TC_MAX_SPLIT; ++s)
@@ -505,8 +508,9 @@ int split_of(long long items, int steps) {
 }
 
 // Activation rows of an item of a dense call: the rows are cut alike into the number of tiles that is expected to cost least. In steps of an item of 256 rows: a round of items takes its steps
-// in proportion to 128 + rows (its weights, its rows), those that share columns meet for six of 128 rows. us, with items of 128 or 256 rows / cut alike: 515 rows of 4096 x 4096 21.9 / 15.4, 1000
-// 24.7 / 18.3, 1500 27.3 / 25.7; 2100 of 1411 x 2560 17.6 / 13.0; 1500 of 4096 x 1408 17.6 / 15.0; 515 of 4096 x 512 6.4 / 5.6
+// in proportion to 128 + rows (its weights, its rows), those that share columns meet for six of 128 rows. us, with items of 128 or 256 rows / cut alike:
+//   rows of 4096 x 4096: 515 21.9 / 15.4, 1000 24.7 / 18.3, 1500 27.3 / 25.7
+//   2100 rows of 1411 x 2560 17.6 / 13.0, 1500 of 4096 x 1408 17.6 / 15.0, 515 of 4096 x 512 6.4 / 5.6
 int dense_rows(int n, int row_blocks, int steps, bool longer, bool two, int sms) {
     const int most = two ? 128 : 256, least = two ? 32 : 96, first = ceil_div(n, most);
     int best = most;
@@ -533,14 +537,21 @@ template <int MATS>
 int32_t i8_gemm(const I8Args & p, long long q_rows, int per_group, int * status, cudaStream_t s) {
     TcArgs c{};
     c.row_blocks = ceil_div(p.rows, MATS == 2 ? 64 : 128);
-    // Items of 256 rows halve what the weights cost in copies and products (8192 x 4096 x 4096: 96 us, with 128 rows 150), items of 128 leave room for six ring
-    // stages instead of four and waste less where an expert has fewer (512 experts at 80 each, gate/up 211 against 225 us; 128 experts at 128 each with a
-    // skewed load 385 and 333); below that nothing is gained (64 rows, 16 each: 248 and 242). Pairs pay from long rows on, where the products of an item outlast what its blocks tell each other: us, single / pair: 8192 x 4096 rows of 4096 columns 96.5 / 87.1, of 2048 59.6 / 60.3,
-    // of 1024 49.1 / 53.6; 8192 x 8192 of 8192 378.6 / 353.0; gate/up, 128 experts of 4096 columns at 16 each 248.5 (items of 128) / 246.2, at 160 344.9 / 326.2, at 320 613 / 584; 512 of 2048 at 160 304 / 318;
-    // down, 512 of 512 columns at 80 193 / 242
-    // Short rows: two blocks an SM with half the ring each, since an item of a few steps takes longer from its first copy to its last store than its copies alone, and one block's items hide
-    // behind the other's. us, one / two: down, 512 experts of 512 columns at one row each 76 / 60, at 80 192 / 178, at 320 650 / 498, of 768 columns at 40 64 / 67; gate/up of 512 columns at 8 107 / 78;
-    // dense 8192 rows, 4096 x 512 44 / 36, 4096 x 1024 49 / 42; gate/up of 2048 columns at 80 242 / 258.
+    // The shape of a launch, by the columns and the rows that an item will have. Times in us.
+    // Items of 256 rows halve what the weights cost in copies and products; items of 128 leave room for six ring stages instead of four and waste less where an expert has fewer. 256 / 128:
+    //   dense 8192 rows of 4096 x 4096                96 / 150
+    //   gate/up, 512 experts at 80 rows each         225 / 211
+    //   gate/up, 128 experts at 128 each, skewed     333 / 385
+    // (64 rows gain nothing further: 248 against 242 with 128, at 16 each.)
+    // Pairs pay from long rows on, where the products of an item outlast what its blocks tell each other. Single / pair:
+    //   dense 8192 rows of 4096 x 4096              96.5 / 87.1      of 4096 x 2048    59.6 / 60.3      of 4096 x 1024    49.1 / 53.6      of 8192 x 8192    378.6 / 353.0
+    //   gate/up, 128 experts of 4096 columns, at 16 each 248.5 (items of 128) / 246.2, at 160 344.9 / 326.2, at 320 613 / 584
+    //   gate/up, 512 experts of 2048 columns, at 160 each 304 / 318      down, 512 of 512 columns at 80 each 193 / 242
+    // Short rows: two blocks an SM with half the ring each. An item of a few steps takes longer from its first copy to its last store than its copies alone, and one block's items hide behind the
+    // other's. One / two:
+    //   down, 512 experts of 512 columns, at one row each 76 / 60, at 80 192 / 178, at 320 650 / 498; of 768 columns at 40 64 / 67
+    //   gate/up of 512 columns at 8 each 107 / 78, of 2048 columns at 80 242 / 258
+    //   dense 8192 rows of 4096 x 512 44 / 36, of 4096 x 1024 49 / 42
     const int sms = sm_count();
     const bool longer = p.cols > 2560, two = p.cols <= I8_SHORT_COLS;
     if (p.plan) c.nt = two ? 128 : per_group > 96 || longer ? 256 : 128;

@@ -127,9 +127,10 @@ __global__ void __launch_bounds__(512) i8_stream_k(const I8Args p) {
 }
 
 // Warps that share a block's columns: eight where a launch has few blocks, else four; sixteen for long rows of a dense call whose blocks are all on the SMs at once. us with 4 / 8 / 16, one row:
-// 4096 x 4096 10.0 / 6.5 / 4.6, 2048 x 8192 15.7 / 9.3 / 6.2, 1411 x 2560 5.1 / 3.6 / 2.9, 1024 x 2048 4.2 / 3.0 / 2.7, 512 x 1024 2.4 / 2.2 / 2.4, 8192 x 1024 3.7 / 3.4 / 5.5; gate/up of one token of
-// ten experts 11.3 / 9.0 / 12.1. Eight steps at once where a warp has as many (8192 x 8192 16.1 -> 15.3, 2048 x 8192 6.1 -> 5.7; down of 64 experts of 4096 x 4096 at
-// three each 181.6 -> 171.8, of eight of 2048 x 4096 17.9 -> 17.0; where it has fewer it loses: 4096 x 4096 4.5 -> 4.8)
+//   4096 x 4096 10.0 / 6.5 / 4.6      2048 x 8192 15.7 / 9.3 / 6.2      1411 x 2560 5.1 / 3.6 / 2.9      1024 x 2048 4.2 / 3.0 / 2.7
+//   512 x 1024   2.4 / 2.2 / 2.4      8192 x 1024  3.7 / 3.4 / 5.5      gate/up of one token of ten experts 11.3 / 9.0 / 12.1
+// Eight steps at once where a warp has as many (before / with): 8192 x 8192 16.1 / 15.3, 2048 x 8192 6.1 / 5.7; down of 64 experts of 4096 x 4096 at three each 181.6 / 171.8, of eight of
+// 2048 x 4096 17.9 / 17.0; where it has fewer it loses: 4096 x 4096 4.5 / 4.8
 template <int MATS, int NT>
 int32_t launch_stream(const I8Args & a, int groups, cudaStream_t s) {
     const int blocks = ceil_div(a.rows, 16), steps = ceil_div(a.cols, 64);
@@ -170,11 +171,15 @@ size_t i8_workspace_bytes(int rows_x, int k) { return i8_rows_bytes(rows_x, k); 
 size_t i8_slot_bytes(int slot_rows, int k) { return i8_rows_bytes(slot_rows, k) + align_up(size_t(slot_rows) * sizeof(int), 256); }
 
 // The form of a product: the streaming kernel for a few rows, the tensor-core GEMM (int8_gemm.cu) for more. us, streamed / GEMM:
-//   dense, from 17 rows on: 4096 x 4096 16 rows 5.5 / 8.0, 24 7.9 / 8.0, 48 13.1 / 8.2; 2048 x 8192 16 6.9 / 8.8, 17 10.4 / 8.9; 1411 x 2560 16 3.6 / 5.9, 32 5.7 / 6.0; 8192 x 8192 16 17.3 / 15.5, 17 22.4 / 15.3
-//   gate/up, from seven rows per expert on: 128 experts of 1408 x 4096 at 4 each 221 / 233, at 8 307 / 245; 512 of 512 x 2048 at 2.5 155 / 168, at 5 184 / 187; 32 of 512 x 1024 at 4 8.9 / 14.2, at 16
-//   17.1 / 15.3 (the GEMM's times have a launch more in them, since its rows lie in slot order)
-//   down, where they are in slot order anyway, also where the SMs get eight items each, and for short rows from three per expert or four items an SM on: 128 of 4096 x 1408 at 0.5 63 / 60, at 1
-//   95 / 80, at 4 138 / 120; 512 of 2048 x 512 two tokens of ten 9.5 / 9.7, four 14.8 / 11.9, 64 110 / 67; 32 of 1024 x 512 at 2 7.8 / 7.7, at 4 9.6 / 7.6
+//   dense, from 17 rows on
+//     4096 x 4096   16 rows 5.5 / 8.0, 24 7.9 / 8.0, 48 13.1 / 8.2          2048 x 8192   16 6.9 / 8.8, 17 10.4 / 8.9
+//     1411 x 2560   16 3.6 / 5.9, 32 5.7 / 6.0                              8192 x 8192   16 17.3 / 15.5, 17 22.4 / 15.3
+//   gate/up, from seven rows per expert on (the GEMM's times have a launch more in them, since its rows lie in slot order)
+//     128 experts of 1408 x 4096   at 4 each 221 / 233, at 8 307 / 245      512 of 512 x 2048   at 2.5 155 / 168, at 5 184 / 187
+//     32 of 512 x 1024   at 4 8.9 / 14.2, at 16 17.1 / 15.3
+//   down, where they are in slot order anyway, also where the SMs get eight items each, and for short rows from three per expert or four items an SM on
+//     128 of 4096 x 1408   at 0.5 63 / 60, at 1 95 / 80, at 4 138 / 120     512 of 2048 x 512   two tokens of ten 9.5 / 9.7, four 14.8 / 11.9, 64 110 / 67
+//     32 of 1024 x 512   at 2 7.8 / 7.7, at 4 9.6 / 7.6
 constexpr int I8_DENSE_ROWS = 16, I8_GEMM_MIN_PER = 7, I8_SHORT_MIN_PER = 3, I8_MANY_ITEMS = 148 * 8, I8_SHORT_ITEMS = 148 * 4;
 bool i8_takes_gemm(int experts, bool worth) {
     const int family = harness_family();

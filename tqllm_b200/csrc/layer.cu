@@ -269,7 +269,7 @@ extern "C" B2MOE_API int32_t b2moe_expert_gateup_swiglu(const b2moe_bank * gate,
     return expert_gateup(gate, up, shared_gate, shared_up, x, x_dtype, plan, n, topk, shared_tokens, act, workspace, workspace_bytes, stream, false);
 }
 
-// plan_ready: the launch before this call's is a gate/up product over the same plan, which another launch made. The LAST kernel of that product (dec4_k, gemm_tc_k; the others have no early release) waits
+// plan_ready: the launch before this call's is a gate/up product over the same plan, which another launch made. The LAST kernel of that product (dec4_k, gemm_tc_k, i8_stream_k, i8_gemm_k; the others have no early release) waits
 // for the launches before it and only then, when its own work is done, lets the next one begin, so whatever begins here finds the plan complete and may ask for weights before it waits. A product
 // that ends with a kernel which releases before its wait, as the conversions in front of the last kernels do, would break this
 static int32_t expert_down(const b2moe_bank * down, const b2moe_bank * shared_down, const float * act, const int32_t * plan, int32_t n, int32_t topk,
