@@ -288,7 +288,7 @@ B2MOE_API int32_t b2moe_linear_i8(const int8_t * q, int64_t ldq, const float * s
  * The auxiliary loss that keeps a router's load even, with the counts per expert and sequence, and its gradient on the
  * logits. It has no counterpart in the reference (which serves).
  *   p[t] = softmax of logits[t][0..experts) (B2MOE_SOFTMAX), or their sigmoids divided by their sum (B2MOE_SIGMOID; no bias);
- *   a row whose logits are all -inf has p = 0; any NaN makes its row, its sequence's means and the loss NaN
+ *   a row whose logits are all -inf has p = 0; any NaN (and, for B2MOE_SOFTMAX, +inf) makes its row, its sequence's means and the loss NaN
  *   tokens[s] = tokens of sequence s that the mask keeps; counts[s][e] = their assignments to e; prob[s][e] = their mean p[t][e]
  *   loss = coef / S * sum over the S sequences with tokens of experts / (topk tokens[s]) * sum_e counts[s][e] prob[s][e]
  * logits fp32, rows ld apart (further columns, as a shared expert's, are not read); ids [n][topk], ids outside [0, experts) are
