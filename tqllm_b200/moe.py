@@ -27,20 +27,24 @@ def _ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
 
-def _stream_of(t: torch.Tensor, *others: torch.Tensor | None) -> int:
-    """the current stream, for tensors that are all on the current device (a launch there on another one's memory would fault)"""
+def _stream_of(t: torch.Tensor, *others: torch.Tensor | None, banks: tuple = ()) -> int:
+    """the current stream, for tensors and banks that are all on the current device (a launch there on another one's memory would fault)"""
     dev = t.get_device()
     if dev >= 0 and dev == torch._C._cuda_getDevice():
         for o in others:
             if o is not None and o.get_device() != dev:
                 break
         else:
-            return torch._C._cuda_getCurrentRawStream(dev)
+            for b in banks:
+                if b is not None and b.index != dev:
+                    break
+            else:
+                return torch._C._cuda_getCurrentRawStream(dev)
     raise capi.B2moeError(capi.ERR_CUDA, "tensors on the current CUDA device are wanted")
 
 
 class DeviceBank:
-    """One stacked expert matrix [experts * rows][cols] in bank layout on the device."""
+    """One stacked expert matrix [experts * rows][cols] in bank layout on the device (`index`: the device's, asked for once; -1 for host memory)."""
 
     def __init__(self, type_id: int, raw: torch.Tensor, experts: int, rows: int, cols: int):
         assert raw.is_cuda and raw.dtype == torch.uint8
@@ -52,7 +56,7 @@ class DeviceBank:
         self.aux = torch.empty(experts * aux_bytes // 4, dtype=torch.float32, device=raw.device) if aux_bytes else None
         check(lib.b2moe_bank_load(type_id, raw.data_ptr(), experts, rows, cols, self.data.data_ptr(), _ptr(self.aux), _stream()),
               "b2moe_bank_load")
-        self.c = capi.Bank(self.data.data_ptr(), _ptr(self.aux), type_id, experts, rows, cols)
+        self.c, self.index = capi.Bank(self.data.data_ptr(), _ptr(self.aux), type_id, experts, rows, cols), self.data.get_device()
 
     @classmethod
     def from_packed(cls, type_id: int, data, aux, experts: int, rows: int, cols: int, device="cuda"):
@@ -63,7 +67,7 @@ class DeviceBank:
             raise capi.B2moeError(capi.ERR_SHAPE, "DeviceBank.from_packed: byte count does not match the shape")
         self.data = torch.as_tensor(data).to(device)
         self.aux = None if aux is None else torch.as_tensor(aux).to(device)
-        self.c = capi.Bank(self.data.data_ptr(), _ptr(self.aux), type_id, experts, rows, cols)
+        self.c, self.index = capi.Bank(self.data.data_ptr(), _ptr(self.aux), type_id, experts, rows, cols), self.data.get_device()
         return self
 
     @classmethod
@@ -81,7 +85,7 @@ class DeviceBank:
         self = cls.__new__(cls)
         self.type, self.experts, self.rows, self.cols = capi.I8, experts, rows, cols
         self.data, self.aux = data, scale
-        self.c = capi.Bank(data.data_ptr(), scale.data_ptr(), capi.I8, experts, rows, cols)
+        self.c, self.index = capi.Bank(data.data_ptr(), scale.data_ptr(), capi.I8, experts, rows, cols), data.get_device()
         return self
 
     @classmethod
@@ -91,15 +95,10 @@ class DeviceBank:
         return cls.from_int8(q.view(w.shape), scale.view(w.shape[:-1]), 1)
 
     def dequant(self) -> torch.Tensor:
-        stream = _stream_of(*_tensors(self))
+        stream = _stream_of(self.data, self.aux)
         out = torch.empty(self.experts * self.rows, self.cols, dtype=torch.float32, device=self.data.device)
         check(lib.b2moe_dequant_dump(C.byref(self.c), out.data_ptr(), stream), "b2moe_dequant_dump")
         return out
-
-
-def _tensors(*banks: DeviceBank | None) -> list:
-    """the arrays of banks, which may be the caller's own (DeviceBank.from_int8) and lie anywhere"""
-    return [t for b in banks if b is not None for t in (b.data, b.aux)]
 
 
 def router(router_w, x, shared_gate=None, ld=None):
@@ -179,7 +178,7 @@ def linear_i8(q: torch.Tensor, scale: torch.Tensor, bank: DeviceBank, out_dtype=
             raise capi.B2moeError(capi.ERR_SHAPE, "linear_i8: an output [n, rows] with contiguous rows is wanted")
         out_dtype = out.dtype
         ldy = out.stride(0) if n > 1 else rows
-    stream = _stream_of(q, scale, bank.data, bank.aux, out, status)
+    stream = _stream_of(q, scale, out, status, banks=(bank,))
     if out is None:
         out = torch.empty(n, rows, dtype=out_dtype, device=q.device)
     check(lib.b2moe_linear_i8(q.data_ptr(), ldq if n > 1 else k, scale.data_ptr(), C.byref(bank.c), n, out.data_ptr(), _DT[out_dtype], ldy, _ptr(status), stream), "b2moe_linear_i8")
@@ -322,7 +321,7 @@ def _bref(b: DeviceBank | None):
 def expert_gateup_swiglu(gate, up, x, plan: Plan, sh_gate=None, sh_up=None, act: torch.Tensor | None = None):
     """act [assignments, ff]; a buffer that is given keeps the rows of skipped assignments, without one they are zeros"""
     total = plan.n * plan.topk + plan.shared_tokens
-    stream = _stream_of(x, plan.buf, act, *_tensors(gate, up, sh_gate, sh_up))
+    stream = _stream_of(x, plan.buf, act, banks=(gate, up, sh_gate, sh_up))
     act = torch.zeros(total, gate.rows, dtype=torch.float32, device=x.device) if act is None else act
     assert act.dtype == torch.float32 and act.shape == (total, gate.rows) and act.is_contiguous()
     # room for a row per assignment: the grouped GEMM reads the rows of an expert as boxes then and does not gather them
@@ -335,7 +334,7 @@ def expert_gateup_swiglu(gate, up, x, plan: Plan, sh_gate=None, sh_up=None, act:
 
 def expert_down(down, act, plan: Plan, sh_down=None, y: torch.Tensor | None = None):
     """y [assignments, hidden]; a buffer that is given keeps the rows of skipped assignments, without one they are zeros"""
-    stream = _stream_of(act, plan.buf, y, *_tensors(down, sh_down))
+    stream = _stream_of(act, plan.buf, y, banks=(down, sh_down))
     y = torch.zeros(act.shape[0], down.rows, dtype=torch.float32, device=act.device) if y is None else y
     assert y.dtype == torch.float32 and y.shape == (act.shape[0], down.rows) and y.is_contiguous()
     ws = _scratch(lib.b2moe_expert_slot_workspace_bytes(_bref(down), act.shape[0], capi.F32), act.device)
@@ -422,7 +421,7 @@ class MoeLayer:
         for t, dims in ((router_w, (banks[0].experts, shape.hidden)), (sel_bias, (banks[0].experts,)), (shared_gate_vec, (shape.hidden,))):
             if t is not None and (t.dtype is not torch.float32 or tuple(t.shape) != dims or not t.is_contiguous()):
                 raise capi.B2moeError(capi.ERR_SHAPE, "MoeLayer.from_banks: contiguous float32 router weights, selection bias and shared gate of the layer's sizes are wanted")
-        _stream_of(router_w, sel_bias, shared_gate_vec, *_tensors(*banks, *(shared_banks or ())))
+        _stream_of(router_w, sel_bias, shared_gate_vec, banks=(*banks, *(shared_banks or ())))
         self = cls.__new__(cls)
         self.shape, self.experts, self.device = shape, banks[0].experts, router_w.device
         self.router_w, self.sel_bias, self.shared_gate_vec = router_w, sel_bias, shared_gate_vec
