@@ -284,6 +284,30 @@ B2MOE_API int32_t b2moe_quantize_rows(const void * x, int32_t x_dtype, int64_t l
 B2MOE_API int32_t b2moe_linear_i8(const int8_t * q, int64_t ldq, const float * scale, const b2moe_bank * w, int32_t n, void * y, int32_t y_dtype,
                         int64_t ldy, int32_t * status, b2moe_stream stream);
 
+/* ---- norm ----------------------------------------------------------------------------------------------------------
+ * The root-mean-square norm in front of a layer or a projection, with the skip connection's addition (the engines' add_sumsq + norm,
+ * src/models/qwen/qwen35/qwen35_forward.cpp:1113) and an output in 8 bits for b2moe_linear_i8, in one pass over the rows.
+ * b2moe_rms_norm: h = x + residual in 32 bits (residual may be null: h = x), sum = h rounded (null: not wanted; needs a residual),
+ *   y = h / sqrt(mean(h^2) + eps) * weight, rounded once (null: not wanted),
+ *   q, scale (null: not wanted): the integers nearest to 127 u / max|u|, halves to even, exactly, with u = h weight as it is before any rounding, and
+ *   scale = max|u| / sqrt(mean(h^2) + eps) / 127. A row of zeros has scale 0; a row with an infinity or a NaN, or a product u that
+ *   passes the range of 32 bits, has a NaN as its scale. At least one of y and q is wanted.
+ *   x, residual, sum and y are rows of dtype, each with its own stride in elements; weight [k] is fp32 or of dtype; eps >= 0 and finite.
+ *   An output may lie on an input of the same stride (sum on residual, y on x). k <= 16384, n below 2^30. Rows of any k and natural alignment; with q, k
+ *   and ldq are multiples of 16, strides whole 16 bytes, pointers 16-byte aligned. Bytes of q between k and ldq are left as they are. Rows that
+ *   begin on 16 bytes and have whole 16 bytes are the fast case everywhere.
+ * b2moe_rms_norm_backward: from h (x, or the sum that the norm wrote) and the gradients of y and (may be null) of the sum:
+ *   grad_x = gradient on h = rho (a - h rho^2 mean(a h)) + grad_sum with a = grad_y weight, rho = 1 / sqrt(mean(h^2) + eps);
+ *   grad_weight fp32 [k] (null: not wanted) = (accumulate: +) sum over the rows of grad_y h rho, in a fixed order. grad_x may lie on h, grad_y
+ *   or grad_sum of the same stride. workspace: b2moe_rms_norm_backward_workspace_bytes(n, k) bytes, 16-byte aligned, used by one call at a time
+ *   (null where grad_weight is). */
+B2MOE_API int32_t b2moe_rms_norm(const void * x, int32_t dtype, int64_t ldx, const void * residual, int64_t ldr, const void * weight, int32_t weight_dtype, float eps,
+                       int32_t n, int32_t k, void * sum, int64_t lds, void * y, int64_t ldy, int8_t * q, int64_t ldq, float * scale, b2moe_stream stream);
+B2MOE_API size_t b2moe_rms_norm_backward_workspace_bytes(int32_t n, int32_t k);
+B2MOE_API int32_t b2moe_rms_norm_backward(const void * h, int32_t dtype, int64_t ldh, const void * weight, int32_t weight_dtype, const void * grad_y, int64_t ldgy,
+                                const void * grad_sum, int64_t ldgs, float eps, int32_t n, int32_t k, void * grad_x, int64_t ldgx, float * grad_weight,
+                                int32_t accumulate, void * workspace, size_t workspace_bytes, b2moe_stream stream);
+
 /* ---- balance loss ------------------------------------------------------------------------------------------------
  * The auxiliary loss that keeps a router's load even, with the counts per expert and sequence, and its gradient on the
  * logits. It has no counterpart in the reference (which serves).

@@ -103,6 +103,9 @@ SIGNATURES = {
     "b2moe_combine_residual": (_i32, [_vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _vp, _i32, _vp]),
     "b2moe_quantize_rows": (_i32, [_vp, _i32, _i64, _i32, _i32, _vp, _i64, _vp, _vp]),
     "b2moe_linear_i8": (_i32, [_vp, _i64, _vp, C.POINTER(Bank), _i32, _vp, _i32, _i64, _vp, _vp]),
+    "b2moe_rms_norm": (_i32, [_vp, _i32, _i64, _vp, _i64, _vp, _i32, _f32, _i32, _i32, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp]),
+    "b2moe_rms_norm_backward_workspace_bytes": (_sz, [_i32, _i32]),
+    "b2moe_rms_norm_backward": (_i32, [_vp, _i32, _i64, _vp, _i32, _vp, _i64, _vp, _i64, _f32, _i32, _i32, _vp, _i64, _vp, _i32, _vp, _sz, _vp]),
     "b2moe_balance_workspace_bytes": (_sz, [_i32, _i32, _i32]),
     "b2moe_balance_loss": (_i32, [_i32, _vp, _i32, _vp, _i32, _vp, _vp, _i32, _i32, _i32, _f32, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "b2moe_balance_loss_backward": (_i32, [_i32, _vp, _i32, _i32, _vp, _vp, _i32, _i32, _i32, _f32, _vp, _vp, _vp, _vp, _i32, _i32, _vp]),

@@ -185,6 +185,92 @@ def linear_i8(q: torch.Tensor, scale: torch.Tensor, bank: DeviceBank, out_dtype=
     return out
 
 
+class Norm(NamedTuple):
+    """what b2moe_rms_norm writes, None where it was not asked for: y, the sum of the skip connection, q and scale"""
+    y: torch.Tensor | None
+    sum: torch.Tensor | None
+    q: torch.Tensor | None
+    scale: torch.Tensor | None
+
+
+def _rows_of(t, n, k, dtype, what):
+    """row stride of a matrix [n, k] of this type with neighbouring values, or a refusal"""
+    if t.dtype is not dtype or t.dim() != 2 or t.shape[0] != n or t.shape[1] != k:
+        raise capi.B2moeError(capi.ERR_SHAPE, f"{what}: rows of one type and size are wanted")
+    ld, one = t.stride()
+    if one != 1 and k > 1:
+        raise capi.B2moeError(capi.ERR_SHAPE, f"{what}: the values of a row have to be neighbours")
+    return ld if n > 1 else k
+
+
+def _norm_args(x, weight, what):
+    if x.dim() != 2 or x.dtype not in _DT:
+        raise capi.B2moeError(capi.ERR_SHAPE, f"{what}: rows [n, k] in float32, float16 or bfloat16 are wanted")
+    n, k = x.shape
+    if max(n, k) > _INT:
+        raise capi.B2moeError(capi.ERR_SHAPE, f"{what}: rows and columns are 32-bit numbers")
+    if weight.dtype not in (torch.float32, x.dtype) or weight.shape != (k,) or not weight.is_contiguous():
+        raise capi.B2moeError(capi.ERR_SHAPE, f"{what}: a contiguous weight for each column, in float32 or the rows' type, is wanted")
+    return n, k, _rows_of(x, n, k, x.dtype, what)
+
+
+def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float, residual: torch.Tensor | None = None, rows: bool = True, quantize: bool = False,
+             out: torch.Tensor | None = None, sum_out: torch.Tensor | None = None) -> Norm:
+    """Norm(y, sum, q, scale) of the rows x + residual (b2moe_rms_norm): y of x's type unless `rows` is false, sum where there is a residual (into `sum_out`, which
+    may be the residual itself), q and scale for linear_i8 with `quantize`. x, residual, out and sum_out may be rows of wider matrices"""
+    n, k, ldx = _norm_args(x, weight, "rms_norm")
+    dtype = x.dtype
+    ldr = lds = ldy = k
+    if residual is not None:
+        ldr = _rows_of(residual, n, k, dtype, "rms_norm")
+        if sum_out is not None:
+            lds = _rows_of(sum_out, n, k, dtype, "rms_norm")
+    elif sum_out is not None:
+        raise capi.B2moeError(capi.ERR_SHAPE, "rms_norm: a sum needs a residual")
+    if out is not None:
+        if not rows:
+            raise capi.B2moeError(capi.ERR_SHAPE, "rms_norm: an output is given for rows that are not wanted")
+        ldy = _rows_of(out, n, k, dtype, "rms_norm")
+    stream = _stream_of(x, weight, residual, out, sum_out)
+    new = torch.empty
+    if residual is not None and sum_out is None:
+        sum_out = new((n, k), dtype=dtype, device=x.device)
+    if rows and out is None:
+        out = new((n, k), dtype=dtype, device=x.device)
+    q = scale = None
+    if quantize:
+        q, scale = new((n, k), dtype=torch.int8, device=x.device), new(n, dtype=torch.float32, device=x.device)
+    check(lib.b2moe_rms_norm(x.data_ptr(), _DT[dtype], ldx, _ptr(residual), ldr, weight.data_ptr(), _DT[weight.dtype], eps, n, k, _ptr(sum_out), lds, _ptr(out), ldy,
+                             _ptr(q), k, _ptr(scale), stream), "b2moe_rms_norm")
+    return Norm(out, sum_out, q, scale)
+
+
+def rms_norm_backward(h: torch.Tensor, weight: torch.Tensor, grad_y: torch.Tensor, eps: float, grad_sum: torch.Tensor | None = None, out: torch.Tensor | None = None,
+                      grad_weight: torch.Tensor | None = None, weight_grad: bool = True):
+    """(gradient on h, gradient on the weight in float32) of rms_norm's rows (b2moe_rms_norm_backward); h is x, or the sum that the norm wrote, grad_sum what reaches the sum
+    through the skip connection. Into a `grad_weight` that is given it is added; without `weight_grad` it is None"""
+    n, k, ldh = _norm_args(h, weight, "rms_norm_backward")
+    ldgy, ldgs, ldgx = _rows_of(grad_y, n, k, h.dtype, "rms_norm_backward"), k, k
+    if grad_sum is not None:
+        ldgs = _rows_of(grad_sum, n, k, h.dtype, "rms_norm_backward")
+    if out is not None:
+        ldgx = _rows_of(out, n, k, h.dtype, "rms_norm_backward")
+    if grad_weight is not None and (not weight_grad or grad_weight.dtype is not torch.float32 or grad_weight.shape != (k,) or not grad_weight.is_contiguous()):
+        raise capi.B2moeError(capi.ERR_SHAPE, "rms_norm_backward: the weight's gradient is a contiguous float32 for each column")
+    stream = _stream_of(h, weight, grad_y, grad_sum, out, grad_weight)
+    add, ws, size = grad_weight is not None, None, 0
+    if out is None:
+        out = torch.empty((n, k), dtype=h.dtype, device=h.device)
+    if weight_grad:
+        size = lib.b2moe_rms_norm_backward_workspace_bytes(n, k)
+        ws = torch.empty(max(4, size // 4), dtype=torch.float32, device=h.device)
+        if not add:
+            grad_weight = torch.empty(k, dtype=torch.float32, device=h.device)
+    check(lib.b2moe_rms_norm_backward(h.data_ptr(), _DT[h.dtype], ldh, weight.data_ptr(), _DT[weight.dtype], grad_y.data_ptr(), ldgy, _ptr(grad_sum), ldgs, eps, n, k, out.data_ptr(),
+                                      ldgx, _ptr(grad_weight), int(add), _ptr(ws), size, stream), "b2moe_rms_norm_backward")
+    return out, grad_weight
+
+
 class Balance(NamedTuple):
     """what b2moe_balance_loss writes: loss (a scalar), counts and prob [sequences, experts], tokens [sequences + 1]"""
     loss: torch.Tensor
