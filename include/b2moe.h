@@ -308,6 +308,39 @@ B2MOE_API int32_t b2moe_rms_norm_backward(const void * h, int32_t dtype, int64_t
                                 const void * grad_sum, int64_t ldgs, float eps, int32_t n, int32_t k, void * grad_x, int64_t ldgx, float * grad_weight,
                                 int32_t accumulate, void * workspace, size_t workspace_bytes, b2moe_stream stream);
 
+/* ---- rows sorted by expert, and back --------------------------------------------------------------------------------
+ * For experts whose products are the caller's own (a tuning run's, in 16 or 32 bits): the rows of a plan's assignments next to each other,
+ * expert by expert, and the way back with the routing weights, each with its gradient. They have no counterpart in the reference, whose lists of
+ * rows (moe_group, src/experts/moe.cu:168-176) are read by its products in place. dtype is that of all rows; hidden and the strides (in elements) are whole 16 bytes,
+ * row pointers 16-byte aligned, n * topk below 2^30.
+ * b2moe_dispatch_rows: rows[slot] = x[token] for every assignment that the plan holds, slot = its place in the plan's permutation; expert e has
+ *   the slots offsets[e] .. offsets[e + 1) and the shared expert the last ones. ids are those that the plan was made of; shared_tokens: the plan's.
+ *   rows has n * topk + shared_tokens rows; those behind the last assignment are left as they are. slots (may be null): int32
+ *   [n * topk + (shared_tokens ? n : 0)], the slot of every assignment and then of every token's shared row, -1 where the plan holds none.
+ *   The gradient on x is b2moe_combine_rows of the gradient of rows, without weights.
+ * b2moe_combine_rows: out[t] = (residual[t] +) sum_s weights[t][s] y[slots[t * topk + s]] + shared_weights[t] y[slots[n * topk + t]] (the latter with
+ *   shared_tokens = n), in 32 bits in this order, rounded once; null weights are one; slots outside [0, rows) are left out, and so are their weights.
+ *   residual and out are of y's type; residual may be out.
+ * b2moe_combine_rows_backward: grad_y[slot] = weight grad_out[t] (grad_y null: not wanted), grad_weights[t][s] = grad_out[t] . y[slot] and grad_shared[t]
+ *   (null: not wanted; 0 where there is no slot). Rows of grad_y without an assignment are left as they are; it may lie on y of the same stride. */
+B2MOE_API int32_t b2moe_dispatch_rows(const void * x, int32_t dtype, int64_t ldx, const int32_t * ids, const int32_t * plan, int32_t n, int32_t topk, int32_t hidden,
+                            int32_t experts, int32_t shared_tokens, void * rows, int64_t ldr, int32_t * slots, b2moe_stream stream);
+B2MOE_API int32_t b2moe_combine_rows(const void * y, int32_t dtype, int64_t ldy, int32_t rows, const int32_t * slots, const float * weights, const float * shared_weights,
+                           const void * residual, int64_t ldr, int32_t n, int32_t topk, int32_t hidden, int32_t shared_tokens, void * out, int64_t ldo,
+                           b2moe_stream stream);
+B2MOE_API int32_t b2moe_combine_rows_backward(const void * grad_out, int32_t dtype, int64_t ldgo, const void * y, int64_t ldy, int32_t rows, const int32_t * slots,
+                                    const float * weights, const float * shared_weights, int32_t n, int32_t topk, int32_t hidden, int32_t shared_tokens,
+                                    void * grad_y, int64_t ldgy, float * grad_weights, float * grad_shared, b2moe_stream stream);
+
+/* The gradient of the routing weights (b2moe_topk_softmax, b2moe_route_sigmoid, b2moe_route_dispatch) on the logits, from what those calls wrote: grad_logits[t][e] = (accumulate: +)
+ *   sum_s grad_weights[t][s] d weights[t][s] / d logits[t][e], with the selection held fixed; zero in the columns that were not selected (accumulate: they stay).
+ *   With grad_shared and shared_weights [n] (the softmax family's), column `experts` is the shared expert's. norm (sigmoid family) and scale as in the routing call. logits: read
+ *   for the sigmoid family only (may be null). An id outside [0, experts) gets no gradient, its weight counts as one of the token's. accumulate adds to
+ *   the gradient that b2moe_balance_loss_backward wrote, say. Columns behind are left as they are. experts <= 4096. */
+B2MOE_API int32_t b2moe_route_backward(int32_t gating, const float * logits, int32_t ld, const int32_t * ids, const float * weights, const float * grad_weights,
+                             const float * shared_weights, const float * grad_shared, int32_t experts, int32_t topk, int32_t norm, float scale, int32_t n,
+                             float * grad_logits, int32_t ldg, int32_t accumulate, b2moe_stream stream);
+
 /* ---- balance loss ------------------------------------------------------------------------------------------------
  * The auxiliary loss that keeps a router's load even, with the counts per expert and sequence, and its gradient on the
  * logits. It has no counterpart in the reference (which serves).

@@ -106,6 +106,10 @@ SIGNATURES = {
     "b2moe_rms_norm": (_i32, [_vp, _i32, _i64, _vp, _i64, _vp, _i32, _f32, _i32, _i32, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp]),
     "b2moe_rms_norm_backward_workspace_bytes": (_sz, [_i32, _i32]),
     "b2moe_rms_norm_backward": (_i32, [_vp, _i32, _i64, _vp, _i32, _vp, _i64, _vp, _i64, _f32, _i32, _i32, _vp, _i64, _vp, _i32, _vp, _sz, _vp]),
+    "b2moe_dispatch_rows": (_i32, [_vp, _i32, _i64, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _vp, _i64, _vp, _vp]),
+    "b2moe_combine_rows": (_i32, [_vp, _i32, _i64, _i32, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _vp, _i64, _vp]),
+    "b2moe_combine_rows_backward": (_i32, [_vp, _i32, _i64, _vp, _i64, _i32, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _vp, _i64, _vp, _vp, _vp]),
+    "b2moe_route_backward": (_i32, [_i32, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _f32, _i32, _vp, _i32, _i32, _vp]),
     "b2moe_balance_workspace_bytes": (_sz, [_i32, _i32, _i32]),
     "b2moe_balance_loss": (_i32, [_i32, _vp, _i32, _vp, _i32, _vp, _vp, _i32, _i32, _i32, _f32, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "b2moe_balance_loss_backward": (_i32, [_i32, _vp, _i32, _i32, _vp, _vp, _i32, _i32, _i32, _f32, _vp, _vp, _vp, _vp, _i32, _i32, _vp]),

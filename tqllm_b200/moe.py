@@ -271,6 +271,42 @@ def rms_norm_backward(h: torch.Tensor, weight: torch.Tensor, grad_y: torch.Tenso
     return out, grad_weight
 
 
+def route_backward(logits, ids, weights, grad_weights, experts, gating=capi.SOFTMAX, norm=True, scale=0.0, shared_weights=None, grad_shared=None, out=None):
+    """The gradient of the routing weights [n, topk] on the logits (b2moe_route_backward), [n, experts] or, with the shared expert's, [n, experts + 1]; into `out` (rows of at least
+    as many columns) it is added. logits may be None for the softmax family"""
+    n, topk = ids.shape
+    cols = experts + (grad_shared is not None)
+    if max(n, cols) > _INT:
+        raise capi.B2moeError(capi.ERR_SHAPE, "route_backward: tokens and columns are 32-bit numbers")
+    if ids.dtype is not torch.int32 or not ids.is_contiguous():
+        raise capi.B2moeError(capi.ERR_SHAPE, "route_backward: contiguous int32 ids [n, topk] are wanted")
+    for w in (weights, grad_weights):
+        if w.dtype is not torch.float32 or w.shape != ids.shape or not w.is_contiguous():
+            raise capi.B2moeError(capi.ERR_SHAPE, "route_backward: contiguous float32 weights and gradients [n, topk] are wanted")
+    if (shared_weights is None) != (grad_shared is None):
+        raise capi.B2moeError(capi.ERR_SHAPE, "route_backward: the shared expert has weights and a gradient, or neither")
+    for w in (shared_weights, grad_shared):
+        if w is not None and (w.dtype is not torch.float32 or w.numel() != n or not w.is_contiguous()):
+            raise capi.B2moeError(capi.ERR_SHAPE, "route_backward: a contiguous float32 for each token is wanted of the shared expert")
+    ld, ldg, add = cols, cols, out is not None
+    if logits is not None:
+        if logits.dtype is not torch.float32 or logits.dim() != 2 or logits.shape[0] != n or logits.shape[1] < experts or (logits.stride(1) != 1 and experts > 1):
+            raise capi.B2moeError(capi.ERR_SHAPE, "route_backward: float32 logits with contiguous rows of at least as many columns as experts are wanted")
+        ld = logits.stride(0) if n > 1 else logits.shape[1]
+    if add:
+        if out.dtype is not torch.float32 or out.dim() != 2 or out.shape[0] != n or out.shape[1] < cols or (out.stride(1) != 1 and cols > 1):
+            raise capi.B2moeError(capi.ERR_SHAPE, "route_backward: the gradient has float32 rows like the logits")
+        ldg = out.stride(0) if n > 1 else out.shape[1]
+    if max(ld, ldg) > _INT:
+        raise capi.B2moeError(capi.ERR_SHAPE, "route_backward: row strides are 32-bit numbers")
+    stream = _stream_of(ids, weights, grad_weights, logits, shared_weights, grad_shared, out)
+    if not add:
+        out = torch.empty((n, cols), dtype=torch.float32, device=ids.device)
+    check(lib.b2moe_route_backward(gating, _ptr(logits), ld, ids.data_ptr(), weights.data_ptr(), grad_weights.data_ptr(), _ptr(shared_weights), _ptr(grad_shared), experts, topk, int(norm), scale, n,
+                                   out.data_ptr(), ldg, int(add), stream), "b2moe_route_backward")
+    return out
+
+
 class Balance(NamedTuple):
     """what b2moe_balance_loss writes: loss (a scalar), counts and prob [sequences, experts], tokens [sequences + 1]"""
     loss: torch.Tensor
@@ -334,6 +370,86 @@ def balance_loss_backward(logits, saved: Balance, topk, coef, gating=capi.SOFTMA
     check(lib.b2moe_balance_loss_backward(gating, logits.data_ptr(), ld, topk, _ptr(mask), _ptr(offsets), seqs, experts, n, coef, saved.counts.data_ptr(),
                                           saved.tokens.data_ptr(), _ptr(grad_loss), grad.data_ptr(), ldg, int(out is not None), stream), "b2moe_balance_loss_backward")
     return grad
+
+
+def dispatch_rows(x: torch.Tensor, ids: torch.Tensor, plan: "Plan", rows: torch.Tensor | None = None):
+    """(rows [assignments + shared, hidden] in slot order, slots int32) of the tokens x [n, hidden] (b2moe_dispatch_rows); ids are those that the plan was made of. A buffer that is given keeps
+    the rows behind the last assignment, without one they are zeros"""
+    n, topk = ids.shape
+    hidden = x.shape[-1]
+    if x.dtype not in _DT or n != plan.n or topk != plan.topk or hidden > _INT:
+        raise capi.B2moeError(capi.ERR_SHAPE, "dispatch_rows: rows and ids of the plan's tokens are wanted")
+    ldx = _rows_of(x, n, hidden, x.dtype, "dispatch_rows")
+    if ids.dtype is not torch.int32 or not ids.is_contiguous():
+        raise capi.B2moeError(capi.ERR_SHAPE, "dispatch_rows: contiguous int32 ids [n, topk] are wanted")
+    shared, ldr = plan.shared_tokens, hidden
+    total = n * topk + shared
+    if rows is not None:
+        ldr = _rows_of(rows, total, hidden, x.dtype, "dispatch_rows")
+    stream = _stream_of(x, ids, plan.buf, rows)
+    if rows is None:
+        rows = torch.zeros((total, hidden), dtype=x.dtype, device=x.device)
+    slots = torch.empty(n * topk + (n if shared else 0), dtype=torch.int32, device=x.device)
+    check(lib.b2moe_dispatch_rows(x.data_ptr(), _DT[x.dtype], ldx, ids.data_ptr(), plan.buf.data_ptr(), n, topk, hidden, plan.experts, shared, rows.data_ptr(), ldr, slots.data_ptr(), stream),
+          "b2moe_dispatch_rows")
+    return rows, slots
+
+
+def _slots_args(rows, slots, weights, shared_weights, n, topk, what):
+    """(tokens of the shared expert, hidden) of a call on rows in slot order"""
+    if rows.dim() != 2 or rows.dtype not in _DT or max(n, topk, *rows.shape) > _INT:
+        raise capi.B2moeError(capi.ERR_SHAPE, f"{what}: rows [slots, hidden] in float32, float16 or bfloat16 are wanted")
+    if slots.dtype is not torch.int32 or not slots.is_contiguous() or slots.numel() not in (n * topk, n * topk + n):
+        raise capi.B2moeError(capi.ERR_SHAPE, f"{what}: contiguous int32 slots of n * topk assignments (and n shared rows) are wanted")
+    shared = n if slots.numel() > n * topk else 0
+    for w, count in ((weights, n * topk), (shared_weights, n)):
+        if w is not None and (w.dtype is not torch.float32 or w.numel() != count or not w.is_contiguous()):
+            raise capi.B2moeError(capi.ERR_SHAPE, f"{what}: contiguous float32 weights are wanted, one for each assignment and shared row")
+    if shared_weights is not None and not shared:
+        raise capi.B2moeError(capi.ERR_SHAPE, f"{what}: weights of shared rows without slots of theirs")
+    return shared, rows.shape[1]
+
+
+def combine_rows(y: torch.Tensor, slots: torch.Tensor, weights: torch.Tensor | None, n: int, topk: int, shared_weights=None, residual: torch.Tensor | None = None,
+                 out: torch.Tensor | None = None) -> torch.Tensor:
+    """out [n, hidden] = (residual +) the weighted sum of the rows y [slots, hidden] of each token's assignments, and of its shared row where `slots` has them (b2moe_combine_rows); residual may be out"""
+    shared, hidden = _slots_args(y, slots, weights, shared_weights, n, topk, "combine_rows")
+    total, dtype = y.shape[0], y.dtype
+    ldy, ldr, ldo = _rows_of(y, total, hidden, dtype, "combine_rows"), hidden, hidden
+    if residual is not None:
+        ldr = _rows_of(residual, n, hidden, dtype, "combine_rows")
+    if out is not None:
+        ldo = _rows_of(out, n, hidden, dtype, "combine_rows")
+    stream = _stream_of(y, slots, weights, shared_weights, residual, out)
+    if out is None:
+        out = torch.empty((n, hidden), dtype=dtype, device=y.device)
+    check(lib.b2moe_combine_rows(y.data_ptr(), _DT[dtype], ldy, total, slots.data_ptr(), _ptr(weights), _ptr(shared_weights), _ptr(residual), ldr, n, topk, hidden, shared, out.data_ptr(), ldo, stream),
+          "b2moe_combine_rows")
+    return out
+
+
+def dispatch_rows_backward(grad_rows: torch.Tensor, slots: torch.Tensor, n: int, topk: int, residual: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """The gradient of dispatch_rows on its tokens: (residual +) the sum of the gradients of a token's rows"""
+    return combine_rows(grad_rows, slots, None, n, topk, residual=residual, out=out)
+
+
+def combine_rows_backward(grad_out: torch.Tensor, y: torch.Tensor, slots: torch.Tensor, weights: torch.Tensor | None, n: int, topk: int, shared_weights=None,
+                          grad_y: torch.Tensor | None = None):
+    """(gradient on y, on the weights [n, topk], on the shared weights [n] or None) of combine_rows (b2moe_combine_rows_backward). A buffer grad_y that is given keeps the rows without an assignment (it may
+    be y), without one they are zeros"""
+    shared, hidden = _slots_args(y, slots, weights, shared_weights, n, topk, "combine_rows_backward")
+    total, dtype = y.shape[0], y.dtype
+    ldgo, ldy, ldgy = _rows_of(grad_out, n, hidden, dtype, "combine_rows_backward"), _rows_of(y, total, hidden, dtype, "combine_rows_backward"), hidden
+    if grad_y is not None:
+        ldgy = _rows_of(grad_y, total, hidden, dtype, "combine_rows_backward")
+    stream = _stream_of(grad_out, y, slots, weights, shared_weights, grad_y)
+    if grad_y is None:
+        grad_y = torch.zeros((total, hidden), dtype=dtype, device=y.device)
+    grad_weights = torch.empty((n, topk), dtype=torch.float32, device=y.device)
+    grad_shared = torch.empty(n, dtype=torch.float32, device=y.device) if shared else None
+    check(lib.b2moe_combine_rows_backward(grad_out.data_ptr(), _DT[dtype], ldgo, y.data_ptr(), ldy, total, slots.data_ptr(), _ptr(weights), _ptr(shared_weights), n, topk, hidden, shared,
+                                          grad_y.data_ptr(), ldgy, grad_weights.data_ptr(), _ptr(grad_shared), stream), "b2moe_combine_rows_backward")
+    return grad_y, grad_weights, grad_shared
 
 
 def count_ids(ids: torch.Tensor, counts: torch.Tensor) -> torch.Tensor:
