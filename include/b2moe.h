@@ -283,6 +283,11 @@ B2MOE_API int32_t b2moe_quantize_rows(const void * x, int32_t x_dtype, int64_t l
                             b2moe_stream stream);
 B2MOE_API int32_t b2moe_linear_i8(const int8_t * q, int64_t ldq, const float * scale, const b2moe_bank * w, int32_t n, void * y, int32_t y_dtype,
                         int64_t ldy, int32_t * status, b2moe_stream stream);
+/* b2moe_linear_i8 with what follows a projection in the same pass: y = act((sum q w) (scale aux) + bias) + residual, in 32 bits and rounded once. bias [rows] fp32 (null: none); residual [n][rows] of
+ *   y_dtype, rows ldr elements apart (null: none; it may be y of the same stride); act: a b2moe_act. */
+enum b2moe_act { B2MOE_ACT_NONE = 0, B2MOE_ACT_RELU = 1, B2MOE_ACT_SILU = 2, B2MOE_ACT_GELU = 3 /* v (1 + erf(v / sqrt 2)) / 2 */, B2MOE_ACT_GELU_TANH = 4 /* v (1 + tanh(sqrt(2 / pi) (v + 0.044715 v^3))) / 2 */ };
+B2MOE_API int32_t b2moe_linear_i8_epilogue(const int8_t * q, int64_t ldq, const float * scale, const b2moe_bank * w, int32_t n, const float * bias, int32_t act, const void * residual,
+                                 int64_t ldr, void * y, int32_t y_dtype, int64_t ldy, int32_t * status, b2moe_stream stream);
 
 /* ---- norm ----------------------------------------------------------------------------------------------------------
  * The root-mean-square norm in front of a layer or a projection, with the skip connection's addition (the engines' add_sumsq + norm,

@@ -19,6 +19,7 @@ IQ3_S_X4 = 0x1015        # bank layout of IQ3_S blocks as 4-bit codes (b2moe_typ
 I8 = 0x1008              # plain 8-bit rows with a scale each (b2moe_type)
 FAMILY = {"auto": 0, "generic": 1, "decode": 2, "gemm": 3, "decode_kernels": 4}
 SOFTMAX, SIGMOID = 1, 2
+ACT = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
 
 
 class B2moeError(RuntimeError):
@@ -103,6 +104,7 @@ SIGNATURES = {
     "b2moe_combine_residual": (_i32, [_vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _vp, _i32, _vp]),
     "b2moe_quantize_rows": (_i32, [_vp, _i32, _i64, _i32, _i32, _vp, _i64, _vp, _vp]),
     "b2moe_linear_i8": (_i32, [_vp, _i64, _vp, C.POINTER(Bank), _i32, _vp, _i32, _i64, _vp, _vp]),
+    "b2moe_linear_i8_epilogue": (_i32, [_vp, _i64, _vp, C.POINTER(Bank), _i32, _vp, _i32, _vp, _i64, _vp, _i32, _i64, _vp, _vp]),
     "b2moe_rms_norm": (_i32, [_vp, _i32, _i64, _vp, _i64, _vp, _i32, _f32, _i32, _i32, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp]),
     "b2moe_rms_norm_backward_workspace_bytes": (_sz, [_i32, _i32]),
     "b2moe_rms_norm_backward": (_i32, [_vp, _i32, _i64, _vp, _i32, _vp, _i64, _vp, _i64, _f32, _i32, _i32, _vp, _i64, _vp, _i32, _vp, _sz, _vp]),

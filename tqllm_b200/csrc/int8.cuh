@@ -34,7 +34,31 @@ struct I8Args {
     void * y;
     int y_dtype;
     long long ldy;
+    // what follows a dense product (null, null, B2MOE_ACT_NONE: nothing): y = act(product + bias) + residual, residual of y's type
+    const float * bias;
+    const void * residual;
+    long long ldr;
+    int act;
 };
+
+inline bool has_epilogue(const I8Args & a) { return a.bias || a.residual || a.act != B2MOE_ACT_NONE; }
+
+// What is small stays exact to its own size: the negative tail of GELU is a complementary error function, (1 + tanh z) / 2 = 1 / (1 + e^-2z)
+__device__ __forceinline__ float activation(int act, float v) {
+    switch (act) {
+        case B2MOE_ACT_RELU: return v < 0.f ? 0.f : v;                 // a NaN stays one
+        case B2MOE_ACT_SILU: return v / (1.f + expf(-v));
+        case B2MOE_ACT_GELU: return 0.5f * v * erfcf(-0.70710678118654752f * v);
+        case B2MOE_ACT_GELU_TANH: return v / (1.f + expf(-1.59576912160573071f * fmaf(0.044715f * v * v, v, v)));
+        default: return v;
+    }
+}
+
+// a product's output with what follows it; every rounding is written out, so that all forms give the same bits
+__device__ __forceinline__ float finished(const I8Args & p, int sum, float scale, float bias, float residual) {
+    const float v = activation(p.act, __fadd_rn(__fmul_rn(float(sum), scale), bias));
+    return p.residual ? __fadd_rn(v, residual) : v;
+}
 
 __device__ __forceinline__ int source_row(const I8Args & p, int slot, int a) {
     return p.slots ? slot : !p.per_token ? a : a < p.assignments ? a / p.topk : a - p.assignments;

@@ -81,14 +81,18 @@ __device__ __forceinline__ void epi_sync() { asm volatile("bar.sync 1, %0;" ::"n
 
 struct TcItem { int e, first, count, rb; };      // expert, first row (slot), rows, block of weight rows
 
+__device__ __forceinline__ float to_float(float v) { return v; }
+__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+
 // this lane's weight row of an item
 template <int MATS>
 __device__ __forceinline__ int weight_row(const TcItem & im, int quarter, int lane) {
     return MATS == 2 ? im.rb * 64 + 16 * quarter + (lane & 15) : im.rb * 128 + 32 * quarter + lane;
 }
-// the item's outputs from tensor memory; t: (output row, scale) of its activation rows, v: the scales of the lane's weight row
-template <int MATS, class T>
-__device__ __forceinline__ void store_item(const I8Args & p, const TcItem & im, uint32_t taddr, const int2 * t, const float (&v)[MATS], int quarter, int half, int lane) {
+// the item's outputs from tensor memory; t: (output row, scale) of its activation rows, v: the scales of the lane's weight row; EPI: what follows the product, with the bias of the lane's weight row
+template <int MATS, bool EPI, class T>
+__device__ __forceinline__ void store_item(const I8Args & p, const TcItem & im, uint32_t taddr, const int2 * t, const float (&v)[MATS], float bias, int quarter, int half, int lane) {
     const bool upper = MATS == 2 && lane >= 16;
     const int row = weight_row<MATS>(im, quarter, lane);
     const bool in = row < p.rows;
@@ -102,6 +106,13 @@ __device__ __forceinline__ void store_item(const I8Args & p, const TcItem & im, 
 #pragma unroll 1
     for (int c = 16 * half; c < im.count; c += 32) {
         uint32_t d[16];
+        T r[16];                                                       // EPI: the residual's values of these 16 rows, asked for together (they may lie under the outputs, and loads stay behind stores)
+        if (EPI && p.residual) {
+            const T * from = static_cast<const T *>(p.residual) + row;
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+                if (in && c + j < im.count) r[j] = from[size_t(uint32_t(t[c + j].x)) * p.ldr];
+        }
         tmem_ld16(taddr + c, d);
         tmem_ld_wait();
 #pragma unroll
@@ -114,6 +125,12 @@ __device__ __forceinline__ void store_item(const I8Args & p, const TcItem & im, 
                 const int gs = int(upper ? other : d[j]), us = int(upper ? d[j + 1] : other);
                 const float s = upper ? s1 : s0, g = float(gs) * (s * v[0]), u = float(us) * (s * v[MATS - 1]);
                 if (in && c + j + int(upper) < im.count) put(upper ? two.z : two.x, g / (1.f + expf(-g)) * u);
+            } else if (EPI) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const float f = finished(p, int(d[j + i]), (i ? s1 : s0) * v[0], bias, to_float(r[j + i]));
+                    if (in && c + j + i < im.count) put(i ? two.z : two.x, f);
+                }
             } else {
                 if (in && c + j < im.count) put(two.x, float(int(d[j])) * (s0 * v[0]));
                 if (in && c + j + 1 < im.count) put(two.z, float(int(d[j + 1])) * (s1 * v[0]));
@@ -134,7 +151,8 @@ __device__ __noinline__ void spoil_rows(void * y, int dtype, long long ldy, int 
 // PAIR (long rows): two blocks take neighbouring blocks of weight rows of the same activation rows, of which each brings a half: the copies from the L2, which set the pace of
 // large calls, are a third fewer. The even block issues the products of both and has the barriers of the operands and of the sums that have been read.
 enum { TC_SPLIT = 1, TC_PAIR = 2 };
-template <int MATS, int MODE>
+// EPI (dense calls): bias, activation and residual follow the product
+template <int MATS, int MODE, bool EPI>
 __global__ void __launch_bounds__(TC_THREADS, MODE ? 1 : 2) i8_gemm_k(const I8Args p, const TcArgs c, const __grid_constant__ TcMaps maps) {
     extern __shared__ __align__(1024) uint8_t tc_mem[];
     __shared__ __align__(16) int2 table[2][256];
@@ -351,12 +369,13 @@ __global__ void __launch_bounds__(TC_THREADS, MODE ? 1 : 2) i8_gemm_k(const I8Ar
         const int tid = threadIdx.x - 32 * TC_EPI_WARP0, quarter = warp & 3, half = (warp - TC_EPI_WARP0) >> 2;
         // what the stores of an item need to know (its rows' places and scales, the weight row's scales) is asked for an item ahead
         int2 mine = make_int2(0, 0);
-        float v[MATS];
+        float v[MATS], bias = 0.f;
         auto fetch = [&](const TcItem & im) {
             if (tid < im.count) mine = make_int2(p.plan ? perm[im.first + tid] : im.first + tid, __float_as_int(p.s[im.first + tid]));
             const int row = weight_row<MATS>(im, quarter, lane);
 #pragma unroll
             for (int m = 0; m < MATS; ++m) v[m] = row < p.rows ? (p.plan && im.e == p.experts ? p.shared_v[m] : p.v[m] + size_t(im.e) * p.rows)[row] : 0.f;
+            if (EPI) bias = p.bias && row < p.rows ? p.bias[row] : 0.f;
         };
         const uint32_t acc_empty0 = PAIR ? at_rank(acc_empty, 0) : acc_empty;
         uint32_t done = 0;
@@ -374,6 +393,7 @@ __global__ void __launch_bounds__(TC_THREADS, MODE ? 1 : 2) i8_gemm_k(const I8Ar
             float scale[MATS];
 #pragma unroll
             for (int m = 0; m < MATS; ++m) scale[m] = v[m];
+            const float add = bias;
             epi_sync();                                                // the table is there; the other one's item has been read by every warp
             if (it + it_step < items) {
                 next = locate(it + it_step);
@@ -383,9 +403,9 @@ __global__ void __launch_bounds__(TC_THREADS, MODE ? 1 : 2) i8_gemm_k(const I8Ar
             fence_after();
             if (ok) {
                 const uint32_t taddr = tmem + h * c.half + (uint32_t(32 * quarter) << 16);
-                if (p.y_dtype == B2MOE_F32) store_item<MATS, float>(p, im, taddr, table[h], scale, quarter, half, lane);
-                else if (p.y_dtype == B2MOE_F16) store_item<MATS, __half>(p, im, taddr, table[h], scale, quarter, half, lane);
-                else store_item<MATS, __nv_bfloat16>(p, im, taddr, table[h], scale, quarter, half, lane);
+                if (p.y_dtype == B2MOE_F32) store_item<MATS, EPI, float>(p, im, taddr, table[h], scale, add, quarter, half, lane);
+                else if (p.y_dtype == B2MOE_F16) store_item<MATS, EPI, __half>(p, im, taddr, table[h], scale, add, quarter, half, lane);
+                else store_item<MATS, EPI, __nv_bfloat16>(p, im, taddr, table[h], scale, add, quarter, half, lane);
             } else {
                 if (lane == 0) give_up();
                 const int row = weight_row<MATS>(im, quarter, lane);
@@ -412,7 +432,7 @@ __global__ void __launch_bounds__(TC_THREADS, MODE ? 1 : 2) i8_gemm_k(const I8Ar
         const TcItem im = locate(blockIdx.x);
         const int parts = gridDim.z, lo = im.count * int(blockIdx.z) / parts, hi = im.count * (int(blockIdx.z) + 1) / parts, r = threadIdx.x & 127, row = 128 * im.rb + r;
         const bool in = row < p.rows;
-        const float v = in ? p.v[0][row] : 0.f;
+        const float v = in ? p.v[0][row] : 0.f, bias = EPI && p.bias && in ? p.bias[row] : 0.f;
         uint32_t place[TC_MAX_SPLIT];
 #pragma unroll
         for (int z = 0; z < TC_MAX_SPLIT; ++z) asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(place[z]) : "r"(saddr(ring) + 4 * r), "r"(z < parts ? z : 0));
@@ -421,11 +441,12 @@ __global__ void __launch_bounds__(TC_THREADS, MODE ? 1 : 2) i8_gemm_k(const I8Ar
         constexpr int STEP = TC_THREADS / 128;
         for (int col = lo + (threadIdx.x >> 7); col < hi && in; col += 4 * STEP) {
             int part[4][TC_MAX_SPLIT];
-            float s[4];
+            float s[4], r[4] = {};
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int at = min(col + i * STEP, hi - 1);
                 s[i] = p.s[im.first + at];
+                if (EPI && p.residual) r[i] = load_act(p.residual, p.y_dtype, size_t(im.first + at) * p.ldr + row);
 #pragma unroll
                 for (int z = 0; z < TC_MAX_SPLIT; ++z)
                     if (z < parts) asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(part[i][z]) : "r"(place[z] + uint32_t(at) * 512u) : "memory");
@@ -436,7 +457,8 @@ __global__ void __launch_bounds__(TC_THREADS, MODE ? 1 : 2) i8_gemm_k(const I8Ar
 #pragma unroll
                 for (int z = 0; z < TC_MAX_SPLIT; ++z)
                     if (z < parts) sum += part[i][z];
-                if (col + i * STEP < hi) store_act(p.y, p.y_dtype, size_t(im.first + col + i * STEP) * p.ldy + row, float(sum) * (s[i] * v));
+                const float out = EPI ? finished(p, sum, s[i] * v, bias, r[i]) : float(sum) * (s[i] * v);
+                if (col + i * STEP < hi) store_act(p.y, p.y_dtype, size_t(im.first + col + i * STEP) * p.ldy + row, out);
             }
         }
         cluster.sync();                                                // the parts stay until every block has read them
@@ -480,7 +502,7 @@ bool map_rows(CUtensorMap & m, const int8_t * base, int cols, long long rows, lo
 int clusters_at_once(int size) {
     static const std::array<int, TC_MAX_SPLIT + 1> most = [] {
         std::array<int, TC_MAX_SPLIT + 1> m{};
-        if (!allow_smem(i8_gemm_k<1, TC_SPLIT>, TC_SMEM_MOST)) return m;
+        if (!allow_smem(i8_gemm_k<1, TC_SPLIT, false>, TC_SMEM_MOST)) return m;
         for (int size = 2; size <= TC_MAX_SPLIT; ++size) {
             cudaLaunchConfig_t cfg{};
             cfg.gridDim = dim3(1, 1, size); cfg.blockDim = dim3(TC_THREADS); cfg.dynamicSmemBytes = TC_SMEM_MOST;
@@ -488,7 +510,7 @@ int clusters_at_once(int size) {
             at[0].id = cudaLaunchAttributeClusterDimension;
             at[0].val.clusterDim.x = 1; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = size;
             cfg.attrs = at; cfg.numAttrs = 1;
-            if (cudaOccupancyMaxActiveClusters(&m[size], i8_gemm_k<1, TC_SPLIT>, &cfg) != cudaSuccess) m[size] = 0;
+            if (cudaOccupancyMaxActiveClusters(&m[size], i8_gemm_k<1, TC_SPLIT, false>, &cfg) != cudaSuccess) m[size] = 0;
         }
         cudaGetLastError();
         return m;
@@ -582,20 +604,26 @@ int32_t i8_gemm(const I8Args & p, long long q_rows, int per_group, int * status,
     if (!ok) return B2MOE_ERR_CUDA;
     const size_t smem = TC_ALIGN + size_t(c.stages) * stage_bytes + table;
     const long long items = (long long)c.tiles * c.row_blocks;
-    if constexpr (MATS == 1)
-        if (split > 1) {
-            if (!allow_smem(i8_gemm_k<1, TC_SPLIT>, TC_SMEM_MOST)) return B2MOE_ERR_CUDA;
-            return launch_cluster(i8_gemm_k<1, TC_SPLIT>, dim3(unsigned(items), 1, split), dim3(1, 1, split), smem, s, p, c, maps);
+    auto launch = [&](auto epi) -> int32_t {
+        constexpr bool EPI = decltype(epi)::value;
+        if constexpr (MATS == 1)
+            if (split > 1) {
+                if (!allow_smem(i8_gemm_k<1, TC_SPLIT, EPI>, TC_SMEM_MOST)) return B2MOE_ERR_CUDA;
+                return launch_cluster(i8_gemm_k<1, TC_SPLIT, EPI>, dim3(unsigned(items), 1, split), dim3(1, 1, split), smem, s, p, c, maps);
+            }
+        if (pair) {
+            if (!allow_smem(i8_gemm_k<MATS, TC_PAIR, EPI>, TC_SMEM_MOST)) return B2MOE_ERR_CUDA;
+            const long long pairs = (long long)c.tiles * ceil_div(c.row_blocks, 2);
+            return launch_cluster(i8_gemm_k<MATS, TC_PAIR, EPI>, dim3(unsigned(2 * (p.plan ? sms / 2 : std::min<long long>(sms / 2, pairs)))), dim3(2), smem, s, p, c, maps);
         }
-    if (pair) {
-        if (!allow_smem(i8_gemm_k<MATS, TC_PAIR>, TC_SMEM_MOST)) return B2MOE_ERR_CUDA;
-        const long long pairs = (long long)c.tiles * ceil_div(c.row_blocks, 2);
-        return launch_cluster(i8_gemm_k<MATS, TC_PAIR>, dim3(unsigned(2 * (p.plan ? sms / 2 : std::min<long long>(sms / 2, pairs)))), dim3(2), smem, s, p, c, maps);
-    }
-    if (!allow_smem(i8_gemm_k<MATS, 0>, TC_SMEM_MOST)) return B2MOE_ERR_CUDA;
-    const int blocks = two ? 2 * sms : sms;
-    launch_overlapped(i8_gemm_k<MATS, 0>, dim3(unsigned(p.plan ? blocks : std::min<long long>(blocks, items))), dim3(TC_THREADS), smem, s, p, c, maps);
-    return launch_status();
+        if (!allow_smem(i8_gemm_k<MATS, 0, EPI>, TC_SMEM_MOST)) return B2MOE_ERR_CUDA;
+        const int blocks = two ? 2 * sms : sms;
+        launch_overlapped(i8_gemm_k<MATS, 0, EPI>, dim3(unsigned(p.plan ? blocks : std::min<long long>(blocks, items))), dim3(TC_THREADS), smem, s, p, c, maps);
+        return launch_status();
+    };
+    if constexpr (MATS == 1)
+        if (has_epilogue(p)) return launch(std::true_type{});
+    return launch(std::false_type{});
 }
 template int32_t i8_gemm<1>(const I8Args &, long long, int, int *, cudaStream_t);
 template int32_t i8_gemm<2>(const I8Args &, long long, int, int *, cudaStream_t);

@@ -28,8 +28,8 @@ __device__ __forceinline__ uint4 load_stream(const int8_t * p) {
 // A few tokens per expert: bound by streaming the weights. A block takes 16 weight rows of one expert (of both matrices with MATS = 2) and all the
 // expert's tokens, 8 NT at a time; its warps share the columns in pieces of 64, 16 bytes a lane and row, straight from memory into the fragments of the tensor
 // core: lane (g, t) holds bytes 16 t.. of rows g and g + 8, so word i of both operands stands for the same four columns, which is all that a sum over columns needs.
-// UNROLL: steps that a warp asks for at once.
-template <int MATS, int NT, int UNROLL>
+// UNROLL: steps that a warp asks for at once. EPI: a dense call with an epilogue.
+template <int MATS, int NT, int UNROLL, bool EPI>
 __global__ void __launch_bounds__(512) i8_stream_k(const I8Args p) {
     extern __shared__ int red[];                                       // [warps][MATS][NT][16 rows][8 tokens]
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, g = lane >> 2, t = lane & 3, r0 = blockIdx.x * 16;
@@ -121,6 +121,7 @@ __global__ void __launch_bounds__(512) i8_stream_k(const I8Args p) {
                 const float u = float(sum[MATS - 1]) * (s * v[MATS - 1][row]);
                 out = out / (1.f + expf(-out)) * u;
             }
+            if (EPI) out = finished(p, sum[0], s * v[0][row], p.bias ? p.bias[row] : 0.f, p.residual ? load_act(p.residual, p.y_dtype, size_t(j) * p.ldr + row) : 0.f);
             store_act(p.y, p.y_dtype, size_t(a) * p.ldy + row, out);
         }
     }
@@ -131,23 +132,23 @@ __global__ void __launch_bounds__(512) i8_stream_k(const I8Args p) {
 //   512 x 1024   2.4 / 2.2 / 2.4      8192 x 1024  3.7 / 3.4 / 5.5      gate/up of one token of ten experts 11.3 / 9.0 / 12.1
 // Eight steps at once where a warp has as many (before / with): 8192 x 8192 16.1 / 15.3, 2048 x 8192 6.1 / 5.7; down of 64 experts of 4096 x 4096 at three each 181.6 / 171.8, of eight of
 // 2048 x 4096 17.9 / 17.0; where it has fewer it loses: 4096 x 4096 4.5 / 4.8
-template <int MATS, int NT>
+template <int MATS, int NT, bool EPI>
 int32_t launch_stream(const I8Args & a, int groups, cudaStream_t s) {
     const int blocks = ceil_div(a.rows, 16), steps = ceil_div(a.cols, 64);
     const int warps = !a.plan && blocks <= 148 * 2 && steps >= 32 ? 16 : (long long)blocks * groups < 148 * 4 ? 8 : 4;
-    auto kernel = i8_stream_k<MATS, NT, (NT > 2 ? 2 : 4)>;
+    auto kernel = i8_stream_k<MATS, NT, (NT > 2 ? 2 : 4), EPI>;
     if constexpr (MATS == 1 && NT == 1)
-        if (steps >= 8 * warps) kernel = i8_stream_k<1, 1, 8>;
+        if (steps >= 8 * warps) kernel = i8_stream_k<1, 1, 8, EPI>;
     launch_overlapped(kernel, dim3(blocks, groups), dim3(32 * warps), size_t(warps) * MATS * NT * 128 * sizeof(int), s, a);
     return launch_status();
 }
-template <int MATS>
+template <int MATS, bool EPI = false>
 int32_t i8_stream(const I8Args & a, int groups, long long tokens, cudaStream_t s) {
     if (groups > 65535) return B2MOE_ERR_SHAPE;                        // the grid's second extent
     // rows that a pass over the weights serves: a second pass of some experts (from the L2) costs less than the registers of 16 rows (512 experts at five each: 184 and 222 us)
-    if (tokens <= 8LL * groups) return launch_stream<MATS, 1>(a, groups, s);
-    if (tokens <= 16LL * groups) return launch_stream<MATS, 2>(a, groups, s);
-    return launch_stream<MATS, 4>(a, groups, s);
+    if (tokens <= 8LL * groups) return launch_stream<MATS, 1, EPI>(a, groups, s);
+    if (tokens <= 16LL * groups) return launch_stream<MATS, 2, EPI>(a, groups, s);
+    return launch_stream<MATS, 4, EPI>(a, groups, s);
 }
 int groups_of(int experts, int n, int topk, int shared_tokens) { return int(std::min((long long)n * topk, (long long)experts)) + (shared_tokens ? 1 : 0); }
 
@@ -239,18 +240,30 @@ int32_t i8_dump(const b2moe_bank & b, float * out, cudaStream_t s) {
 
 using namespace b2;
 
-extern "C" B2MOE_API int32_t b2moe_linear_i8(const int8_t * q, int64_t ldq, const float * scale, const b2moe_bank * w, int32_t n, void * y, int32_t y_dtype, int64_t ldy, int32_t * status,
-                                             b2moe_stream stream) {
+static int32_t linear_any(const int8_t * q, int64_t ldq, const float * scale, const b2moe_bank * w, int32_t n, const float * bias, int32_t act, const void * residual, int64_t ldr, void * y,
+                          int32_t y_dtype, int64_t ldy, int32_t * status, b2moe_stream stream) {
     if (int32_t rc = check_bank(w)) return rc;
     if (w->type != B2MOE_I8) return B2MOE_ERR_FORMAT;
     if (n <= 0 || n > I8_MAX_ROWS || w->experts != 1 || !valid_dtype(y_dtype) || ldq < w->cols || ldq % 16 || ldy < w->rows) return B2MOE_ERR_SHAPE;
+    if (act < B2MOE_ACT_NONE || act > B2MOE_ACT_GELU_TANH || (residual && ldr < w->rows)) return B2MOE_ERR_SHAPE;
     if (!q || !scale || !y) return B2MOE_ERR_NULL;
     if (!aligned16(q) || !aligned_to(y, dtype_bytes(y_dtype)) || !aligned_to(scale, 4) || !aligned_to(status, 4)) return B2MOE_ERR_ALIGN;
+    if (!aligned_to(bias, 4) || !aligned_to(residual, dtype_bytes(y_dtype))) return B2MOE_ERR_ALIGN;
     I8Args p{};
     p.w[0] = static_cast<const int8_t *>(w->data); p.v[0] = static_cast<const float *>(w->aux);
     p.experts = 1; p.rows = w->rows; p.cols = w->cols;
     p.q = q; p.ldq = ldq; p.s = scale; p.n = n;
     p.y = y; p.y_dtype = y_dtype; p.ldy = ldy;
+    p.bias = bias; p.residual = residual; p.ldr = ldr; p.act = act;
     if (i8_takes_gemm(1, n > I8_DENSE_ROWS)) return i8_gemm<1>(p, n, n, status, as_stream(stream));
-    return i8_stream<1>(p, 1, n, as_stream(stream));
+    return has_epilogue(p) ? i8_stream<1, true>(p, 1, n, as_stream(stream)) : i8_stream<1>(p, 1, n, as_stream(stream));
+}
+
+extern "C" B2MOE_API int32_t b2moe_linear_i8(const int8_t * q, int64_t ldq, const float * scale, const b2moe_bank * w, int32_t n, void * y, int32_t y_dtype, int64_t ldy, int32_t * status,
+                                             b2moe_stream stream) {
+    return linear_any(q, ldq, scale, w, n, nullptr, B2MOE_ACT_NONE, nullptr, 0, y, y_dtype, ldy, status, stream);
+}
+extern "C" B2MOE_API int32_t b2moe_linear_i8_epilogue(const int8_t * q, int64_t ldq, const float * scale, const b2moe_bank * w, int32_t n, const float * bias, int32_t act, const void * residual,
+                                                      int64_t ldr, void * y, int32_t y_dtype, int64_t ldy, int32_t * status, b2moe_stream stream) {
+    return linear_any(q, ldq, scale, w, n, bias, act, residual, ldr, y, y_dtype, ldy, status, stream);
 }

@@ -159,12 +159,14 @@ def quantize_rows(x: torch.Tensor):
     return q, scale
 
 
-def linear_i8(q: torch.Tensor, scale: torch.Tensor, bank: DeviceBank, out_dtype=torch.bfloat16, out: torch.Tensor | None = None, status: torch.Tensor | None = None):
+def linear_i8(q: torch.Tensor, scale: torch.Tensor, bank: DeviceBank, out_dtype=torch.bfloat16, out: torch.Tensor | None = None, status: torch.Tensor | None = None,
+              bias: torch.Tensor | None = None, activation: str = "none", residual: torch.Tensor | None = None):
     """y [n, rows] = (q . w) * scale[t] * bank scale[r] of 8-bit rows (b2moe_linear_i8); q and out may be rows of wider matrices. A launch that gives up a bounded
-    wait leaves NaN in what it did not finish, and a nonzero value in `status` where that is given"""
+    wait leaves NaN in what it did not finish, and a nonzero value in `status` where that is given. With a bias (float32 [rows]), an activation ("relu", "silu", "gelu", "gelu_tanh") or a
+    residual (of the output's type, rows like it; it may be `out`): activation(y + bias) + residual in the same pass (b2moe_linear_i8_epilogue)"""
     n, k = q.shape
     ldq, one = q.stride()
-    ldy = rows = bank.rows
+    ldr = ldy = rows = bank.rows
     if q.dtype is not torch.int8 or k != bank.cols or scale.dtype is not torch.float32 or scale.numel() != n or not scale.is_contiguous():
         raise capi.B2moeError(capi.ERR_SHAPE, "linear_i8: int8 rows of the bank's columns and a float32 scale for each are wanted")
     if one != 1 and k > 1:
@@ -178,10 +180,21 @@ def linear_i8(q: torch.Tensor, scale: torch.Tensor, bank: DeviceBank, out_dtype=
             raise capi.B2moeError(capi.ERR_SHAPE, "linear_i8: an output [n, rows] with contiguous rows is wanted")
         out_dtype = out.dtype
         ldy = out.stride(0) if n > 1 else rows
-    stream = _stream_of(q, scale, out, status, banks=(bank,))
+    act = capi.ACT.get(activation)
+    if act is None:
+        raise capi.B2moeError(capi.ERR_SHAPE, f"linear_i8: no activation of the name {activation!r}")
+    if bias is not None and (bias.dtype is not torch.float32 or bias.numel() != rows or not bias.is_contiguous()):
+        raise capi.B2moeError(capi.ERR_SHAPE, "linear_i8: the bias is a contiguous float32 for each row of the bank")
+    if residual is not None:
+        ldr = _rows_of(residual, n, rows, out_dtype, "linear_i8")
+    stream = _stream_of(q, scale, out, status, bias, residual, banks=(bank,))
     if out is None:
         out = torch.empty(n, rows, dtype=out_dtype, device=q.device)
-    check(lib.b2moe_linear_i8(q.data_ptr(), ldq if n > 1 else k, scale.data_ptr(), C.byref(bank.c), n, out.data_ptr(), _DT[out_dtype], ldy, _ptr(status), stream), "b2moe_linear_i8")
+    if act or bias is not None or residual is not None:
+        check(lib.b2moe_linear_i8_epilogue(q.data_ptr(), ldq if n > 1 else k, scale.data_ptr(), C.byref(bank.c), n, _ptr(bias), act, _ptr(residual), ldr, out.data_ptr(), _DT[out_dtype], ldy, _ptr(status),
+                                           stream), "b2moe_linear_i8_epilogue")
+    else:
+        check(lib.b2moe_linear_i8(q.data_ptr(), ldq if n > 1 else k, scale.data_ptr(), C.byref(bank.c), n, out.data_ptr(), _DT[out_dtype], ldy, _ptr(status), stream), "b2moe_linear_i8")
     return out
 
 
