@@ -23,7 +23,11 @@ namespace b2 {
 namespace {
 using namespace tc;
 
-constexpr int TC_THREADS = 384, TC_EPI_WARP0 = 4, TC_EPI_WARPS = 8, TC_EPI_THREADS = 32 * TC_EPI_WARPS, TC_MAX_STAGES = 12, TC_MAX_EXPERTS = 4096;
+constexpr int TC_EPI_WARP0 = 4, TC_MAX_STAGES = 12, TC_MAX_EXPERTS = 4096;
+// warps that empty the accumulators: more with an epilogue, since what they do to a value is no longer little. 4096 rows of 4096 x 4096 with GELU, bias and residual, 8 / 12 / 16 warps: 74 / 70 / 76 us,
+// of 4096 x 512 49 / 45 / 51 (16 leave a thread 96 registers)
+constexpr int epi_warps(bool epi) { return epi ? 12 : 8; }
+constexpr int tc_threads(bool epi) { return 32 * (TC_EPI_WARP0 + epi_warps(epi)); }
 constexpr int TC_A_BYTES = 128 * 128, TC_SMEM = 227 * 1024, TC_MAX_SPLIT = 8;
 // static arrays and the alignment of the ring; what a launch asks for at most
 constexpr int TC_FIXED = 8 * 1024, TC_ALIGN = 1024, TC_SMEM_MOST = TC_SMEM - TC_FIXED + TC_ALIGN;
@@ -77,13 +81,18 @@ __device__ __forceinline__ uint32_t at_rank(uint32_t addr, int rank) {
     return r;
 }
 __device__ __forceinline__ void bar_arrive_cluster(uint32_t bar) { asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
-__device__ __forceinline__ void epi_sync() { asm volatile("bar.sync 1, %0;" ::"n"(TC_EPI_THREADS) : "memory"); }
+template <bool EPI> __device__ __forceinline__ void epi_sync() { asm volatile("bar.sync 1, %0;" ::"n"(32 * epi_warps(EPI)) : "memory"); }
 
 struct TcItem { int e, first, count, rb; };      // expert, first row (slot), rows, block of weight rows
 
 __device__ __forceinline__ float to_float(float v) { return v; }
 __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
 __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <class T> __device__ __forceinline__ T to_type(float f) {
+    if constexpr (std::is_same<T, float>::value) return f;
+    else if constexpr (std::is_same<T, __half>::value) return __float2half_rn(f);
+    else return __float2bfloat16_rn(f);
+}
 
 // this lane's weight row of an item
 template <int MATS>
@@ -91,27 +100,78 @@ __device__ __forceinline__ int weight_row(const TcItem & im, int quarter, int la
     return MATS == 2 ? im.rb * 64 + 16 * quarter + (lane & 15) : im.rb * 128 + 32 * quarter + lane;
 }
 // the item's outputs from tensor memory; t: (output row, scale) of its activation rows, v: the scales of the lane's weight row; EPI: what follows the product, with the bias of the lane's weight row
-template <int MATS, bool EPI, class T>
-__device__ __forceinline__ void store_item(const I8Args & p, const TcItem & im, uint32_t taddr, const int2 * t, const float (&v)[MATS], float bias, int quarter, int half, int lane) {
+// ready(): waits for the sums; false where that ran out, and nothing is stored
+template <int MATS, bool EPI, class T, class F>
+__device__ __forceinline__ bool store_item(const I8Args & p, const TcItem & im, uint32_t taddr, const int2 * t, const float (&v)[MATS], float bias, int quarter, int half, int lane, F ready) {
+    constexpr int STRIDE = 4 * epi_warps(EPI);                         // the warps of a quarter take 16 columns in turn
     const bool upper = MATS == 2 && lane >= 16;
     const int row = weight_row<MATS>(im, quarter, lane);
     const bool in = row < p.rows;
     T * const y = static_cast<T *>(p.y) + row;
-    auto put = [&](int at, float f) {
-        T * d = y + size_t(uint32_t(at)) * p.ldy;
-        if constexpr (std::is_same<T, float>::value) *d = f;
-        else if constexpr (std::is_same<T, __half>::value) *d = __float2half_rn(f);
-        else *d = __float2bfloat16_rn(f);
-    };
-#pragma unroll 1
-    for (int c = 16 * half; c < im.count; c += 32) {
-        uint32_t d[16];
-        T r[16];                                                       // EPI: the residual's values of these 16 rows, asked for together (they may lie under the outputs, and loads stay behind stores)
-        if (EPI && p.residual) {
-            const T * from = static_cast<const T *>(p.residual) + row;
+    auto put = [&](int at, float f) { y[size_t(uint32_t(at)) * p.ldy] = to_type<T>(f); };
+    // The residual's values of the next 16 rows are asked for before the ones at hand are worked on, the first before the sums are there: behind the copies of the operands a load takes thousands of cycles
+    // (4096 rows of 4096 x 4096: 76 us without, 66 with). Rows behind the last and lanes without a weight row read one that is there: loads under a condition each wait for one another (135 us)
+    T next[16];
+    auto ask = [&](int c) {
+        const T * from = static_cast<const T *>(p.residual) + size_t(im.first + c) * p.ldr + min(row, p.rows - 1);
+        const int last = im.count - 1 - c;
+        if (last >= 15) {
 #pragma unroll
-            for (int j = 0; j < 16; ++j)
-                if (in && c + j < im.count) r[j] = from[size_t(uint32_t(t[c + j].x)) * p.ldr];
+            for (int j = 0; j < 16; ++j, from += p.ldr) next[j] = *from;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) next[j] = from[(long long)min(j, last) * p.ldr];
+        }
+    };
+    if (EPI && p.residual && 16 * half < im.count) ask(16 * half);
+    const bool ok = ready();
+#pragma unroll 1
+    for (int c = 16 * half; ok && c < im.count; c += STRIDE) {
+        uint32_t d[16];
+        if constexpr (EPI) {                                           // a dense call: the item's rows follow one another
+            T now[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) now[j] = next[j];
+            if (p.residual && c + STRIDE < im.count) ask(c + STRIDE);
+            tmem_ld16(taddr + c, d);
+            tmem_ld_wait();
+            T * to = y + size_t(im.first + c) * p.ldy;
+            const int rows = im.count - c;
+#pragma unroll
+            for (int j0 = 0; j0 < 16; j0 += 8) {
+                float r[8];
+                Two scale[4], f[4];
+                int sum[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    sum[j] = int(d[j0 + j]);
+                    r[j] = to_float(now[j0 + j]);
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int4 pair = *reinterpret_cast<const int4 *>(t + c + j0 + 2 * j);
+                    scale[j] = two(__int_as_float(pair.y), __int_as_float(pair.w)) * two(v[0]);
+                }
+                finish(p, sum, scale, bias, r, f);
+                T out[8];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float2 g = apart(f[j]);
+                    out[2 * j] = to_type<T>(g.x);
+                    out[2 * j + 1] = to_type<T>(g.y);
+                }
+                if (in) {
+                    if (rows >= 16) {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j, to += p.ldy) *to = out[j];
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j, to += p.ldy)
+                            if (j0 + j < rows) *to = out[j];
+                    }
+                }
+            }
+            continue;
         }
         tmem_ld16(taddr + c, d);
         tmem_ld_wait();
@@ -125,24 +185,19 @@ __device__ __forceinline__ void store_item(const I8Args & p, const TcItem & im, 
                 const int gs = int(upper ? other : d[j]), us = int(upper ? d[j + 1] : other);
                 const float s = upper ? s1 : s0, g = float(gs) * (s * v[0]), u = float(us) * (s * v[MATS - 1]);
                 if (in && c + j + int(upper) < im.count) put(upper ? two.z : two.x, g / (1.f + expf(-g)) * u);
-            } else if (EPI) {
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const float f = finished(p, int(d[j + i]), (i ? s1 : s0) * v[0], bias, to_float(r[j + i]));
-                    if (in && c + j + i < im.count) put(i ? two.z : two.x, f);
-                }
             } else {
                 if (in && c + j < im.count) put(two.x, float(int(d[j])) * (s0 * v[0]));
                 if (in && c + j + 1 < im.count) put(two.z, float(int(d[j + 1])) * (s1 * v[0]));
             }
         }
     }
+    return ok;
 }
 
-// The outputs of an item that was left unfinished by a wait that ran out: NaN, since the call may have no status word to tell. One weight row; of the item's activation rows this half's 16 of every 32.
+// The outputs of an item that was left unfinished by a wait that ran out: NaN, since the call may have no status word to tell. One weight row; of the item's activation rows this warp's 16 of every `stride`.
 // Not inlined, so that it takes no registers from what happens
-__device__ __noinline__ void spoil_rows(void * y, int dtype, long long ldy, int row, const int2 * t, int count, int half) {
-    for (int c = 16 * half; c < count; c += 32)
+__device__ __noinline__ void spoil_rows(void * y, int dtype, long long ldy, int row, const int2 * t, int count, int half, int stride) {
+    for (int c = 16 * half; c < count; c += stride)
         for (int j = c; j < min(c + 16, count); ++j) store_act(y, dtype, size_t(uint32_t(t[j].x)) * ldy + row, __int_as_float(0x7fc00000));
 }
 
@@ -153,11 +208,12 @@ __device__ __noinline__ void spoil_rows(void * y, int dtype, long long ldy, int 
 enum { TC_SPLIT = 1, TC_PAIR = 2 };
 // EPI (dense calls): bias, activation and residual follow the product
 template <int MATS, int MODE, bool EPI>
-__global__ void __launch_bounds__(TC_THREADS, MODE ? 1 : 2) i8_gemm_k(const I8Args p, const TcArgs c, const __grid_constant__ TcMaps maps) {
+__global__ void __launch_bounds__(tc_threads(EPI), MODE || EPI ? 1 : 2) i8_gemm_k(const I8Args p, const TcArgs c, const __grid_constant__ TcMaps maps) {
     extern __shared__ __align__(1024) uint8_t tc_mem[];
     __shared__ __align__(16) int2 table[2][256];
     __shared__ __align__(8) uint64_t bars[2 * TC_MAX_STAGES + 5];
-    __shared__ int scan[TC_THREADS / 32];
+    constexpr int THREADS = tc_threads(EPI), EPI_WARPS = epi_warps(EPI);
+    __shared__ int scan[THREADS / 32];
     __shared__ uint32_t tmem_slot;
     __shared__ volatile int abort_flag;
     constexpr bool SPLIT = MODE == TC_SPLIT, PAIR = MODE == TC_PAIR;
@@ -170,7 +226,7 @@ __global__ void __launch_bounds__(TC_THREADS, MODE ? 1 : 2) i8_gemm_k(const I8Ar
     const uint32_t full = saddr(bars), empty = full + 8 * TC_MAX_STAGES, acc_full = empty + 8 * TC_MAX_STAGES, acc_empty = acc_full + 16, drain = acc_empty + 16;
     if (threadIdx.x == 0) {
         for (int i = 0; i < c.stages; ++i) { bar_init(full + 8 * i, 1); bar_init(empty + 8 * i, 1); }
-        for (int i = 0; i < 2; ++i) { bar_init(acc_full + 8 * i, 1); bar_init(acc_empty + 8 * i, (PAIR ? 2 : 1) * TC_EPI_WARPS); }
+        for (int i = 0; i < 2; ++i) { bar_init(acc_full + 8 * i, 1); bar_init(acc_empty + 8 * i, (PAIR ? 2 : 1) * EPI_WARPS); }
         bar_init(drain, 1);
         bar_init_fence();
         abort_flag = 0;
@@ -193,7 +249,7 @@ __global__ void __launch_bounds__(TC_THREADS, MODE ? 1 : 2) i8_gemm_k(const I8Ar
     int tiles = c.tiles;
     if (p.plan) {
         // inclusive prefix sums of the experts' tiles: a span of experts a thread (a call without a shared expert leaves that of the plan out)
-        const int span = (ne + TC_THREADS - 1) / TC_THREADS, lo = min(ne, int(threadIdx.x) * span), hi = min(ne, lo + span);
+        const int span = (ne + THREADS - 1) / THREADS, lo = min(ne, int(threadIdx.x) * span), hi = min(ne, lo + span);
         int mine = 0;
         for (int e = lo; e < hi; ++e) mine += (counts[e] + c.nt - 1) / c.nt;
         int run = mine;
@@ -354,7 +410,7 @@ __global__ void __launch_bounds__(TC_THREADS, MODE ? 1 : 2) i8_gemm_k(const I8Ar
         if (warp_wait(acc_full, 0)) {
             fence_after();
 #pragma unroll 1
-            for (int col = 16 * half; col < im.count; col += 32) {
+            for (int col = 16 * half; col < im.count; col += 4 * EPI_WARPS) {
                 uint32_t d[16];
                 tmem_ld16(tmem + (uint32_t(32 * quarter) << 16) + col, d);
                 tmem_ld_wait();
@@ -365,7 +421,7 @@ __global__ void __launch_bounds__(TC_THREADS, MODE ? 1 : 2) i8_gemm_k(const I8Ar
             give_up();
         }
     } else if (!SPLIT && warp >= TC_EPI_WARP0) {
-        // ---- results: warp q of either half reads the lanes 32 (q mod 4) of tensor memory, the halves take 16 columns in turn ----
+        // ---- results: warp q reads the lanes 32 (q mod 4) of tensor memory, those of the same lanes take 16 columns in turn ----
         const int tid = threadIdx.x - 32 * TC_EPI_WARP0, quarter = warp & 3, half = (warp - TC_EPI_WARP0) >> 2;
         // what the stores of an item need to know (its rows' places and scales, the weight row's scales) is asked for an item ahead
         int2 mine = make_int2(0, 0);
@@ -375,7 +431,15 @@ __global__ void __launch_bounds__(TC_THREADS, MODE ? 1 : 2) i8_gemm_k(const I8Ar
             const int row = weight_row<MATS>(im, quarter, lane);
 #pragma unroll
             for (int m = 0; m < MATS; ++m) v[m] = row < p.rows ? (p.plan && im.e == p.experts ? p.shared_v[m] : p.v[m] + size_t(im.e) * p.rows)[row] : 0.f;
-            if (EPI) bias = p.bias && row < p.rows ? p.bias[row] : 0.f;
+            if (EPI) {
+                bias = p.bias && row < p.rows ? p.bias[row] : 0.f;
+                // the item's part of the residual, into the L2: a row's 128 values a thread
+                if (p.residual && tid < im.count) {
+                    const int size = p.y_dtype == B2MOE_F32 ? 4 : 2;
+                    const char * from = static_cast<const char *>(p.residual) + size_t(mine.x) * p.ldr * size;
+                    for (int j = 128 * im.rb; j < min(p.rows, 128 * im.rb + 128); j += 128 / size) asm volatile("prefetch.global.L2 [%0];" ::"l"(from + size_t(j) * size));
+                }
+            }
         };
         const uint32_t acc_empty0 = PAIR ? at_rank(acc_empty, 0) : acc_empty;
         uint32_t done = 0;
@@ -394,22 +458,24 @@ __global__ void __launch_bounds__(TC_THREADS, MODE ? 1 : 2) i8_gemm_k(const I8Ar
 #pragma unroll
             for (int m = 0; m < MATS; ++m) scale[m] = v[m];
             const float add = bias;
-            epi_sync();                                                // the table is there; the other one's item has been read by every warp
+            epi_sync<EPI>();                                                // the table is there; the other one's item has been read by every warp
             if (it + it_step < items) {
                 next = locate(it + it_step);
                 fetch(next);
             }
-            ok = ok && !abort_flag && warp_wait(acc_full + 8 * h, (done >> 1) & 1u);
-            fence_after();
-            if (ok) {
-                const uint32_t taddr = tmem + h * c.half + (uint32_t(32 * quarter) << 16);
-                if (p.y_dtype == B2MOE_F32) store_item<MATS, EPI, float>(p, im, taddr, table[h], scale, add, quarter, half, lane);
-                else if (p.y_dtype == B2MOE_F16) store_item<MATS, EPI, __half>(p, im, taddr, table[h], scale, add, quarter, half, lane);
-                else store_item<MATS, EPI, __nv_bfloat16>(p, im, taddr, table[h], scale, add, quarter, half, lane);
-            } else {
+            auto ready = [&]() {
+                ok = ok && !abort_flag && warp_wait(acc_full + 8 * h, (done >> 1) & 1u);
+                fence_after();
+                return ok;
+            };
+            const uint32_t taddr = tmem + h * c.half + (uint32_t(32 * quarter) << 16);
+            if (p.y_dtype == B2MOE_F32) store_item<MATS, EPI, float>(p, im, taddr, table[h], scale, add, quarter, half, lane, ready);
+            else if (p.y_dtype == B2MOE_F16) store_item<MATS, EPI, __half>(p, im, taddr, table[h], scale, add, quarter, half, lane, ready);
+            else store_item<MATS, EPI, __nv_bfloat16>(p, im, taddr, table[h], scale, add, quarter, half, lane, ready);
+            if (!ok) {
                 if (lane == 0) give_up();
                 const int row = weight_row<MATS>(im, quarter, lane);
-                if (row < p.rows) spoil_rows(p.y, p.y_dtype, p.ldy, row, table[h], im.count, half);
+                if (row < p.rows) spoil_rows(p.y, p.y_dtype, p.ldy, row, table[h], im.count, half, 4 * epi_warps(EPI));
             }
             fence_before();
             __syncwarp();
@@ -438,7 +504,7 @@ __global__ void __launch_bounds__(TC_THREADS, MODE ? 1 : 2) i8_gemm_k(const I8Ar
         for (int z = 0; z < TC_MAX_SPLIT; ++z) asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(place[z]) : "r"(saddr(ring) + 4 * r), "r"(z < parts ? z : 0));
         cluster.sync();
         // four activation rows of a thread at a time: a read of another block's memory takes several hundred cycles
-        constexpr int STEP = TC_THREADS / 128;
+        constexpr int STEP = THREADS / 128;
         for (int col = lo + (threadIdx.x >> 7); col < hi && in; col += 4 * STEP) {
             int part[4][TC_MAX_SPLIT];
             float s[4], r[4] = {};
@@ -457,7 +523,8 @@ __global__ void __launch_bounds__(TC_THREADS, MODE ? 1 : 2) i8_gemm_k(const I8Ar
 #pragma unroll
                 for (int z = 0; z < TC_MAX_SPLIT; ++z)
                     if (z < parts) sum += part[i][z];
-                const float out = EPI ? finished(p, sum, s[i] * v, bias, r[i]) : float(sum) * (s[i] * v);
+                float out = float(sum) * (s[i] * v);
+                if (EPI) out = finish_one(p, sum, s[i] * v, bias, r[i]);
                 if (col + i * STEP < hi) store_act(p.y, p.y_dtype, size_t(im.first + col + i * STEP) * p.ldy + row, out);
             }
         }
@@ -475,9 +542,9 @@ int sm_count() {
     return count;
 }
 template <class K>
-int32_t launch_cluster(K kernel, dim3 grid, dim3 cluster, size_t smem, cudaStream_t s, const I8Args & p, const TcArgs & c, const TcMaps & maps) {
+int32_t launch_cluster(K kernel, int threads, dim3 grid, dim3 cluster, size_t smem, cudaStream_t s, const I8Args & p, const TcArgs & c, const TcMaps & maps) {
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = grid; cfg.blockDim = dim3(TC_THREADS); cfg.dynamicSmemBytes = smem; cfg.stream = s;
+    cfg.gridDim = grid; cfg.blockDim = dim3(threads); cfg.dynamicSmemBytes = smem; cfg.stream = s;
     cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = cluster.x; at[0].val.clusterDim.y = cluster.y; at[0].val.clusterDim.z = cluster.z;
@@ -505,7 +572,7 @@ int clusters_at_once(int size) {
         if (!allow_smem(i8_gemm_k<1, TC_SPLIT, false>, TC_SMEM_MOST)) return m;
         for (int size = 2; size <= TC_MAX_SPLIT; ++size) {
             cudaLaunchConfig_t cfg{};
-            cfg.gridDim = dim3(1, 1, size); cfg.blockDim = dim3(TC_THREADS); cfg.dynamicSmemBytes = TC_SMEM_MOST;
+            cfg.gridDim = dim3(1, 1, size); cfg.blockDim = dim3(tc_threads(false)); cfg.dynamicSmemBytes = TC_SMEM_MOST;
             cudaLaunchAttribute at[1];
             at[0].id = cudaLaunchAttributeClusterDimension;
             at[0].val.clusterDim.x = 1; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = size;
@@ -575,7 +642,7 @@ int32_t i8_gemm(const I8Args & p, long long q_rows, int per_group, int * status,
     //   gate/up of 512 columns at 8 each 107 / 78, of 2048 columns at 80 242 / 258
     //   dense 8192 rows of 4096 x 512 44 / 36, of 4096 x 1024 49 / 42
     const int sms = sm_count();
-    const bool longer = p.cols > 2560, two = p.cols <= I8_SHORT_COLS;
+    const bool longer = p.cols > 2560, two = p.cols <= I8_SHORT_COLS && !has_epilogue(p);
     if (p.plan) c.nt = two ? 128 : per_group > 96 || longer ? 256 : 128;
     else c.nt = dense_rows(p.n, c.row_blocks, ceil_div(p.cols, 128), longer, two, sms);
     c.tiles = p.plan ? 0 : ceil_div(p.n, c.nt);
@@ -609,16 +676,16 @@ int32_t i8_gemm(const I8Args & p, long long q_rows, int per_group, int * status,
         if constexpr (MATS == 1)
             if (split > 1) {
                 if (!allow_smem(i8_gemm_k<1, TC_SPLIT, EPI>, TC_SMEM_MOST)) return B2MOE_ERR_CUDA;
-                return launch_cluster(i8_gemm_k<1, TC_SPLIT, EPI>, dim3(unsigned(items), 1, split), dim3(1, 1, split), smem, s, p, c, maps);
+                return launch_cluster(i8_gemm_k<1, TC_SPLIT, EPI>, tc_threads(EPI), dim3(unsigned(items), 1, split), dim3(1, 1, split), smem, s, p, c, maps);
             }
         if (pair) {
             if (!allow_smem(i8_gemm_k<MATS, TC_PAIR, EPI>, TC_SMEM_MOST)) return B2MOE_ERR_CUDA;
             const long long pairs = (long long)c.tiles * ceil_div(c.row_blocks, 2);
-            return launch_cluster(i8_gemm_k<MATS, TC_PAIR, EPI>, dim3(unsigned(2 * (p.plan ? sms / 2 : std::min<long long>(sms / 2, pairs)))), dim3(2), smem, s, p, c, maps);
+            return launch_cluster(i8_gemm_k<MATS, TC_PAIR, EPI>, tc_threads(EPI), dim3(unsigned(2 * (p.plan ? sms / 2 : std::min<long long>(sms / 2, pairs)))), dim3(2), smem, s, p, c, maps);
         }
         if (!allow_smem(i8_gemm_k<MATS, 0, EPI>, TC_SMEM_MOST)) return B2MOE_ERR_CUDA;
         const int blocks = two ? 2 * sms : sms;
-        launch_overlapped(i8_gemm_k<MATS, 0, EPI>, dim3(unsigned(p.plan ? blocks : std::min<long long>(blocks, items))), dim3(TC_THREADS), smem, s, p, c, maps);
+        launch_overlapped(i8_gemm_k<MATS, 0, EPI>, dim3(unsigned(p.plan ? blocks : std::min<long long>(blocks, items))), dim3(tc_threads(EPI)), smem, s, p, c, maps);
         return launch_status();
     };
     if constexpr (MATS == 1)

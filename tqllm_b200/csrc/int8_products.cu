@@ -121,7 +121,7 @@ __global__ void __launch_bounds__(512) i8_stream_k(const I8Args p) {
                 const float u = float(sum[MATS - 1]) * (s * v[MATS - 1][row]);
                 out = out / (1.f + expf(-out)) * u;
             }
-            if (EPI) out = finished(p, sum[0], s * v[0][row], p.bias ? p.bias[row] : 0.f, p.residual ? load_act(p.residual, p.y_dtype, size_t(j) * p.ldr + row) : 0.f);
+            if (EPI) out = finish_one(p, sum[0], s * v[0][row], p.bias ? p.bias[row] : 0.f, p.residual ? load_act(p.residual, p.y_dtype, size_t(j) * p.ldr + row) : 0.f);
             store_act(p.y, p.y_dtype, size_t(a) * p.ldy + row, out);
         }
     }
