@@ -180,7 +180,7 @@ def check_gradient(h, w, g, s, got, weight, dtype, before=None):
     d, bound, dw, size = gradient(h, w, g, s)
     near(got, d, bound, dtype)
     n, k = h.shape
-    blocks = min(n, 148 * max(1, min(16, 8192 // k)))
+    blocks = min((n + 7) // 8 * 8, 148 * max(1, min(8, 8192 // k)) // 8 * 8)
     before = 0.0 if before is None else before.double()
     room = (27 + n // blocks + 1 + blocks // 8 + 10) * U * size + U * (dw + before).abs() + 2.0 ** -149
     assert bool(((weight.cpu().double() - dw - before).abs() <= room).all())
@@ -198,6 +198,33 @@ def test_gradient(n, k, dtype, wdtype, skip):
     check_gradient(x, w, g, s, got, weight, dtype)
     again, none = moe.rms_norm_backward(x.cuda(), w.cuda(), g.cuda(), EPS, up(s), weight_grad=False)
     assert none is None and torch.equal(again, got)
+
+
+@pytest.mark.parametrize("dtype", (BF16, F16, F32))
+@pytest.mark.parametrize("k,ld,begin", ((33, 48, 3), (101, 101, 5), (101, 108, 5), (1031, 1040, 1), (2050, 2051, 7), (5000, 5002, 2), (8193, 8193, 1), (16370, 16371, 6), (64, 72, 4), (64, 64, 1), (4096, 4099, 0)))
+def test_rows_that_begin_anywhere(dtype, k, ld, begin):
+    """rows that begin behind 16 bytes, in all matrices alike or in one otherwise; nothing beside them is touched"""
+    from tqllm_b200 import moe
+    n = 19
+    x, r, w, gen = make(n, k, dtype, F32, k + ld)
+    g = torch.randn(n, k, generator=gen).to(dtype)
+    for lone in (None, 0, 4):
+        bufs = [torch.full((n * ld + 16,), 3.0, dtype=dtype, device="cuda") for _ in range(8)]
+        view = [b[begin + (i == lone):].as_strided((n, k), (ld, 1)) for i, b in enumerate(bufs)]
+        for v, t in zip(view, (x, r, x, r, x, g, r, x)):
+            v.copy_(t)
+        keep = [b.clone() for b in bufs]
+        out = moe.rms_norm(view[0], w.cuda(), EPS, view[1], out=view[2], sum_out=view[3])
+        check_norm(x, r, w, out, dtype)
+        check_norm(x, None, w, moe.rms_norm(view[0], w.cuda(), EPS, out=view[2]), dtype)
+        got, weight = moe.rms_norm_backward(view[4], w.cuda(), view[5], EPS, view[6], out=view[7])
+        got = got.clone()
+        check_gradient(x, w, g, r, got, weight, dtype)
+        for i, (b, v, t) in enumerate(zip(bufs, view, (x, r, x, r, x, g, r, x))):
+            v.copy_(t)
+            assert torch.equal(b, keep[i])
+        moe.rms_norm_backward(view[4], w.cuda(), view[5], EPS, view[6], out=view[5])
+        assert torch.equal(view[5], got) if lone is None else True
 
 
 def test_gradient_is_added_and_lies_on_its_inputs():

@@ -6,6 +6,7 @@
 //
 // One pass: the row stays in registers between its sums and its outputs. Bound by memory.
 #include <algorithm>
+#include <type_traits>
 
 #include "int8.cuh"
 
@@ -35,7 +36,26 @@ template <int DT, int V> struct Piece {
 #pragma unroll
         for (int j = 0; j < WORDS; ++j) w[j] = make_uint4(0, 0, 0, 0);
     }
+    __device__ __forceinline__ uint32_t & word(int j) { return j % 4 == 0 ? w[j / 4].x : j % 4 == 1 ? w[j / 4].y : j % 4 == 2 ? w[j / 4].z : w[j / 4].w; }
     __device__ __forceinline__ uint32_t word(int j) const { return j % 4 == 0 ? w[j / 4].x : j % 4 == 1 ? w[j / 4].y : j % 4 == 2 ? w[j / 4].z : w[j / 4].w; }
+    // those of the values i .. i + V - 1 of a row that lie in [0, k), one by one; the piece is zero before
+    __device__ __forceinline__ void load_some(const void * row, int i, int k) {
+#pragma unroll
+        for (int l = 0; l < V; ++l)
+            if (unsigned(i + l) < unsigned(k)) {
+                if constexpr (DT == B2MOE_F32) word(l) = static_cast<const uint32_t *>(row)[i + l];
+                else word(l / 2) |= uint32_t(static_cast<const uint16_t *>(row)[i + l]) << (16 * (l & 1));
+            }
+    }
+    // values outside of [0, k) become zero
+    __device__ __forceinline__ void trim(int i, int k) {
+#pragma unroll
+        for (int l = 0; l < V; ++l)
+            if (unsigned(i + l) >= unsigned(k)) {
+                if constexpr (DT == B2MOE_F32) word(l) = 0u;
+                else word(l / 2) &= l & 1 ? 0x0000ffffu : 0xffff0000u;
+            }
+    }
     __device__ __forceinline__ float operator[](int i) const {
         if (DT == B2MOE_F32) return __uint_as_float(word(i));
         const uint32_t u = word(i / 2);
@@ -46,9 +66,15 @@ template <int DT, int V> struct Piece {
 template <int DT> struct Piece<DT, 1> {
     float v;
     __device__ __forceinline__ void load(const void * p, size_t i) { v = load_act(p, DT, i); }
+    __device__ __forceinline__ void load_some(const void * row, int i, int k) { if (unsigned(i) < unsigned(k)) load(row, i); }
     __device__ __forceinline__ void zero() { v = 0.f; }
     __device__ __forceinline__ float operator[](int) const { return v; }
 };
+template <int DT, int V> __device__ __forceinline__ void store_some(void * row, int i, int k, const float (&v)[V]) {
+#pragma unroll
+    for (int l = 0; l < V; ++l)
+        if (unsigned(i + l) < unsigned(k)) store_act(row, DT, size_t(i + l), v[l]);
+}
 template <int DT, int V> __device__ __forceinline__ void store_piece(void * p, size_t i, const float (&v)[V]) {
     using T = typename Elem<DT>::type;
     T * at = static_cast<T *>(p) + i;
@@ -76,6 +102,34 @@ template <int DT, int V> __device__ __forceinline__ void store_piece(void * p, s
     }
 }
 
+// The pieces of a row. As it is: piece c holds the values from c V on, every row begins on 16 bytes and ends with a whole piece. SHIFT: rows begin `phase` values behind 16 bytes, in all matrices alike (odd k, a
+// view of a wider matrix): piece c holds the values from c V - phase on, the first and the last are not whole and go value by value
+template <int V, bool SHIFT> struct Grid {
+    int k, phase;
+    __device__ __forceinline__ int first(int c) const { return c * V - (SHIFT ? phase : 0); }
+    __device__ __forceinline__ bool any(int j) const { return j < k && (!SHIFT || j + V > 0); }
+    __device__ __forceinline__ bool whole(int j) const { return !SHIFT || (j >= 0 && j + V <= k); }
+};
+template <int V> __device__ __forceinline__ int phase_of(const void * row, int size) { return V == 1 ? 0 : int(reinterpret_cast<uintptr_t>(row) / size % V); }
+template <int DT, int V, bool SHIFT>
+__device__ __forceinline__ void get(Piece<DT, V> & v, const void * base, size_t row, int j, const Grid<V, SHIFT> & grid) {
+    const void * at = static_cast<const typename Elem<DT>::type *>(base) + row;
+    if (grid.whole(j)) v.load(at, j);
+    else v.load_some(at, j, grid.k);
+}
+template <int DT, int V, bool SHIFT>
+__device__ __forceinline__ void put(void * base, size_t row, int j, const Grid<V, SHIFT> & grid, const float (&v)[V]) {
+    void * at = static_cast<typename Elem<DT>::type *>(base) + row;
+    if (grid.whole(j)) store_piece<DT, V>(at, j, v);
+    else store_some<DT, V>(at, j, grid.k, v);
+}
+// the norm's weight begins on 16 bytes where the rows do, and is read value by value where they do not
+template <int WDT, int V, bool SHIFT>
+__device__ __forceinline__ void get_weight(Piece<WDT, V> & w, const void * base, int j, const Grid<V, SHIFT> & grid) {
+    if (SHIFT) w.load_some(base, j, grid.k);
+    else w.load(base, j);
+}
+
 struct NormArgs {
     const void * x, * r, * w;
     long long ldx, ldr, lds, ldy, ldq;
@@ -98,6 +152,11 @@ __device__ __forceinline__ T over_row(T v, T none, T * red, F join) {
     if (warps == 1) return v;
     if (lane == 0) red[threadIdx.x >> 5] = v;
     __syncthreads();
+    if (warps <= 4) {
+        v = red[0];
+        for (int i = 1; i < warps; ++i) v = join(v, red[i]);
+        return v;
+    }
     v = lane < warps ? red[lane] : none;
 #pragma unroll
     for (int d = 16; d; d >>= 1) v = join(v, shuffled(v, d));
@@ -121,7 +180,7 @@ __device__ __noinline__ int nearest_product(float h, float w, double top) {
 constexpr float UNIT = 0x1p-80f;
 
 // P pieces of V values a thread; WARP: a warp a row, eight rows a block; otherwise the block takes a row. WDT: the weight's type; Q: 8-bit rows are wanted
-template <int DT, int WDT, int V, int P, bool WARP, bool Q>
+template <int DT, int WDT, int V, int P, bool WARP, bool Q, bool SHIFT>
 __global__ void __launch_bounds__(WARP ? 256 : 512) norm_k(const NormArgs p) {
     __shared__ float2 red[32], red_again[32];
     __shared__ double red_exact[32];
@@ -130,20 +189,23 @@ __global__ void __launch_bounds__(WARP ? 256 : 512) norm_k(const NormArgs p) {
     const int nt = WARP ? 32 : blockDim.x, tid = WARP ? threadIdx.x & 31 : threadIdx.x;
     const int row = WARP ? blockIdx.x * 8 + (threadIdx.x >> 5) : blockIdx.x;
     if (WARP && row >= p.n) return;                                    // no barrier follows in this form
+    using T = typename Elem<DT>::type;
+    const size_t x0 = size_t(row) * p.ldx;
+    const Grid<V, SHIFT> grid{p.k, SHIFT ? phase_of<V>(static_cast<const T *>(p.x) + x0, sizeof(T)) : 0};
     float h[P][V];
     Piece<WDT, V> w[P];
     {
         Piece<DT, V> x[P], r[P];
 #pragma unroll
         for (int i = 0; i < P; ++i) {
-            const int j = (i * nt + tid) * V;
+            const int j = grid.first(i * nt + tid);
             x[i].zero();
             r[i].zero();
             w[i].zero();
-            if (j >= p.k) continue;
-            x[i].load(p.x, size_t(row) * p.ldx + j);
-            if (p.r) r[i].load(p.r, size_t(row) * p.ldr + j);
-            w[i].load(p.w, j);
+            if (!grid.any(j)) continue;
+            get(x[i], p.x, x0, j, grid);
+            if (p.r) get(r[i], p.r, size_t(row) * p.ldr, j, grid);
+            get_weight(w[i], p.w, j, grid);
         }
 #pragma unroll
         for (int i = 0; i < P; ++i)
@@ -169,8 +231,8 @@ __global__ void __launch_bounds__(WARP ? 256 : 512) norm_k(const NormArgs p) {
     if (p.sum) {
 #pragma unroll
         for (int i = 0; i < P; ++i) {
-            const int j = (i * nt + tid) * V;
-            if (j < p.k) store_piece<DT, V>(p.sum, size_t(row) * p.lds + j, h[i]);
+            const int j = grid.first(i * nt + tid);
+            if (grid.any(j)) put<DT>(p.sum, size_t(row) * p.lds, j, grid, h[i]);
         }
     }
     float2 all = join(mine, red);
@@ -189,16 +251,43 @@ __global__ void __launch_bounds__(WARP ? 256 : 512) norm_k(const NormArgs p) {
     if (p.y) {
 #pragma unroll
         for (int i = 0; i < P; ++i) {
-            const int j = (i * nt + tid) * V;
-            if (j >= p.k) continue;
+            const int j = grid.first(i * nt + tid);
+            if (!grid.any(j)) continue;
             float y[V];
 #pragma unroll
             for (int l = 0; l < V; ++l) y[l] = h[i][l] * rho * w[i][l];
-            store_piece<DT, V>(p.y, size_t(row) * p.ldy + j, y);
+            put<DT>(p.y, size_t(row) * p.ldy, j, grid, y);
         }
     }
     if constexpr (Q) {
         const float top = all.y;
+        if (tid == 0) p.scale[row] = fine ? top * rho / 127.f : __int_as_float(0x7fc00000);
+        const bool tiny = top < 0x1p-100f, all_exact = fine && tiny && top > 0.f;      // products have lost bits there
+        const float inv = tiny || !fine ? 0.f : __fdiv_rn(127.f, top);
+        // u, top and inv are off by 2^-24 of themselves each, the quotient t by 3 |t| 2^-24: those that close to a half are done again, exactly. (One row of 4096 in thirty has such a value.) The
+        // nearest integer m comes from t + 1.5 * 2^23; |t| <= |m| + 1/2
+        constexpr float MAGIC = 12582912.f, OFF = 3.2f * 0x1p-24f;
+        float off = 0.f;
+        int8_t * const q = p.q + size_t(row) * p.ldq;
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            uint32_t b[V], o[V / 4];
+#pragma unroll
+            for (int l = 0; l < V; ++l) {
+                const float u = h[i][l] * w[i][l], f = __fmaf_rn(u, inv, MAGIC), m = MAGIC - f;
+                b[l] = __float_as_uint(f);
+                off = fmaxf(off, fmaf(fabsf(m), OFF, fabsf(__fmaf_rn(u, inv, m))));
+            }
+#pragma unroll
+            for (int l = 0; l < V / 4; ++l) o[l] = fine ? __byte_perm(__byte_perm(b[4 * l], b[4 * l + 1], 0x0040), __byte_perm(b[4 * l + 2], b[4 * l + 3], 0x0040), 0x5410) : 0u;
+            const int j = grid.first(i * nt + tid);
+            if (j >= p.k) continue;
+            if constexpr (V == 8) *reinterpret_cast<uint2 *>(q + j) = make_uint2(o[0], o[1]);
+            else *reinterpret_cast<uint32_t *>(q + j) = o[0];
+        }
+        bool close = fine && (off > 0.5f - OFF || all_exact);
+        close = WARP ? __any_sync(0xffffffffu, close) : __syncthreads_or(close);
+        if (!close) return;
         // the largest product exactly: among those that round to the largest
         double exact = 0.0;
         if (mine.y == top) {
@@ -209,57 +298,40 @@ __global__ void __launch_bounds__(WARP ? 256 : 512) norm_k(const NormArgs p) {
                     if (fabsf(h[i][l] * w[i][l]) == top) exact = fmax(exact, fabs(double(h[i][l]) * double(w[i][l])));
         }
         exact = over_row<WARP>(exact, 0.0, red_exact, Max());
-        if (tid == 0) p.scale[row] = fine ? top * rho / 127.f : __int_as_float(0x7fc00000);
-        const bool tiny = top < 0x1p-100f;                             // products have lost bits there
-        const float inv = tiny || !fine ? 0.f : __fdiv_rn(127.f, top);
-        // u, top and inv are off by 2^-24 each, their quotient by 127 times the sum: those that close to a half are done again
-        const float near = !fine || top == 0.f ? 1.f : tiny ? -1.f : 0.5f - 5e-5f;
-        constexpr float MAGIC = 12582912.f;                            // u * inv + 1.5 * 2^23: the nearest integer in the low bits
 #pragma unroll
-        for (int i = 0; i < P; ++i) {
-            const int j = (i * nt + tid) * V;
-            if (j >= p.k) continue;
-            uint32_t b[V];
-            float off = 0.f;
+        for (int i = 0; i < P; ++i)
 #pragma unroll
             for (int l = 0; l < V; ++l) {
-                const float u = fine ? h[i][l] * w[i][l] : 0.f, f = __fmaf_rn(u, inv, MAGIC);
-                b[l] = __float_as_uint(f);
-                off = fmaxf(off, fabsf(__fmaf_rn(u, inv, MAGIC - f)));
+                const float u = h[i][l] * w[i][l], f = __fmaf_rn(u, inv, MAGIC), m = MAGIC - f;
+                const int j = grid.first(i * nt + tid) + l;
+                if (j < p.k && (all_exact || fmaf(fabsf(m), OFF, fabsf(__fmaf_rn(u, inv, m))) > 0.5f - OFF)) q[j] = int8_t(nearest_product(h[i][l], w[i][l], exact));
             }
-            if (off > near) {
-#pragma unroll
-                for (int l = 0; l < V; ++l) {
-                    const float u = h[i][l] * w[i][l], f = __uint_as_float(b[l]);
-                    if (fabsf(__fmaf_rn(u, inv, MAGIC - f)) > near) b[l] = uint32_t(nearest_product(h[i][l], w[i][l], exact));
-                }
-            }
-            uint32_t o[V / 4];
-#pragma unroll
-            for (int l = 0; l < V / 4; ++l) o[l] = __byte_perm(__byte_perm(b[4 * l], b[4 * l + 1], 0x0040), __byte_perm(b[4 * l + 2], b[4 * l + 3], 0x0040), 0x5410);
-            int8_t * at = p.q + size_t(row) * p.ldq + j;
-            if constexpr (V == 8) *reinterpret_cast<uint2 *>(at) = make_uint2(o[0], o[1]);
-            else *reinterpret_cast<uint32_t *>(at) = o[0];
-        }
     }
 }
 
+// how the rows of a call lie
+enum Form { WHOLE, SHIFTED, SINGLE };            // whole pieces of 16 bytes; pieces behind a phase that all matrices share; value by value
+
 template <int DT, int WDT, bool Q>
-void launch_norm_wide(const NormArgs & a, cudaStream_t s) {
+void launch_norm_whole(const NormArgs & a, cudaStream_t s) {
     constexpr int V = DT == B2MOE_F32 ? 4 : 8, MOST = NORM_MAX_COLS / V / 512;
     const int by_warp = ceil_div(a.k / V, 32);
     auto go = [&](auto kernel, int blocks, int threads) { launch_overlapped(kernel, dim3(blocks), dim3(threads), 0, s, a); };
-    if (by_warp <= 4 && a.n >= SMS * 16) go(norm_k<DT, WDT, V, 4, true, Q>, ceil_div(a.n, 8), 256);
-    else if (by_warp <= 16 && a.n < SMS * 16) go(norm_k<DT, WDT, V, 1, false, Q>, a.n, by_warp * 32);
-    else if (by_warp <= 64) go(norm_k<DT, WDT, V, 4, false, Q>, a.n, ceil_div(by_warp, 4) * 32);
-    else go(norm_k<DT, WDT, V, MOST, false, Q>, a.n, ceil_div(by_warp, MOST) * 32);
+    if (by_warp <= 4 && a.n >= SMS * 16) go(norm_k<DT, WDT, V, 4, true, Q, false>, ceil_div(a.n, 8), 256);
+    else if (by_warp <= 16 && a.n < SMS * 16) go(norm_k<DT, WDT, V, 1, false, Q, false>, a.n, by_warp * 32);
+    else if (by_warp <= 64) go(norm_k<DT, WDT, V, 4, false, Q, false>, a.n, ceil_div(by_warp, 4) * 32);
+    else go(norm_k<DT, WDT, V, MOST, false, Q, false>, a.n, ceil_div(by_warp, MOST) * 32);
 }
 template <int DT, int WDT>
-int32_t launch_norm(const NormArgs & a, bool wide, cudaStream_t s) {
-    if (wide && a.q) launch_norm_wide<DT, WDT, true>(a, s);
-    else if (wide) launch_norm_wide<DT, WDT, false>(a, s);
-    else if (a.k <= 2048) launch_overlapped(norm_k<DT, WDT, 1, 4, false, false>, dim3(a.n), dim3(ceil_div(a.k, 128) * 32), 0, s, a);
-    else launch_overlapped(norm_k<DT, WDT, 1, 32, false, false>, dim3(a.n), dim3(ceil_div(a.k, 1024) * 32), 0, s, a);
+int32_t launch_norm(const NormArgs & a, Form form, cudaStream_t s) {
+    constexpr int V = DT == B2MOE_F32 ? 4 : 8, MOST = NORM_MAX_COLS / V / 512;
+    auto go = [&](auto kernel, int threads) { launch_overlapped(kernel, dim3(a.n), dim3(threads), 0, s, a); };
+    const int by_warp = ceil_div(a.k + V - 1, 32 * V);                 // SHIFTED: a phase of V - 1 at most
+    if (form == WHOLE && a.q) launch_norm_whole<DT, WDT, true>(a, s);
+    else if (form == WHOLE) launch_norm_whole<DT, WDT, false>(a, s);
+    else if (form == SHIFTED && by_warp <= 16 * MOST) by_warp <= 4 ? go(norm_k<DT, WDT, V, 1, false, false, true>, by_warp * 32) : go(norm_k<DT, WDT, V, MOST, false, false, true>, ceil_div(by_warp, MOST) * 32);
+    else if (a.k <= 2048) go(norm_k<DT, WDT, 1, 4, false, false, false>, ceil_div(a.k, 128) * 32);
+    else go(norm_k<DT, WDT, 1, 32, false, false, false>, ceil_div(a.k, 1024) * 32);
     return launch_status();
 }
 
@@ -267,125 +339,219 @@ struct NormGradArgs {
     const void * h, * w, * dy, * ds;
     long long ldh, ldy, lds, ldx;
     float eps;
-    int n, k;
+    int n, k, stages;
     void * dx;
     float * parts;                     // [blocks][k]: each block's sums for the weight's gradient (null: not wanted)
 };
 
-template <int DT, int WDT, int V, int P>
-__global__ void __launch_bounds__(512) norm_grad_k(const NormGradArgs p) {
+__device__ __forceinline__ void copy16(void * shared, const void * global) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(uint32_t(__cvta_generic_to_shared(shared))), "l"(__cvta_generic_to_global(global)) : "memory");
+}
+
+// A block walks rows, the weight's gradient in registers. V > 1: the pieces of the rows to come are on their way into shared memory (`stages` rows of them), each thread's own, so that no barrier is needed for them;
+// V = 1: one row after the other. SHIFT: the grid is a multiple of V, so that all rows of a block have the same phase and a thread its columns
+// WARP (short rows): a warp a row, eight rows a block at a time and no barrier; the warps' sums for the weight's gradient meet at the end
+template <int DT, int WDT, int V, int P, bool SHIFT, bool WARP>
+__global__ void __launch_bounds__(WARP ? 256 : 512) norm_grad_k(const NormGradArgs p) {
+    extern __shared__ __align__(16) uint4 ahead[];                     // [stages][h, dy, ds][P][threads]
     __shared__ float2 red[2][32], red_again[2][32];
     grid_release();
     grid_wait();
-    const int nt = blockDim.x, tid = threadIdx.x;
+    const int nt = WARP ? 32 : blockDim.x, tid = WARP ? threadIdx.x & 31 : threadIdx.x, warp = threadIdx.x >> 5;
+    const int row0 = WARP ? blockIdx.x * 8 + warp : blockIdx.x, step = WARP ? gridDim.x * 8 : gridDim.x;
+    constexpr bool COPIES = V > 1;
+    uint4 * const ring = ahead + (WARP ? size_t(warp) * p.stages * 3 * P * 32 : 0);
+    using T = typename Elem<DT>::type;
+    const Grid<V, SHIFT> grid{p.k, SHIFT ? phase_of<V>(static_cast<const T *>(p.h) + size_t(row0) * p.ldh, sizeof(T)) : 0};
     Piece<WDT, V> w[P];
     float dw[P][V];
 #pragma unroll
     for (int i = 0; i < P; ++i) {
-        const int j = (i * nt + tid) * V;
+        const int j = grid.first(i * nt + tid);
         w[i].zero();
-        if (j < p.k) w[i].load(p.w, j);
+        if (grid.any(j)) get_weight(w[i], p.w, j, grid);
 #pragma unroll
         for (int l = 0; l < V; ++l) dw[i][l] = 0.f;
     }
-    int turn = 0;                                                      // two sets of words in turn: one barrier a row
-    for (int row = blockIdx.x; row < p.n; row += gridDim.x, turn ^= 1) {
-        Piece<DT, V> h[P], g[P], s[P];
+    // A piece that is not whole comes with its neighbours in the matrix, which `trim` drops; only in front of the matrix and behind it there may be nothing to read
+    auto bring = [&](uint4 * to, const void * base, int row, long long ld, int j) {
+        const T * at = static_cast<const T *>(base) + size_t(row) * ld;
+        if (grid.whole(j) || ((j >= 0 || row > 0) && (j + V <= p.k || row + 1 < p.n))) return copy16(to, at + j);
+        Piece<DT, V> some;
+        some.zero();
+        some.load_some(at, j, p.k);
+        if constexpr (COPIES) *to = some.w[0];
+    };
+    auto copy = [&](int row, int stage) {
+        if (row < p.n) {
+            uint4 * at = ring + size_t(stage) * 3 * P * nt + tid;
 #pragma unroll
-        for (int i = 0; i < P; ++i) {
-            const int j = (i * nt + tid) * V;
-            h[i].zero();
-            g[i].zero();
-            s[i].zero();
-            if (j >= p.k) continue;
-            h[i].load(p.h, size_t(row) * p.ldh + j);
-            g[i].load(p.dy, size_t(row) * p.ldy + j);
-            if (p.ds) s[i].load(p.ds, size_t(row) * p.lds + j);
+            for (int i = 0; i < P; ++i, at += nt) {
+                const int j = grid.first(i * nt + tid);
+                if (!grid.any(j)) continue;
+                bring(at, p.h, row, p.ldh, j);
+                bring(at + P * nt, p.dy, row, p.ldy, j);
+                if (p.ds) bring(at + 2 * P * nt, p.ds, row, p.lds, j);
+            }
         }
+        asm volatile("cp.async.commit_group;" ::: "memory");           // an empty one behind the last row: the count stays
+    };
+    if (COPIES)
+        for (int s = 0; s < p.stages; ++s) copy(row0 + s * step, s);
+    int turn = 0, stage = 0;                                           // two sets of words in turn: one barrier a row
+    for (int row = row0; row < p.n; row += step, turn ^= 1) {
+        if (COPIES) {
+            if (p.stages == 1) asm volatile("cp.async.wait_group 0;" ::: "memory");
+            else if (p.stages == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
+            else asm volatile("cp.async.wait_group 2;" ::: "memory");
+        }
+        // piece i of the row's matrix m (h, dy, ds), read where it is wanted: the row is not held in registers across the barrier (that took twice as many, and half of the blocks)
+        auto piece = [&](int m, int i, int j) {
+            Piece<DT, V> v;
+            if constexpr (COPIES) {
+                v.w[0] = ring[(size_t(stage) * 3 + m) * P * nt + i * nt + tid];
+                if (SHIFT && !grid.whole(j)) v.trim(j, p.k);
+            } else {
+                v.load(m == 0 ? p.h : m == 1 ? p.dy : p.ds, size_t(row) * (m == 0 ? p.ldh : m == 1 ? p.ldy : p.lds) + j);
+            }
+            return v;
+        };
         float unit = 1.f;
         auto sums = [&]() {
             float2 v = make_float2(0.f, 0.f);
 #pragma unroll
-            for (int i = 0; i < P; ++i)
+            for (int i = 0; i < P; ++i) {
+                const int j = grid.first(i * nt + tid);
+                if (!grid.any(j)) continue;
+                const Piece<DT, V> h = piece(0, i, j), g = piece(1, i, j);
 #pragma unroll
                 for (int l = 0; l < V; ++l) {
-                    const float f = h[i][l] * unit;
+                    const float f = h[l] * unit;
                     v.x = fmaf(f, f, v.x);
-                    v.y = fmaf(g[i][l] * w[i][l], f, v.y);
+                    v.y = fmaf(g[l] * w[i][l], f, v.y);
                 }
+            }
             return v;
         };
-        float2 v = over_row<false>(sums(), make_float2(0.f, 0.f), red[turn], Add2());
+        float2 v = over_row<WARP>(sums(), make_float2(0.f, 0.f), red[turn], Add2());
         if (!(v.x < INFINITY)) {
             unit = UNIT;
-            v = over_row<false>(sums(), make_float2(0.f, 0.f), red_again[turn], Add2());
+            v = over_row<WARP>(sums(), make_float2(0.f, 0.f), red_again[turn], Add2());
         }
         // in the unit: rho h as it is, rho the unit times as large
         const float m = v.x / float(p.k) + p.eps * unit * unit, rho = 1.f / sqrtf(m), t = v.y / float(p.k) / m, out = rho * unit;
 #pragma unroll
         for (int i = 0; i < P; ++i) {
-            const int j = (i * nt + tid) * V;
-            if (j >= p.k) continue;
+            const int j = grid.first(i * nt + tid);
+            if (!grid.any(j)) continue;
+            const Piece<DT, V> h = piece(0, i, j), g = piece(1, i, j);
+            Piece<DT, V> s;
+            s.zero();
+            if (p.ds) s = piece(2, i, j);
             float d[V];
 #pragma unroll
             for (int l = 0; l < V; ++l) {
-                const float f = h[i][l] * unit;
-                d[l] = fmaf(out, fmaf(-f, t, g[i][l] * w[i][l]), s[i][l]);
-                dw[i][l] = fmaf(g[i][l], f * rho, dw[i][l]);
+                const float f = h[l] * unit;
+                d[l] = fmaf(out, fmaf(-f, t, g[l] * w[i][l]), s[l]);
+                dw[i][l] = fmaf(g[l], f * rho, dw[i][l]);
             }
-            store_piece<DT, V>(p.dx, size_t(row) * p.ldx + j, d);
+            put<DT>(p.dx, size_t(row) * p.ldx, j, grid, d);
+        }
+        if (COPIES) {                                                  // this row's pieces have been read
+            copy(row + p.stages * step, stage);
+            if (++stage == p.stages) stage = 0;
         }
     }
     if (p.parts) {
+        if (WARP) __syncthreads();                                     // the ring is free: a row of sums a warp
+        float * const at = WARP ? reinterpret_cast<float *>(ahead) + warp * (32 * P * V) : p.parts + size_t(blockIdx.x) * p.k;
 #pragma unroll
         for (int i = 0; i < P; ++i) {
-            const int j = (i * nt + tid) * V;
-            if (j >= p.k) continue;
+            const int j = grid.first(i * nt + tid);
+            if (!grid.any(j)) continue;
+            if constexpr (COPIES && !SHIFT) {
 #pragma unroll
-            for (int l = 0; l < V; ++l) p.parts[size_t(blockIdx.x) * p.k + j + l] = dw[i][l];
+                for (int l = 0; l < V; l += 4) *reinterpret_cast<float4 *>(at + j + l) = make_float4(dw[i][l], dw[i][l + 1], dw[i][l + 2], dw[i][l + 3]);
+            } else {
+#pragma unroll
+                for (int l = 0; l < V; ++l)
+                    if (unsigned(j + l) < unsigned(p.k)) at[j + l] = dw[i][l];
+            }
+        }
+        if (WARP) {
+            __syncthreads();
+            for (int j = threadIdx.x; j < p.k; j += 256) {
+                const float * from = reinterpret_cast<const float *>(ahead) + j;
+                float sum = from[0];
+#pragma unroll
+                for (int i = 1; i < 8; ++i) sum += from[i * (32 * P * V)];
+                p.parts[size_t(blockIdx.x) * p.k + j] = sum;
+            }
         }
     }
 }
 
-// dw[j] = (accumulate: +) the sum over the blocks' parts, in a fixed order: 32 columns a block, eight threads a column
-__global__ void __launch_bounds__(256) norm_weight_grad_k(const float * parts, int blocks, int k, float * dw, int accumulate) {
-    __shared__ float part[8][32];
+// dw[j] = (accumulate: +) the sum over the blocks' parts, in a fixed order: 32 columns a block, a warp takes every 32nd part (eight warps: 8 us of 58 for 8192 x 4096, 32: XX)
+__global__ void __launch_bounds__(1024) norm_weight_grad_k(const float * parts, int blocks, int k, float * dw, int accumulate) {
+    __shared__ float part[32][33];
     grid_release();
     grid_wait();
-    const int j = blockIdx.x * 32 + (threadIdx.x & 31), y = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, j = blockIdx.x * 32 + lane;
     float s = 0.f;
     if (j < k)
-#pragma unroll 8
-        for (int b = y; b < blocks; b += 8) s += parts[size_t(b) * k + j];
-    part[y][threadIdx.x & 31] = s;
+#pragma unroll 10
+        for (int b = warp; b < blocks; b += 32) s += parts[size_t(b) * k + j];
+    part[warp][lane] = s;
     __syncthreads();
-    if (y || j >= k) return;
+    // the 32 sums of a column by a warp
+    s = part[lane][warp];
 #pragma unroll
-    for (int i = 1; i < 8; ++i) s += part[i][threadIdx.x];
-    dw[j] = accumulate ? dw[j] + s : s;
+    for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+    const int c = blockIdx.x * 32 + warp;
+    if (lane || c >= k) return;
+    dw[c] = accumulate ? dw[c] + s : s;
 }
 
-int grad_blocks(int n, int k) { return std::min(n, SMS * std::max(1, std::min(16, 8192 / k))); }
+// Blocks that walk the rows, and so the parts of the weight's gradient. Long rows: as many of an SM as 32 KB of 16-bit values in a row each make, eight at most; a multiple of eight, the most phases that rows
+// have. Short ones, a warp each: four blocks an SM, or two where a row takes four pieces a lane
+constexpr int GRAD_NUM = 16384;
+int grad_blocks_most(int n, int k) { return std::min((n + 7) / 8 * 8, SMS * std::max(4, std::min(8, GRAD_NUM / k)) / 8 * 8); }
 
 template <int DT, int WDT>
-void launch_norm_grad(const NormGradArgs & a, bool wide, cudaStream_t s) {
-    constexpr int V = DT == B2MOE_F32 ? 4 : 8, MOST = NORM_MAX_COLS / V / 512;
-    auto go = [&](auto kernel, int threads) { launch_overlapped(kernel, dim3(a.parts ? grad_blocks(a.n, a.k) : a.n), dim3(threads), 0, s, a); };
-    if (!wide) return a.k <= 2048 ? go(norm_grad_k<DT, WDT, 1, 4>, ceil_div(a.k, 128) * 32) : go(norm_grad_k<DT, WDT, 1, 32>, ceil_div(a.k, 1024) * 32);
-    const int by_warp = ceil_div(a.k / V, 32);
-    if (by_warp <= 8) go(norm_grad_k<DT, WDT, V, 1>, by_warp * 32);
-    else if (by_warp <= 32) go(norm_grad_k<DT, WDT, V, 2>, ceil_div(by_warp, 2) * 32);
-    else go(norm_grad_k<DT, WDT, V, MOST>, ceil_div(by_warp, MOST) * 32);
+int32_t launch_norm_grad(NormGradArgs a, Form form, cudaStream_t s, int & blocks) {
+    constexpr int V = DT == B2MOE_F32 ? 4 : 8, MOST = NORM_MAX_COLS / V / 512, SMEM = 216 * 1024;
+    // per_sm blocks fill an SM's shared memory, so that a launch that becomes resident while the one before it runs spreads over all SMs (69 us instead of 49 for 8192 x 4096, with more than two of an SM)
+    auto go = [&](auto kernel, bool by_row, int threads, int pieces, int per_sm) -> int32_t {
+        const size_t row = size_t(3) * pieces * threads * 16;          // of a stage
+        a.stages = int(std::min<size_t>(3, std::max<size_t>(1, SMEM / per_sm / (row ? row : SMEM))));
+        if (row && !allow_smem(kernel, SMEM)) return B2MOE_ERR_CUDA;
+        blocks = by_row ? std::min(ceil_div(a.n, 8), SMS * per_sm) : std::min((a.n + 7) / 8 * 8, SMS * per_sm / 8 * 8);
+        launch_overlapped(kernel, dim3(blocks), dim3(threads), row ? std::max<size_t>(a.stages * row, SMEM / per_sm) : 0, s, a);
+        return launch_status();
+    };
+    const int by_warp = ceil_div(form == SHIFTED ? a.k + V - 1 : a.k, 32 * V), per_sm = std::max(1, std::min(8, GRAD_NUM / a.k));      // a warp's pieces
+    if (form == SINGLE || by_warp > 16 * MOST) {
+        if (a.k <= 2048) return go(norm_grad_k<DT, WDT, 1, 4, false, false>, false, ceil_div(a.k, 128) * 32, 0, per_sm);
+        return go(norm_grad_k<DT, WDT, 1, 32, false, false>, false, ceil_div(a.k, 1024) * 32, 0, per_sm);
+    }
+    auto with = [&](auto shift) -> int32_t {
+        constexpr bool SHIFT = decltype(shift)::value;
+        if (by_warp <= 1) return go(norm_grad_k<DT, WDT, V, 1, SHIFT, true>, true, 256, 1, 4);
+        if (by_warp <= 2) return go(norm_grad_k<DT, WDT, V, 2, SHIFT, true>, true, 256, 2, 4);
+        if (by_warp <= 4) return go(norm_grad_k<DT, WDT, V, 4, SHIFT, true>, true, 256, 4, 2);
+        if (by_warp <= 32) return go(norm_grad_k<DT, WDT, V, 2, SHIFT, false>, false, ceil_div(by_warp, 2) * 32, 2, per_sm);
+        return go(norm_grad_k<DT, WDT, V, MOST, SHIFT, false>, false, ceil_div(by_warp, MOST) * 32, MOST, per_sm);
+    };
+    return form == SHIFTED ? with(std::true_type{}) : with(std::false_type{});
 }
 
-// rows of 16-byte pieces: the columns, every row's first value and the strides
-struct Rows { const void * p; long long ld; int dtype; };
-bool in_pieces(int k, std::initializer_list<Rows> rows) {
-    for (const Rows & r : rows) {
-        const int per = 16 / int(dtype_bytes(r.dtype));
-        if (r.p && (k % per || r.ld % per || !aligned16(r.p))) return false;
-    }
-    return true;
+struct Rows { const void * p; long long ld; };
+Form form_of(int k, int dtype, const void * weight, std::initializer_list<Rows> rows) {
+    const int size = int(dtype_bytes(dtype)), per = 16 / size, phase = int(reinterpret_cast<uintptr_t>(rows.begin()->p) / size % per), ld = int(rows.begin()->ld % per);
+    bool whole = k % per == 0 && phase == 0 && ld == 0 && aligned16(weight), shared = true;
+    for (const Rows & r : rows)
+        if (r.p) shared = shared && int(reinterpret_cast<uintptr_t>(r.p) / size % per) == phase && int(r.ld % per) == ld;
+    return shared ? (whole ? WHOLE : SHIFTED) : SINGLE;
 }
 bool weight_type(int dtype, int weight_dtype) { return weight_dtype == B2MOE_F32 || weight_dtype == dtype; }
 
@@ -401,18 +567,18 @@ extern "C" B2MOE_API int32_t b2moe_rms_norm(const void * x, int32_t dtype, int64
     if (!x || !weight || (!y && !q) || (q && !scale) || (sum && !residual)) return B2MOE_ERR_NULL;
     const size_t e = dtype_bytes(dtype);
     if (!aligned_to(x, e) || !aligned_to(residual, e) || !aligned_to(sum, e) || !aligned_to(y, e) || !aligned_to(weight, dtype_bytes(weight_dtype)) || !aligned16(q) || !aligned_to(scale, 4)) return B2MOE_ERR_ALIGN;
-    const bool wide = in_pieces(k, {{x, ldx, dtype}, {residual, ldr, dtype}, {sum, lds, dtype}, {y, ldy, dtype}, {weight, 0, weight_dtype}});
-    if (q && !wide) return B2MOE_ERR_ALIGN;                            // rows in 8 bits come from rows in pieces of 16 bytes
+    const Form form = form_of(k, dtype, weight, {{x, ldx}, {residual, ldr}, {sum, lds}, {y, ldy}});
+    if (q && form != WHOLE) return B2MOE_ERR_ALIGN;                            // rows in 8 bits come from rows in pieces of 16 bytes
     const NormArgs a{x, residual, weight, ldx, ldr, lds, ldy, ldq, eps, n, k, sum, y, q, scale};
     cudaStream_t s = as_stream(stream);
-    if (dtype == B2MOE_F32) return launch_norm<B2MOE_F32, B2MOE_F32>(a, wide, s);
-    if (dtype == B2MOE_F16) return weight_dtype == B2MOE_F32 ? launch_norm<B2MOE_F16, B2MOE_F32>(a, wide, s) : launch_norm<B2MOE_F16, B2MOE_F16>(a, wide, s);
-    return weight_dtype == B2MOE_F32 ? launch_norm<B2MOE_BF16, B2MOE_F32>(a, wide, s) : launch_norm<B2MOE_BF16, B2MOE_BF16>(a, wide, s);
+    if (dtype == B2MOE_F32) return launch_norm<B2MOE_F32, B2MOE_F32>(a, form, s);
+    if (dtype == B2MOE_F16) return weight_dtype == B2MOE_F32 ? launch_norm<B2MOE_F16, B2MOE_F32>(a, form, s) : launch_norm<B2MOE_F16, B2MOE_F16>(a, form, s);
+    return weight_dtype == B2MOE_F32 ? launch_norm<B2MOE_BF16, B2MOE_F32>(a, form, s) : launch_norm<B2MOE_BF16, B2MOE_BF16>(a, form, s);
 }
 
 extern "C" B2MOE_API size_t b2moe_rms_norm_backward_workspace_bytes(int32_t n, int32_t k) {
     if (n <= 0 || n > I8_MAX_ROWS || k <= 0 || k > NORM_MAX_COLS) return 0;
-    return align_up(size_t(grad_blocks(n, k)) * k * sizeof(float), 16);
+    return align_up(size_t(grad_blocks_most(n, k)) * k * sizeof(float), 16);
 }
 
 extern "C" B2MOE_API int32_t b2moe_rms_norm_backward(const void * h, int32_t dtype, int64_t ldh, const void * weight, int32_t weight_dtype, const void * grad_y, int64_t ldgy,
@@ -425,16 +591,15 @@ extern "C" B2MOE_API int32_t b2moe_rms_norm_backward(const void * h, int32_t dty
     if (!aligned_to(h, e) || !aligned_to(grad_y, e) || !aligned_to(grad_sum, e) || !aligned_to(grad_x, e) || !aligned_to(weight, dtype_bytes(weight_dtype)) || !aligned_to(grad_weight, 4) ||
         (grad_weight && !aligned16(workspace))) return B2MOE_ERR_ALIGN;
     if (grad_weight && workspace_bytes < b2moe_rms_norm_backward_workspace_bytes(n, k)) return B2MOE_ERR_WORKSPACE;
-    const bool wide = in_pieces(k, {{h, ldh, dtype}, {grad_y, ldgy, dtype}, {grad_sum, ldgs, dtype}, {grad_x, ldgx, dtype}, {weight, 0, weight_dtype}});
-    const NormGradArgs a{h, weight, grad_y, grad_sum, ldh, ldgy, ldgs, ldgx, eps, n, k, grad_x, grad_weight ? static_cast<float *>(workspace) : nullptr};
+    const Form form = form_of(k, dtype, weight, {{h, ldh}, {grad_y, ldgy}, {grad_sum, ldgs}, {grad_x, ldgx}});
+    const NormGradArgs a{h, weight, grad_y, grad_sum, ldh, ldgy, ldgs, ldgx, eps, n, k, 1, grad_x, grad_weight ? static_cast<float *>(workspace) : nullptr};
     cudaStream_t s = as_stream(stream);
-    if (dtype == B2MOE_F32) launch_norm_grad<B2MOE_F32, B2MOE_F32>(a, wide, s);
-    else if (dtype == B2MOE_F16 && weight_dtype == B2MOE_F32) launch_norm_grad<B2MOE_F16, B2MOE_F32>(a, wide, s);
-    else if (dtype == B2MOE_F16) launch_norm_grad<B2MOE_F16, B2MOE_F16>(a, wide, s);
-    else if (weight_dtype == B2MOE_F32) launch_norm_grad<B2MOE_BF16, B2MOE_F32>(a, wide, s);
-    else launch_norm_grad<B2MOE_BF16, B2MOE_BF16>(a, wide, s);
-    if (int32_t rc = launch_status()) return rc;
+    int32_t rc, blocks = 0;
+    if (dtype == B2MOE_F32) rc = launch_norm_grad<B2MOE_F32, B2MOE_F32>(a, form, s, blocks);
+    else if (dtype == B2MOE_F16) rc = weight_dtype == B2MOE_F32 ? launch_norm_grad<B2MOE_F16, B2MOE_F32>(a, form, s, blocks) : launch_norm_grad<B2MOE_F16, B2MOE_F16>(a, form, s, blocks);
+    else rc = weight_dtype == B2MOE_F32 ? launch_norm_grad<B2MOE_BF16, B2MOE_F32>(a, form, s, blocks) : launch_norm_grad<B2MOE_BF16, B2MOE_BF16>(a, form, s, blocks);
+    if (rc) return rc;
     if (!grad_weight) return B2MOE_OK;
-    launch_overlapped(norm_weight_grad_k, dim3(ceil_div(k, 32)), dim3(256), 0, s, static_cast<const float *>(workspace), grad_blocks(n, k), k, grad_weight, accumulate);
+    launch_overlapped(norm_weight_grad_k, dim3(ceil_div(k, 32)), dim3(1024), 0, s, static_cast<const float *>(workspace), blocks, k, grad_weight, accumulate);
     return launch_status();
 }
