@@ -3,6 +3,7 @@
 #include <algorithm>
 
 #include "common.cuh"
+#include "two.cuh"
 
 namespace b2 {
 
@@ -43,14 +44,6 @@ struct I8Args {
 
 inline bool has_epilogue(const I8Args & a) { return a.bias || a.residual || a.act != B2MOE_ACT_NONE; }
 
-// two 32-bit values in one instruction, each rounded as by itself
-struct Two { unsigned long long v; };
-__device__ __forceinline__ Two two(float a, float b) { Two r; asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b)); return r; }
-__device__ __forceinline__ Two two(float a) { return two(a, a); }
-__device__ __forceinline__ float2 apart(Two a) { float2 r; asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a.v)); return r; }
-__device__ __forceinline__ Two operator*(Two a, Two b) { Two r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v)); return r; }
-__device__ __forceinline__ Two operator+(Two a, Two b) { Two r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v)); return r; }
-__device__ __forceinline__ Two fma2(Two a, Two b, Two c) { Two r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v)); return r; }
 __device__ __forceinline__ Two reciprocal(Two a) {                     // off by one step; 1 / inf = 0
     float2 f = apart(a);
     asm("rcp.approx.f32 %0, %0;" : "+f"(f.x));

@@ -21,6 +21,12 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
+__device__ __forceinline__ float largest(float a, Two b) {             // of three magnitudes; a NaN where there is one
+    const float2 f = apart(b);
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(fabsf(f.x)), "f"(fabsf(f.y)));
+    return r;
+}
 
 // V neighbouring values as they lie in memory: 16 bytes where rows allow it (V > 1), else one. 16-bit values are unpacked where they are used and take half a register each until then
 template <int DT, int V> struct Piece {
@@ -56,6 +62,7 @@ template <int DT, int V> struct Piece {
                 else word(l / 2) &= l & 1 ? 0x0000ffffu : 0xffff0000u;
             }
     }
+    __device__ __forceinline__ Two pair(int l) const { return two((*this)[2 * l], (*this)[2 * l + 1]); }
     __device__ __forceinline__ float operator[](int i) const {
         if (DT == B2MOE_F32) return __uint_as_float(word(i));
         const uint32_t u = word(i / 2);
@@ -69,6 +76,7 @@ template <int DT> struct Piece<DT, 1> {
     __device__ __forceinline__ void load_some(const void * row, int i, int k) { if (unsigned(i) < unsigned(k)) load(row, i); }
     __device__ __forceinline__ void zero() { v = 0.f; }
     __device__ __forceinline__ float operator[](int) const { return v; }
+    __device__ __forceinline__ Two pair(int) const { return two(v, 0.f); }
 };
 template <int DT, int V> __device__ __forceinline__ void store_some(void * row, int i, int k, const float (&v)[V]) {
 #pragma unroll
@@ -123,6 +131,13 @@ __device__ __forceinline__ void put(void * base, size_t row, int j, const Grid<V
     if (grid.whole(j)) store_piece<DT, V>(at, j, v);
     else store_some<DT, V>(at, j, grid.k, v);
 }
+template <int DT, int V, bool SHIFT>
+__device__ __forceinline__ void put(void * base, size_t row, int j, const Grid<V, SHIFT> & grid, const Two (&v)[(V + 1) / 2]) {
+    float f[V];
+#pragma unroll
+    for (int l = 0; l < V; ++l) f[l] = l & 1 ? apart(v[l / 2]).y : apart(v[l / 2]).x;
+    put<DT>(base, row, j, grid, f);
+}
 // the norm's weight begins on 16 bytes where the rows do, and is read value by value where they do not
 template <int WDT, int V, bool SHIFT>
 __device__ __forceinline__ void get_weight(Piece<WDT, V> & w, const void * base, int j, const Grid<V, SHIFT> & grid) {
@@ -133,7 +148,7 @@ __device__ __forceinline__ void get_weight(Piece<WDT, V> & w, const void * base,
 struct NormArgs {
     const void * x, * r, * w;
     long long ldx, ldr, lds, ldy, ldq;
-    float eps;
+    float eps, inv_k;
     int n, k;
     void * sum, * y;
     int8_t * q;
@@ -167,21 +182,65 @@ struct Add2 { __device__ float2 operator()(float2 a, float2 b) const { return ma
 struct AddMax { __device__ float2 operator()(float2 a, float2 b) const { return make_float2(a.x + b.x, max_nan(a.y, b.y)); } };
 struct Max { __device__ double operator()(double a, double b) const { return fmax(a, b); } };
 
-// The integer nearest to 127 u / top for products u = h w that 64 bits hold exactly, halves to even, exactly: 127 u and (m + 1/2) top are compared through what rounding
-// the latter leaves over
-__device__ __noinline__ int nearest_product(float h, float w, double top) {
-    const double u = double(h) * double(w), a = fabs(u), m = floor(127.0 * a / top), half = m + 0.5;
-    const double p = half * top, over = fma(127.0, a, -p), rest = fma(half, top, -p);
-    const int lo = int(m), q = over > rest ? lo + 1 : over < rest ? lo : lo + (lo & 1);
+// The integer nearest to 127 u / top for a product u = h w, which 64 bits hold exactly, halves to even, where it is `low` or the next: 127 |u| and (low + 1/2) top are compared through what rounding the
+// latter leaves over. off: what the top may be off by; 128 where that leaves it open
+__device__ __forceinline__ int decide(float h, float w, double low, double top, double off) {
+    const double u = double(h) * double(w), half = low + 0.5, p = half * top, diff = fma(127.0, fabs(u), -p) - fma(half, top, -p);
+    if (fabs(diff) < half * off) return 128;
+    const int lo = int(low), q = diff > 0.0 ? lo + 1 : diff < 0.0 ? lo : lo + (lo & 1);
     return u < 0.0 ? -q : q;
+}
+
+// 1 / sqrt(v): the approximation and a step of Newton's, off by 1.5 steps of 2^-24. (Root and quotients by their own rounded instructions, done by every thread of a row: 53 us instead of 51 for 8192 x 4096 to 8 bits, 65 instead of 57 for 4097 columns)
+__device__ __forceinline__ float inverse_root(float v) {
+    float r;
+    asm("rsqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
+    const float half = fmaf(-v * r, r, 1.f) * 0.5f;
+    return v > 0x1p-126f && v < INFINITY ? fmaf(r, half, r) : r;       // 0, infinities and NaN as they come
+}
+
+constexpr float MAGIC = 12582912.f, OFF = 5.2f * 0x1p-24f;
+__device__ __forceinline__ bool near_half(float u, float inv) {
+    const float m = MAGIC - __fmaf_rn(u, inv, MAGIC);
+    return fmaf(fabsf(m), OFF, fabsf(__fmaf_rn(u, inv, m))) > 0.5f - OFF;
+}
+template <int WDT, int V, int P> struct Held { Two h[P][(V + 1) / 2]; Piece<WDT, V> w[P]; };
+// The integers of a row's products whose quotient is close to a half once more, exactly, over those that are there. A function of its own: the registers of what is rare do not count in the kernel
+template <int WDT, int V, int P, bool WARP>
+__device__ __noinline__ void redo_close(const Held<WDT, V, P> & row, int8_t * q, int k, int nt, int tid, float mine, float top, float inv, bool close, bool all, double * red) {
+    auto value = [&](int i, int l) {
+        const float2 h = apart(row.h[i][l / 2]);
+        return make_float2(l & 1 ? h.y : h.x, row.w[i][l]);
+    };
+    // the largest product exactly: among those that round to the largest
+    double exact = 0.0;
+    if (mine == top)
+#pragma unroll 1
+        for (int i = 0; i < P; ++i)
+#pragma unroll
+            for (int l = 0; l < V; ++l) {
+                const float2 v = value(i, l);
+                if (fabsf(v.x * v.y) == top) exact = fmax(exact, fabs(double(v.x) * double(v.y)));
+            }
+    exact = over_row<WARP>(exact, 0.0, red, Max());
+    if (!close) return;
+#pragma unroll 1
+    for (int i = 0; i < P; ++i)
+#pragma unroll
+        for (int l = 0; l < V; ++l) {
+            const float2 v = value(i, l);
+            const int j = (i * nt + tid) * V + l;
+            if (j < k && (all || near_half(v.x * v.y, inv))) q[j] = int8_t(decide(v.x, v.y, floor(127.0 * fabs(double(v.x) * double(v.y)) / exact), exact, 0.0));
+        }
 }
 
 // Squares that pass the range of 32 bits: the row is taken once more in this unit, in which they do not (16384 squares of 2^48 at most), nor does what is small count there
 constexpr float UNIT = 0x1p-80f;
 
-// P pieces of V values a thread; WARP: a warp a row, eight rows a block; otherwise the block takes a row. WDT: the weight's type; Q: 8-bit rows are wanted
-template <int DT, int WDT, int V, int P, bool WARP, bool Q, bool SHIFT>
-__global__ void __launch_bounds__(WARP ? 256 : 512) norm_k(const NormArgs p) {
+// P pieces of V values a thread, in pairs (V = 1: a value and a zero); WARP: a warp a row, eight rows a block; otherwise the block, of MOST threads at most, takes a row. WDT: the weight's type; Q: 8-bit
+// rows are wanted. With 128 threads a row the registers are held to what five or six blocks of an SM have
+template <int DT, int WDT, int V, int P, bool WARP, bool Q, bool SHIFT, int MOST>
+__global__ void __launch_bounds__(MOST, MOST == 128 && V > 1 ? (Q ? 5 : 6) : WARP ? 2 : 1) norm_k(const NormArgs p) {
     __shared__ float2 red[32], red_again[32];
     __shared__ double red_exact[32];
     grid_release();
@@ -190,9 +249,10 @@ __global__ void __launch_bounds__(WARP ? 256 : 512) norm_k(const NormArgs p) {
     const int row = WARP ? blockIdx.x * 8 + (threadIdx.x >> 5) : blockIdx.x;
     if (WARP && row >= p.n) return;                                    // no barrier follows in this form
     using T = typename Elem<DT>::type;
+    constexpr int H = (V + 1) / 2;
     const size_t x0 = size_t(row) * p.ldx;
     const Grid<V, SHIFT> grid{p.k, SHIFT ? phase_of<V>(static_cast<const T *>(p.x) + x0, sizeof(T)) : 0};
-    float h[P][V];
+    Two h[P][H];
     Piece<WDT, V> w[P];
     {
         Piece<DT, V> x[P], r[P];
@@ -210,18 +270,20 @@ __global__ void __launch_bounds__(WARP ? 256 : 512) norm_k(const NormArgs p) {
 #pragma unroll
         for (int i = 0; i < P; ++i)
 #pragma unroll
-            for (int l = 0; l < V; ++l) h[i][l] = p.r ? x[i][l] + r[i][l] : x[i][l];
+            for (int l = 0; l < H; ++l) h[i][l] = x[i].pair(l) + r[i].pair(l);
     }
     auto sums = [&]() {                                                // squares, the largest product
-        float2 v = make_float2(0.f, 0.f);
+        Two squares = two(0.f);
+        float top = 0.f;
 #pragma unroll
         for (int i = 0; i < P; ++i)
 #pragma unroll
-            for (int l = 0; l < V; ++l) {
-                v.x = fmaf(h[i][l], h[i][l], v.x);
-                if (Q) v.y = max_nan(v.y, fabsf(h[i][l] * w[i][l]));
+            for (int l = 0; l < H; ++l) {
+                squares = fma2(h[i][l], h[i][l], squares);
+                if (Q) top = largest(top, h[i][l] * w[i].pair(l));
             }
-        return v;
+        const float2 s = apart(squares);
+        return make_float2(s.x + s.y, top);
     };
     auto join = [&](float2 v, float2 * red) {
         if constexpr (Q) return over_row<WARP>(v, make_float2(0.f, 0.f), red, AddMax());
@@ -243,19 +305,19 @@ __global__ void __launch_bounds__(WARP ? 256 : 512) norm_k(const NormArgs p) {
 #pragma unroll
         for (int i = 0; i < P; ++i)
 #pragma unroll
-            for (int l = 0; l < V; ++l) h[i][l] *= UNIT;
+            for (int l = 0; l < H; ++l) h[i][l] = h[i][l] * two(UNIT);
         mine = sums();
         all = join(mine, red_again);
     }
-    const float rho = 1.f / sqrtf(all.x / float(p.k) + p.eps * unit * unit);
+    const float rho = inverse_root(fmaf(all.x, p.inv_k, p.eps * unit * unit));
     if (p.y) {
 #pragma unroll
         for (int i = 0; i < P; ++i) {
             const int j = grid.first(i * nt + tid);
             if (!grid.any(j)) continue;
-            float y[V];
+            Two y[H];
 #pragma unroll
-            for (int l = 0; l < V; ++l) y[l] = h[i][l] * rho * w[i][l];
+            for (int l = 0; l < H; ++l) y[l] = h[i][l] * two(rho) * w[i].pair(l);
             put<DT>(p.y, size_t(row) * p.ldy, j, grid, y);
         }
     }
@@ -263,20 +325,27 @@ __global__ void __launch_bounds__(WARP ? 256 : 512) norm_k(const NormArgs p) {
         const float top = all.y;
         if (tid == 0) p.scale[row] = fine ? top * rho / 127.f : __int_as_float(0x7fc00000);
         const bool tiny = top < 0x1p-100f, all_exact = fine && tiny && top > 0.f;      // products have lost bits there
-        const float inv = tiny || !fine ? 0.f : __fdiv_rn(127.f, top);
-        // u, top and inv are off by 2^-24 of themselves each, the quotient t by 3 |t| 2^-24: those that close to a half are done again, exactly. (One row of 4096 in thirty has such a value.) The
-        // nearest integer m comes from t + 1.5 * 2^23; |t| <= |m| + 1/2
-        constexpr float MAGIC = 12582912.f, OFF = 3.2f * 0x1p-24f;
-        float off = 0.f;
+        float inv;
+        asm("rcp.approx.f32 %0, %1;" : "=f"(inv) : "f"(top));
+        inv = tiny || !fine ? 0.f : inv * 127.f;
+        // (OFF) u and top are off by 2^-24 of themselves, inv by 3 times that (its reciprocal 2, the product 1), the quotient t by 5 |t| 2^-24: those that close to a half are done again, exactly. The
+        // nearest integer m comes from t + 1.5 * 2^23; |t| <= |m| + 1/2. A piece is looked at by its largest m and its largest distance from an integer (one row of 4096 in ten has such a piece), then its
+        // values in 64 bits with the top as it is, which decides all but a sixth of them; rows of the others (one in a hundred) take the exact top
+        bool close = all_exact;
+        uint32_t some = 0;                                             // pieces with such a value
         int8_t * const q = p.q + size_t(row) * p.ldq;
 #pragma unroll
         for (int i = 0; i < P; ++i) {
             uint32_t b[V], o[V / 4];
+            float far = 0.f, big = 0.f;
 #pragma unroll
-            for (int l = 0; l < V; ++l) {
-                const float u = h[i][l] * w[i][l], f = __fmaf_rn(u, inv, MAGIC), m = MAGIC - f;
-                b[l] = __float_as_uint(f);
-                off = fmaxf(off, fmaf(fabsf(m), OFF, fabsf(__fmaf_rn(u, inv, m))));
+            for (int l = 0; l < H; ++l) {
+                const Two u = h[i][l] * w[i].pair(l), f = fma2(u, two(inv), two(MAGIC)), m = fma2(f, two(-1.f), two(MAGIC));
+                const float2 g = apart(f);
+                b[2 * l] = __float_as_uint(g.x);
+                b[2 * l + 1] = __float_as_uint(g.y);
+                big = largest(big, m);
+                far = largest(far, fma2(u, two(inv), m));
             }
 #pragma unroll
             for (int l = 0; l < V / 4; ++l) o[l] = fine ? __byte_perm(__byte_perm(b[4 * l], b[4 * l + 1], 0x0040), __byte_perm(b[4 * l + 2], b[4 * l + 3], 0x0040), 0x5410) : 0u;
@@ -284,28 +353,31 @@ __global__ void __launch_bounds__(WARP ? 256 : 512) norm_k(const NormArgs p) {
             if (j >= p.k) continue;
             if constexpr (V == 8) *reinterpret_cast<uint2 *>(q + j) = make_uint2(o[0], o[1]);
             else *reinterpret_cast<uint32_t *>(q + j) = o[0];
+            if (fmaf(big, OFF, far) > 0.5f - OFF) some |= 1u << i;
         }
-        bool close = fine && (off > 0.5f - OFF || all_exact);
-        close = WARP ? __any_sync(0xffffffffu, close) : __syncthreads_or(close);
-        if (!close) return;
-        // the largest product exactly: among those that round to the largest
-        double exact = 0.0;
-        if (mine.y == top) {
+        if (some && fine && !tiny) {
 #pragma unroll
             for (int i = 0; i < P; ++i)
+                if (some >> i & 1u)
 #pragma unroll
-                for (int l = 0; l < V; ++l)
-                    if (fabsf(h[i][l] * w[i][l]) == top) exact = fmax(exact, fabs(double(h[i][l]) * double(w[i][l])));
+                    for (int l = 0; l < V; ++l) {
+                        const float hl = l & 1 ? apart(h[i][l / 2]).y : apart(h[i][l / 2]).x;
+                        if (!near_half(hl * w[i][l], inv)) continue;
+                        const int exactly = decide(hl, w[i][l], floorf(fabsf(hl * w[i][l] * inv)), top, double(top) * 0x1.01p-24);
+                        if (exactly > 127) close = true;
+                        else q[grid.first(i * nt + tid) + l] = int8_t(exactly);
+                    }
         }
-        exact = over_row<WARP>(exact, 0.0, red_exact, Max());
+        close = close && fine;
+        if (!(WARP ? __any_sync(0xffffffffu, close) : __syncthreads_or(close))) return;
+        Held<WDT, V, P> held;
 #pragma unroll
-        for (int i = 0; i < P; ++i)
+        for (int i = 0; i < P; ++i) {
+            held.w[i] = w[i];
 #pragma unroll
-            for (int l = 0; l < V; ++l) {
-                const float u = h[i][l] * w[i][l], f = __fmaf_rn(u, inv, MAGIC), m = MAGIC - f;
-                const int j = grid.first(i * nt + tid) + l;
-                if (j < p.k && (all_exact || fmaf(fabsf(m), OFF, fabsf(__fmaf_rn(u, inv, m))) > 0.5f - OFF)) q[j] = int8_t(nearest_product(h[i][l], w[i][l], exact));
-            }
+            for (int l = 0; l < H; ++l) held.h[i][l] = h[i][l];
+        }
+        redo_close<WDT, V, P, WARP>(held, q, p.k, nt, tid, mine.y, top, inv, close, all_exact, red_exact);
     }
 }
 
@@ -317,10 +389,10 @@ void launch_norm_whole(const NormArgs & a, cudaStream_t s) {
     constexpr int V = DT == B2MOE_F32 ? 4 : 8, MOST = NORM_MAX_COLS / V / 512;
     const int by_warp = ceil_div(a.k / V, 32);
     auto go = [&](auto kernel, int blocks, int threads) { launch_overlapped(kernel, dim3(blocks), dim3(threads), 0, s, a); };
-    if (by_warp <= 4 && a.n >= SMS * 16) go(norm_k<DT, WDT, V, 4, true, Q, false>, ceil_div(a.n, 8), 256);
-    else if (by_warp <= 16 && a.n < SMS * 16) go(norm_k<DT, WDT, V, 1, false, Q, false>, a.n, by_warp * 32);
-    else if (by_warp <= 64) go(norm_k<DT, WDT, V, 4, false, Q, false>, a.n, ceil_div(by_warp, 4) * 32);
-    else go(norm_k<DT, WDT, V, MOST, false, Q, false>, a.n, ceil_div(by_warp, MOST) * 32);
+    if (by_warp <= 4 && a.n >= SMS * 16) go(norm_k<DT, WDT, V, 4, true, Q, false, 256>, ceil_div(a.n, 8), 256);
+    else if (by_warp <= 16 && a.n < SMS * 16) go(norm_k<DT, WDT, V, 1, false, Q, false, 512>, a.n, by_warp * 32);
+    else if (by_warp <= 16) go(norm_k<DT, WDT, V, 4, false, Q, false, 128>, a.n, ceil_div(by_warp, 4) * 32);
+    else go(norm_k<DT, WDT, V, MOST, false, Q, false, 512>, a.n, ceil_div(by_warp, MOST) * 32);
 }
 template <int DT, int WDT>
 int32_t launch_norm(const NormArgs & a, Form form, cudaStream_t s) {
@@ -329,16 +401,16 @@ int32_t launch_norm(const NormArgs & a, Form form, cudaStream_t s) {
     const int by_warp = ceil_div(a.k + V - 1, 32 * V);                 // SHIFTED: a phase of V - 1 at most
     if (form == WHOLE && a.q) launch_norm_whole<DT, WDT, true>(a, s);
     else if (form == WHOLE) launch_norm_whole<DT, WDT, false>(a, s);
-    else if (form == SHIFTED && by_warp <= 16 * MOST) by_warp <= 4 ? go(norm_k<DT, WDT, V, 1, false, false, true>, by_warp * 32) : go(norm_k<DT, WDT, V, MOST, false, false, true>, ceil_div(by_warp, MOST) * 32);
-    else if (a.k <= 2048) go(norm_k<DT, WDT, 1, 4, false, false, false>, ceil_div(a.k, 128) * 32);
-    else go(norm_k<DT, WDT, 1, 32, false, false, false>, ceil_div(a.k, 1024) * 32);
+    else if (form == SHIFTED && by_warp <= 16 * MOST) by_warp <= 4 ? go(norm_k<DT, WDT, V, 1, false, false, true, 512>, by_warp * 32) : go(norm_k<DT, WDT, V, MOST, false, false, true, 512>, ceil_div(by_warp, MOST) * 32);
+    else if (a.k <= 2048) go(norm_k<DT, WDT, 1, 4, false, false, false, 512>, ceil_div(a.k, 128) * 32);
+    else go(norm_k<DT, WDT, 1, 32, false, false, false, 512>, ceil_div(a.k, 1024) * 32);
     return launch_status();
 }
 
 struct NormGradArgs {
     const void * h, * w, * dy, * ds;
     long long ldh, ldy, lds, ldx;
-    float eps;
+    float eps, inv_k;
     int n, k, stages;
     void * dx;
     float * parts;                     // [blocks][k]: each block's sums for the weight's gradient (null: not wanted)
@@ -352,7 +424,7 @@ __device__ __forceinline__ void copy16(void * shared, const void * global) {
 // V = 1: one row after the other. SHIFT: the grid is a multiple of V, so that all rows of a block have the same phase and a thread its columns
 // WARP (short rows): a warp a row, eight rows a block at a time and no barrier; the warps' sums for the weight's gradient meet at the end
 template <int DT, int WDT, int V, int P, bool SHIFT, bool WARP>
-__global__ void __launch_bounds__(WARP ? 256 : 512) norm_grad_k(const NormGradArgs p) {
+__global__ void __launch_bounds__(WARP ? 256 : 512, (WARP ? 2 : 1) * (P <= 2 ? 2 : 1)) norm_grad_k(const NormGradArgs p) {
     extern __shared__ __align__(16) uint4 ahead[];                     // [stages][h, dy, ds][P][threads]
     __shared__ float2 red[2][32], red_again[2][32];
     grid_release();
@@ -439,7 +511,7 @@ __global__ void __launch_bounds__(WARP ? 256 : 512) norm_grad_k(const NormGradAr
             v = over_row<WARP>(sums(), make_float2(0.f, 0.f), red_again[turn], Add2());
         }
         // in the unit: rho h as it is, rho the unit times as large
-        const float m = v.x / float(p.k) + p.eps * unit * unit, rho = 1.f / sqrtf(m), t = v.y / float(p.k) / m, out = rho * unit;
+        const float m = fmaf(v.x, p.inv_k, p.eps * unit * unit), rho = inverse_root(m), t = v.y * p.inv_k * rho * rho, out = rho * unit;
 #pragma unroll
         for (int i = 0; i < P; ++i) {
             const int j = grid.first(i * nt + tid);
@@ -491,7 +563,7 @@ __global__ void __launch_bounds__(WARP ? 256 : 512) norm_grad_k(const NormGradAr
     }
 }
 
-// dw[j] = (accumulate: +) the sum over the blocks' parts, in a fixed order: 32 columns a block, a warp takes every 32nd part (eight warps: 8 us of 58 for 8192 x 4096, 32: XX)
+// dw[j] = (accumulate: +) the sum over the blocks' parts, in a fixed order: 32 columns a block, a warp takes every 32nd part (with eight warps 8192 x 4096 take a microsecond more, 30000 x 256 four)
 __global__ void __launch_bounds__(1024) norm_weight_grad_k(const float * parts, int blocks, int k, float * dw, int accumulate) {
     __shared__ float part[32][33];
     grid_release();
@@ -569,7 +641,7 @@ extern "C" B2MOE_API int32_t b2moe_rms_norm(const void * x, int32_t dtype, int64
     if (!aligned_to(x, e) || !aligned_to(residual, e) || !aligned_to(sum, e) || !aligned_to(y, e) || !aligned_to(weight, dtype_bytes(weight_dtype)) || !aligned16(q) || !aligned_to(scale, 4)) return B2MOE_ERR_ALIGN;
     const Form form = form_of(k, dtype, weight, {{x, ldx}, {residual, ldr}, {sum, lds}, {y, ldy}});
     if (q && form != WHOLE) return B2MOE_ERR_ALIGN;                            // rows in 8 bits come from rows in pieces of 16 bytes
-    const NormArgs a{x, residual, weight, ldx, ldr, lds, ldy, ldq, eps, n, k, sum, y, q, scale};
+    const NormArgs a{x, residual, weight, ldx, ldr, lds, ldy, ldq, eps, 1.f / float(k), n, k, sum, y, q, scale};
     cudaStream_t s = as_stream(stream);
     if (dtype == B2MOE_F32) return launch_norm<B2MOE_F32, B2MOE_F32>(a, form, s);
     if (dtype == B2MOE_F16) return weight_dtype == B2MOE_F32 ? launch_norm<B2MOE_F16, B2MOE_F32>(a, form, s) : launch_norm<B2MOE_F16, B2MOE_F16>(a, form, s);
@@ -592,7 +664,7 @@ extern "C" B2MOE_API int32_t b2moe_rms_norm_backward(const void * h, int32_t dty
         (grad_weight && !aligned16(workspace))) return B2MOE_ERR_ALIGN;
     if (grad_weight && workspace_bytes < b2moe_rms_norm_backward_workspace_bytes(n, k)) return B2MOE_ERR_WORKSPACE;
     const Form form = form_of(k, dtype, weight, {{h, ldh}, {grad_y, ldgy}, {grad_sum, ldgs}, {grad_x, ldgx}});
-    const NormGradArgs a{h, weight, grad_y, grad_sum, ldh, ldgy, ldgs, ldgx, eps, n, k, 1, grad_x, grad_weight ? static_cast<float *>(workspace) : nullptr};
+    const NormGradArgs a{h, weight, grad_y, grad_sum, ldh, ldgy, ldgs, ldgx, eps, 1.f / float(k), n, k, 1, grad_x, grad_weight ? static_cast<float *>(workspace) : nullptr};
     cudaStream_t s = as_stream(stream);
     int32_t rc, blocks = 0;
     if (dtype == B2MOE_F32) rc = launch_norm_grad<B2MOE_F32, B2MOE_F32>(a, form, s, blocks);
