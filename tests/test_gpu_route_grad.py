@@ -176,4 +176,5 @@ def test_router_tuning_step():
     total = (want * d.double()).sum() + coef * e / (k * n) * (counts * p.mean(0)).sum()
     gl, gxx = torch.autograd.grad(total, (lx, xx))
     # sums of 64 products in 32 bits, of sizes around 8: 1e-4 is 200 u of the largest terms of a sum of this length
+    want = want.detach()
     assert float((out.cpu().double() - want).abs().max()) < 1e-4 and float((grad.cpu().double() - gl).abs().max()) < 1e-4 and float((gx.cpu().double() - gxx).abs().max()) < 1e-4

@@ -19,7 +19,7 @@ struct RouteGradArgs {
     const float * w, * g, * sw, * gs;            // weights and their gradients, the shared expert's (null: none)
     float * out;
     long long ld, ldg;
-    int experts, topk, n, sigmoid, norm, add;
+    int experts, topk, n, sigmoid, norm, add, together;
     float scale;
 };
 
@@ -28,11 +28,21 @@ __global__ void __launch_bounds__(32 * GRAD_WARPS) route_grad_k(const RouteGradA
     grid_release();
     grid_wait();
     const int t = blockIdx.x * GRAD_WARPS + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    // rows one behind the other: the block's four begin on 16 bytes and are zeroed together
+    if (p.together) {
+        float * const rows = p.out + size_t(blockIdx.x) * GRAD_WARPS * p.ldg;
+        const int count = int(min((long long)GRAD_WARPS, (long long)p.n - (long long)blockIdx.x * GRAD_WARPS) * p.ldg);
+        for (int c = 4 * threadIdx.x; c < count; c += 4 * 32 * GRAD_WARPS) {
+            if (c + 4 <= count) *reinterpret_cast<float4 *>(rows + c) = make_float4(0.f, 0.f, 0.f, 0.f);
+            else for (int l = c; l < count; ++l) rows[l] = 0.f;
+        }
+        __syncthreads();
+    }
     if (t >= p.n) return;
     const int * ids = p.ids + size_t(t) * p.topk;
     const float * w = p.w + size_t(t) * p.topk, * g = p.g + size_t(t) * p.topk, * logits = p.logits + size_t(t) * p.ld;
     float * out = p.out + size_t(t) * p.ldg;
-    if (!p.add)
+    if (!p.add && !p.together)
         for (int c = lane; c < p.experts; c += 32) out[c] = 0.f;
     // sigmoid: is the selected ones' sum above the clamp
     bool coupled = p.norm;
@@ -99,7 +109,7 @@ extern "C" B2MOE_API int32_t b2moe_route_backward(int32_t gating, const float * 
                            static_cast<const void *>(shared_weights), static_cast<const void *>(grad_shared), static_cast<const void *>(grad_logits)})
         if (!aligned_to(p, 4)) return B2MOE_ERR_ALIGN;
     const RouteGradArgs a{logits, ids, weights, grad_weights, shared_weights, grad_shared, grad_logits, ld, ldg, experts, topk, n, gating == B2MOE_SIGMOID, gating == B2MOE_SOFTMAX || norm, accumulate,
-                          scale == 0.f ? 1.f : scale};
+                          !accumulate && ldg == experts + (grad_shared ? 1 : 0) && aligned16(grad_logits), scale == 0.f ? 1.f : scale};
     launch_overlapped(route_grad_k, dim3(ceil_div(n, GRAD_WARPS)), dim3(32 * GRAD_WARPS), 0, as_stream(stream), a);
     return launch_status();
 }

@@ -50,45 +50,82 @@ __device__ __forceinline__ int find_slot(const ThereArgs & p, int a, int e) {
     return -1;
 }
 
-constexpr int THERE_LIST = 32;                   // slots of a token that are looked for before they are written
-template <int P>
+// A warp takes an assignment: its token's row, of which the first pieces are on their way while the slot is looked for, to its slot. (The other warps of the token find the row in the L1.)
+constexpr int THERE_PIECES = 8;
 __global__ void __launch_bounds__(256) there_k(const ThereArgs p) {
-    __shared__ int list[THERE_LIST];
     grid_release();
     grid_wait();
-    const int t = blockIdx.x, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, lane = threadIdx.x & 31, A = p.n * p.topk;
-    const int step = gridDim.y * blockDim.x * P, all = p.topk + (p.shared ? 1 : 0);
+    const int i = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31, A = p.n * p.topk;
+    const bool shared = i >= A;
+    if (i >= A + (p.shared ? p.n : 0)) return;
+    const int t = shared ? i - A : i / p.topk, e = shared ? p.experts : p.ids[i];
     const uint4 * x = p.x + size_t(t) * p.ldx;
-    for (int j0 = blockIdx.y * blockDim.x * P; j0 < p.pieces; j0 += step) {
+    uint4 v[THERE_PIECES];
+    auto load = [&](int j0) {
+#pragma unroll
+        for (int c = 0; c < THERE_PIECES; ++c)
+            if (j0 + 32 * c + lane < p.pieces) v[c] = x[j0 + 32 * c + lane];
+    };
+    load(0);
+    const int slot = shared || e < p.experts ? find_slot(p, i, e) : -1;
+    if (p.slots && lane == 0) p.slots[i] = slot;
+    if (slot < 0) return;
+    uint4 * row = p.rows + size_t(slot) * p.ldr;
+    for (int j0 = 0; j0 < p.pieces; j0 += 32 * THERE_PIECES) {
+        if (j0) load(j0);
+#pragma unroll
+        for (int c = 0; c < THERE_PIECES; ++c)
+            if (j0 + 32 * c + lane < p.pieces) row[j0 + 32 * c + lane] = v[c];
+    }
+}
+
+// The slot of every assignment of the plan, for launches of many tokens. Words of assignments that the plan does not hold stay as they are: whoever reads one looks whether the plan leads back
+__global__ void __launch_bounds__(256) slots_k(const ThereArgs p) {
+    grid_release();
+    grid_wait();
+    const int i = blockIdx.x * 256 + threadIdx.x, e1 = p.experts + 1, A = p.n * p.topk;
+    if (i >= min(p.plan[PLAN_NGROUPED], A + p.shared)) return;
+    const int a = p.plan[PLAN_HDR + 3 * e1 + 1 + i];
+    if (unsigned(a) < unsigned(A + (p.shared ? p.n : 0))) p.slots[a] = i;
+}
+// A warp (short rows) or a block takes a token: its row is read once, P pieces a thread at a time, and written to all its slots
+template <int P, bool WARP>
+__global__ void __launch_bounds__(256) there_token_k(const ThereArgs p) {
+    __shared__ int list[32];
+    grid_release();
+    grid_wait();
+    const int lane = threadIdx.x & 31, nt = WARP ? 32 : blockDim.x, tid = WARP ? lane : threadIdx.x, t = WARP ? blockIdx.x * 8 + (threadIdx.x >> 5) : blockIdx.x;
+    if (t >= p.n) return;
+    const int A = p.n * p.topk, e1 = p.experts + 1, all = p.topk + (p.shared ? 1 : 0), * perm = p.plan + PLAN_HDR + 3 * e1 + 1, total = min(p.plan[PLAN_NGROUPED], A + p.shared);
+    const uint4 * x = p.x + size_t(t) * p.ldx;
+    for (int first = 0; first < p.pieces; first += P * nt) {
+        const int j0 = first + tid;
         uint4 v[P];
 #pragma unroll
-        for (int i = 0; i < P; ++i) {
-            const int j = j0 + i * blockDim.x + threadIdx.x;
-            if (j < p.pieces) v[i] = x[j];
-        }
-        for (int s0 = 0; s0 < all; s0 += THERE_LIST) {
-            const bool again = j0 == int(blockIdx.y * blockDim.x * P) || all > THERE_LIST;      // the list of a token with few slots stays from its first pieces on
-            if (again) {
-                __syncthreads();
-                for (int s = s0 + warp; s < min(all, s0 + THERE_LIST); s += warps) {
-                    const bool shared = s == p.topk;
-                    const int a = shared ? A + t : t * p.topk + s, e = shared ? p.experts : p.ids[a], slot = shared || e < p.experts ? find_slot(p, a, e) : -1;
-                    if (lane == 0) {
-                        list[s - s0] = slot;
-                        if (p.slots && j0 == 0) p.slots[a] = slot;
-                    }
+        for (int c = 0; c < P; ++c)
+            if (j0 + nt * c < p.pieces) v[c] = x[j0 + nt * c];
+        for (int s0 = 0; s0 < all; s0 += 32) {
+            int slot = -1;
+            if (s0 + lane < all && tid < 32) {
+                const int a = s0 + lane < p.topk ? t * p.topk + s0 + lane : A + t;
+                slot = p.slots[a];
+                if (unsigned(slot) >= unsigned(total) || perm[slot] != a) {
+                    slot = -1;
+                    p.slots[a] = -1;
                 }
+            }
+            if (!WARP) {
+                if (first + s0) __syncthreads();                       // the slots before have been read
+                if (tid < 32) list[lane] = slot;
                 __syncthreads();
             }
-            for (int s = s0; s < min(all, s0 + THERE_LIST); ++s) {
-                const int slot = list[s - s0];
-                if (slot < 0) continue;
-                uint4 * row = p.rows + size_t(slot) * p.ldr;
+            for (int s = 0; s < min(32, all - s0); ++s) {
+                const int at = WARP ? __shfl_sync(0xffffffffu, slot, s) : list[s];
+                if (at < 0) continue;
+                uint4 * row = p.rows + size_t(at) * p.ldr;
 #pragma unroll
-                for (int i = 0; i < P; ++i) {
-                    const int j = j0 + i * blockDim.x + threadIdx.x;
-                    if (j < p.pieces) row[j] = v[i];
-                }
+                for (int c = 0; c < P; ++c)
+                    if (j0 + nt * c < p.pieces) row[j0 + nt * c] = v[c];
             }
         }
     }
@@ -140,9 +177,11 @@ struct BackArgs {
     int pieces, n, topk, shared, rows;           // shared: the slots of the always-on expert follow the routed ones; rows: of y, nothing is read behind them
 };
 
-constexpr int BACK_SLOTS = 5;                    // slots whose rows are asked for at once
-template <int DT>
-__global__ void __launch_bounds__(256) back_k(const BackArgs p) {
+// S: slots whose rows are asked for at once, with the registers that let eight blocks or five of an SM run. us with 5 slots (five blocks) / 3 (eight) / 2 (eight):
+//   4096 tokens of 2048 from ten slots 34.3 / 50.3 / 37.7, 4093 of 4096 from nine 63.8 / 87.1 / 65.5, 8192 of 4096 from two 57.2 / 56.7 / 45.0
+// A thread takes a piece of a token, and the blocks of a token lie next to one another. (A warp that goes over a token's pieces with the slots in its lanes takes 58 us where this takes 33: 4096 tokens of 2048 from ten slots.)
+template <int DT, int S>
+__global__ void __launch_bounds__(256, S <= 2 ? 8 : 5) back_k(const BackArgs p) {
     constexpr int N = Vec<DT>::N;
     grid_release();
     grid_wait();
@@ -154,24 +193,25 @@ __global__ void __launch_bounds__(256) back_k(const BackArgs p) {
 #pragma unroll
         for (int l = 0; l < N; ++l) acc[l] = 0.f;
     const int all = p.topk + (p.shared ? 1 : 0);
-    for (int s0 = 0; s0 < all; s0 += BACK_SLOTS) {
-        uint4 v[BACK_SLOTS];
-        float w[BACK_SLOTS];
-        bool live[BACK_SLOTS];
+    for (int s0 = 0; s0 < all; s0 += S) {
+        uint4 v[S];
+        float w[S];
+        int slot[S];
 #pragma unroll
-        for (int i = 0; i < BACK_SLOTS; ++i) {
+        for (int i = 0; i < S; ++i) {
             const int s = s0 + i;
-            live[i] = false;
+            slot[i] = -1;
             if (s >= all) continue;
             const size_t a = s < p.topk ? size_t(t) * p.topk + s : size_t(p.n) * p.topk + t;
-            const int slot = p.slots[a];
-            live[i] = unsigned(slot) < unsigned(p.rows);
+            slot[i] = p.slots[a];
             w[i] = s < p.topk ? (p.w ? p.w[a] : 1.f) : p.sw ? p.sw[t] : 1.f;
-            if (live[i]) v[i] = p.y[size_t(slot) * p.ldy + j];
         }
 #pragma unroll
-        for (int i = 0; i < BACK_SLOTS; ++i)
-            if (live[i]) {
+        for (int i = 0; i < S; ++i)
+            if (unsigned(slot[i]) < unsigned(p.rows)) v[i] = p.y[size_t(slot[i]) * p.ldy + j];
+#pragma unroll
+        for (int i = 0; i < S; ++i)
+            if (unsigned(slot[i]) < unsigned(p.rows)) {
                 Vec<DT>::open(v[i], f);
 #pragma unroll
                 for (int l = 0; l < N; ++l) acc[l] = fmaf(w[i], f[l], acc[l]);
@@ -190,51 +230,82 @@ struct BackGradArgs {
     int pieces, n, topk, shared, rows;
 };
 
-// a block takes an assignment: its part of the token's gradient, its row, and the product of the two
-template <int DT>
+// A warp takes W assignments at a time (more of short rows), or (W = 0, launches of few assignments) a block takes one: the token's gradient, the row, and the product of the two
+template <int DT, int W>
 __global__ void __launch_bounds__(256) back_grad_k(const BackGradArgs p) {
-    constexpr int N = Vec<DT>::N;
+    constexpr int N = Vec<DT>::N, M = W ? W : 1, P = 4 / M;            // pieces of an assignment in flight
     __shared__ float red[8];
     grid_release();
     grid_wait();
-    const int all = p.topk + (p.shared ? 1 : 0), t = blockIdx.x / all, s = blockIdx.x % all;
-    const size_t a = s < p.topk ? size_t(t) * p.topk + s : size_t(p.n) * p.topk + t;
-    const int slot = p.slots[a];
-    const bool live = unsigned(slot) < unsigned(p.rows);
-    float dot = 0.f;
-    if (live) {
-        const float w = s < p.topk ? (p.w ? p.w[a] : 1.f) : p.sw ? p.sw[t] : 1.f;
-        const uint4 * d = p.dout + size_t(t) * p.ldo, * y = p.y + size_t(slot) * p.ldy;
-        uint4 * dy = p.dy + size_t(slot) * p.ldd;
-        for (int j = threadIdx.x; j < p.pieces; j += blockDim.x) {
-            float g[N], f[N];
-            Vec<DT>::open(d[j], g);
-            if (p.y) {
-                Vec<DT>::open(y[j], f);
+    const int nt = W ? 32 : blockDim.x, tid = W ? threadIdx.x & 31 : threadIdx.x, i0 = W ? (blockIdx.x * 8 + (threadIdx.x >> 5)) * M : blockIdx.x;
+    const int A = p.n * p.topk, all = A + (p.shared ? p.n : 0);
+    if (i0 >= all) return;
+    int t[M], slot[M];
+    float w[M], dot[M];
 #pragma unroll
-                for (int l = 0; l < N; ++l) dot = fmaf(g[l], f[l], dot);
-            }
-            if (p.dy) {
+    for (int m = 0; m < M; ++m) {
+        const int i = i0 + m;
+        t[m] = i < A ? i / p.topk : i - A;
+        slot[m] = i < all ? p.slots[i] : -1;
+        w[m] = i >= all ? 0.f : i >= A ? (p.sw ? p.sw[t[m]] : 1.f) : p.w ? p.w[i] : 1.f;
+        dot[m] = 0.f;
+    }
+    for (int j0 = tid; j0 < p.pieces; j0 += P * nt) {
+        uint4 g[M][P], v[M][P];
 #pragma unroll
-                for (int l = 0; l < N; ++l) g[l] *= w;
-                dy[j] = Vec<DT>::close(g);
-            }
+        for (int m = 0; m < M; ++m)
+#pragma unroll
+            for (int c = 0; c < P; ++c)
+                if (unsigned(slot[m]) < unsigned(p.rows) && j0 + c * nt < p.pieces) {
+                    if (p.y) v[m][c] = p.y[size_t(slot[m]) * p.ldy + j0 + c * nt];
+                    g[m][c] = p.dout[size_t(t[m]) * p.ldo + j0 + c * nt];
+                }
+#pragma unroll
+        for (int m = 0; m < M; ++m)
+#pragma unroll
+            for (int c = 0; c < P; ++c)
+                if (unsigned(slot[m]) < unsigned(p.rows) && j0 + c * nt < p.pieces) {
+                    float a[N], f[N];
+                    Vec<DT>::open(g[m][c], a);
+                    if (p.y) {
+                        Vec<DT>::open(v[m][c], f);
+#pragma unroll
+                        for (int l = 0; l < N; ++l) dot[m] = fmaf(a[l], f[l], dot[m]);
+                    }
+                    if (p.dy) {
+#pragma unroll
+                        for (int l = 0; l < N; ++l) a[l] *= w[m];
+                        p.dy[size_t(slot[m]) * p.ldd + j0 + c * nt] = Vec<DT>::close(a);
+                    }
+                }
+    }
+    if (!p.dw && !p.dsw) return;
+#pragma unroll
+    for (int m = 0; m < M; ++m)
+#pragma unroll
+        for (int d = 16; d; d >>= 1) dot[m] += __shfl_xor_sync(0xffffffffu, dot[m], d);
+    if (!W) {
+        if ((tid & 31) == 0) red[tid >> 5] = dot[0];
+        __syncthreads();
+        for (int u = 1; u < int(blockDim.x >> 5) && tid == 0; ++u) dot[0] += red[u];
+    }
+    if (tid) return;
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+        const int i = i0 + m;
+        if (i < A) {
+            if (p.dw) p.dw[i] = dot[m];
+        } else if (i < all && p.dsw) {
+            p.dsw[t[m]] = dot[m];
         }
     }
-    float * out = s < p.topk ? (p.dw ? p.dw + a : nullptr) : p.dsw ? p.dsw + t : nullptr;
-    if (!out) return;
-#pragma unroll
-    for (int d = 16; d; d >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, d);
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = dot;
-    __syncthreads();
-    if (threadIdx.x) return;
-    for (int w = 1; w < int(blockDim.x >> 5); ++w) dot += red[w];
-    *out = dot;
 }
 
 // what the calls have in common; pieces of 16 bytes
+// n * (topk + 1) stays inside 32 bits: topk >= 1 and n topk < 2^30
 bool batch(int n, int topk, int hidden, int dtype) { return n > 0 && topk > 0 && (long long)n * topk <= MAX_ASSIGNMENTS && hidden > 0 && valid_dtype(dtype) && hidden % (16 / int(dtype_bytes(dtype))) == 0; }
 bool stride(const void * p, long long ld, int hidden, int dtype) { return !p || (ld >= hidden && ld % (16 / (long long)dtype_bytes(dtype)) == 0); }
+constexpr int MANY_TOKENS = 148 * 8, GRAD_MANY = 148 * 16;
 int threads_for(int pieces) { return std::min(256, ceil_div(pieces, 32) * 32); }
 
 }  // namespace
@@ -247,9 +318,18 @@ extern "C" B2MOE_API int32_t b2moe_dispatch_rows(const void * x, int32_t dtype, 
     if (!batch(n, topk, hidden, dtype) || experts <= 0 || shared_tokens < 0 || shared_tokens > n || !stride(x, ldx, hidden, dtype) || !stride(rows, ldr, hidden, dtype)) return B2MOE_ERR_SHAPE;
     if (!x || !ids || !plan || !rows) return B2MOE_ERR_NULL;
     if (!aligned16(x) || !aligned16(rows) || !aligned_to(ids, 4) || !aligned_to(plan, 4) || !aligned_to(slots, 4)) return B2MOE_ERR_ALIGN;
-    const int per = 16 / int(dtype_bytes(dtype)), pieces = hidden / per, threads = threads_for(pieces);
+    const int per = 16 / int(dtype_bytes(dtype)), pieces = hidden / per;
     const ThereArgs a{static_cast<const uint4 *>(x), static_cast<uint4 *>(rows), ids, plan, slots, ldx / per, ldr / per, pieces, n, topk, experts, shared_tokens};
-    launch_overlapped(there_k<2>, dim3(n), dim3(threads), 0, as_stream(stream), a);
+    const long long all = n * (long long)topk + (shared_tokens ? n : 0);
+    cudaStream_t s = as_stream(stream);
+    if (!slots || n < MANY_TOKENS) {
+        launch_overlapped(there_k, dim3(unsigned((all + 7) / 8)), dim3(256), 0, s, a);
+        return launch_status();
+    }
+    launch_overlapped(slots_k, dim3(unsigned((all + 255) / 256)), dim3(256), 0, s, a);
+    if (int32_t rc = launch_status()) return rc;
+    if (pieces <= 64) launch_overlapped(there_token_k<2, true>, dim3(ceil_div(n, 8)), dim3(256), 0, s, a);
+    else launch_overlapped(there_token_k<2, false>, dim3(n), dim3(std::min(256, ceil_div(pieces, 64) * 32)), 0, s, a);
     return launch_status();
 }
 
@@ -261,11 +341,12 @@ extern "C" B2MOE_API int32_t b2moe_combine_rows(const void * y, int32_t dtype, i
     if (!aligned16(y) || !aligned16(residual) || !aligned16(out) || !aligned_to(slots, 4) || !aligned_to(weights, 4) || !aligned_to(shared_weights, 4)) return B2MOE_ERR_ALIGN;
     const int per = 16 / int(dtype_bytes(dtype)), pieces = hidden / per, threads = threads_for(pieces);
     const BackArgs a{static_cast<const uint4 *>(y), static_cast<const uint4 *>(residual), static_cast<uint4 *>(out), slots, weights, shared_weights, ldy / per, ldr / per, ldo / per, pieces, n, topk, shared_tokens ? 1 : 0, rows};
-    const dim3 grid(n, ceil_div(pieces, threads));
     cudaStream_t s = as_stream(stream);
-    if (dtype == B2MOE_F32) launch_overlapped(back_k<B2MOE_F32>, grid, dim3(threads), 0, s, a);
-    else if (dtype == B2MOE_F16) launch_overlapped(back_k<B2MOE_F16>, grid, dim3(threads), 0, s, a);
-    else launch_overlapped(back_k<B2MOE_BF16>, grid, dim3(threads), 0, s, a);
+    const dim3 grid(n, ceil_div(pieces, threads));
+    auto go = [&](auto two, auto five) { launch_overlapped(topk + (shared_tokens ? 1 : 0) <= 2 ? two : five, grid, dim3(threads), 0, s, a); };
+    if (dtype == B2MOE_F32) go(back_k<B2MOE_F32, 2>, back_k<B2MOE_F32, 5>);
+    else if (dtype == B2MOE_F16) go(back_k<B2MOE_F16, 2>, back_k<B2MOE_F16, 5>);
+    else go(back_k<B2MOE_BF16, 2>, back_k<B2MOE_BF16, 5>);
     return launch_status();
 }
 
@@ -281,10 +362,15 @@ extern "C" B2MOE_API int32_t b2moe_combine_rows_backward(const void * grad_out, 
     const bool dots = grad_weights || grad_shared;
     const BackGradArgs a{static_cast<const uint4 *>(grad_out), dots ? static_cast<const uint4 *>(y) : nullptr, static_cast<uint4 *>(grad_y), slots, weights, shared_weights, grad_weights, grad_shared,
                          ldgo / per, ldy / per, ldgy / per, pieces, n, topk, shared_tokens ? 1 : 0, rows};
-    const dim3 grid(unsigned(n) * unsigned(topk + (shared_tokens ? 1 : 0)));
+    const long long all = (long long)n * topk + (shared_tokens ? n : 0);
     cudaStream_t s = as_stream(stream);
-    if (dtype == B2MOE_F32) launch_overlapped(back_grad_k<B2MOE_F32>, grid, dim3(threads), 0, s, a);
-    else if (dtype == B2MOE_F16) launch_overlapped(back_grad_k<B2MOE_F16>, grid, dim3(threads), 0, s, a);
-    else launch_overlapped(back_grad_k<B2MOE_BF16>, grid, dim3(threads), 0, s, a);
+    auto go = [&](auto block, auto one, auto two, auto four) {
+        if (all < GRAD_MANY) return launch_overlapped(block, dim3(unsigned(all)), dim3(threads), 0, s, a);
+        const int each = pieces > 64 ? 1 : pieces > 32 ? 2 : 4;
+        launch_overlapped(each == 1 ? one : each == 2 ? two : four, dim3(unsigned((all + 8 * each - 1) / (8 * each))), dim3(256), 0, s, a);
+    };
+    if (dtype == B2MOE_F32) go(back_grad_k<B2MOE_F32, 0>, back_grad_k<B2MOE_F32, 1>, back_grad_k<B2MOE_F32, 2>, back_grad_k<B2MOE_F32, 4>);
+    else if (dtype == B2MOE_F16) go(back_grad_k<B2MOE_F16, 0>, back_grad_k<B2MOE_F16, 1>, back_grad_k<B2MOE_F16, 2>, back_grad_k<B2MOE_F16, 4>);
+    else go(back_grad_k<B2MOE_BF16, 0>, back_grad_k<B2MOE_BF16, 1>, back_grad_k<B2MOE_BF16, 2>, back_grad_k<B2MOE_BF16, 4>);
     return launch_status();
 }
