@@ -208,7 +208,7 @@ class Norm(NamedTuple):
 
 def _rows_of(t, n, k, dtype, what):
     """row stride of a matrix [n, k] of this type with neighbouring values, or a refusal"""
-    if t.dtype is not dtype or t.dim() != 2 or t.shape[0] != n or t.shape[1] != k:
+    if t.dtype is not dtype or t.shape != (n, k):
         raise capi.B2moeError(capi.ERR_SHAPE, f"{what}: rows of one type and size are wanted")
     ld, one = t.stride()
     if one != 1 and k > 1:
@@ -220,7 +220,7 @@ def _norm_args(x, weight, what):
     if x.dim() != 2 or x.dtype not in _DT:
         raise capi.B2moeError(capi.ERR_SHAPE, f"{what}: rows [n, k] in float32, float16 or bfloat16 are wanted")
     n, k = x.shape
-    if max(n, k) > _INT:
+    if n > _INT or k > _INT:
         raise capi.B2moeError(capi.ERR_SHAPE, f"{what}: rows and columns are 32-bit numbers")
     if weight.dtype not in (torch.float32, x.dtype) or weight.shape != (k,) or not weight.is_contiguous():
         raise capi.B2moeError(capi.ERR_SHAPE, f"{what}: a contiguous weight for each column, in float32 or the rows' type, is wanted")
@@ -245,14 +245,13 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float, residual: torch.
             raise capi.B2moeError(capi.ERR_SHAPE, "rms_norm: an output is given for rows that are not wanted")
         ldy = _rows_of(out, n, k, dtype, "rms_norm")
     stream = _stream_of(x, weight, residual, out, sum_out)
-    new = torch.empty
+    new, q, scale = x.new_empty, None, None
     if residual is not None and sum_out is None:
-        sum_out = new((n, k), dtype=dtype, device=x.device)
+        sum_out = new((n, k))
     if rows and out is None:
-        out = new((n, k), dtype=dtype, device=x.device)
-    q = scale = None
+        out = new((n, k))
     if quantize:
-        q, scale = new((n, k), dtype=torch.int8, device=x.device), new(n, dtype=torch.float32, device=x.device)
+        q, scale = new((n, k), dtype=torch.int8), new(n, dtype=torch.float32)
     check(lib.b2moe_rms_norm(x.data_ptr(), _DT[dtype], ldx, _ptr(residual), ldr, weight.data_ptr(), _DT[weight.dtype], eps, n, k, _ptr(sum_out), lds, _ptr(out), ldy,
                              _ptr(q), k, _ptr(scale), stream), "b2moe_rms_norm")
     return Norm(out, sum_out, q, scale)
@@ -273,12 +272,12 @@ def rms_norm_backward(h: torch.Tensor, weight: torch.Tensor, grad_y: torch.Tenso
     stream = _stream_of(h, weight, grad_y, grad_sum, out, grad_weight)
     add, ws, size = grad_weight is not None, None, 0
     if out is None:
-        out = torch.empty((n, k), dtype=h.dtype, device=h.device)
+        out = h.new_empty((n, k))
     if weight_grad:
         size = lib.b2moe_rms_norm_backward_workspace_bytes(n, k)
-        ws = torch.empty(max(4, size // 4), dtype=torch.float32, device=h.device)
+        ws = h.new_empty(max(16, size), dtype=torch.uint8)
         if not add:
-            grad_weight = torch.empty(k, dtype=torch.float32, device=h.device)
+            grad_weight = h.new_empty(k, dtype=torch.float32)
     check(lib.b2moe_rms_norm_backward(h.data_ptr(), _DT[h.dtype], ldh, weight.data_ptr(), _DT[weight.dtype], grad_y.data_ptr(), ldgy, _ptr(grad_sum), ldgs, eps, n, k, out.data_ptr(),
                                       ldgx, _ptr(grad_weight), int(add), _ptr(ws), size, stream), "b2moe_rms_norm_backward")
     return out, grad_weight
@@ -314,7 +313,7 @@ def route_backward(logits, ids, weights, grad_weights, experts, gating=capi.SOFT
         raise capi.B2moeError(capi.ERR_SHAPE, "route_backward: row strides are 32-bit numbers")
     stream = _stream_of(ids, weights, grad_weights, logits, shared_weights, grad_shared, out)
     if not add:
-        out = torch.empty((n, cols), dtype=torch.float32, device=ids.device)
+        out = weights.new_empty((n, cols))
     check(lib.b2moe_route_backward(gating, _ptr(logits), ld, ids.data_ptr(), weights.data_ptr(), grad_weights.data_ptr(), _ptr(shared_weights), _ptr(grad_shared), experts, topk, int(norm), scale, n,
                                    out.data_ptr(), ldg, int(add), stream), "b2moe_route_backward")
     return out
@@ -401,8 +400,8 @@ def dispatch_rows(x: torch.Tensor, ids: torch.Tensor, plan: "Plan", rows: torch.
         ldr = _rows_of(rows, total, hidden, x.dtype, "dispatch_rows")
     stream = _stream_of(x, ids, plan.buf, rows)
     if rows is None:
-        rows = torch.zeros((total, hidden), dtype=x.dtype, device=x.device)
-    slots = torch.empty(n * topk + (n if shared else 0), dtype=torch.int32, device=x.device)
+        rows = x.new_zeros((total, hidden))
+    slots = ids.new_empty(n * topk + (n if shared else 0))
     check(lib.b2moe_dispatch_rows(x.data_ptr(), _DT[x.dtype], ldx, ids.data_ptr(), plan.buf.data_ptr(), n, topk, hidden, plan.experts, shared, rows.data_ptr(), ldr, slots.data_ptr(), stream),
           "b2moe_dispatch_rows")
     return rows, slots
@@ -435,7 +434,7 @@ def combine_rows(y: torch.Tensor, slots: torch.Tensor, weights: torch.Tensor | N
         ldo = _rows_of(out, n, hidden, dtype, "combine_rows")
     stream = _stream_of(y, slots, weights, shared_weights, residual, out)
     if out is None:
-        out = torch.empty((n, hidden), dtype=dtype, device=y.device)
+        out = y.new_empty((n, hidden))
     check(lib.b2moe_combine_rows(y.data_ptr(), _DT[dtype], ldy, total, slots.data_ptr(), _ptr(weights), _ptr(shared_weights), _ptr(residual), ldr, n, topk, hidden, shared, out.data_ptr(), ldo, stream),
           "b2moe_combine_rows")
     return out
@@ -457,9 +456,9 @@ def combine_rows_backward(grad_out: torch.Tensor, y: torch.Tensor, slots: torch.
         ldgy = _rows_of(grad_y, total, hidden, dtype, "combine_rows_backward")
     stream = _stream_of(grad_out, y, slots, weights, shared_weights, grad_y)
     if grad_y is None:
-        grad_y = torch.zeros((total, hidden), dtype=dtype, device=y.device)
-    grad_weights = torch.empty((n, topk), dtype=torch.float32, device=y.device)
-    grad_shared = torch.empty(n, dtype=torch.float32, device=y.device) if shared else None
+        grad_y = y.new_zeros((total, hidden))
+    grad_weights = y.new_empty((n, topk), dtype=torch.float32)
+    grad_shared = y.new_empty(n, dtype=torch.float32) if shared else None
     check(lib.b2moe_combine_rows_backward(grad_out.data_ptr(), _DT[dtype], ldgo, y.data_ptr(), ldy, total, slots.data_ptr(), _ptr(weights), _ptr(shared_weights), n, topk, hidden, shared,
                                           grad_y.data_ptr(), ldgy, grad_weights.data_ptr(), _ptr(grad_shared), stream), "b2moe_combine_rows_backward")
     return grad_y, grad_weights, grad_shared
