@@ -201,7 +201,7 @@ def test_gradient(n, k, dtype, wdtype, skip):
 
 
 @pytest.mark.parametrize("dtype", (BF16, F16, F32))
-@pytest.mark.parametrize("k,ld,begin", ((33, 48, 3), (101, 101, 5), (101, 108, 5), (1031, 1040, 1), (2050, 2051, 7), (5000, 5002, 2), (8193, 8193, 1), (16370, 16371, 6), (64, 72, 4), (64, 64, 1), (4096, 4099, 0)))
+@pytest.mark.parametrize("k,ld,begin", ((1, 1, 0), (1, 1, 3), (2, 3, 1), (5, 5, 7), (33, 48, 3), (101, 101, 5), (101, 108, 5), (1031, 1040, 1), (2050, 2051, 7), (5000, 5002, 2), (8193, 8193, 1), (16370, 16371, 6), (64, 72, 4), (64, 64, 1), (4096, 4099, 0)))
 def test_rows_that_begin_anywhere(dtype, k, ld, begin):
     """rows that begin behind 16 bytes, in all matrices alike or in one otherwise; nothing beside them is touched"""
     from tqllm_b200 import moe
@@ -314,3 +314,24 @@ def test_captured():
         for _, (out, (grad, weight)) in graphs:
             check_norm(a, b, w, out, BF16)
             check_gradient(out.sum.cpu(), w, gs.cpu(), gs.cpu(), grad, weight, BF16)
+
+
+def test_zero_rows_without_eps():
+    """0 / sqrt(0) is not a number; the 8-bit row of zeros has scale 0 all the same"""
+    from tqllm_b200 import moe
+    x = torch.zeros(2, 64)
+    x[1] = 1.0
+    out = moe.rms_norm(x.cuda(), torch.ones(64).cuda(), 0.0, quantize=True)
+    assert out.y[0].isnan().all() and not out.q[0].any() and out.scale[0] == 0
+    assert bool((out.y[1] == 1).all()) and bool((out.q[1] == 127).all())
+
+
+def test_long_batches():
+    """more rows than a launch has blocks, in every form of the gradient"""
+    from tqllm_b200 import moe
+    for n, k, dtype in ((30011, 64, BF16), (20000, 77, F16), (9001, 520, F32), (3001, 2056, BF16), (2003, 4099, F32)):
+        x, r, w, gen = make(n, k, dtype, F32, n)
+        g = torch.randn(n, k, generator=gen).to(dtype)
+        got, weight = moe.rms_norm_backward(x.cuda(), w.cuda(), g.cuda(), EPS, r.cuda())
+        check_gradient(x, w, g, r, got, weight, dtype)
+        check_norm(x, r, w, moe.rms_norm(x.cuda(), w.cuda(), EPS, r.cuda()), dtype)

@@ -323,7 +323,7 @@ __global__ void __launch_bounds__(MOST, MOST == 128 && V > 1 ? (Q ? 5 : 6) : WAR
     }
     if constexpr (Q) {
         const float top = all.y;
-        if (tid == 0) p.scale[row] = fine ? top * rho / 127.f : __int_as_float(0x7fc00000);
+        if (tid == 0) p.scale[row] = !fine ? __int_as_float(0x7fc00000) : top > 0.f ? top * rho / 127.f : 0.f;
         const bool tiny = top < 0x1p-100f, all_exact = fine && tiny && top > 0.f;      // products have lost bits there
         float inv;
         asm("rcp.approx.f32 %0, %1;" : "=f"(inv) : "f"(top));
@@ -445,10 +445,10 @@ __global__ void __launch_bounds__(WARP ? 256 : 512, (WARP ? 2 : 1) * (P <= 2 ? 2
 #pragma unroll
         for (int l = 0; l < V; ++l) dw[i][l] = 0.f;
     }
-    // A piece that is not whole comes with its neighbours in the matrix, which `trim` drops; only in front of the matrix and behind it there may be nothing to read
+    // A piece that is not whole comes with its neighbours in the matrix, which `trim` drops; in front of the matrix and behind it there may be nothing to read
     auto bring = [&](uint4 * to, const void * base, int row, long long ld, int j) {
         const T * at = static_cast<const T *>(base) + size_t(row) * ld;
-        if (grid.whole(j) || ((j >= 0 || row > 0) && (j + V <= p.k || row + 1 < p.n))) return copy16(to, at + j);
+        if (grid.whole(j) || (row * ld + j >= 0 && row * ld + j + V <= (p.n - 1) * ld + p.k)) return copy16(to, at + j);
         Piece<DT, V> some;
         some.zero();
         some.load_some(at, j, p.k);
@@ -591,14 +591,14 @@ int grad_blocks_most(int n, int k) { return std::min((n + 7) / 8 * 8, SMS * std:
 
 template <int DT, int WDT>
 int32_t launch_norm_grad(NormGradArgs a, Form form, cudaStream_t s, int & blocks) {
-    constexpr int V = DT == B2MOE_F32 ? 4 : 8, MOST = NORM_MAX_COLS / V / 512, SMEM = 216 * 1024;
+    constexpr int V = DT == B2MOE_F32 ? 4 : 8, MOST = NORM_MAX_COLS / V / 512;
     // per_sm blocks fill an SM's shared memory, so that a launch that becomes resident while the one before it runs spreads over all SMs (69 us instead of 49 for 8192 x 4096, with more than two of an SM)
     auto go = [&](auto kernel, bool by_row, int threads, int pieces, int per_sm) -> int32_t {
-        const size_t row = size_t(3) * pieces * threads * 16;          // of a stage
-        a.stages = int(std::min<size_t>(3, std::max<size_t>(1, SMEM / per_sm / (row ? row : SMEM))));
-        if (row && !allow_smem(kernel, SMEM)) return B2MOE_ERR_CUDA;
+        const size_t row = size_t(3) * pieces * threads * 16, room = 228 * 1024 / per_sm - 2048;      // of a stage; of a block (an SM's 228 KB, less a block's own 1 KB and its static words)
+        a.stages = int(std::min<size_t>(3, std::max<size_t>(1, row ? room / row : 1)));
+        if (row && !allow_smem(kernel, 226 * 1024)) return B2MOE_ERR_CUDA;
         blocks = by_row ? std::min(ceil_div(a.n, 8), SMS * per_sm) : std::min((a.n + 7) / 8 * 8, SMS * per_sm / 8 * 8);
-        launch_overlapped(kernel, dim3(blocks), dim3(threads), row ? std::max<size_t>(a.stages * row, SMEM / per_sm) : 0, s, a);
+        launch_overlapped(kernel, dim3(blocks), dim3(threads), row ? std::max(a.stages * row, room) : 0, s, a);
         return launch_status();
     };
     const int by_warp = ceil_div(form == SHIFTED ? a.k + V - 1 : a.k, 32 * V), per_sm = std::max(1, std::min(8, GRAD_NUM / a.k));      // a warp's pieces

@@ -96,7 +96,7 @@ __global__ void __launch_bounds__(256) there_token_k(const ThereArgs p) {
     grid_wait();
     const int lane = threadIdx.x & 31, nt = WARP ? 32 : blockDim.x, tid = WARP ? lane : threadIdx.x, t = WARP ? blockIdx.x * 8 + (threadIdx.x >> 5) : blockIdx.x;
     if (t >= p.n) return;
-    const int A = p.n * p.topk, e1 = p.experts + 1, all = p.topk + (p.shared ? 1 : 0), * perm = p.plan + PLAN_HDR + 3 * e1 + 1, total = min(p.plan[PLAN_NGROUPED], A + p.shared);
+    const int A = p.n * p.topk, e1 = p.experts + 1, all = p.topk + (p.shared ? 1 : 0), * perm = p.plan + PLAN_HDR + 3 * e1 + 1, total = max(0, min(p.plan[PLAN_NGROUPED], A + p.shared));
     const uint4 * x = p.x + size_t(t) * p.ldx;
     for (int first = 0; first < p.pieces; first += P * nt) {
         const int j0 = first + tid;
