@@ -180,13 +180,11 @@ __device__ __forceinline__ T over_row(T v, T none, T * red, F join) {
 struct Add { __device__ float operator()(float a, float b) const { return a + b; } };
 struct Add2 { __device__ float2 operator()(float2 a, float2 b) const { return make_float2(a.x + b.x, a.y + b.y); } };
 struct AddMax { __device__ float2 operator()(float2 a, float2 b) const { return make_float2(a.x + b.x, max_nan(a.y, b.y)); } };
-struct Max { __device__ double operator()(double a, double b) const { return fmax(a, b); } };
 
 // The integer nearest to 127 u / top for a product u = h w, which 64 bits hold exactly, halves to even, where it is `low` or the next: 127 |u| and (low + 1/2) top are compared through what rounding the
-// latter leaves over. off: what the top may be off by; 128 where that leaves it open
-__device__ __forceinline__ int decide(float h, float w, double low, double top, double off) {
+// latter leaves over
+__device__ __forceinline__ int decide(float h, float w, double low, double top) {
     const double u = double(h) * double(w), half = low + 0.5, p = half * top, diff = fma(127.0, fabs(u), -p) - fma(half, top, -p);
-    if (fabs(diff) < half * off) return 128;
     const int lo = int(low), q = diff > 0.0 ? lo + 1 : diff < 0.0 ? lo : lo + (lo & 1);
     return u < 0.0 ? -q : q;
 }
@@ -199,41 +197,11 @@ __device__ __forceinline__ float inverse_root(float v) {
     return v > 0x1p-126f && v < INFINITY ? fmaf(r, half, r) : r;       // 0, infinities and NaN as they come
 }
 
-constexpr float MAGIC = 12582912.f, OFF = 5.2f * 0x1p-24f;
+constexpr float MAGIC = 12582912.f, OFF = 3.2f * 0x1p-24f;
 __device__ __forceinline__ bool near_half(float u, float inv) {
     const float m = MAGIC - __fmaf_rn(u, inv, MAGIC);
     return fmaf(fabsf(m), OFF, fabsf(__fmaf_rn(u, inv, m))) > 0.5f - OFF;
 }
-template <int WDT, int V, int P> struct Held { Two h[P][(V + 1) / 2]; Piece<WDT, V> w[P]; };
-// The integers of a row's products whose quotient is close to a half once more, exactly, over those that are there. A function of its own: the registers of what is rare do not count in the kernel
-template <int WDT, int V, int P, bool WARP>
-__device__ __noinline__ void redo_close(const Held<WDT, V, P> & row, int8_t * q, int k, int nt, int tid, float mine, float top, float inv, bool close, bool all, double * red) {
-    auto value = [&](int i, int l) {
-        const float2 h = apart(row.h[i][l / 2]);
-        return make_float2(l & 1 ? h.y : h.x, row.w[i][l]);
-    };
-    // the largest product exactly: among those that round to the largest
-    double exact = 0.0;
-    if (mine == top)
-#pragma unroll 1
-        for (int i = 0; i < P; ++i)
-#pragma unroll
-            for (int l = 0; l < V; ++l) {
-                const float2 v = value(i, l);
-                if (fabsf(v.x * v.y) == top) exact = fmax(exact, fabs(double(v.x) * double(v.y)));
-            }
-    exact = over_row<WARP>(exact, 0.0, red, Max());
-    if (!close) return;
-#pragma unroll 1
-    for (int i = 0; i < P; ++i)
-#pragma unroll
-        for (int l = 0; l < V; ++l) {
-            const float2 v = value(i, l);
-            const int j = (i * nt + tid) * V + l;
-            if (j < k && (all || near_half(v.x * v.y, inv))) q[j] = int8_t(decide(v.x, v.y, floor(127.0 * fabs(double(v.x) * double(v.y)) / exact), exact, 0.0));
-        }
-}
-
 // Squares that pass the range of 32 bits: the row is taken once more in this unit, in which they do not (16384 squares of 2^48 at most), nor does what is small count there
 constexpr float UNIT = 0x1p-80f;
 
@@ -242,10 +210,12 @@ constexpr float UNIT = 0x1p-80f;
 template <int DT, int WDT, int V, int P, bool WARP, bool Q, bool SHIFT, int MOST>
 __global__ void __launch_bounds__(MOST, MOST == 128 && V > 1 ? (Q ? 5 : 6) : WARP ? 2 : 1) norm_k(const NormArgs p) {
     __shared__ float2 red[32], red_again[32];
-    __shared__ double red_exact[32];
+    __shared__ unsigned long long exact_top[WARP ? 8 : 1];
     grid_release();
     grid_wait();
     const int nt = WARP ? 32 : blockDim.x, tid = WARP ? threadIdx.x & 31 : threadIdx.x;
+    unsigned long long * const exact = exact_top + (WARP ? threadIdx.x >> 5 : 0);
+    if (Q && tid == 0) *exact = 0;
     const int row = WARP ? blockIdx.x * 8 + (threadIdx.x >> 5) : blockIdx.x;
     if (WARP && row >= p.n) return;                                    // no barrier follows in this form
     using T = typename Elem<DT>::type;
@@ -267,21 +237,32 @@ __global__ void __launch_bounds__(MOST, MOST == 128 && V > 1 ? (Q ? 5 : 6) : WAR
             if (p.r) get(r[i], p.r, size_t(row) * p.ldr, j, grid);
             get_weight(w[i], p.w, j, grid);
         }
+        if (p.r) {
 #pragma unroll
-        for (int i = 0; i < P; ++i)
+            for (int i = 0; i < P; ++i)
 #pragma unroll
-            for (int l = 0; l < H; ++l) h[i][l] = x[i].pair(l) + r[i].pair(l);
+                for (int l = 0; l < H; ++l) h[i][l] = x[i].pair(l) + r[i].pair(l);
+        } else {
+#pragma unroll
+            for (int i = 0; i < P; ++i)
+#pragma unroll
+                for (int l = 0; l < H; ++l) h[i][l] = x[i].pair(l);
+        }
     }
+    float tops[Q ? P : 1];                                             // of the pieces
     auto sums = [&]() {                                                // squares, the largest product
         Two squares = two(0.f);
         float top = 0.f;
 #pragma unroll
-        for (int i = 0; i < P; ++i)
+        for (int i = 0; i < P; ++i) {
+            if (Q) tops[i] = 0.f;
 #pragma unroll
             for (int l = 0; l < H; ++l) {
                 squares = fma2(h[i][l], h[i][l], squares);
-                if (Q) top = largest(top, h[i][l] * w[i].pair(l));
+                if (Q) tops[i] = largest(tops[i], h[i][l] * w[i].pair(l));
             }
+            if (Q) top = max_nan(top, tops[i]);
+        }
         const float2 s = apart(squares);
         return make_float2(s.x + s.y, top);
     };
@@ -324,14 +305,24 @@ __global__ void __launch_bounds__(MOST, MOST == 128 && V > 1 ? (Q ? 5 : 6) : WAR
     if constexpr (Q) {
         const float top = all.y;
         if (tid == 0) p.scale[row] = !fine ? __int_as_float(0x7fc00000) : top > 0.f ? top * rho / 127.f : 0.f;
-        const bool tiny = top < 0x1p-100f, all_exact = fine && tiny && top > 0.f;      // products have lost bits there
-        float inv;
-        asm("rcp.approx.f32 %0, %1;" : "=f"(inv) : "f"(top));
-        inv = tiny || !fine ? 0.f : inv * 127.f;
-        // (OFF) u and top are off by 2^-24 of themselves, inv by 3 times that (its reciprocal 2, the product 1), the quotient t by 5 |t| 2^-24: those that close to a half are done again, exactly. The
-        // nearest integer m comes from t + 1.5 * 2^23; |t| <= |m| + 1/2. A piece is looked at by its largest m and its largest distance from an integer (one row of 4096 in ten has such a piece), then its
-        // values in 64 bits with the top as it is, which decides all but a sixth of them; rows of the others (one in a hundred) take the exact top
-        bool close = all_exact;
+        if (WARP || blockDim.x == 32) __syncwarp();
+        // the largest product exactly, from the pieces of those that round to the largest (numbers above zero are ordered as their bits are)
+        if (mine.y == top && top > 0.f) {
+            double most = 0.0;
+#pragma unroll
+            for (int i = 0; i < P; ++i)
+                if (tops[i] == top)
+#pragma unroll
+                    for (int l = 0; l < V; ++l) {
+                        const float hl = l & 1 ? apart(h[i][l / 2]).y : apart(h[i][l / 2]).x;
+                        if (fabsf(hl * w[i][l]) == top) most = fmax(most, fabs(double(hl) * double(w[i][l])));
+                    }
+            atomicMax(exact, (unsigned long long)__double_as_longlong(most));
+        }
+        const bool tiny = top < 0x1p-100f;                             // products have lost bits there: all are taken exactly
+        const float inv = tiny || !fine ? 0.f : __fdiv_rn(127.f, top);
+        // (OFF) u, top and inv are off by 2^-24 of themselves each, the quotient t by 3 |t| 2^-24: those that close to a half are done again, exactly. The nearest integer m comes from t + 1.5 * 2^23;
+        // |t| <= |m| + 1/2. A piece is looked at by its largest m and its largest distance from an integer (one row of 4096 in fifteen has such a piece)
         uint32_t some = 0;                                             // pieces with such a value
         int8_t * const q = p.q + size_t(row) * p.ldq;
 #pragma unroll
@@ -353,31 +344,22 @@ __global__ void __launch_bounds__(MOST, MOST == 128 && V > 1 ? (Q ? 5 : 6) : WAR
             if (j >= p.k) continue;
             if constexpr (V == 8) *reinterpret_cast<uint2 *>(q + j) = make_uint2(o[0], o[1]);
             else *reinterpret_cast<uint32_t *>(q + j) = o[0];
-            if (fmaf(big, OFF, far) > 0.5f - OFF) some |= 1u << i;
+            if (tiny || fmaf(big, OFF, far) > 0.5f - OFF) some |= 1u << i;
         }
-        if (some && fine && !tiny) {
+        if (WARP || blockDim.x == 32) __syncwarp();
+        else __syncthreads();                                          // the exact top is there
+        if (!some || !fine || top == 0.f) return;
+        const double largest_product = __longlong_as_double((long long)*exact);
 #pragma unroll
-            for (int i = 0; i < P; ++i)
-                if (some >> i & 1u)
+        for (int i = 0; i < P; ++i)
+            if (some >> i & 1u)
 #pragma unroll
-                    for (int l = 0; l < V; ++l) {
-                        const float hl = l & 1 ? apart(h[i][l / 2]).y : apart(h[i][l / 2]).x;
-                        if (!near_half(hl * w[i][l], inv)) continue;
-                        const int exactly = decide(hl, w[i][l], floorf(fabsf(hl * w[i][l] * inv)), top, double(top) * 0x1.01p-24);
-                        if (exactly > 127) close = true;
-                        else q[grid.first(i * nt + tid) + l] = int8_t(exactly);
-                    }
-        }
-        close = close && fine;
-        if (!(WARP ? __any_sync(0xffffffffu, close) : __syncthreads_or(close))) return;
-        Held<WDT, V, P> held;
-#pragma unroll
-        for (int i = 0; i < P; ++i) {
-            held.w[i] = w[i];
-#pragma unroll
-            for (int l = 0; l < H; ++l) held.h[i][l] = h[i][l];
-        }
-        redo_close<WDT, V, P, WARP>(held, q, p.k, nt, tid, mine.y, top, inv, close, all_exact, red_exact);
+                for (int l = 0; l < V; ++l) {
+                    const float hl = l & 1 ? apart(h[i][l / 2]).y : apart(h[i][l / 2]).x, u = hl * w[i][l];
+                    if (!tiny && !near_half(u, inv)) continue;
+                    const double low = tiny ? floor(127.0 * fabs(double(hl) * double(w[i][l])) / largest_product) : double(floorf(fabsf(u * inv)));
+                    q[grid.first(i * nt + tid) + l] = int8_t(decide(hl, w[i][l], low, largest_product));
+                }
     }
 }
 
@@ -596,7 +578,7 @@ int32_t launch_norm_grad(NormGradArgs a, Form form, cudaStream_t s, int & blocks
     auto go = [&](auto kernel, bool by_row, int threads, int pieces, int per_sm) -> int32_t {
         const size_t row = size_t(3) * pieces * threads * 16, room = 228 * 1024 / per_sm - 2048;      // of a stage; of a block (an SM's 228 KB, less a block's own 1 KB and its static words)
         a.stages = int(std::min<size_t>(3, std::max<size_t>(1, row ? room / row : 1)));
-        if (row && !allow_smem(kernel, 226 * 1024)) return B2MOE_ERR_CUDA;
+        if (room > 48 * 1024 && !allow_smem(kernel, 226 * 1024)) return B2MOE_ERR_CUDA;
         blocks = by_row ? std::min(ceil_div(a.n, 8), SMS * per_sm) : std::min((a.n + 7) / 8 * 8, SMS * per_sm / 8 * 8);
         launch_overlapped(kernel, dim3(blocks), dim3(threads), row ? std::max(a.stages * row, room) : 0, s, a);
         return launch_status();

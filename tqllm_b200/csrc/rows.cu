@@ -50,7 +50,7 @@ __device__ __forceinline__ int find_slot(const ThereArgs & p, int a, int e) {
     return -1;
 }
 
-// A warp takes an assignment: its token's row, of which the first pieces are on their way while the slot is looked for, to its slot. (The other warps of the token find the row in the L1.)
+// A warp takes an assignment, or (grid.y) a part of its row: the row of its token, whose first pieces are on their way while the slot is looked for, to its slot. (The other warps of the token find the row in the L1.)
 constexpr int THERE_PIECES = 8;
 __global__ void __launch_bounds__(256) there_k(const ThereArgs p) {
     grid_release();
@@ -60,22 +60,23 @@ __global__ void __launch_bounds__(256) there_k(const ThereArgs p) {
     if (i >= A + (p.shared ? p.n : 0)) return;
     const int t = shared ? i - A : i / p.topk, e = shared ? p.experts : p.ids[i];
     const uint4 * x = p.x + size_t(t) * p.ldx;
+    const int share = (p.pieces + 32 * gridDim.y - 1) / (32 * gridDim.y) * 32, begin = blockIdx.y * share, end = min(p.pieces, begin + share);
     uint4 v[THERE_PIECES];
     auto load = [&](int j0) {
 #pragma unroll
         for (int c = 0; c < THERE_PIECES; ++c)
-            if (j0 + 32 * c + lane < p.pieces) v[c] = x[j0 + 32 * c + lane];
+            if (j0 + 32 * c + lane < end) v[c] = x[j0 + 32 * c + lane];
     };
-    load(0);
+    load(begin);
     const int slot = shared || e < p.experts ? find_slot(p, i, e) : -1;
-    if (p.slots && lane == 0) p.slots[i] = slot;
+    if (p.slots && lane == 0 && blockIdx.y == 0) p.slots[i] = slot;
     if (slot < 0) return;
     uint4 * row = p.rows + size_t(slot) * p.ldr;
-    for (int j0 = 0; j0 < p.pieces; j0 += 32 * THERE_PIECES) {
-        if (j0) load(j0);
+    for (int j0 = begin; j0 < end; j0 += 32 * THERE_PIECES) {
+        if (j0 > begin) load(j0);
 #pragma unroll
         for (int c = 0; c < THERE_PIECES; ++c)
-            if (j0 + 32 * c + lane < p.pieces) row[j0 + 32 * c + lane] = v[c];
+            if (j0 + 32 * c + lane < end) row[j0 + 32 * c + lane] = v[c];
     }
 }
 
@@ -177,11 +178,11 @@ struct BackArgs {
     int pieces, n, topk, shared, rows;           // shared: the slots of the always-on expert follow the routed ones; rows: of y, nothing is read behind them
 };
 
-// S: slots whose rows are asked for at once, with the registers that let eight blocks or five of an SM run. us with 5 slots (five blocks) / 3 (eight) / 2 (eight):
+// S: slots whose rows are asked for at once, with the registers that let eight blocks or five of an SM run; twelve where there is a block or two an SM (64 tokens of 2048 from eleven slots: 3.9 us with five, 2.9 with twelve). us with 5 slots (five blocks) / 3 (eight) / 2 (eight):
 //   4096 tokens of 2048 from ten slots 34.3 / 50.3 / 37.7, 4093 of 4096 from nine 63.8 / 87.1 / 65.5, 8192 of 4096 from two 57.2 / 56.7 / 45.0
 // A thread takes a piece of a token, and the blocks of a token lie next to one another. (A warp that goes over a token's pieces with the slots in its lanes takes 58 us where this takes 33: 4096 tokens of 2048 from ten slots.)
 template <int DT, int S>
-__global__ void __launch_bounds__(256, S <= 2 ? 8 : 5) back_k(const BackArgs p) {
+__global__ void __launch_bounds__(256, S <= 2 ? 8 : S <= 5 ? 5 : 2) back_k(const BackArgs p) {
     constexpr int N = Vec<DT>::N;
     grid_release();
     grid_wait();
@@ -305,7 +306,11 @@ __global__ void __launch_bounds__(256) back_grad_k(const BackGradArgs p) {
 // n * (topk + 1) stays inside 32 bits: topk >= 1 and n topk < 2^30
 bool batch(int n, int topk, int hidden, int dtype) { return n > 0 && topk > 0 && (long long)n * topk <= MAX_ASSIGNMENTS && hidden > 0 && valid_dtype(dtype) && hidden % (16 / int(dtype_bytes(dtype))) == 0; }
 bool stride(const void * p, long long ld, int hidden, int dtype) { return !p || (ld >= hidden && ld % (16 / (long long)dtype_bytes(dtype)) == 0); }
-constexpr int MANY_TOKENS = 148 * 8, GRAD_MANY = 148 * 16;
+// From how many tokens on a launch looks the slots up first; parts of rows that the launches of fewer have at most. us, there: 64 tokens of 2048 to eleven slots whole / in parts 3.1 / 2.3, 140 of 4096 to eight 5.7 / 4.1; 1000 of 2048 to four
+// in parts beyond this number 5.5 instead of 4.5
+constexpr int MANY_TOKENS = 148 * 8, THERE_WARPS = 148 * 16;
+// From how many assignments on a warp takes one in the gradient. us, block / warp: 640 of 2048 4.2 / 3.4, 2240 of 2048 8.2 / 4.6, 1120 of 4096 5.3 / 6.9, 41,000 of 2048 82 / 56
+inline int grad_many(int pieces) { return 148 * (pieces <= 256 ? 4 : 8); }
 int threads_for(int pieces) { return std::min(256, ceil_div(pieces, 32) * 32); }
 
 }  // namespace
@@ -323,7 +328,8 @@ extern "C" B2MOE_API int32_t b2moe_dispatch_rows(const void * x, int32_t dtype, 
     const long long all = n * (long long)topk + (shared_tokens ? n : 0);
     cudaStream_t s = as_stream(stream);
     if (!slots || n < MANY_TOKENS) {
-        launch_overlapped(there_k, dim3(unsigned((all + 7) / 8)), dim3(256), 0, s, a);
+        const int parts = int(std::max(1LL, std::min<long long>(ceil_div(pieces, 64), THERE_WARPS / all)));      // of a row, while that makes no more warps than run at once
+        launch_overlapped(there_k, dim3(unsigned((all + 7) / 8), parts), dim3(256), 0, s, a);
         return launch_status();
     }
     launch_overlapped(slots_k, dim3(unsigned((all + 255) / 256)), dim3(256), 0, s, a);
@@ -343,10 +349,12 @@ extern "C" B2MOE_API int32_t b2moe_combine_rows(const void * y, int32_t dtype, i
     const BackArgs a{static_cast<const uint4 *>(y), static_cast<const uint4 *>(residual), static_cast<uint4 *>(out), slots, weights, shared_weights, ldy / per, ldr / per, ldo / per, pieces, n, topk, shared_tokens ? 1 : 0, rows};
     cudaStream_t s = as_stream(stream);
     const dim3 grid(n, ceil_div(pieces, threads));
-    auto go = [&](auto two, auto five) { launch_overlapped(topk + (shared_tokens ? 1 : 0) <= 2 ? two : five, grid, dim3(threads), 0, s, a); };
-    if (dtype == B2MOE_F32) go(back_k<B2MOE_F32, 2>, back_k<B2MOE_F32, 5>);
-    else if (dtype == B2MOE_F16) go(back_k<B2MOE_F16, 2>, back_k<B2MOE_F16, 5>);
-    else go(back_k<B2MOE_BF16, 2>, back_k<B2MOE_BF16, 5>);
+    const int all = topk + (shared_tokens ? 1 : 0);
+    const bool few = (long long)n * grid.y <= 2 * 148;
+    auto go = [&](auto two, auto five, auto twelve) { launch_overlapped(all <= 2 ? two : few && all > 5 ? twelve : five, grid, dim3(threads), 0, s, a); };
+    if (dtype == B2MOE_F32) go(back_k<B2MOE_F32, 2>, back_k<B2MOE_F32, 5>, back_k<B2MOE_F32, 12>);
+    else if (dtype == B2MOE_F16) go(back_k<B2MOE_F16, 2>, back_k<B2MOE_F16, 5>, back_k<B2MOE_F16, 12>);
+    else go(back_k<B2MOE_BF16, 2>, back_k<B2MOE_BF16, 5>, back_k<B2MOE_BF16, 12>);
     return launch_status();
 }
 
@@ -365,7 +373,7 @@ extern "C" B2MOE_API int32_t b2moe_combine_rows_backward(const void * grad_out, 
     const long long all = (long long)n * topk + (shared_tokens ? n : 0);
     cudaStream_t s = as_stream(stream);
     auto go = [&](auto block, auto one, auto two, auto four) {
-        if (all < GRAD_MANY) return launch_overlapped(block, dim3(unsigned(all)), dim3(threads), 0, s, a);
+        if (all < grad_many(pieces)) return launch_overlapped(block, dim3(unsigned(all)), dim3(threads), 0, s, a);
         const int each = pieces > 64 ? 1 : pieces > 32 ? 2 : 4;
         launch_overlapped(each == 1 ? one : each == 2 ? two : four, dim3(unsigned((all + 8 * each - 1) / (8 * each))), dim3(256), 0, s, a);
     };
