@@ -545,17 +545,37 @@ __global__ void __launch_bounds__(WARP ? 256 : 512, (WARP ? 2 : 1) * (P <= 2 ? 2
     }
 }
 
-// dw[j] = (accumulate: +) the sum over the blocks' parts, in a fixed order: 32 columns a block, a warp takes every 32nd part (with eight warps 8192 x 4096 take a microsecond more, 30000 x 256 four)
+// dw[j] = (accumulate: +) the sum over the blocks' parts, in a fixed order: 32 columns a block; a warp takes one part, or (WIDE: rows of whole 16 bytes) four with 16 bytes a lane, and all parts are on their way
+// at once. (30000 x 256: 14.1 us a value a lane, 12.5 with 16 bytes; with eight warps four more)
+template <bool WIDE>
 __global__ void __launch_bounds__(1024) norm_weight_grad_k(const float * parts, int blocks, int k, float * dw, int accumulate) {
     __shared__ float part[32][33];
     grid_release();
     grid_wait();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, j = blockIdx.x * 32 + lane;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     float s = 0.f;
-    if (j < k)
+    if (WIDE) {
+        const int j = blockIdx.x * 32 + (lane & 7) * 4;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (j < k)
+#pragma unroll 5
+            for (int b = warp * 4 + (lane >> 3); b < blocks; b += 128) {
+                const float4 a = *reinterpret_cast<const float4 *>(parts + size_t(b) * k + j);
+                v.x += a.x; v.y += a.y; v.z += a.z; v.w += a.w;
+            }
+#pragma unroll
+        for (int d = 8; d <= 16; d <<= 1) {
+            v.x += __shfl_xor_sync(0xffffffffu, v.x, d); v.y += __shfl_xor_sync(0xffffffffu, v.y, d);
+            v.z += __shfl_xor_sync(0xffffffffu, v.z, d); v.w += __shfl_xor_sync(0xffffffffu, v.w, d);
+        }
+        if (lane < 8) { part[warp][4 * lane] = v.x; part[warp][4 * lane + 1] = v.y; part[warp][4 * lane + 2] = v.z; part[warp][4 * lane + 3] = v.w; }
+    } else {
+        const int j = blockIdx.x * 32 + lane;
+        if (j < k)
 #pragma unroll 10
-        for (int b = warp; b < blocks; b += 32) s += parts[size_t(b) * k + j];
-    part[warp][lane] = s;
+            for (int b = warp; b < blocks; b += 32) s += parts[size_t(b) * k + j];
+        part[warp][lane] = s;
+    }
     __syncthreads();
     // the 32 sums of a column by a warp
     s = part[lane][warp];
@@ -654,6 +674,10 @@ extern "C" B2MOE_API int32_t b2moe_rms_norm_backward(const void * h, int32_t dty
     else rc = weight_dtype == B2MOE_F32 ? launch_norm_grad<B2MOE_BF16, B2MOE_F32>(a, form, s, blocks) : launch_norm_grad<B2MOE_BF16, B2MOE_BF16>(a, form, s, blocks);
     if (rc) return rc;
     if (!grad_weight) return B2MOE_OK;
-    launch_overlapped(norm_weight_grad_k, dim3(ceil_div(k, 32)), dim3(1024), 0, s, static_cast<const float *>(workspace), blocks, k, grad_weight, accumulate);
+    // in plain stream order: as an early resident it takes the registers of the rows' last blocks (8192 x 4096: 52.4 us, 49.8 so)
+    const dim3 grid(ceil_div(k, 32)), block(1024);
+    const float * parts = static_cast<const float *>(workspace);
+    if (k % 4) norm_weight_grad_k<false><<<grid, block, 0, s>>>(parts, blocks, k, grad_weight, accumulate);
+    else norm_weight_grad_k<true><<<grid, block, 0, s>>>(parts, blocks, k, grad_weight, accumulate);
     return launch_status();
 }
