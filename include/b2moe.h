@@ -298,7 +298,7 @@ B2MOE_API int32_t b2moe_linear_i8_epilogue(const int8_t * q, int64_t ldq, const 
  *   scale = max|u| / sqrt(mean(h^2) + eps) / 127. A row of zeros has scale 0; a row with an infinity or a NaN, or a product u that
  *   passes the range of 32 bits, has a NaN as its scale. At least one of y and q is wanted.
  *   x, residual, sum and y are rows of dtype, each with its own stride in elements; weight [k] is fp32 or of dtype; eps >= 0 and finite.
- *   An output may lie on an input of the same stride (sum on residual, y on x). k <= 16384, n below 2^30. Rows of any k and natural alignment; with q, k
+ *   An output may lie on an input of the same stride (sum on residual, y on x), outputs not on one another. k <= 16384, n below 2^30. Rows of any k and natural alignment; with q, k
  *   and ldq are multiples of 16, strides whole 16 bytes, pointers 16-byte aligned. Bytes of q between k and ldq are left as they are. Rows that
  *   begin on 16 bytes and have whole 16 bytes are the fast case everywhere.
  * b2moe_rms_norm_backward: from h (x, or the sum that the norm wrote) and the gradients of y and (may be null) of the sum:
@@ -325,7 +325,7 @@ B2MOE_API int32_t b2moe_rms_norm_backward(const void * h, int32_t dtype, int64_t
  *   The gradient on x is b2moe_combine_rows of the gradient of rows, without weights.
  * b2moe_combine_rows: out[t] = (residual[t] +) sum_s weights[t][s] y[slots[t * topk + s]] + shared_weights[t] y[slots[n * topk + t]] (the latter with
  *   shared_tokens = n), in 32 bits in this order, rounded once; null weights are one; slots outside [0, rows) are left out, and so are their weights.
- *   residual and out are of y's type; residual may be out.
+ *   residual and out are of y's type; residual may be out, y may not.
  * b2moe_combine_rows_backward: grad_y[slot] = weight grad_out[t] (grad_y null: not wanted), grad_weights[t][s] = grad_out[t] . y[slot] and grad_shared[t]
  *   (null: not wanted; 0 where there is no slot). Rows of grad_y without an assignment are left as they are; it may lie on y of the same stride. */
 B2MOE_API int32_t b2moe_dispatch_rows(const void * x, int32_t dtype, int64_t ldx, const int32_t * ids, const int32_t * plan, int32_t n, int32_t topk, int32_t hidden,
