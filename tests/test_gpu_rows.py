@@ -43,7 +43,8 @@ def sorted_plain(ids, e, shared):
 
 
 CASES = [dict(n=1, h=8, e=1, k=1), dict(n=1, h=2048, e=512, k=10), dict(n=3, h=40, e=5, k=2), dict(n=64, h=2048, e=64, k=10), dict(n=33, h=264, e=7, k=7, skip=0.5), dict(n=129, h=1032, e=3, k=1),
-         dict(n=40, h=16, e=8, k=2, skip=1.0), dict(n=700, h=72, e=9, k=3, one=True), dict(n=2500, h=24, e=4, k=2, one=True), dict(n=20, h=136, e=60, k=40), dict(n=5, h=4104, e=16, k=4), dict(n=2, h=16392, e=40, k=33)]
+         dict(n=40, h=16, e=8, k=2, skip=1.0), dict(n=700, h=72, e=9, k=3, one=True), dict(n=2500, h=24, e=4, k=2, one=True), dict(n=20, h=136, e=60, k=40), dict(n=5, h=4104, e=16, k=4), dict(n=2, h=16392, e=40, k=33),
+         dict(n=1300, h=40, e=60, k=40, skip=0.3), dict(n=1190, h=1096, e=50, k=35, skip=0.1), dict(n=1500, h=520, e=70, k=9), dict(n=1184, h=8, e=2, k=1, skip=1.0)]
 
 
 def run(case, dtype, shared, weights=True):
@@ -175,6 +176,34 @@ def test_plans_in_another_order_and_repeated_experts():
     want = torch.full((n * k,), -1, dtype=torch.int32)
     want[perm] = torch.arange(perm.numel(), dtype=torch.int32)
     assert torch.equal(slots.cpu(), want) and torch.equal(rows[: perm.numel()].cpu(), x[perm // k])
+
+
+@pytest.mark.parametrize("n", (30, 1300))
+def test_shared_expert_for_a_part_of_the_tokens(n):
+    """the plan of a rank that evaluates the shared expert for its own tokens: the others have no shared slot"""
+    from tqllm_b200 import capi, moe
+    from tqllm_b200.capi import check, lib
+    k, e, h, first, count = 3, 7, 64, 5, 11
+    ids, x, w, sw, g = make(n, h, e, k, BF16, 3, skip=0.4)
+    di, dx = ids.cuda(), x.cuda()
+    plan = moe.Plan(e, n, k, count, "cuda")
+    ws = torch.empty(max(16, lib.b2moe_dispatch_workspace_bytes(e, n * k)), dtype=torch.uint8, device="cuda")
+    stream = torch.cuda.current_stream().cuda_stream
+    check(lib.b2moe_dispatch_range(di.data_ptr(), n, k, e, first, count, plan.buf.data_ptr(), ws.data_ptr(), ws.numel(), stream), "range")
+    rows, slots = moe.dispatch_rows(dx, di, plan)
+    routed, token = sorted_plain(ids, e, False)
+    live = token.numel()
+    want = torch.cat([routed, torch.full((n,), -1, dtype=torch.int32)])
+    want[n * k + first : n * k + first + count] = torch.arange(live, live + count, dtype=torch.int32)
+    assert slots.numel() == n * k + n and torch.equal(slots.cpu(), want)
+    assert torch.equal(rows[:live].cpu(), x[token]) and torch.equal(rows[live : live + count].cpu(), x[first : first + count]) and not rows[live + count :].any()
+    out = moe.combine_rows(rows, slots, w.cuda(), n, k, shared_weights=sw.cuda())
+    total, size = plain_back(rows.cpu(), want, w, sw, None, n, k, True)
+    near(out, total, (k + 3) * U * size, BF16)
+    gy, gw, gs = moe.combine_rows_backward(dx, rows, slots, w.cuda(), n, k, shared_weights=sw.cuda())
+    own = torch.zeros(n, dtype=torch.bool)
+    own[first : first + count] = True
+    assert not gs.cpu()[~own].any() and bool((gs.cpu()[own] > 0).all())
 
 
 def test_slots_that_lead_nowhere_and_ids_of_another_plan():
