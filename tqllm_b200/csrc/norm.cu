@@ -173,6 +173,7 @@ __device__ __forceinline__ T over_row(T v, T none, T * red, F join) {
     return v;
 }
 struct Add { __device__ float operator()(float a, float b) const { return a + b; } };
+struct Max { __device__ float operator()(float a, float b) const { return fmaxf(a, b); } };
 struct Add2 { __device__ float2 operator()(float2 a, float2 b) const { return make_float2(a.x + b.x, a.y + b.y); } };
 struct AddMax { __device__ float2 operator()(float2 a, float2 b) const { return make_float2(a.x + b.x, max_nan(a.y, b.y)); } };
 
@@ -197,14 +198,28 @@ __device__ __forceinline__ bool near_half(float u, float inv) {
     const float m = MAGIC - __fmaf_rn(u, inv, MAGIC);
     return fmaf(fabsf(m), OFF, fabsf(__fmaf_rn(u, inv, m))) > 0.5f - OFF;
 }
-// Squares that pass the range of 32 bits: the row is taken once more in this unit, in which they do not (16384 squares of 2^48 at most), nor does what is small count there
-constexpr float UNIT = 0x1p-80f;
+// Rows whose mean square (with eps) lies outside of this range: squares have passed 32 bits, or lost bits below their normal numbers. They are taken once more in a unit of their own
+constexpr float LEAST = 0x1p-64f;
+__device__ __forceinline__ bool ordinary(float m) { return m >= LEAST && m < INFINITY; }
+// a power of two that brings a row's largest value to 2^48 (to 2^-49 at least, from below the normal numbers): 16384 squares stay inside of 32 bits, and only what is 2^-111 of the largest square loses bits
+__device__ __forceinline__ float unit_of(float largest) { return __uint_as_float(uint32_t(min(227, 302 - int(__float_as_uint(largest) >> 23))) << 23); }
+constexpr float UNIT = 0x1p-80f;                 // of the gradient's rows whose squares pass the range
 
 // P pieces of V values a thread, in pairs (V = 1: a value and a zero); WARP: a warp a row, eight rows a block; otherwise the block, of MOST threads at most, takes a row. WDT: the weight's type; Q: 8-bit
-// rows are wanted. With 128 threads a row the registers are held to what five or six blocks of an SM have
+// rows are wanted. Registers are held to what this many blocks of an SM have: left alone, the second look at rows that are not ordinary takes up to 38 more than the rest needs (8192 x 256 bf16: 4.4 us
+// instead of 3.5, 512 x 4096 2.9 instead of 2.6)
 template <int DT, int WDT, int V, int P, bool WARP, bool Q, bool SHIFT, int MOST>
-__global__ void __launch_bounds__(MOST, MOST == 128 && V > 1 ? (Q ? 5 : 6) : WARP ? 2 : 1) norm_k(const NormArgs p) {
-    __shared__ float2 red[SHIFT ? 2 : 1][32], red_again[SHIFT ? 2 : 1][32];
+constexpr int norm_blocks() {
+    constexpr bool narrow = V == 8 && WDT == DT && !Q;
+    if (SHIFT) return P == 1 ? 10 : 1;
+    if (WARP) return narrow ? 3 : 2;
+    if (V > 1 && MOST == 128) return Q ? 5 : 6;
+    return P == 1 && narrow ? 4 : 1;
+}
+template <int DT, int WDT, int V, int P, bool WARP, bool Q, bool SHIFT, int MOST>
+__global__ void __launch_bounds__(MOST, norm_blocks<DT, WDT, V, P, WARP, Q, SHIFT, MOST>()) norm_k(const NormArgs p) {
+    __shared__ float2 red[SHIFT ? 2 : 1][32];
+    __shared__ float red_again[32];
     __shared__ unsigned long long exact_top[WARP ? 8 : 1];
     grid_release();
     grid_wait();
@@ -270,27 +285,19 @@ __global__ void __launch_bounds__(MOST, MOST == 128 && V > 1 ? (Q ? 5 : 6) : WAR
             }
         }
         float tops[Q ? P : 1];                                             // of the pieces
-        auto sums = [&]() {                                                // squares, the largest product
-            Two squares = two(0.f);
-            float top = 0.f;
+        Two squares = two(0.f);
+        float2 mine = make_float2(0.f, 0.f);                               // squares, the largest product
 #pragma unroll
-            for (int i = 0; i < P; ++i) {
-                if (Q) tops[i] = 0.f;
+        for (int i = 0; i < P; ++i) {
+            if (Q) tops[i] = 0.f;
 #pragma unroll
-                for (int l = 0; l < H; ++l) {
-                    squares = fma2(h[i][l], h[i][l], squares);
-                    if (Q) tops[i] = largest(tops[i], h[i][l] * w[i].pair(l));
-                }
-                if (Q) top = max_nan(top, tops[i]);
+            for (int l = 0; l < H; ++l) {
+                squares = fma2(h[i][l], h[i][l], squares);
+                if (Q) tops[i] = largest(tops[i], h[i][l] * w[i].pair(l));
             }
-            const float2 s = apart(squares);
-            return make_float2(s.x + s.y, top);
-        };
-        auto join = [&](float2 v, float2 * red) {
-            if constexpr (Q) return over_row<WARP>(v, make_float2(0.f, 0.f), red, AddMax());
-            else return make_float2(over_row<WARP>(v.x, 0.f, reinterpret_cast<float *>(red), Add()), 0.f);
-        };
-        float2 mine = sums();
+            if (Q) mine.y = max_nan(mine.y, tops[i]);
+        }
+        mine.x = apart(squares).x + apart(squares).y;
         if (p.sum) {
 #pragma unroll
             for (int i = 0; i < P; ++i) {
@@ -298,19 +305,31 @@ __global__ void __launch_bounds__(MOST, MOST == 128 && V > 1 ? (Q ? 5 : 6) : WAR
                 if (grid.any(j)) put<DT>(p.sum, size_t(row) * p.lds, j, grid, h[i]);
             }
         }
-        float2 all = join(mine, red[turn]);
+        float2 all;
+        if constexpr (Q) all = over_row<WARP>(mine, make_float2(0.f, 0.f), red[turn], AddMax());
+        else all = make_float2(over_row<WARP>(mine.x, 0.f, reinterpret_cast<float *>(red[turn]), Add()), 0.f);
         const bool fine = all.y < INFINITY;                                // no infinity, no NaN, no product beyond 32 bits
-        float unit = 1.f;
-        if (!(all.x < INFINITY)) {
-            unit = UNIT;
+        float unit = 1.f, m = fmaf(all.x, p.inv_k, p.eps);
+        if (!ordinary(m)) {
+            float most = 0.f;
 #pragma unroll
             for (int i = 0; i < P; ++i)
 #pragma unroll
-                for (int l = 0; l < H; ++l) h[i][l] = h[i][l] * two(UNIT);
-            mine = sums();
-            all = join(mine, red_again[turn]);
+                for (int l = 0; l < H; ++l) most = fmaxf(most, fmaxf(fabsf(apart(h[i][l]).x), fabsf(apart(h[i][l]).y)));
+            unit = unit_of(over_row<WARP>(most, 0.f, red_again, Max()));
+            squares = two(0.f);
+#pragma unroll
+            for (int i = 0; i < P; ++i)
+#pragma unroll
+                for (int l = 0; l < H; ++l) {
+                    const Two f = h[i][l] * two(unit);
+                    squares = fma2(f, f, squares);
+                    if (!Q) h[i][l] = f;                                   // with 8-bit rows the products stay those of the values as they came
+                }
+            if (!WARP) __syncthreads();                                    // the maxima have been read
+            m = fmaf(over_row<WARP>(apart(squares).x + apart(squares).y, 0.f, red_again, Add()), p.inv_k, p.eps * unit * unit);
         }
-        const float rho = inverse_root(fmaf(all.x, p.inv_k, p.eps * unit * unit));
+        const float rho = inverse_root(m);                                 // in the unit
         if (p.y) {
 #pragma unroll
             for (int i = 0; i < P; ++i) {
@@ -318,13 +337,18 @@ __global__ void __launch_bounds__(MOST, MOST == 128 && V > 1 ? (Q ? 5 : 6) : WAR
                 if (!grid.any(j)) continue;
                 Two y[H];
 #pragma unroll
-                for (int l = 0; l < H; ++l) y[l] = h[i][l] * two(rho) * w[i].pair(l);
+                for (int l = 0; l < H; ++l) y[l] = (Q ? h[i][l] * two(unit) : h[i][l]) * two(rho) * w[i].pair(l);
                 put<DT>(p.y, size_t(row) * p.ldy, j, grid, y);
             }
         }
         if constexpr (Q) {
+            // the products are worked out again below: kept since the sums they would take 32 registers (and spill)
+#pragma unroll
+            for (int i = 0; i < P; ++i)
+#pragma unroll
+                for (int l = 0; l < H; ++l) asm("" : "+l"(h[i][l].v));
             const float top = all.y;
-            if (tid == 0) p.scale[row] = !fine ? __int_as_float(0x7fc00000) : top > 0.f ? top * rho / 127.f : 0.f;
+            if (tid == 0) p.scale[row] = !fine ? __int_as_float(0x7fc00000) : !(top > 0.f) ? 0.f : unit == 1.f ? top * rho / 127.f : float(double(top) * rho * unit / 127.0);
             if (WARP || blockDim.x == 32) __syncwarp();
             // the largest product exactly, from the pieces of those that round to the largest (numbers above zero are ordered as their bits are)
             if (mine.y == top && top > 0.f) {
@@ -408,7 +432,7 @@ int32_t launch_norm(const NormArgs & a, Form form, cudaStream_t s) {
         // blocks that walk rows, a multiple of eight: 1024 threads an SM, of short rows 2048 (8192 x 333: 13.2 and 9.7 us)
         const int threads = by_warp <= 4 ? by_warp * 32 : ceil_div(by_warp, MOST) * 32;
         const dim3 blocks(std::min((a.n + 7) / 8 * 8, SMS * std::max(1, (by_warp <= 4 ? 2048 : 1024) / threads) / 8 * 8));
-        if (by_warp <= 4) launch_overlapped(norm_k<DT, WDT, V, 1, false, false, true, 512>, blocks, dim3(threads), 0, s, a);
+        if (by_warp <= 4) launch_overlapped(norm_k<DT, WDT, V, 1, false, false, true, 128>, blocks, dim3(threads), 0, s, a);
         else launch_overlapped(norm_k<DT, WDT, V, MOST, false, false, true, 512>, blocks, dim3(threads), 0, s, a);
     }
     else if (a.k <= 2048) go(norm_k<DT, WDT, 1, 4, false, false, false, 512>, ceil_div(a.k, 128) * 32);
