@@ -363,7 +363,7 @@ __global__ void __launch_bounds__(MOST, norm_blocks<DT, WDT, V, P, WARP, Q, SHIF
                         }
                 atomicMax(exact, (unsigned long long)__double_as_longlong(most));
             }
-            const bool tiny = top < 0x1p-100f;                             // products have lost bits there: all are taken exactly
+            const bool tiny = top < 0x1p-100f;                             // products have lost bits there, or all of theirs
             const float inv = tiny || !fine ? 0.f : __fdiv_rn(127.f, top);
             // (OFF) u, top and inv are off by 2^-24 of themselves each, the quotient t by 3 |t| 2^-24: those that close to a half are done again, exactly. The nearest integer m comes from t + 1.5 * 2^23;
             // |t| <= |m| + 1/2. A piece is looked at by its largest m and its largest distance from an integer (one row of 4096 in fifteen has such a piece)
@@ -388,11 +388,41 @@ __global__ void __launch_bounds__(MOST, norm_blocks<DT, WDT, V, P, WARP, Q, SHIF
                 if (j >= p.k) continue;
                 if constexpr (V == 8) *reinterpret_cast<uint2 *>(q + j) = make_uint2(o[0], o[1]);
                 else *reinterpret_cast<uint32_t *>(q + j) = o[0];
-                if (tiny || fmaf(big, OFF, far) > 0.5f - OFF) some |= 1u << i;
+                if (fmaf(big, OFF, far) > 0.5f - OFF) some |= 1u << i;
             }
             if (WARP || blockDim.x == 32) __syncwarp();
             else __syncthreads();                                          // the exact top is there
-            if (!some || !fine || top == 0.f) return;
+            if (tiny) {
+                // all products exactly, then the largest, the scale and every integer from it
+                double most = 0.0;
+#pragma unroll
+                for (int i = 0; i < P; ++i) {
+                    unsigned long long bits = 0;
+#pragma unroll
+                    for (int l = 0; l < H; ++l) bits |= h[i][l].v;
+                    if (bits & 0x7fffffff7fffffffull)                      // rows of zeros have nothing to work out
+#pragma unroll
+                        for (int l = 0; l < V; ++l) most = fmax(most, fabs(double(l & 1 ? apart(h[i][l / 2]).y : apart(h[i][l / 2]).x) * double(w[i][l])));
+                }
+                if (most > 0.0) atomicMax(exact, (unsigned long long)__double_as_longlong(most));
+                if (WARP || blockDim.x == 32) __syncwarp();
+                else __syncthreads();
+                most = __longlong_as_double((long long)*exact);
+                if (most == 0.0) return;
+                if (tid == 0) p.scale[row] = float(most * rho * unit / 127.0);
+#pragma unroll
+                for (int i = 0; i < P; ++i) {
+                    const int j = grid.first(i * nt + tid);
+                    if (j < p.k)
+#pragma unroll
+                        for (int l = 0; l < V; ++l) {
+                            const float hl = l & 1 ? apart(h[i][l / 2]).y : apart(h[i][l / 2]).x;
+                            q[j + l] = int8_t(decide(hl, w[i][l], floor(127.0 * fabs(double(hl) * double(w[i][l])) / most), most));
+                        }
+                }
+                return;
+            }
+            if (!some || !fine) return;
             const double largest_product = __longlong_as_double((long long)*exact);
 #pragma unroll
             for (int i = 0; i < P; ++i)
@@ -400,9 +430,7 @@ __global__ void __launch_bounds__(MOST, norm_blocks<DT, WDT, V, P, WARP, Q, SHIF
 #pragma unroll
                     for (int l = 0; l < V; ++l) {
                         const float hl = l & 1 ? apart(h[i][l / 2]).y : apart(h[i][l / 2]).x, u = hl * w[i][l];
-                        if (!tiny && !near_half(u, inv)) continue;
-                        const double low = tiny ? floor(127.0 * fabs(double(hl) * double(w[i][l])) / largest_product) : double(floorf(fabsf(u * inv)));
-                        q[grid.first(i * nt + tid) + l] = int8_t(decide(hl, w[i][l], low, largest_product));
+                        if (near_half(u, inv)) q[grid.first(i * nt + tid) + l] = int8_t(decide(hl, w[i][l], double(floorf(fabsf(u * inv))), largest_product));
                     }
         }
     }
