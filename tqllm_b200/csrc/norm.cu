@@ -203,7 +203,6 @@ constexpr float LEAST = 0x1p-64f;
 __device__ __forceinline__ bool ordinary(float m) { return m >= LEAST && m < INFINITY; }
 // a power of two that brings a row's largest value to 2^48 (to 2^-49 at least, from below the normal numbers): 16384 squares stay inside of 32 bits, and only what is 2^-111 of the largest square loses bits
 __device__ __forceinline__ float unit_of(float largest) { return __uint_as_float(uint32_t(min(227, 302 - int(__float_as_uint(largest) >> 23))) << 23); }
-constexpr float UNIT = 0x1p-80f;                 // of the gradient's rows whose squares pass the range
 
 // P pieces of V values a thread, in pairs (V = 1: a value and a zero); WARP: a warp a row, eight rows a block; otherwise the block, of MOST threads at most, takes a row. WDT: the weight's type; Q: 8-bit
 // rows are wanted. Registers are held to what this many blocks of an SM have: left alone, the second look at rows that are not ordinary takes up to 38 more than the rest needs (8192 x 256 bf16: 4.4 us
@@ -487,7 +486,7 @@ __device__ __forceinline__ void copy16(void * shared, const void * global) {
 template <int DT, int WDT, int V, int P, bool SHIFT, bool WARP>
 __global__ void __launch_bounds__(WARP ? 256 : 512, (WARP ? 2 : 1) * (P <= 2 ? 2 : 1)) norm_grad_k(const NormGradArgs p) {
     extern __shared__ __align__(16) uint4 ahead[];                     // [stages][h, dy, ds][P][threads]
-    __shared__ float2 red[2][32], red_again[2][32];
+    __shared__ float2 red[2][32], red_again[32];
     grid_release();
     grid_wait();
     const int nt = WARP ? 32 : blockDim.x, tid = WARP ? threadIdx.x & 31 : threadIdx.x, warp = threadIdx.x >> 5;
@@ -549,47 +548,76 @@ __global__ void __launch_bounds__(WARP ? 256 : 512, (WARP ? 2 : 1) * (P <= 2 ? 2
             }
             return v;
         };
+        // FAR: the row is taken in a unit of its own
         float unit = 1.f;
-        auto sums = [&]() {
+        auto sums = [&](auto FAR) {
             float2 v = make_float2(0.f, 0.f);
+            auto add = [&](int i, const Piece<WDT, V> & w) {
+                const int j = grid.first(i * nt + tid);
+                if (!grid.any(j)) return;
+                const Piece<DT, V> h = piece(0, i, j), g = piece(1, i, j);
+#pragma unroll
+                for (int l = 0; l < V; ++l) {
+                    const float f = FAR ? h[l] * unit : h[l];
+                    v.x = fmaf(f, f, v.x);
+                    v.y = fmaf(g[l] * w[l], f, v.y);
+                }
+            };
+            if constexpr (FAR && !COPIES) {                            // the weight once more, so that these loops need no registers beside the other ones'
+#pragma unroll 2
+                for (int i = 0; i < P; ++i) {
+                    Piece<WDT, V> again;
+                    again.zero();
+                    if (grid.any(grid.first(i * nt + tid))) get_weight(again, p.w, grid.first(i * nt + tid), grid);
+                    add(i, again);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < P; ++i) add(i, w[i]);
+            }
+            return v;
+        };
+        auto finish = [&](auto FAR, float rho, float t) {
 #pragma unroll
             for (int i = 0; i < P; ++i) {
                 const int j = grid.first(i * nt + tid);
                 if (!grid.any(j)) continue;
                 const Piece<DT, V> h = piece(0, i, j), g = piece(1, i, j);
+                Piece<DT, V> s;
+                s.zero();
+                if (p.ds) s = piece(2, i, j);
+                float d[V];
 #pragma unroll
                 for (int l = 0; l < V; ++l) {
-                    const float f = h[l] * unit;
-                    v.x = fmaf(f, f, v.x);
-                    v.y = fmaf(g[l] * w[i][l], f, v.y);
+                    const float f = FAR ? h[l] * unit : h[l], a = fmaf(-f, t, g[l] * w[i][l]);
+                    d[l] = FAR && (COPIES || unit != 1.f) ? fmaf(rho * a, unit, s[l]) : fmaf(rho, a, s[l]);
+                    dw[i][l] = fmaf(g[l], f * rho, dw[i][l]);
                 }
+                put<DT>(p.dx, size_t(row) * p.ldx, j, grid, d);
             }
-            return v;
         };
-        float2 v = over_row<WARP>(sums(), make_float2(0.f, 0.f), red[turn], Add2());
-        if (!(v.x < INFINITY)) {
-            unit = UNIT;
-            v = over_row<WARP>(sums(), make_float2(0.f, 0.f), red_again[turn], Add2());
+        float2 v = over_row<WARP>(sums(std::false_type{}), make_float2(0.f, 0.f), red[turn], Add2());
+        float m = fmaf(v.x, p.inv_k, p.eps);
+        if (!ordinary(m)) {
+            v = make_float2(0.f, 0.f);
+#pragma unroll (COPIES ? P : 2)
+            for (int i = 0; i < P; ++i) {
+                const int j = grid.first(i * nt + tid);
+                if (!grid.any(j)) continue;
+                const Piece<DT, V> h = piece(0, i, j);
+#pragma unroll
+                for (int l = 0; l < V; ++l) v.x = fmaxf(v.x, fabsf(h[l]));
+            }
+            unit = unit_of(over_row<WARP>(v.x, 0.f, reinterpret_cast<float *>(red_again), Max()));
+            if (!WARP) __syncthreads();                                // the maxima have been read
+            v = over_row<WARP>(sums(std::true_type{}), make_float2(0.f, 0.f), red_again, Add2());
+            m = fmaf(v.x, p.inv_k, p.eps * unit * unit);
         }
         // in the unit: rho h as it is, rho the unit times as large
-        const float m = fmaf(v.x, p.inv_k, p.eps * unit * unit), rho = inverse_root(m), t = v.y * p.inv_k * rho * rho, out = rho * unit;
-#pragma unroll
-        for (int i = 0; i < P; ++i) {
-            const int j = grid.first(i * nt + tid);
-            if (!grid.any(j)) continue;
-            const Piece<DT, V> h = piece(0, i, j), g = piece(1, i, j);
-            Piece<DT, V> s;
-            s.zero();
-            if (p.ds) s = piece(2, i, j);
-            float d[V];
-#pragma unroll
-            for (int l = 0; l < V; ++l) {
-                const float f = h[l] * unit;
-                d[l] = fmaf(out, fmaf(-f, t, g[l] * w[i][l]), s[l]);
-                dw[i][l] = fmaf(g[l], f * rho, dw[i][l]);
-            }
-            put<DT>(p.dx, size_t(row) * p.ldx, j, grid, d);
-        }
+        const float rho = inverse_root(m), t = v.y * p.inv_k * rho * rho;
+        // (value by value there is one form: two of 32 values a thread spill, 2048 x 4097 62 us instead of 55)
+        if (COPIES && unit == 1.f) finish(std::false_type{}, rho, t);
+        else finish(std::true_type{}, rho, t);
         if (COPIES) {                                                  // this row's pieces have been read
             copy(row + p.stages * step, stage);
             if (++stage == p.stages) stage = 0;
