@@ -302,7 +302,7 @@ B2MOE_API int32_t b2moe_linear_i8_epilogue(const int8_t * q, int64_t ldq, const 
  *   and ldq are multiples of 16, strides whole 16 bytes, pointers 16-byte aligned. Bytes of q between k and ldq are left as they are. Rows that
  *   begin on 16 bytes and have whole 16 bytes are the fast case everywhere.
  * b2moe_rms_norm_backward: from h (x, or the sum that the norm wrote) and the gradients of y and (may be null) of the sum:
- *   grad_x = gradient on h = rho (a - h rho^2 mean(a h)) + grad_sum with a = grad_y weight, rho = 1 / sqrt(mean(h^2) + eps);
+ *   grad_x = gradient on h = rho (a - h rho^2 mean(a h)) + grad_sum with a = grad_y weight (infinite where the product passes 32 bits), rho = 1 / sqrt(mean(h^2) + eps);
  *   grad_weight fp32 [k] (null: not wanted) = (accumulate: +) sum over the rows of grad_y h rho, in a fixed order. grad_x may lie on h, grad_y
  *   or grad_sum of the same stride. workspace: b2moe_rms_norm_backward_workspace_bytes(n, k) bytes, 16-byte aligned, used by one call at a time
  *   (null where grad_weight is). */

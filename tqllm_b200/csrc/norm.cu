@@ -174,6 +174,7 @@ __device__ __forceinline__ T over_row(T v, T none, T * red, F join) {
 }
 struct Add { __device__ float operator()(float a, float b) const { return a + b; } };
 struct Max { __device__ float operator()(float a, float b) const { return fmaxf(a, b); } };
+struct Max2 { __device__ float2 operator()(float2 a, float2 b) const { return make_float2(fmaxf(a.x, b.x), fmaxf(a.y, b.y)); } };
 struct Add2 { __device__ float2 operator()(float2 a, float2 b) const { return make_float2(a.x + b.x, a.y + b.y); } };
 struct AddMax { __device__ float2 operator()(float2 a, float2 b) const { return make_float2(a.x + b.x, max_nan(a.y, b.y)); } };
 
@@ -200,6 +201,8 @@ __device__ __forceinline__ bool near_half(float u, float inv) {
 }
 // Rows whose mean square (with eps) lies outside of this range: squares have passed 32 bits, or lost bits below their normal numbers. They are taken once more in a unit of their own
 constexpr float LEAST = 0x1p-64f;
+__device__ __forceinline__ int exponent_of(float power) { return int(__float_as_uint(power) >> 23) - 127; }
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float(uint32_t(e + 127) << 23); }
 __device__ __forceinline__ bool ordinary(float m) { return m >= LEAST && m < INFINITY; }
 // a power of two that brings a row's largest value to 2^48 (to 2^-49 at least, from below the normal numbers): 16384 squares stay inside of 32 bits, and only what is 2^-111 of the largest square loses bits
 __device__ __forceinline__ float unit_of(float largest) { return __uint_as_float(uint32_t(min(227, 302 - int(__float_as_uint(largest) >> 23))) << 23); }
@@ -548,28 +551,26 @@ __global__ void __launch_bounds__(WARP ? 256 : 512, (WARP ? 2 : 1) * (P <= 2 ? 2
             }
             return v;
         };
-        // FAR: the row is taken in a unit of its own
-        float unit = 1.f;
-        auto sums = [&](auto FAR) {
+        // FAR: the row and a = dy w are taken in units of their own
+        float unit = 1.f, unit_a = 1.f;
+        // what(h, a, so far) over the row's values. Value by value a second look takes the weight once more, so that it needs no registers beside the first one's
+        auto look = [&](auto what, auto again) {
             float2 v = make_float2(0.f, 0.f);
             auto add = [&](int i, const Piece<WDT, V> & w) {
                 const int j = grid.first(i * nt + tid);
                 if (!grid.any(j)) return;
                 const Piece<DT, V> h = piece(0, i, j), g = piece(1, i, j);
 #pragma unroll
-                for (int l = 0; l < V; ++l) {
-                    const float f = FAR ? h[l] * unit : h[l];
-                    v.x = fmaf(f, f, v.x);
-                    v.y = fmaf(g[l] * w[l], f, v.y);
-                }
+                for (int l = 0; l < V; ++l) v = what(h[l], g[l] * w[l], v);
             };
-            if constexpr (FAR && !COPIES) {                            // the weight once more, so that these loops need no registers beside the other ones'
+            if constexpr (again && !COPIES) {
 #pragma unroll 2
                 for (int i = 0; i < P; ++i) {
-                    Piece<WDT, V> again;
-                    again.zero();
-                    if (grid.any(grid.first(i * nt + tid))) get_weight(again, p.w, grid.first(i * nt + tid), grid);
-                    add(i, again);
+                    const int j = grid.first(i * nt + tid);
+                    Piece<WDT, V> once;
+                    once.zero();
+                    if (grid.any(j)) get_weight(once, p.w, j, grid);
+                    add(i, once);
                 }
             } else {
 #pragma unroll
@@ -577,7 +578,12 @@ __global__ void __launch_bounds__(WARP ? 256 : 512, (WARP ? 2 : 1) * (P <= 2 ? 2
             }
             return v;
         };
+        auto sums = [](float h, float a, float2 v) { return make_float2(fmaf(h, h, v.x), fmaf(a, h, v.y)); };
         auto finish = [&](auto FAR, float rho, float t) {
+            // a product of the units that may pass 32 bits by itself, in two halves
+            const int e = exponent_of(unit) - exponent_of(unit_a);
+            const float half = power_of_two(e / 2), rest = power_of_two(e - e / 2);
+            const bool far = FAR && (COPIES || unit != 1.f || unit_a != 1.f);
 #pragma unroll
             for (int i = 0; i < P; ++i) {
                 const int j = grid.first(i * nt + tid);
@@ -589,34 +595,28 @@ __global__ void __launch_bounds__(WARP ? 256 : 512, (WARP ? 2 : 1) * (P <= 2 ? 2
                 float d[V];
 #pragma unroll
                 for (int l = 0; l < V; ++l) {
-                    const float f = FAR ? h[l] * unit : h[l], a = fmaf(-f, t, g[l] * w[i][l]);
-                    d[l] = FAR && (COPIES || unit != 1.f) ? fmaf(rho * a, unit, s[l]) : fmaf(rho, a, s[l]);
+                    const float f = FAR ? h[l] * unit : h[l], a = fmaf(-f, t, FAR ? g[l] * w[i][l] * unit_a : g[l] * w[i][l]);
+                    d[l] = far ? fmaf(rho * a * half, rest, s[l]) : fmaf(rho, a, s[l]);
                     dw[i][l] = fmaf(g[l], f * rho, dw[i][l]);
                 }
                 put<DT>(p.dx, size_t(row) * p.ldx, j, grid, d);
             }
         };
-        float2 v = over_row<WARP>(sums(std::false_type{}), make_float2(0.f, 0.f), red[turn], Add2());
-        float m = fmaf(v.x, p.inv_k, p.eps);
-        if (!ordinary(m)) {
-            v = make_float2(0.f, 0.f);
-#pragma unroll (COPIES ? P : 2)
-            for (int i = 0; i < P; ++i) {
-                const int j = grid.first(i * nt + tid);
-                if (!grid.any(j)) continue;
-                const Piece<DT, V> h = piece(0, i, j);
-#pragma unroll
-                for (int l = 0; l < V; ++l) v.x = fmaxf(v.x, fabsf(h[l]));
-            }
-            unit = unit_of(over_row<WARP>(v.x, 0.f, reinterpret_cast<float *>(red_again), Max()));
+        float2 v = over_row<WARP>(look(sums, std::false_type{}), make_float2(0.f, 0.f), red[turn], Add2());
+        float m = fmaf(v.x, p.inv_k, p.eps), rho = inverse_root(m), t = v.y * p.inv_k * rho * rho;
+        if (!ordinary(m) || !(fabsf(t) < INFINITY)) {
+            const float2 largest = over_row<WARP>(look([&](float h, float a, float2 v) { return make_float2(fmaxf(v.x, fabsf(h)), fmaxf(v.y, fabsf(a))); }, std::true_type{}), make_float2(0.f, 0.f), red_again, Max2());
+            unit = unit_of(largest.x);
+            unit_a = unit_of(largest.y);
             if (!WARP) __syncthreads();                                // the maxima have been read
-            v = over_row<WARP>(sums(std::true_type{}), make_float2(0.f, 0.f), red_again, Add2());
+            v = over_row<WARP>(look([&](float h, float a, float2 v) { return sums(h * unit, a * unit_a, v); }, std::true_type{}), make_float2(0.f, 0.f), red_again, Add2());
             m = fmaf(v.x, p.inv_k, p.eps * unit * unit);
+            // in the units: rho h as it is, rho and t h in theirs
+            rho = inverse_root(m);
+            t = v.y * p.inv_k * rho * rho;
         }
-        // in the unit: rho h as it is, rho the unit times as large
-        const float rho = inverse_root(m), t = v.y * p.inv_k * rho * rho;
         // (value by value there is one form: two of 32 values a thread spill, 2048 x 4097 62 us instead of 55)
-        if (COPIES && unit == 1.f) finish(std::false_type{}, rho, t);
+        if (COPIES && unit == 1.f && unit_a == 1.f) finish(std::false_type{}, rho, t);
         else finish(std::true_type{}, rho, t);
         if (COPIES) {                                                  // this row's pieces have been read
             copy(row + p.stages * step, stage);
