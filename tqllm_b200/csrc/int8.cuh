@@ -72,7 +72,8 @@ __device__ __forceinline__ Two normal_tail(Two x) {
     return exp2_near(two(-0.72134752f) * x * x) * (t * q);
 }
 // 2 N values at a time under one switch, so that they are in flight together. What is small stays exact to its own size: the negative tail of GELU is a complementary error function,
-// (1 + tanh z) / 2 = 1 / (1 + e^-2z). A NaN stays one
+// (1 + tanh z) / 2 = 1 / (1 + e^-2z), and where e^-v passes 32 bits before v / (1 + e^-v) leaves them, that is v e^(v / 2) e^(v / 2). A NaN stays one
+constexpr float FAR_SILU = -80.f;                // (selects instead of the branch: 4096 rows of 4096 x 512 36.6 us instead of 33.3)
 template <int N>
 __device__ __forceinline__ void activate(int act, Two (&f)[N]) {
     if (act == B2MOE_ACT_RELU) {
@@ -82,10 +83,24 @@ __device__ __forceinline__ void activate(int act, Two (&f)[N]) {
             f[i] = two(v.x < 0.f ? 0.f : v.x, v.y < 0.f ? 0.f : v.y);
         }
     } else if (act == B2MOE_ACT_SILU) {
+        float least = 0.f;
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const float2 v = apart(f[i]);
-            f[i] = f[i] * reciprocal(two(expf(-v.x), expf(-v.y)) + two(1.f));
+        for (int i = 0; i < N; ++i) least = fminf(least, fminf(apart(f[i]).x, apart(f[i]).y));
+        if (least >= FAR_SILU) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const float2 v = apart(f[i]);
+                f[i] = f[i] * reciprocal(two(expf(-v.x), expf(-v.y)) + two(1.f));
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const float2 v = apart(f[i]);
+                const bool x = v.x < FAR_SILU, y = v.y < FAR_SILU;
+                const Two e = two(expf(x ? 0.5f * v.x : -v.x), expf(y ? 0.5f * v.y : -v.y));
+                const float2 near = apart(f[i] * reciprocal(e + two(1.f))), far = apart(f[i] * e * e);
+                f[i] = two(x ? far.x : near.x, y ? far.y : near.y);
+            }
         }
     } else if (act == B2MOE_ACT_GELU) {
 #pragma unroll
