@@ -44,17 +44,27 @@ __global__ void __launch_bounds__(32 * GRAD_WARPS) route_grad_k(const RouteGradA
     float * out = p.out + size_t(t) * p.ldg;
     if (!p.add && !p.together)
         for (int c = lane; c < p.experts; c += 32) out[c] = 0.f;
-    // sigmoid: is the selected ones' sum above the clamp
+    // sigmoid: is the selected ones' sum above the clamp. Without the logits of ids outside of the experts, the weights tell: they add up to the scale where it was, and to less of it where the clamp was divided by
     bool coupled = p.norm;
     if (p.sigmoid && p.norm) {
         float sum = 0.f;
+        bool all = true;
         for (int s = lane; s < p.topk; s += 32) {
             const int id = ids[s];
             if (unsigned(id) < unsigned(p.experts)) sum += 1.f / (1.f + expf(-logits[id]));
+            else all = false;
         }
 #pragma unroll
         for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
         coupled = sum > 6.103515625e-5f;
+        if (!coupled && !__all_sync(0xffffffffu, all)) {
+            float total = 0.f;
+            for (int s = lane; s < p.topk; s += 32) total += w[s];
+#pragma unroll
+            for (int d = 16; d; d >>= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
+            // (weights of three roundings each, added up in 128 steps and five at most: 2^-16)
+            coupled = total / p.scale > 1.f - 0x1p-16f;
+        }
     }
     __syncwarp();                                                      // the zeros come before the values
     for (int s0 = 0; s0 < p.topk; s0 += 32) {
