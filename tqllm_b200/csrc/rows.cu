@@ -231,7 +231,7 @@ struct BackGradArgs {
     int pieces, n, topk, shared, rows;
 };
 
-// A warp takes W assignments at a time (more of short rows), or (W = 0, launches of few assignments) a block takes one: the token's gradient, the row, and the product of the two
+// A warp takes W assignments at a time (two of short rows), or (W = 0, launches of few assignments) a block takes one: the token's gradient, the row, and the product of the two
 template <int DT, int W>
 __global__ void __launch_bounds__(256) back_grad_k(const BackGradArgs p) {
     constexpr int N = Vec<DT>::N, M = W ? W : 1, P = 4 / M;            // pieces of an assignment in flight
@@ -311,6 +311,9 @@ bool stride(const void * p, long long ld, int hidden, int dtype) { return !p || 
 constexpr int MANY_TOKENS = 148 * 8, THERE_WARPS = 148 * 16;
 // From how many assignments on a warp takes one in the gradient. us, block / warp: 640 of 2048 4.2 / 3.4, 2240 of 2048 8.2 / 4.6, 1120 of 4096 5.3 / 6.9, 41,000 of 2048 82 / 56
 inline int grad_many(int pieces) { return 148 * (pieces <= 256 ? 4 : 8); }
+// Up to how many pieces a row has two assignments go to a warp there. us, one / two / four a warp, bf16: 8192 tokens of 128 to four 9.7 / 8.0 / 9.0, of 512 12.3 / 10.5 / 13.5, of 1024 26.2 / 24.7 / 32.2, of 2048 46.5 / 48.0 / 58.3; 40,000 of
+// 256 to two 35.3 / 23.3 / 26.1; 1000 of 256 to two 2.1 / 2.7 / 2.8, of 1024 3.1 / 4.6 / 5.1
+constexpr int GRAD_ONE = 64;
 int threads_for(int pieces) { return std::min(256, ceil_div(pieces, 32) * 32); }
 
 }  // namespace
@@ -372,13 +375,13 @@ extern "C" B2MOE_API int32_t b2moe_combine_rows_backward(const void * grad_out, 
                          ldgo / per, ldy / per, ldgy / per, pieces, n, topk, shared_tokens ? 1 : 0, rows};
     const long long all = (long long)n * topk + (shared_tokens ? n : 0);
     cudaStream_t s = as_stream(stream);
-    auto go = [&](auto block, auto one, auto two, auto four) {
+    auto go = [&](auto block, auto one, auto two) {
         if (all < grad_many(pieces)) return launch_overlapped(block, dim3(unsigned(all)), dim3(threads), 0, s, a);
-        const int each = pieces > 64 ? 1 : pieces > 32 ? 2 : 4;
-        launch_overlapped(each == 1 ? one : each == 2 ? two : four, dim3(unsigned((all + 8 * each - 1) / (8 * each))), dim3(256), 0, s, a);
+        const int each = pieces > GRAD_ONE ? 1 : 2;
+        launch_overlapped(each == 1 ? one : two, dim3(unsigned((all + 8 * each - 1) / (8 * each))), dim3(256), 0, s, a);
     };
-    if (dtype == B2MOE_F32) go(back_grad_k<B2MOE_F32, 0>, back_grad_k<B2MOE_F32, 1>, back_grad_k<B2MOE_F32, 2>, back_grad_k<B2MOE_F32, 4>);
-    else if (dtype == B2MOE_F16) go(back_grad_k<B2MOE_F16, 0>, back_grad_k<B2MOE_F16, 1>, back_grad_k<B2MOE_F16, 2>, back_grad_k<B2MOE_F16, 4>);
-    else go(back_grad_k<B2MOE_BF16, 0>, back_grad_k<B2MOE_BF16, 1>, back_grad_k<B2MOE_BF16, 2>, back_grad_k<B2MOE_BF16, 4>);
+    if (dtype == B2MOE_F32) go(back_grad_k<B2MOE_F32, 0>, back_grad_k<B2MOE_F32, 1>, back_grad_k<B2MOE_F32, 2>);
+    else if (dtype == B2MOE_F16) go(back_grad_k<B2MOE_F16, 0>, back_grad_k<B2MOE_F16, 1>, back_grad_k<B2MOE_F16, 2>);
+    else go(back_grad_k<B2MOE_BF16, 0>, back_grad_k<B2MOE_BF16, 1>, back_grad_k<B2MOE_BF16, 2>);
     return launch_status();
 }
