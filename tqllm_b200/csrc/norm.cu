@@ -186,7 +186,7 @@ __device__ __forceinline__ int decide(float h, float w, double low, double top) 
     return u < 0.0 ? -q : q;
 }
 
-// 1 / sqrt(v): the approximation and a step of Newton's, off by 1.5 steps of 2^-24. (Root and quotients by their own rounded instructions, done by every thread of a row: 53 us instead of 51 for 8192 x 4096 to 8 bits)
+// 1 / sqrt(v): the approximation and a step of Newton's, off by 1.5 steps of 2^-24. (Root and reciprocal by their own rounded instructions, done by every thread of a row: 8192 x 4096 to 8 bits 35.3 us instead of 34.6)
 __device__ __forceinline__ float inverse_root(float v) {
     float r;
     asm("rsqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
@@ -441,6 +441,8 @@ __global__ void __launch_bounds__(MOST, norm_blocks<DT, WDT, V, P, WARP, Q, SHIF
 // how the rows of a call lie
 enum Form { WHOLE, SHIFTED, SINGLE };            // whole pieces of 16 bytes; pieces behind a phase that all matrices share; value by value
 
+// us, a warp a row / a piece a thread / 128 threads (bf16): 1024 x 256 1.8 / 1.6 / 1.8, 2368 x 256 1.8 / 2.8 / 2.8, 2368 x 1024 2.6 / 3.4 / 2.8, 8192 x 256 3.5 / 8.9 / 9.1, 8192 x 1024 5.0 / 9.0 / 9.0, 512 x 4096 - / 2.5 / 2.8,
+// 2368 x 4096 - / 7.5 / 6.0, 8192 x 4096 - / 30.0 / 24.3; to 8 bits 1024 x 1024 4.0 / 3.2 / 4.3, 8192 x 1024 11.3 / 12.9 / 11.4, 512 x 4096 - / 4.8 / 4.4, 2368 x 4096 - / 16.5 / 11.3, 512 x 2048 fp32 - / 4.0 / 3.0
 template <int DT, int WDT, bool Q>
 void launch_norm_whole(const NormArgs & a, cudaStream_t s) {
     constexpr int V = DT == B2MOE_F32 ? 4 : 8, MOST = NORM_MAX_COLS / V / 512;
@@ -694,7 +696,8 @@ __global__ void __launch_bounds__(1024) norm_weight_grad_k(const float * parts, 
 }
 
 // Blocks that walk the rows, and so the parts of the weight's gradient. Long rows: as many of an SM as 32 KB of 16-bit values in a row each make, eight at most; a multiple of eight, the most phases that rows
-// have. Short ones, a warp each: four blocks an SM, or two where a row takes four pieces a lane
+// have. Short ones, a warp each: four blocks an SM, or two where a row takes four pieces a lane. us, half of these / these / twice as many blocks, bf16: 8192 x 4096 48.8 / 50.9 / 53.1, 8192 x 2048 27.6 / 30.1 / 30.1,
+// 4096 x 8192 51.5 / 49.1 / 55.1, 2048 x 16384 50.4 / 50.4 / 63.5, 600 x 4096 8.7 / 8.8 / 9.9; a warp each: 30000 x 256 13.0 / 12.8 / 14.4, 30000 x 512 24.9 / 25.8 / 26.2, 8192 x 1024 13.2 / 12.6 / 14.7, 16000 x 128 8.8 / 8.9 / 10.5
 constexpr int GRAD_NUM = 16384;
 int grad_blocks_most(int n, int k) { return std::min((n + 7) / 8 * 8, SMS * std::max(4, std::min(8, GRAD_NUM / k)) / 8 * 8); }
 
