@@ -204,8 +204,9 @@ constexpr float LEAST = 0x1p-64f;
 __device__ __forceinline__ int exponent_of(float power) { return int(__float_as_uint(power) >> 23) - 127; }
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float(uint32_t(e + 127) << 23); }
 __device__ __forceinline__ bool ordinary(float m) { return m >= LEAST && m < INFINITY; }
-// a power of two that brings a row's largest value to 2^48 (to 2^-49 at least, from below the normal numbers): 16384 squares stay inside of 32 bits, and only what is 2^-111 of the largest square loses bits
-__device__ __forceinline__ float unit_of(float largest) { return __uint_as_float(uint32_t(min(227, 302 - int(__float_as_uint(largest) >> 23))) << 23); }
+// a power of two that brings a row's largest value to 2^48 (to 2^-59 at least, from below the normal numbers; 2^90 at most, whose square leaves an eps below LEAST inside of 32 bits): 16384 squares stay inside of
+// 32 bits, and only what is 2^-111 of the largest square loses bits
+__device__ __forceinline__ float unit_of(float largest) { return __uint_as_float(uint32_t(min(217, 302 - int(__float_as_uint(largest) >> 23))) << 23); }
 
 // P pieces of V values a thread, in pairs (V = 1: a value and a zero); WARP: a warp a row, eight rows a block; otherwise the block, of MOST threads at most, takes a row. WDT: the weight's type; Q: 8-bit
 // rows are wanted. Registers are held to what this many blocks of an SM have: left alone, the second look at rows that are not ordinary takes up to 38 more than the rest needs (8192 x 256 bf16: 4.4 us
