@@ -204,9 +204,11 @@ constexpr float LEAST = 0x1p-64f;
 __device__ __forceinline__ int exponent_of(float power) { return int(__float_as_uint(power) >> 23) - 127; }
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float(uint32_t(e + 127) << 23); }
 __device__ __forceinline__ bool ordinary(float m) { return m >= LEAST && m < INFINITY; }
-// a power of two that brings a row's largest value to 2^48 (to 2^-59 at least, from below the normal numbers; 2^90 at most, whose square leaves an eps below LEAST inside of 32 bits): 16384 squares stay inside of
-// 32 bits, and only what is 2^-111 of the largest square loses bits
-__device__ __forceinline__ float unit_of(float largest) { return __uint_as_float(uint32_t(min(217, 302 - int(__float_as_uint(largest) >> 23))) << 23); }
+// A power of two that brings a row's largest value to 2^48: 16384 squares stay inside of 32 bits, and only what is 2^-111 of the largest square loses bits. 2^90 at most (values below the normal numbers become
+// 2^-59 at least), and at most what takes eps to 2^100, beside which smaller squares do not count
+__device__ __forceinline__ float unit_of(float largest, float eps) {
+    return power_of_two(min(min(90, 175 - int(__float_as_uint(largest) >> 23)), (100 - exponent_of(eps)) / 2));
+}
 
 // P pieces of V values a thread, in pairs (V = 1: a value and a zero); WARP: a warp a row, eight rows a block; otherwise the block, of MOST threads at most, takes a row. WDT: the weight's type; Q: 8-bit
 // rows are wanted. Registers are held to what this many blocks of an SM have: left alone, the second look at rows that are not ordinary takes up to 38 more than the rest needs (8192 x 256 bf16: 4.4 us
@@ -319,7 +321,7 @@ __global__ void __launch_bounds__(MOST, norm_blocks<DT, WDT, V, P, WARP, Q, SHIF
             for (int i = 0; i < P; ++i)
 #pragma unroll
                 for (int l = 0; l < H; ++l) most = fmaxf(most, fmaxf(fabsf(apart(h[i][l]).x), fabsf(apart(h[i][l]).y)));
-            unit = unit_of(over_row<WARP>(most, 0.f, red_again, Max()));
+            unit = unit_of(over_row<WARP>(most, 0.f, red_again, Max()), p.eps);
             squares = two(0.f);
 #pragma unroll
             for (int i = 0; i < P; ++i)
@@ -609,8 +611,8 @@ __global__ void __launch_bounds__(WARP ? 256 : 512, (WARP ? 2 : 1) * (P <= 2 ? 2
         float m = fmaf(v.x, p.inv_k, p.eps), rho = inverse_root(m), t = v.y * p.inv_k * rho * rho;
         if (!ordinary(m) || !(fabsf(t) < INFINITY)) {
             const float2 largest = over_row<WARP>(look([&](float h, float a, float2 v) { return make_float2(fmaxf(v.x, fabsf(h)), fmaxf(v.y, fabsf(a))); }, std::true_type{}), make_float2(0.f, 0.f), red_again, Max2());
-            unit = unit_of(largest.x);
-            unit_a = unit_of(largest.y);
+            unit = unit_of(largest.x, p.eps);
+            unit_a = unit_of(largest.y, 0.f);
             if (!WARP) __syncthreads();                                // the maxima have been read
             v = over_row<WARP>(look([&](float h, float a, float2 v) { return sums(h * unit, a * unit_a, v); }, std::true_type{}), make_float2(0.f, 0.f), red_again, Add2());
             m = fmaf(v.x, p.inv_k, p.eps * unit * unit);
